@@ -282,8 +282,8 @@ def _linear_plain(s):
         return out
 
 
-# The rounding of 8-bit states is random, with numbers that are a function of the optimiser's seed, the step and the element's place: a product
-# and two rounds of xor-shift and product, in 32 bits that wrap around.
+# The rounding of 8-bit states is random, with numbers that are a function of the optimiser's seed, the step and the element's place: two rounds of
+# xor-shift and product, in 32 bits that wrap around, for a pair of neighbours, 16 bits for each.
 _PLACE, _ROUND1, _ROUND2, _STEP = 0x9E3779B1, 0x6A09E667, 0xBB67AE85, 0x3C6EF373
 
 
@@ -300,10 +300,10 @@ def _mix(h):
 
 
 def _noise(n, seed, step):
-    """Two 16-bit numbers an element."""
+    """A 16-bit number an element."""
     key = _mix(torch.tensor([_int32(seed + step * _STEP)], dtype=torch.int32, device='cuda'))
-    h = _mix(torch.arange(n, dtype=torch.int32, device='cuda') * _int32(_PLACE) + key)
-    return h & 0xFFFF, (h >> 16) & 0xFFFF
+    h = _mix(torch.arange(n // 2, dtype=torch.int32, device='cuda') * _int32(_PLACE) + key)
+    return torch.stack((h & 0xFFFF, (h >> 16) & 0xFFFF), dim=1).view(-1)
 
 
 def _to_8_bits(x, noise, keep_positive):
@@ -311,7 +311,7 @@ def _to_8_bits(x, noise, keep_positive):
     blocks = x.view(-1, BLOCK)
     most = blocks.abs().amax(1)
     scale = most * (1 / LARGEST)
-    fine = most >= 1e-30
+    fine = ~(most < 1e-30)                            # a NaN stays one
     factor = torch.where(fine, LARGEST * (1 / most), torch.zeros_like(most))
     q = (blocks.abs() * factor[:, None]).view(-1).clamp(max=LARGEST)
     low = 2.0 ** -6                                   # below it e4m3 steps by 2^-9, as it does right above
@@ -347,8 +347,8 @@ def _adamw_plain(s):
     p = p - m / (root * (1 / math.sqrt(1 - h['beta2'] ** t)) + h['eps']) * (h['lr'] / (1 - h['beta1'] ** t))
     s['p'].copy_(p)
     if small:
-        for_m, for_r = _noise(m.numel(), s['seed'], t)
-        for x, noise, codes, scales, positive in ((m, for_m, s['m'], s['ms'], False), (root, for_r, s['v'], s['vs'], True)):
+        noise = _noise(m.numel(), s['seed'], t)
+        for x, codes, scales, positive in ((m, s['m'], s['ms'], False), (root, s['v'], s['vs'], True)):
             q, scale = _to_8_bits(x, noise, positive)
             codes.copy_(q)
             scales.copy_(scale)
@@ -436,13 +436,13 @@ def _exact_adamw(s):
     del update
     if c['bits'] == 32:
         return dict(out, m=first, v=second)
-    low, high = _noise(first.numel(), s['seed'], t)
-    for name, value, noise in (('m', first, low), ('v', second.sqrt_(), high)):
+    noise = _noise(first.numel(), s['seed'], t).double() / 65536
+    for name, value in (('m', first), ('v', second.sqrt_())):
         size = value.abs()
         top = size.view(-1, BLOCK).max(dim=1).values
         q = size / top.clamp(min=1e-30).repeat_interleave(BLOCK) * LARGEST
         grid = torch.exp2(torch.frexp(q).exponent.clamp(min=-5).double() - 4)           # the distance of e4m3's neighbours
-        q = torch.floor(q / grid + noise.double() / 65536).mul_(grid)
+        q = torch.floor(q / grid + noise).mul_(grid)
         if name == 'v':
             q = torch.where((q == 0) & (size > 0), torch.full_like(q, 2.0 ** -9), q)
         out[name], out[name + '_scale'] = torch.copysign(q, value), top / LARGEST
