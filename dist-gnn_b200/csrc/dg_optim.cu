@@ -1,0 +1,457 @@
+// One AdamW step over all tensors of a model, states in 32 bits or in 8, and the norm of all gradients that clips them.
+//
+//   g' = g min(1, max_norm / (|g| + 1e-6)),  m = b1 m + (1 - b1) g',  v = b2 v + (1 - b2) g'^2,  r = sqrt(v)
+//   p  = p (1 - lr wd) - lr / (1 - b1^t)  m / (r / sqrt(1 - b2^t) + eps)
+//
+// All of it in fp32, whatever the type of p and g, each operation rounded by itself, p rounded once to its type.  In 8 bits m and r are kept (r, not
+// v: its range is half as many octaves) as e4m3 numbers times a scale for every 256 elements, the block's largest magnitude / 448.  Rounding to
+// nearest would freeze such an average, which moves by 0.05 % of itself a step on a grid of 6 to 12 %; so the rounding is random, up with the probability
+// of the distance to the neighbour below, with numbers that are a function of (seed, step, place): a step can be repeated bit for bit.  An r above zero is
+// never rounded to zero, or the next step would divide an m that is not by eps.  A block that holds an infinity or a NaN is non-finite from then on.
+//
+// What bounds it: HBM for tables (28 bytes an element with 32-bit states, 10 with bf16 and 8), the launch for small models.
+#include <algorithm>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include "dg_internal.h"
+
+namespace {
+
+constexpr int kThreads = 256, kEach = 8, kChunk = kThreads * kEach;      // a lane takes 8 neighbouring elements, a warp one block of 256
+constexpr int kBlock = 256;
+constexpr int kNormCtas = 148 * 4;
+constexpr float kLargest = 448.f, kSmallestNormal = 0.015625f, kSmallest = 0.001953125f;
+
+// Tensors of one launch.  Their table travels with the launch, so that a captured graph holds it and nothing has to be copied ahead: 40 entries
+// are 3.4 KB of arguments, 376 the 32 KB that a launch can have.
+template <int CAP> struct Table {
+    dg_adamw_tensor t[CAP];
+    int32_t first[CAP + 1];               // running count of chunks
+    int32_t count;
+    uint32_t wide[(CAP + 31) / 32];       // bit: every address on the boundary that whole loads want
+};
+constexpr int kFew = 40, kMany = 376;
+
+struct Factors {
+    double lr, beta1, beta2;
+    float b1, a1, b2, a2, eps, keep;      // a = 1 - b; keep = 1 - lr wd
+    uint32_t seed;
+};
+
+template <class T> __device__ __forceinline__ float to_float(T v);
+template <> __device__ __forceinline__ float to_float(float v) { return v; }
+template <> __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <> __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+template <class T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
+
+// Eight neighbouring elements, as whole 16-byte pieces (8 bytes for codes) or one by one; elements from n on are zero and not stored.
+template <class T> __device__ __forceinline__ void load8(const T* p, int n, bool wide, float* v)
+{
+    if (wide && n >= 8) {
+        if constexpr (sizeof(T) == 4) {
+            const float4 a = __ldcs(reinterpret_cast<const float4*>(p)), b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
+            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        } else {
+            const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p));
+            const T* e = reinterpret_cast<const T*>(&a);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = to_float(e[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < n ? to_float(p[i]) : 0.f;
+    }
+}
+template <class T> __device__ __forceinline__ void store8(T* p, int n, bool wide, const float* v)
+{
+    if (wide && n >= 8) {
+        if constexpr (sizeof(T) == 4) {
+            __stcs(reinterpret_cast<float4*>(p), make_float4(v[0], v[1], v[2], v[3]));
+            __stcs(reinterpret_cast<float4*>(p) + 1, make_float4(v[4], v[5], v[6], v[7]));
+        } else {
+            uint4 a;
+            T* e = reinterpret_cast<T*>(&a);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) e[i] = from_float<T>(v[i]);
+            __stcs(reinterpret_cast<uint4*>(p), a);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) p[i] = from_float<T>(v[i]);
+    }
+}
+__device__ __forceinline__ uint2 load_codes(const uint8_t* p, int n, bool wide)
+{
+    if (wide && n >= 8) return __ldcs(reinterpret_cast<const uint2*>(p));
+    uint2 c = make_uint2(0u, 0u);
+    for (int i = 0; i < 8 && i < n; ++i) (i < 4 ? c.x : c.y) |= (uint32_t)p[i] << (i % 4 * 8);
+    return c;
+}
+__device__ __forceinline__ void store_codes(uint8_t* p, int n, bool wide, uint2 c)
+{
+    if (wide && n >= 8) {
+        __stcs(reinterpret_cast<uint2*>(p), c);
+        return;
+    }
+    for (int i = 0; i < 8 && i < n; ++i) p[i] = (uint8_t)((i < 4 ? c.x : c.y) >> (i % 4 * 8));
+}
+__device__ __forceinline__ void decode(uint2 c, float scale, float* v)
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t w = i < 2 ? c.x : c.y;
+        const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> (i % 2 * 16)), __NV_E4M3)));
+        v[2 * i] = __fmul_rn(f.x, scale);
+        v[2 * i + 1] = __fmul_rn(f.y, scale);
+    }
+}
+
+// Random numbers: xor-shift and product, twice, for a pair of neighbours, 16 bits for each.  The odd factors are the leading bits of the golden
+// ratio's and of square roots' fractions.
+__device__ __forceinline__ uint32_t mix(uint32_t h)
+{
+    h = (h ^ h >> 16) * 0x6A09E667u;
+    h = (h ^ h >> 15) * 0xBB67AE85u;
+    return h ^ h >> 16;
+}
+__device__ __forceinline__ uint32_t key_of(uint32_t seed, int64_t step) { return mix(seed + (uint32_t)step * 0x3C6EF373u); }
+
+// A block's values, eight a lane, as codes and a scale.  q = |x| 448 / largest; below 2^-6, where e4m3 steps by 2^-9, 2^-6 more gives a number that steps
+// by as much in its third mantissa bit: the noise is added below that bit, which is then the last one kept.
+template <bool POSITIVE> __device__ __forceinline__ uint2 encode(const float* x, const uint32_t* noise, float* scale)
+{
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+    const float most = __uint_as_float(__reduce_max_sync(0xffffffffu, top));            // magnitudes are ordered as their bits, NaN above all
+    const bool none = most < 1e-30f;
+    const float factor = none ? 0.f : __fmul_rn(__frcp_rn(most), kLargest);
+    *scale = none ? 0.f : __fmul_rn(most, 1.f / kLargest);
+    uint32_t c[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float y[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const float v = x[2 * i + j], q = fminf(__fmul_rn(fabsf(v), factor), kLargest);
+            const float lift = q < kSmallestNormal ? kSmallestNormal : 0.f;
+            const uint32_t bits = (__float_as_uint(__fadd_rn(q, lift)) + ((j ? noise[i] >> 16 : noise[i] & 0xFFFFu) << 4)) & 0xFFF00000u;
+            y[j] = __fsub_rn(__uint_as_float(bits), lift);
+            if (POSITIVE) y[j] = q > 0.f ? fmaxf(y[j], kSmallest) : y[j];
+            else y[j] = v < 0.f ? -y[j] : y[j];
+        }
+        c[i] = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
+    }
+    return make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
+}
+
+// b^t by squaring: log2(t) dependent products.
+__device__ __forceinline__ void powers(double b1, double b2, int64_t t, double* p1, double* p2)
+{
+    double x = 1.0, y = 1.0;
+    for (; t > 0; t >>= 1, b1 *= b1, b2 *= b2)
+        if (t & 1) x *= b1, y *= b2;
+    *p1 = x, *p2 = y;
+}
+
+template <int CAP> __device__ __forceinline__ int find(const Table<CAP>& tab, int chunk)
+{
+    int lo = 0, hi = tab.count - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (tab.first[mid] <= chunk) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+template <class T, bool SMALL, int CAP>
+__global__ void __launch_bounds__(kThreads) k_adamw(const __grid_constant__ Table<CAP> tab, const Factors f, const float* __restrict__ clip, int* __restrict__ arrived)
+{
+    __shared__ float shared_factor[2];
+    __shared__ uint32_t shared_key;
+    __shared__ int last;
+    const int chunks = tab.first[tab.count];
+    int at = -1;
+    float rate = 0.f, correction = 0.f;
+    uint32_t key = 0;
+    const float coef = clip ? __ldg(clip) : 1.f;
+    for (int chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
+        int i = at;
+        if (at < 0) i = find(tab, chunk);
+        else
+            while (tab.first[i + 1] <= chunk) ++i;
+        const dg_adamw_tensor& t = tab.t[i];
+        const bool wide = tab.wide[i / 32] >> (i % 32) & 1;
+        const int64_t e0 = (int64_t)(chunk - tab.first[i]) * kChunk + threadIdx.x * kEach;
+        const int n = (int)max((int64_t)0, min((int64_t)kEach, t.n - e0));
+        float p[8], g[8], m[8], v[8], r[8];
+        uint2 cm, cr;
+        float sm = 0.f, sr = 0.f;
+        const int64_t block = e0 / kBlock;
+        load8(reinterpret_cast<const T*>(t.p) + e0, n, wide, p);
+        load8(reinterpret_cast<const T*>(t.g) + e0, n, wide, g);
+        if constexpr (SMALL) {
+            cm = load_codes(reinterpret_cast<const uint8_t*>(t.m) + e0, n, wide);
+            cr = load_codes(reinterpret_cast<const uint8_t*>(t.v) + e0, n, wide);
+            if (block * kBlock < t.n) sm = t.m_scale[block], sr = t.v_scale[block];
+        } else {
+            load8(reinterpret_cast<const float*>(t.m) + e0, n, wide, m);
+            load8(reinterpret_cast<const float*>(t.v) + e0, n, wide, v);
+        }
+        if (i != at) {                                            // the same for all threads
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                const int64_t step = *t.step + 1;
+                double p1, p2;
+                powers(f.beta1, f.beta2, step, &p1, &p2);
+                shared_factor[0] = (float)(f.lr / (1.0 - p1));
+                shared_factor[1] = (float)(1.0 / sqrt(1.0 - p2));
+                shared_key = key_of(f.seed, step);
+            }
+            __syncthreads();
+            rate = shared_factor[0], correction = shared_factor[1], key = shared_key;
+            at = i;
+        }
+        if constexpr (SMALL) {
+            decode(cm, sm, m);
+            decode(cr, sr, r);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = __fmul_rn(r[j], r[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float h = clip ? __fmul_rn(g[j], coef) : g[j];
+            m[j] = __fadd_rn(__fmul_rn(m[j], f.b1), __fmul_rn(h, f.a1));
+            v[j] = __fadd_rn(__fmul_rn(v[j], f.b2), __fmul_rn(__fmul_rn(h, h), f.a2));
+            r[j] = __fsqrt_rn(v[j]);
+            const float u = __fdiv_rn(m[j], __fadd_rn(__fmul_rn(r[j], correction), f.eps));
+            p[j] = __fsub_rn(__fmul_rn(p[j], f.keep), __fmul_rn(u, rate));
+        }
+        store8(reinterpret_cast<T*>(t.p) + e0, n, wide, p);
+        if constexpr (SMALL) {
+            uint32_t noise[4];
+            const uint32_t place = (uint32_t)((t.place + e0) >> 1);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) noise[j] = mix((place + j) * 0x9E3779B1u + key);
+            if (n < kEach)                                        // what lies beyond the tensor is no part of its block
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (j >= n) m[j] = r[j] = 0.f;
+            float scale_m, scale_r;
+            cm = encode<false>(m, noise, &scale_m);
+            cr = encode<true>(r, noise, &scale_r);
+            store_codes(reinterpret_cast<uint8_t*>(t.m) + e0, n, wide, cm);
+            store_codes(reinterpret_cast<uint8_t*>(t.v) + e0, n, wide, cr);
+            if (threadIdx.x % 32 == 0 && block * kBlock < t.n) t.m_scale[block] = scale_m, t.v_scale[block] = scale_r;
+        } else {
+            store8(reinterpret_cast<float*>(t.m) + e0, n, wide, m);
+            store8(reinterpret_cast<float*>(t.v) + e0, n, wide, v);
+        }
+    }
+    // The steps are counted by the CTA that comes last: all others have read them.
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        __threadfence();
+        last = atomicAdd(arrived, 1) == (int)gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!last) return;
+    for (int i = threadIdx.x; i < tab.count; i += kThreads) ++*tab.t[i].step;
+    if (threadIdx.x == 0) *arrived = 0;
+}
+
+// Sum of squares in 64 bits, every CTA's in its own place; the CTA that comes last of the last launch adds them in order.
+template <class T, int CAP>
+__global__ void __launch_bounds__(kThreads) k_grad_norm(const __grid_constant__ Table<CAP> tab, double* __restrict__ partial, int total, double max_norm,
+                                                        float* __restrict__ result, int* __restrict__ arrived)
+{
+    __shared__ double warp_sum[kThreads / 32];
+    __shared__ int last;
+    auto sum_of_cta = [&](double s) {
+        for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+        __syncthreads();
+        if (threadIdx.x % 32 == 0) warp_sum[threadIdx.x / 32] = s;
+        __syncthreads();
+        s = 0.0;
+        for (int w = 0; w < kThreads / 32; ++w) s += warp_sum[w];
+        return s;
+    };
+    const int chunks = tab.first[tab.count];
+    double sum = 0.0;
+    int i = -1;
+    for (int chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
+        if (i < 0) i = find(tab, chunk);
+        else
+            while (tab.first[i + 1] <= chunk) ++i;
+        const dg_adamw_tensor& t = tab.t[i];
+        const int64_t e0 = (int64_t)(chunk - tab.first[i]) * kChunk + threadIdx.x * kEach;
+        const int n = (int)max((int64_t)0, min((int64_t)kEach, t.n - e0));
+        float g[8];
+        load8(reinterpret_cast<const T*>(t.g) + e0, n, tab.wide[i / 32] >> (i % 32) & 1, g);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum += (double)g[j] * (double)g[j];
+    }
+    sum = sum_of_cta(sum);
+    if (threadIdx.x == 0) partial[blockIdx.x] = sum;
+    if (!result) return;
+    if (threadIdx.x == 0) {
+        __threadfence();
+        last = atomicAdd(arrived, 1) == (int)gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    const double* all = partial + gridDim.x - total;              // this launch's places are the last ones
+    double s = 0.0;
+    for (int j = threadIdx.x; j < total; j += kThreads) s += __ldcg(all + j);
+    s = sum_of_cta(s);
+    if (threadIdx.x == 0) {
+        const double norm = sqrt(s), coef = max_norm / (norm + 1e-6);
+        result[0] = (float)norm;
+        result[1] = (float)(coef > 1.0 ? 1.0 : coef);             // a NaN stays
+        *arrived = 0;
+    }
+}
+
+bool aligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+int64_t chunks_of(int64_t n) { return (n + kChunk - 1) / kChunk; }
+
+// Fills a table with as many of the tensors [at, count) of `type` as it holds; returns where the next one starts.
+template <int CAP> int fill(Table<CAP>* tab, const dg_adamw_tensor* t, int at, int count, int32_t type, bool norm, int32_t bits)
+{
+    int64_t chunks = 0;
+    tab->count = 0;
+    for (uint32_t& w : tab->wide) w = 0;
+    for (; at < count && tab->count < CAP; ++at) {
+        if (t[at].type != type || t[at].n == 0) continue;
+        const int64_t more = chunks_of(t[at].n);
+        if (chunks + more >= (int64_t)1 << 30) break;             // chunk numbers, with a stride added, stay within 31 bits
+        const int k = tab->count++;
+        tab->t[k] = t[at];
+        tab->first[k] = (int32_t)chunks;
+        chunks += more;
+        bool wide = aligned(t[at].g, 16);
+        if (!norm) wide = wide && aligned(t[at].p, 16) && aligned(t[at].m, bits == 8 ? 8 : 16) && aligned(t[at].v, bits == 8 ? 8 : 16);
+        if (wide) tab->wide[k / 32] |= 1u << (k % 32);
+    }
+    tab->first[tab->count] = (int32_t)chunks;
+    return at;
+}
+
+int check(const dg_adamw_tensor* t, int32_t count, int32_t bits, bool norm)
+{
+    if (count < 0 || (bits != 8 && bits != 32)) return DG_ERR_DIMS;
+    if (count > 0 && !t) return DG_ERR_NULL;
+    for (int32_t i = 0; i < count; ++i) {
+        if (t[i].n < 0 || t[i].n >= (int64_t)1 << 40 || t[i].type < 0 || t[i].type > 2) return DG_ERR_DIMS;
+        if (t[i].n == 0) continue;
+        const size_t item = t[i].type == DG_FLOAT32 ? 4 : 2, state = bits == 8 ? 1 : 4;
+        if (!t[i].g) return DG_ERR_NULL;
+        if (!aligned(t[i].g, item)) return DG_ERR_DIMS;
+        if (norm) continue;
+        if (!t[i].p || !t[i].m || !t[i].v || !t[i].step || (bits == 8 && (!t[i].m_scale || !t[i].v_scale))) return DG_ERR_NULL;
+        if (!aligned(t[i].p, item) || !aligned(t[i].m, state) || !aligned(t[i].v, state) || !aligned(t[i].step, 8) || !aligned(t[i].m_scale, 4) ||
+            !aligned(t[i].v_scale, 4))
+            return DG_ERR_DIMS;
+    }
+    return DG_OK;
+}
+
+// `use(table, type constant, first?)` for as many tables as the tensors need; the form by how many there are.
+template <class Use> int each_table(const dg_adamw_tensor* t, int32_t count, bool norm, int32_t bits, Use use)
+{
+    auto run = [&](auto* tab, int32_t type, auto value) {
+        for (int at = 0; at < count;) {
+            at = fill(tab, t, at, count, type, norm, bits);
+            if (tab->count == 0) continue;
+            const int rc = use(*tab, value);
+            if (rc) return rc;
+        }
+        return (int)DG_OK;
+    };
+    Table<kFew> few;
+    Table<kMany> many;
+    for (int32_t type = 0; type < 3; ++type) {
+        int have = 0;
+        for (int32_t i = 0; i < count; ++i) have += t[i].type == type && t[i].n > 0;
+        if (have == 0) continue;
+        auto with = [&](auto value) { return have <= kFew ? run(&few, type, value) : run(&many, type, value); };
+        const int rc = type == DG_FLOAT32 ? with(float{}) : type == DG_BFLOAT16 ? with(__nv_bfloat16{}) : with(__half{});
+        if (rc) return rc;
+    }
+    return DG_OK;
+}
+
+}  // namespace
+
+extern "C" int64_t dg_adamw_workspace(const dg_adamw_tensor* host_tensors, int32_t count)
+{
+    int64_t tables = 0;
+    if (count < 0 || (count > 0 && !host_tensors)) return DG_ERR_NULL;
+    for (int32_t type = 0; type < 3; ++type) {
+        int64_t have = 0, chunks = 0;
+        for (int32_t i = 0; i < count; ++i)
+            if (host_tensors[i].type == type) ++have, chunks += chunks_of(std::max<int64_t>(host_tensors[i].n, 0));
+        tables += have / kFew + 1 + chunks / ((int64_t)1 << 29);
+    }
+    return 16 + 8 * tables * kNormCtas;
+}
+
+extern "C" int dg_grad_norm(const dg_adamw_tensor* host_tensors, int32_t count, double max_norm, float* result, void* workspace, int64_t workspace_bytes,
+                            void* stream)
+{
+    int rc = check(host_tensors, count, 32, true);
+    if (rc) return rc;
+    if (!result || !workspace) return DG_ERR_NULL;
+    if (!(max_norm > 0.0) || !aligned(workspace, 16)) return DG_ERR_DIMS;
+    if (workspace_bytes < dg_adamw_workspace(host_tensors, count)) return DG_ERR_SCRATCH;
+    // every launch's CTAs first, then the last launch once more with the result: so the tables are counted ahead
+    int launches = 0;
+    rc = each_table(host_tensors, count, true, 32, [&](auto&, auto) { return ++launches, (int)DG_OK; });
+    if (rc) return rc;
+    int* arrived = reinterpret_cast<int*>(workspace);
+    double* partial = reinterpret_cast<double*>(reinterpret_cast<char*>(workspace) + 16);
+    if (launches == 0) {
+        const float none[2] = {0.f, 1.f};
+        return (int)cudaMemcpyAsync(result, none, sizeof none, cudaMemcpyHostToDevice, (cudaStream_t)stream);
+    }
+    int total = 0, done = 0;
+    return each_table(host_tensors, count, true, 32, [&](auto& tab, auto value) {
+        const int grid = std::min(kNormCtas, (int)tab.first[tab.count]);
+        const bool end = ++done == launches;
+        k_grad_norm<decltype(value)><<<grid, kThreads, 0, (cudaStream_t)stream>>>(tab, partial + total, total + grid, max_norm, end ? result : nullptr, arrived);
+        total += grid;
+        return (int)cudaGetLastError();
+    });
+}
+
+extern "C" int dg_adamw_step(const dg_adamw_tensor* host_tensors, int32_t count, const dg_adamw_options* options, const float* clip, void* workspace,
+                             int64_t workspace_bytes, void* stream)
+{
+    if (!options || !workspace) return DG_ERR_NULL;
+    const int rc = check(host_tensors, count, options->bits, false);
+    if (rc) return rc;
+    if (!(options->beta1 >= 0.0 && options->beta1 < 1.0 && options->beta2 >= 0.0 && options->beta2 < 1.0 && options->eps >= 0.0 && options->lr >= 0.0 &&
+          options->weight_decay >= 0.0) || !aligned(workspace, 16))
+        return DG_ERR_DIMS;
+    if (workspace_bytes < 16) return DG_ERR_SCRATCH;
+    Factors f{};
+    f.lr = options->lr, f.beta1 = options->beta1, f.beta2 = options->beta2;
+    f.b1 = (float)options->beta1, f.a1 = (float)(1.0 - options->beta1), f.b2 = (float)options->beta2, f.a2 = (float)(1.0 - options->beta2);
+    f.eps = (float)options->eps, f.keep = (float)(1.0 - options->lr * options->weight_decay), f.seed = options->seed;
+    int* arrived = reinterpret_cast<int*>(workspace) + 1;
+    const bool small = options->bits == 8;
+    return each_table(host_tensors, count, false, options->bits, [&](auto& tab, auto value) {
+        using T = decltype(value);
+        const int grid = std::min(148 * 8, (int)tab.first[tab.count]);
+        if (small) k_adamw<T, true><<<grid, kThreads, 0, (cudaStream_t)stream>>>(tab, f, clip, arrived);
+        else k_adamw<T, false><<<grid, kThreads, 0, (cudaStream_t)stream>>>(tab, f, clip, arrived);
+        return (int)cudaGetLastError();
+    });
+}

@@ -11,6 +11,7 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <atomic>
+#include <functional>
 #include <mutex>
 #include <unordered_map>
 #include "dist_gnn_b200.h"
@@ -391,11 +392,144 @@ Tensor row_cross_entropy(const Tensor& x, const Tensor& targets, int64_t count)
     return loss;
 }
 
+// ---- AdamW over all tensors of an optimiser ----------------------------------------------------------------------------------
+// What spmm_cpp.AdamW steps: its parameters and their state, group after group.  A step takes the gradients' addresses anew; whether the optimiser's state
+// is still the one this was made from is asked by identity (same_state), without hashing a parameter.
+struct AdamwEntry {
+    Tensor p, m, v, m_scale, v_scale, step;
+    int64_t place;
+    int32_t group;
+};
+
+int32_t type_of(const Tensor& t)
+{
+    switch (t.scalar_type()) {
+        case at::kFloat: return DG_FLOAT32;
+        case at::kBFloat16: return DG_BFLOAT16;
+        case at::kHalf: return DG_FLOAT16;
+        default: return -1;
+    }
+}
+
+struct AdamwTable {
+    std::vector<AdamwEntry> entries;
+    std::vector<py::object> seen;         // every parameter of the state, its dict and that dict's values, in their order
+    Tensor workspace, norm;
+    int32_t bits;
+
+    static void walk(PyObject* state, const std::function<bool(PyObject*)>& use)
+    {
+        PyObject *key, *value, *name, *item;
+        Py_ssize_t i = 0;
+        while (PyDict_Next(state, &i, &key, &value)) {
+            if (!use(key) || !use(value)) return;
+            if (!PyDict_Check(value)) continue;
+            Py_ssize_t j = 0;
+            while (PyDict_Next(value, &j, &name, &item))
+                if (!use(item)) return;
+        }
+    }
+    AdamwTable(const py::dict& state, const std::vector<std::tuple<Tensor, Tensor, Tensor, std::optional<Tensor>, std::optional<Tensor>, Tensor, int64_t, int32_t>>& rows,
+               int32_t bits_) : bits(bits_)
+    {
+        walk(state.ptr(), [&](PyObject* o) { return seen.push_back(py::reinterpret_borrow<py::object>(o)), true; });
+        const auto kept = bits == 8 ? at::kFloat8_e4m3fn : at::kFloat;
+        for (const auto& [p, m, v, ms, vs, step, place, group] : rows) {
+            const at::Device device = std::get<0>(rows[0]).device();
+            const int64_t n = p.numel(), blocks = (n + 255) / 256;
+            auto fits = [&](const Tensor& t, at::ScalarType type, int64_t count) {
+                return t.device() == device && t.scalar_type() == type && t.is_contiguous() && t.numel() == count;
+            };
+            if (!p.is_cuda()) throw std::runtime_error("parameters must be CUDA tensors: this library has no CPU path");
+            if (p.device() != device) throw std::runtime_error("parameters must be on one device");
+            if (type_of(p) < 0 || !p.is_contiguous()) throw std::runtime_error("parameters must be contiguous fp32, bf16 or fp16 tensors");
+            if (!fits(m, kept, n) || !fits(v, kept, n) || !fits(step, at::kLong, 1))
+                throw std::runtime_error("optimiser state does not fit its parameter: expected contiguous " + std::string(bits == 8 ? "float8_e4m3fn" : "float32") +
+                                         " tensors of its size and an int64 step, on its device");
+            if (bits == 8 && (!ms || !vs || !fits(*ms, at::kFloat, blocks) || !fits(*vs, at::kFloat, blocks)))
+                throw std::runtime_error("optimiser state does not fit its parameter: expected one float32 scale for every 256 elements");
+            entries.push_back({p, m, v, ms.value_or(Tensor()), vs.value_or(Tensor()), step, place, group});
+        }
+        if (entries.empty()) return;
+        c10::cuda::CUDAGuard guard(entries[0].p.device());
+        std::vector<dg_adamw_tensor> all;
+        for (const AdamwEntry& e : entries) {
+            dg_adamw_tensor t{};
+            t.n = e.p.numel(), t.type = type_of(e.p);
+            all.push_back(t);
+        }
+        const int64_t bytes = dg_adamw_workspace(all.data(), (int32_t)all.size());
+        if (bytes < 0) check((int)bytes);
+        workspace = at::zeros({bytes}, entries[0].p.options().dtype(at::kByte).requires_grad(false));
+        norm = at::zeros({2}, entries[0].p.options().dtype(at::kFloat).requires_grad(false));
+    }
+    bool same_state(const py::dict& state) const
+    {
+        size_t i = 0;
+        bool same = true;
+        walk(state.ptr(), [&](PyObject* o) { return same = i < seen.size() && seen[i++].ptr() == o; });
+        return same && i == seen.size();
+    }
+    // groups: (lr, beta1, beta2, eps, weight decay) each
+    void step(const std::vector<std::tuple<double, double, double, double, double>>& groups, double max_norm, uint32_t seed)
+    {
+        if (entries.empty()) return;
+        const at::Device device = entries[0].p.device();
+        c10::cuda::CUDAGuard guard(device);
+        std::vector<dg_adamw_tensor> all;
+        std::vector<Tensor> copies;                       // of gradients whose elements do not lie side by side
+        std::vector<size_t> end(groups.size(), 0);
+        all.reserve(entries.size());
+        for (const AdamwEntry& e : entries) {
+            const Tensor& grad = e.p.grad();
+            if (grad.defined() && e.p.numel() > 0) {
+                if (grad.layout() != at::kStrided) throw std::runtime_error("AdamW takes dense gradients only");
+                if (e.p.device() != device || e.p.numel() != e.m.numel() || !e.p.is_contiguous() || grad.device() != device ||
+                    grad.scalar_type() != e.p.scalar_type() || grad.sizes() != e.p.sizes())
+                    throw std::runtime_error("a parameter or its gradient has changed its device, type, size or layout");
+                const Tensor* g = &grad;
+                if (!grad.is_contiguous()) {
+                    copies.push_back(grad.contiguous());
+                    g = &copies.back();
+                }
+                const bool small = bits == 8;
+                all.push_back({e.p.data_ptr(), g->data_ptr(), e.m.data_ptr(), e.v.data_ptr(), small ? e.m_scale.data_ptr<float>() : nullptr,
+                               small ? e.v_scale.data_ptr<float>() : nullptr, e.step.data_ptr<int64_t>(), e.p.numel(), e.place, type_of(e.p), 0});
+            }
+            end[e.group] = all.size();
+        }
+        if (all.empty()) return;
+        void* stream = stream_of(entries[0].p);
+        const bool clipped = max_norm > 0;
+        if (clipped) check(dg_grad_norm(all.data(), (int32_t)all.size(), max_norm, norm.data_ptr<float>(), workspace.data_ptr(), workspace.numel(), stream));
+        size_t first = 0;
+        for (size_t k = 0; k < groups.size(); ++k) {
+            const size_t last = std::max(end[k], first);
+            const auto& [lr, beta1, beta2, eps, decay] = groups[k];
+            const dg_adamw_options options{lr, beta1, beta2, eps, decay, seed, bits};
+            if (last > first)
+                check(dg_adamw_step(all.data() + first, (int32_t)(last - first), &options, clipped ? norm.data_ptr<float>() + 1 : nullptr, workspace.data_ptr(),
+                                    workspace.numel(), stream));
+            first = last;
+        }
+        for (const AdamwEntry& e : entries) {             // copies that are kept of a weight go by its version
+            if (!e.p.grad().defined()) continue;
+            for (const Tensor* t : {&e.p, &e.m, &e.v, &e.m_scale, &e.v_scale, &e.step})
+                if (t->defined()) t->unsafeGetTensorImpl()->bump_version();
+        }
+    }
+};
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
 {
     py::class_<PlanRef, std::shared_ptr<PlanRef>>(m, "PlanRef").def(py::init<int64_t, Tensor, Tensor>());
+    py::class_<AdamwTable>(m, "AdamwTable")
+        .def(py::init<const py::dict&, const std::vector<std::tuple<Tensor, Tensor, Tensor, std::optional<Tensor>, std::optional<Tensor>, Tensor, int64_t, int32_t>>&, int32_t>())
+        .def("same_state", &AdamwTable::same_state)
+        .def("step", &AdamwTable::step)
+        .def_readonly("norm", &AdamwTable::norm);
     m.def("spmm", &spmm);
     m.def("gcn", &gcn);
     m.def("readable_padded", &readable_padded);

@@ -60,11 +60,20 @@ def _class_targets(g, outputs, loss_func, rows, labels):
     return targets, count
 
 
-def train(g, env, total_epoch, hidden_dim=256, num_layers=3, weights=None, log_every=10, **model_options):
+def make_optimizer(name, parameters):
+    """'adam' is the reference's (dist_train.py:31); 'adamw' and 'adamw8' are spmm_cpp.AdamW with states in 32 and in 8 bits, at the same rate."""
+    if name == 'adam':
+        return torch.optim.Adam(parameters, lr=0.01)
+    if name in ('adamw', 'adamw8'):
+        return spmm_cpp.AdamW(parameters, lr=0.01, state_bits=8 if name == 'adamw8' else 32)
+    raise ValueError(f"optimizer must be 'adam', 'adamw' or 'adamw8', got {name!r}")
+
+
+def train(g, env, total_epoch, hidden_dim=256, num_layers=3, weights=None, log_every=10, optimizer='adam', **model_options):
     """The reference's epoch loop (dist_train.py:26-55).  model_options go to GCN (cache_input_product,
     input_gradient_shortcut); the defaults recompute everything every epoch, as the reference does."""
     model = GCN(g, env, hidden_dim=hidden_dim, num_layers=num_layers, weights=weights, **model_options)
-    optimizer = torch.optim.Adam(model.parameters(), lr=0.01)
+    optimizer = make_optimizer(optimizer, model.parameters())
     loss_func = nn.CrossEntropyLoss() if g.labels.dim() == 1 else nn.BCEWithLogitsLoss(reduction='mean')
     losses = []
     for epoch in range(total_epoch):
@@ -97,5 +106,6 @@ def main(env, args):
         parts = env.world_size // env.rep
         g = Parted_COO_Graph(args.dataset, rank=env.rank // env.rep, num_parts=parts, device=env.device)
         env.logger.log('graph loaded', g)
-        train(g, env, total_epoch=args.epoch, hidden_dim=getattr(args, 'hidden', 256), num_layers=getattr(args, 'layers', 3))
+        train(g, env, total_epoch=args.epoch, hidden_dim=getattr(args, 'hidden', 256), num_layers=getattr(args, 'layers', 3),
+              optimizer=getattr(args, 'optimizer', 'adam'))
     env.logger.log(env.timer.summary_all(), rank=0)

@@ -1,5 +1,5 @@
 """Launcher with the flags of light_dist_gnn/main.py:24-33 (--nprocs --epoch --backend --dataset) plus --layers,
---hidden and --rep (1.5D replication factor).  One process per GPU, spawned on this host."""
+--hidden, --rep (1.5D replication factor) and --optimizer.  One process per GPU, spawned on this host."""
 import argparse
 import os
 
@@ -30,5 +30,6 @@ if __name__ == '__main__':
     parser.add_argument('--layers', type=int, default=3)
     parser.add_argument('--hidden', type=int, default=256)
     parser.add_argument('--rep', type=int, default=1)
+    parser.add_argument('--optimizer', choices=('adam', 'adamw', 'adamw8'), default='adam')
     args = parser.parse_args()
     torch.multiprocessing.spawn(process_wrapper, (args, dist_train.main), args.nprocs)

@@ -842,3 +842,106 @@ def dense_wait_selftest():
     out = ctypes.c_int(-1)
     check(lib().dg_dense_wait_selftest(ctypes.byref(out), _stream()))
     return out.value == 1
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW with decoupled weight decay over all parameters in one launch (dg_adamw_step), for fp32, bf16 and fp16 parameters.
+
+    state_bits  32: running means exp_avg and exp_avg_sq in fp32.  8: exp_avg and root, the square root of the second mean, as float8_e4m3fn
+                times exp_avg_scale and root_scale, one fp32 number for every 256 elements of a parameter: 2.03 bytes an element instead of 8.
+                They are rounded at random (a mean that moves by 0.05 % a step would stand still on a grid of 6 %), with numbers that are a
+                function of `seed`, the step and the element's place, so that a run can be repeated; ranks that hold copies of a weight
+                keep equal copies if they have the same seed.
+    max_norm    gradients are scaled by min(1, max_norm / (norm + 1e-6)), norm being the 2-norm of all of them, inside the step (the .grad
+                tensors stay as they are); grad_norm is that norm, a 0-dim CUDA tensor.  None: no clipping.
+
+    Parameters are contiguous CUDA tensors of one device; those without a gradient are left as they are.  An infinity or a NaN
+    in a gradient makes its element's parameter and means non-finite, with 8 bits the means of its block of 256, and with max_norm all of them.
+    Steps are counted on the device (state 'step', int64), so a step can be captured into a CUDA graph and replayed; the hyperparameters
+    are those of the capture.  Steps of one optimiser run one after the other: a graph of it and an eager step, or two graphs, not at once."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, max_norm=None, seed=0):
+        if state_bits not in (8, 32):
+            raise ValueError(f'state_bits must be 8 or 32, got {state_bits}')
+        if max_norm is not None and not 0.0 < max_norm < float('inf'):
+            raise ValueError(f'max_norm must be None or a positive number, got {max_norm}')
+        self._check_group(dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+        self.state_bits, self.max_norm, self.seed, self._table = state_bits, max_norm, int(seed) & 0xFFFFFFFF, None
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+
+    @staticmethod
+    def _check_group(group):
+        for name, value in (('lr', group['lr']), ('eps', group['eps']), ('weight_decay', group['weight_decay'])):
+            if isinstance(value, torch.Tensor) or not 0.0 <= value < float('inf'):
+                raise ValueError(f'{name} must be a non-negative number, got {value}')
+        if len(group['betas']) != 2 or not all(0.0 <= b < 1.0 for b in group['betas']):
+            raise ValueError(f'betas must be two numbers of [0, 1), got {group["betas"]}')
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        self._check_group(self.param_groups[-1])
+        self._table = None
+
+    def __getstate__(self):
+        return dict(super().__getstate__(), state_bits=self.state_bits, max_norm=self.max_norm, seed=self.seed)
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._table = None
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        # the base class casts a parameter's state to the parameter's type; these means have types of their own
+        saved = [i for group in state_dict['param_groups'] for i in group['params']]
+        own = [p for group in self.param_groups for p in group['params']]
+        for i, p in zip(saved, own):
+            if i in state_dict['state']:
+                self.state[p] = {name: torch.as_tensor(value, device=p.device).clone() for name, value in state_dict['state'][i].items()}
+        self._table = None
+
+    def _new_state(self, p):
+        options = dict(device=p.device)
+        step = torch.zeros((), dtype=torch.int64, **options)
+        if self.state_bits == 32:
+            return dict(step=step, exp_avg=torch.zeros(p.shape, dtype=torch.float32, **options), exp_avg_sq=torch.zeros(p.shape, dtype=torch.float32, **options))
+        blocks = (p.numel() + 255) // 256
+        return dict(step=step, exp_avg=torch.zeros(p.shape, dtype=torch.float8_e4m3fn, **options), exp_avg_scale=torch.zeros(blocks, **options, dtype=torch.float32),
+                    root=torch.zeros(p.shape, dtype=torch.float8_e4m3fn, **options), root_scale=torch.zeros(blocks, **options, dtype=torch.float32))
+
+    def _make_table(self):
+        rows, place = [], 0
+        names = ('exp_avg', 'exp_avg_sq', None, None) if self.state_bits == 32 else ('exp_avg', 'root', 'exp_avg_scale', 'root_scale')
+        for k, group in enumerate(self.param_groups):
+            for p in group['params']:
+                if not p.is_cuda:
+                    raise RuntimeError('parameters must be CUDA tensors: this library has no CPU path')
+                if not self.state[p]:
+                    self.state[p].update(self._new_state(p))
+                s = self.state[p]
+                try:
+                    rows.append((p, *(None if name is None else s[name] for name in names), s['step'], place, k))
+                except KeyError as missing:
+                    raise RuntimeError(f'optimiser state of {self.state_bits} bits has no {missing}') from None
+                place += p.numel() + (-p.numel()) % 256
+        return binding().AdamwTable(self.state, rows, self.state_bits)
+
+    @property
+    def grad_norm(self):
+        """Norm of all gradients in the last step, before they were scaled (None without max_norm, or before the first step)."""
+        return self._table.norm[0] if self.max_norm is not None and self._table is not None else None
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        table = self._table
+        if table is None or not table.same_state(self.state):
+            table = self._table = self._make_table()
+        groups = []
+        for group in self.param_groups:
+            self._check_group(group)
+            groups.append((group['lr'], *group['betas'], group['eps'], group['weight_decay']))
+        table.step(groups, self.max_norm or 0.0, self.seed)
+        return loss

@@ -387,6 +387,46 @@ int dg_rows_cross_entropy(const float* x, int64_t ld, int64_t n, int32_t C, cons
 int dg_rows_cross_entropy_grad(const float* x, int64_t ld, int64_t n, int32_t C, const int32_t* target, int64_t count,
                                const float* lse, const float* upstream, float* grad, int64_t ldg, void* stream);
 
+/* ---- AdamW over many tensors at once (the reference trains with torch.optim.Adam, light_dist_gnn/dist_train.py:31) ---------------
+ * One step of p <- p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps) with the running means m of the gradients
+ * and v of their squares, for all tensors of a model in one launch (a launch for every type, and for every 376 tensors).  Arithmetic in fp32; p
+ * and g are of the tensor's type, p is rounded once.
+ *   bits == 32   m and v: fp32, n numbers each
+ *   bits == 8    m and the root of v (in the place of v): e4m3, n codes each, times m_scale and v_scale, one fp32 number for every 256 elements (the
+ *                last block may be shorter): the block's largest magnitude / 448.  Rounded at random, up with the probability of the distance to
+ *                the neighbour below; the random numbers are a function of seed, step and place + element, so a step repeats bit for bit.  A root
+ *                above zero never becomes zero.
+ *   step         steps taken so far, on the device; counted up by the call.  One for every tensor.
+ *   place        number of the tensor's first element among the optimiser's (8 bits: a multiple of 256, no two tensors' ranges overlapping)
+ * clip: NULL, or the second number that dg_grad_norm left (a factor for all gradients), on the device.
+ * dg_grad_norm: result[0] = the 2-norm of all gradients (sums in 64 bits, in a fixed order), result[1] = min(1, max_norm / (norm + 1e-6)); only g, n
+ * and type are read.
+ * workspace: 16-byte aligned, dg_adamw_workspace bytes, zero before its first use; steps that use one workspace run one after the other. */
+#define DG_FLOAT32 0
+#define DG_BFLOAT16 1
+#define DG_FLOAT16 2
+typedef struct dg_adamw_tensor {
+    void* p;
+    const void* g;
+    void* m;
+    void* v;
+    float* m_scale;
+    float* v_scale;
+    int64_t* step;
+    int64_t n;
+    int64_t place;
+    int32_t type, pad;
+} dg_adamw_tensor;
+typedef struct dg_adamw_options {
+    double lr, beta1, beta2, eps, weight_decay;
+    uint32_t seed;
+    int32_t bits;
+} dg_adamw_options;
+int64_t dg_adamw_workspace(const dg_adamw_tensor* host_tensors, int32_t count);
+int dg_grad_norm(const dg_adamw_tensor* host_tensors, int32_t count, double max_norm, float* result, void* workspace, int64_t workspace_bytes, void* stream);
+int dg_adamw_step(const dg_adamw_tensor* host_tensors, int32_t count, const dg_adamw_options* options, const float* clip, void* workspace,
+                  int64_t workspace_bytes, void* stream);
+
 /* Time marks: CUDA events from a pool, named by small ids, for timers around regions that are too short for anything
  * dearer.  dg_mark_record records one on `stream` (a stream of the current device) and returns its id, or a negative
  * DG_ERR_*; dg_mark_elapsed gives the milliseconds between two recorded marks that have both been reached (cudaErrorNotReady
