@@ -18,13 +18,11 @@
 // epilogue warps (wider results; by_pairs).  k_dense_tn (further down): the weight gradient X^T * G,
 // both operands MN-major, split-K over the CTAs with periodic accumulator flushes.
 // Every mbarrier wait is bounded; a role that gives up sets the status word and the CTA still frees its TMEM.
-#include <cuda.h>
 #include <algorithm>
-#include <atomic>
-#include <cstdint>
 #include <cstring>
+#include "dg_act.h"
 #include "dg_internal.h"
-#include "dg_umma.h"
+#include "dg_tma.h"
 
 namespace {
 
@@ -44,26 +42,47 @@ struct DenseArgs {
     const float* mask;              // optional [M x N]: the result is zeroed where mask <= 0 (ReLU backward), else nullptr
     int64_t ldm;
     int* status;
+    // the linear layer's epilogue; its residual takes the mask's place
+    const float* bias;
+    float* z;                       // x w + b, or nullptr
+    uint32_t* bits;                 // a bit an element where that is above zero, or nullptr
+    int64_t ldz, ldbits;
+    int32_t act;
 };
+constexpr int kPlain = 0, kMasked = 1, kLinear = 2;
 
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar)
+// A lane's 32 columns of its row: the bias is added, and where asked the signs are kept.
+__device__ __forceinline__ void add_bias(const DenseArgs& a, uint32_t* r, int c0, int64_t row)
 {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-                 ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1) : "memory");
+    if (a.bias) {
+        if (c0 + 32 <= a.N && (reinterpret_cast<uintptr_t>(a.bias) & 15) == 0) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float4 b = __ldg(reinterpret_cast<const float4*>(a.bias + c0) + j);
+                r[4 * j] = __float_as_uint(__uint_as_float(r[4 * j]) + b.x);
+                r[4 * j + 1] = __float_as_uint(__uint_as_float(r[4 * j + 1]) + b.y);
+                r[4 * j + 2] = __float_as_uint(__uint_as_float(r[4 * j + 2]) + b.z);
+                r[4 * j + 3] = __float_as_uint(__uint_as_float(r[4 * j + 3]) + b.w);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+                if (c0 + j < a.N) r[j] = __float_as_uint(__uint_as_float(r[j]) + __ldg(a.bias + c0 + j));
+        }
+    }
+    if (a.bits && row < a.M) {
+        uint32_t word = 0;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) word |= (__uint_as_float(r[j]) <= 0.f ? 0u : 1u) << j;
+        a.bits[row * a.ldbits + c0 / 32] = word;
+    }
 }
-// Shared-memory matrix descriptor of a K-major tile stored as 128-byte rows with the 128B swizzle: 8-row groups are
-// 1024 bytes apart (stride byte offset), the leading byte offset is unused for this layout, descriptor version 1.
-__device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t smem_addr)
+__device__ __forceinline__ float activate(int act, float z)
 {
-    uint64_t d = 0;
-    d |= (uint64_t)((smem_addr & 0x3FFFF) >> 4);            // start address, 16-byte units
-    d |= (uint64_t)1 << 16;                                   // leading byte offset (ignored with swizzle), 16-byte units
-    d |= (uint64_t)(1024 >> 4) << 32;                         // stride byte offset between 8-row groups
-    d |= (uint64_t)1 << 46;                                   // descriptor version for sm_100
-    d |= (uint64_t)2 << 61;                                   // layout type: SWIZZLE_128B
-    return d;
+    return act == DG_ACT_RELU ? act_value<DG_ACT_RELU>(z) : act == DG_ACT_GELU ? act_value<DG_ACT_GELU>(z) : act == DG_ACT_SILU ? act_value<DG_ACT_SILU>(z) : z;
 }
-// The same for rows of 64 bytes with the 64B swizzle: 8-row groups are 512 bytes apart.
+
+// umma_desc_sw128 for rows of 64 bytes with the 64B swizzle: 8-row groups are 512 bytes apart.
 __device__ __forceinline__ uint64_t umma_desc_sw64(uint32_t smem_addr)
 {
     return (uint64_t)((smem_addr & 0x3FFFF) >> 4) | (uint64_t)1 << 16 | (uint64_t)(512 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)4 << 61;
@@ -96,10 +115,11 @@ namespace {
 // registers touch 32 cache lines an instruction (and so do the mask's loads); the piece goes through `stage` in shared memory
 // (32 rows of 36 floats, conflict-free both ways) and leaves as whole 128-byte row pieces, four rows an instruction.
 constexpr int kStagePitch = 36, kStageBytes = 32 * kStagePitch * 4;
-__device__ __forceinline__ void store_rows(const DenseArgs& a, uint32_t acc, float* stage, int64_t row0, int lane)
+template <bool LINEAR> __device__ __forceinline__ void store_rows(const DenseArgs& a, uint32_t acc, float* stage, int64_t row0, int lane)
 {
     const bool vec = a.ldc % 4 == 0 && (reinterpret_cast<uintptr_t>(a.C) & 15) == 0 &&
-                     (!a.mask || (a.ldm % 4 == 0 && (reinterpret_cast<uintptr_t>(a.mask) & 15) == 0));
+                     (!a.mask || (a.ldm % 4 == 0 && (reinterpret_cast<uintptr_t>(a.mask) & 15) == 0)) &&
+                     (!LINEAR || !a.z || (a.ldz % 4 == 0 && (reinterpret_cast<uintptr_t>(a.z) & 15) == 0));
     const int rows = (int)min((int64_t)32, a.M - row0);
     for (int c0 = 0; c0 < a.n_pad; c0 += 32) {
         const bool pieces = vec && c0 + 32 <= a.N;                // whole 128-byte pieces of every row
@@ -114,6 +134,7 @@ __device__ __forceinline__ void store_rows(const DenseArgs& a, uint32_t acc, flo
         tmem_ld16(acc + (uint32_t)c0, r);
         if (c0 + 16 < a.n_pad) tmem_ld16(acc + (uint32_t)c0 + 16, r + 16);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        if constexpr (LINEAR) add_bias(a, r, c0, row0 + lane);
         float4* mine = reinterpret_cast<float4*>(stage + lane * kStagePitch);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
@@ -124,6 +145,13 @@ __device__ __forceinline__ void store_rows(const DenseArgs& a, uint32_t acc, flo
             for (int i = 0; i < 8; ++i) {
                 if (i * 4 + r4 >= rows) continue;
                 float4 v = *reinterpret_cast<const float4*>(stage + (i * 4 + r4) * kStagePitch + (lane & 7) * 4);
+                if constexpr (LINEAR) {
+                    if (a.z) __stcs(reinterpret_cast<float4*>(a.z + (row0 + i * 4 + r4) * a.ldz + col4), v);
+                    v = make_float4(activate(a.act, v.x), activate(a.act, v.y), activate(a.act, v.z), activate(a.act, v.w));
+                    if (a.mask) v = make_float4(v.x + mk[i].x, v.y + mk[i].y, v.z + mk[i].z, v.w + mk[i].w);
+                    __stcs(reinterpret_cast<float4*>(a.C + (row0 + i * 4 + r4) * a.ldc + col4), v);
+                    continue;
+                }
                 if (a.relu) v = make_float4(fmaxf(v.x, 0.f), fmaxf(v.y, 0.f), fmaxf(v.z, 0.f), fmaxf(v.w, 0.f));
                 if (a.mask) {
                     if (!(mk[i].x > 0.f)) v.x = 0.f;
@@ -146,6 +174,13 @@ __device__ __forceinline__ void store_rows(const DenseArgs& a, uint32_t acc, flo
                 for (int i = 0; i < 8; ++i) {
                     if (i0 + i >= rows) break;
                     float v = stage[(i0 + i) * kStagePitch + lane];
+                    if constexpr (LINEAR) {
+                        if (a.z) a.z[(row0 + i0 + i) * a.ldz + c] = v;
+                        v = activate(a.act, v);
+                        if (a.mask) v += mrow[i];
+                        __stcs(a.C + (row0 + i0 + i) * a.ldc + c, v);
+                        continue;
+                    }
                     if (a.relu) v = fmaxf(v, 0.f);
                     if (a.mask && !(mrow[i] > 0.f)) v = 0.f;
                     __stcs(a.C + (row0 + i0 + i) * a.ldc + c, v);
@@ -156,6 +191,7 @@ __device__ __forceinline__ void store_rows(const DenseArgs& a, uint32_t acc, flo
     }
 }
 
+template <bool LINEAR>
 __global__ void __launch_bounds__(kThreads, 1)
 k_dense_nt(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmBh,
            const __grid_constant__ CUtensorMap tmBt, const DenseArgs a)
@@ -259,7 +295,7 @@ k_dense_nt(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
             const int q = warp & 3;                               // a warp may only read its own quarter of the TMEM lanes
             // every load has landed and every MMA has read its operands: the stages are free for the staging of the rows
             if (m0 + q * 32 < a.M)
-                store_rows(a, tmem + ((uint32_t)(q * 32) << 16), reinterpret_cast<float*>(gbase + q * kStageBytes), m0 + q * 32, lane);
+                store_rows<LINEAR>(a, tmem + ((uint32_t)(q * 32) << 16), reinterpret_cast<float*>(gbase + q * kStageBytes), m0 + q * 32, lane);
         }
     }
     if (!ok) atomicExch(a.status, 1);
@@ -303,7 +339,7 @@ __device__ __forceinline__ void umma_tf32_pair(uint32_t tmem_d, uint64_t a_desc,
         ::"r"(tmem_d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
 }
 
-template <bool MASK>
+template <int EPI>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadsPair, 1)
 k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmBh,
                 const __grid_constant__ CUtensorMap tmBt, const DenseArgs a, const int n_tiles, const int stages)
@@ -454,7 +490,9 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         const uint32_t leader_acc_empty0 = in_leader(acc_empty0);
         float4* stage = reinterpret_cast<float4*>(gbase + staging + (warp - 2 - kSplitWarps) * kPieceBytes);
         const bool vec = a.ldc % 4 == 0 && (reinterpret_cast<uintptr_t>(a.C) & 15) == 0 &&
-                         (!MASK || (a.ldm % 4 == 0 && (reinterpret_cast<uintptr_t>(a.mask) & 15) == 0));
+                         (EPI == kPlain || !a.mask || (a.ldm % 4 == 0 && (reinterpret_cast<uintptr_t>(a.mask) & 15) == 0)) &&
+                         (EPI != kLinear || !a.z || (a.ldz % 4 == 0 && (reinterpret_cast<uintptr_t>(a.z) & 15) == 0));
+        const bool side = EPI == kMasked || (EPI == kLinear && a.mask);
         const int r4 = lane >> 3, piece = lane & 7;
         int lt = 0;
         for (int tile = pair; tile < n_tiles; tile += pairs, ++lt) {
@@ -465,7 +503,7 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             for (int c0 = first; c0 < a.n_pad; c0 += step) {
                 const bool whole = vec && c0 + 32 <= a.N;         // 128-byte pieces of every row, four rows an instruction
                 [[maybe_unused]] float4 mk[8];
-                if (MASK && whole) {                              // under way while the accumulator is waited for and read
+                if (side && whole) {                              // under way while the accumulator is waited for and read
                     const float* m = a.mask + (row0 + r4) * a.ldm + c0 + piece * 4;
 #pragma unroll
                     for (int i = 0; i < 8; ++i, m += 4 * a.ldm)
@@ -486,6 +524,7 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                         __syncwarp();
                         if (lane == 0) mbar_arrive_cluster(leader_acc_empty0 + 8 * b);
                     }
+                    if constexpr (EPI == kLinear) add_bias(a, r, c0, row0 + lane);
 #pragma unroll
                     for (int j = 0; j < 8; ++j)                   // a lane holds one row: through shared memory, conflict-free both ways
                         stage[lane * 8 + (j ^ (lane & 7))] = make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]), __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3]));
@@ -498,8 +537,16 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                     float* c = a.C + (row0 + r4) * a.ldc + c0 + piece * 4;
 #pragma unroll
                     for (int i = 0; i < 8; ++i, c += 4 * a.ldc) {
+                        if constexpr (EPI == kLinear) {
+                            if (i * 4 + r4 >= rows) continue;
+                            if (a.z) __stcs(reinterpret_cast<float4*>(a.z + (row0 + i * 4 + r4) * a.ldz + c0 + piece * 4), x[i]);
+                            x[i] = make_float4(activate(a.act, x[i].x), activate(a.act, x[i].y), activate(a.act, x[i].z), activate(a.act, x[i].w));
+                            if (a.mask) x[i] = make_float4(x[i].x + mk[i].x, x[i].y + mk[i].y, x[i].z + mk[i].z, x[i].w + mk[i].w);
+                            __stcs(reinterpret_cast<float4*>(c), x[i]);
+                            continue;
+                        }
                         if (a.relu) x[i] = make_float4(fmaxf(x[i].x, 0.f), fmaxf(x[i].y, 0.f), fmaxf(x[i].z, 0.f), fmaxf(x[i].w, 0.f));
-                        if (MASK) {
+                        if (EPI == kMasked) {
                             if (!(mk[i].x > 0.f)) x[i].x = 0.f;
                             if (!(mk[i].y > 0.f)) x[i].y = 0.f;
                             if (!(mk[i].z > 0.f)) x[i].z = 0.f;
@@ -511,7 +558,7 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                     const float* flat = reinterpret_cast<const float*>(stage);
                     for (int i0 = 0; i0 < rows; i0 += 8) {        // eight rows' mask values in flight
                         [[maybe_unused]] float mrow[8];
-                        if (MASK) {
+                        if (side) {
 #pragma unroll
                             for (int i = 0; i < 8; ++i)
                                 if (i0 + i < rows) mrow[i] = __ldg(a.mask + (row0 + i0 + i) * a.ldm + c0 + lane);
@@ -520,8 +567,15 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                         for (int i = 0; i < 8; ++i) {
                             if (i0 + i >= rows) break;
                             float x = flat[((i0 + i) * 8 + ((lane >> 2) ^ ((i0 + i) & 7))) * 4 + (lane & 3)];
+                            if constexpr (EPI == kLinear) {
+                                if (a.z) a.z[(row0 + i0 + i) * a.ldz + c0 + lane] = x;
+                                x = activate(a.act, x);
+                                if (a.mask) x += mrow[i];
+                                __stcs(a.C + (row0 + i0 + i) * a.ldc + c0 + lane, x);
+                                continue;
+                            }
                             if (a.relu) x = fmaxf(x, 0.f);
-                            if (MASK && !(mrow[i] > 0.f)) x = 0.f;
+                            if (EPI == kMasked && !(mrow[i] > 0.f)) x = 0.f;
                             __stcs(a.C + (row0 + i0 + i) * a.ldc + c0 + lane, x);
                         }
                     }
@@ -584,51 +638,6 @@ __global__ void __launch_bounds__(256) k_tf32_split_operands(const __grid_consta
     }
 }
 
-// Raises a kernel's dynamic shared-memory limit to the most a CTA can have, once per device instead of before every launch.
-int allow_smem(const void* kernel, std::atomic<bool>* done)
-{
-    int dev = 0;
-    DG_CUDA(cudaGetDevice(&dev));
-    if (dev < 0 || dev >= 64) return DG_ERR_STATE;
-    if (done[dev].load(std::memory_order_relaxed)) return DG_OK;
-    DG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
-    done[dev].store(true, std::memory_order_relaxed);
-    return DG_OK;
-}
-
-int sm_count()
-{
-    static std::atomic<int> count[64];
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
-    int n = count[dev].load(std::memory_order_relaxed);
-    if (n == 0) {
-        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-        count[dev].store(n, std::memory_order_relaxed);
-    }
-    return n;
-}
-
-}  // namespace
-
-namespace {
-
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_tiled()
-{
-    static EncodeTiledFn fn = [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
-            p = nullptr;
-        return reinterpret_cast<EncodeTiledFn>(p);
-    }();
-    return fn;
-}
-
 // 2-D fp32 row-major matrix [rows x cols] with leading dimension ld, boxes of box_cols (32: 128B swizzle, 16: 64B swizzle) columns x box_rows rows,
 // out-of-range elements read as zero.
 int make_map(CUtensorMap* map, const float* ptr, int64_t rows, int64_t cols, int64_t ld, int box_rows, int box_cols = BK)
@@ -662,6 +671,49 @@ bool by_pairs(int64_t M, int n_pad, int K, bool masked, int sms)
     const bool half_slab = (K - 1) % BK < BK / 2;
     if (tiles <= sms) return n_pad > 128 || half_slab || K > (n_pad > 80 ? 96 : 128);
     return n_pad > 80 || (tiles > 2 * sms && (!masked || K > 64));
+}
+
+// One panel (up to 256 columns) of a product with the epilogue that `a` describes.
+int launch_nt(const float* A, int64_t lda, const float* Bt_head, const float* Bt_tail, int64_t ldb, DenseArgs a, int epilogue, cudaStream_t stream)
+{
+    a.n_pad = (a.N + 15) / 16 * 16;
+    a.status = dg_status_word();
+    if (!a.status) return DG_ERR_STATE;
+    const int sms = sm_count();
+    if (sms <= 0) return DG_ERR_STATE;
+    const bool pair = by_pairs(a.M, a.n_pad, a.K, a.mask != nullptr, sms);
+    CUtensorMap tmA, tmBh, tmBt;
+    int rc;
+    if (!pair) {
+        const size_t smem = STAGES * (size_t)BK * 4 * (2 * BM + 2 * a.n_pad) + 24 * STAGES + 48 + 1024;
+        if ((rc = make_map(&tmA, A, a.M, a.K, lda, BM)) || (rc = make_map(&tmBh, Bt_head, a.N, a.K, ldb, a.n_pad)) ||
+            (rc = make_map(&tmBt, Bt_tail, a.N, a.K, ldb, a.n_pad)))
+            return rc;
+        auto run = [&](auto* kernel, std::atomic<bool>* granted) {
+            const int code = allow_smem((const void*)kernel, granted);
+            if (code) return code;
+            kernel<<<(unsigned)((a.M + BM - 1) / BM), kThreads, smem, stream>>>(tmA, tmBh, tmBt, a);
+            return (int)cudaGetLastError();
+        };
+        static std::atomic<bool> granted[64], granted_linear[64];
+        return epilogue == kLinear ? run(k_dense_nt<true>, granted_linear) : run(k_dense_nt<false>, granted);
+    }
+    a.n_pad = (a.N + 31) / 32 * 32;                               // both CTAs hold whole groups of 16 of its rows
+    if ((rc = make_map(&tmA, A, a.M, a.K, lda, BM, PK)) || (rc = make_map(&tmBh, Bt_head, a.N, a.K, ldb, a.n_pad / 2, PK)) ||
+        (rc = make_map(&tmBt, Bt_tail, a.N, a.K, ldb, a.n_pad / 2, PK)))
+        return rc;
+    const size_t stage = (size_t)PK * 4 * (2 * BM + a.n_pad), rest = kEpilogueWarps * kPieceBytes + kPairBarBytes + 1024;
+    const int stages = (int)std::min<size_t>(kMaxPairStages, (227 * 1024 - rest) / stage);
+    const int n_tiles = (int)((a.M + 2 * BM - 1) / (2 * BM));
+    auto run = [&](auto* kernel, std::atomic<bool>* granted) {
+        const int code = allow_smem((const void*)kernel, granted);
+        if (code) return code;
+        kernel<<<2u * (unsigned)std::min(n_tiles, sms / 2), kThreadsPair, stages * stage + rest, stream>>>(tmA, tmBh, tmBt, a, n_tiles, stages);
+        return (int)cudaGetLastError();
+    };
+    static std::atomic<bool> granted[64], granted_masked[64], granted_linear[64];
+    return epilogue == kLinear ? run(k_dense_nt_pair<kLinear>, granted_linear) : epilogue == kMasked ? run(k_dense_nt_pair<kMasked>, granted_masked)
+                                                                                               : run(k_dense_nt_pair<kPlain>, granted);
 }
 
 }  // namespace
@@ -730,38 +782,29 @@ extern "C" int dg_dense_nt_masked(const float* A, int64_t lda, const float* Bt_h
         return DG_OK;
     }
     DenseArgs a{};
-    a.C = C; a.ldc = ldc; a.M = M; a.N = N; a.K = K; a.n_pad = (N + 15) / 16 * 16; a.relu = relu ? 1u : 0u;
+    a.C = C; a.ldc = ldc; a.M = M; a.N = N; a.K = K; a.relu = relu ? 1u : 0u;
     a.mask = mask; a.ldm = ldm;
-    a.status = dg_status_word();
-    if (!a.status) return DG_ERR_STATE;
-    const int sms = sm_count();
-    if (sms <= 0) return DG_ERR_STATE;
-    const bool pair = by_pairs(M, a.n_pad, K, mask != nullptr, sms);
-    CUtensorMap tmA, tmBh, tmBt;
-    int rc;
-    if (!pair) {
-        const size_t smem = STAGES * (size_t)BK * 4 * (2 * BM + 2 * a.n_pad) + 24 * STAGES + 48 + 1024;
-        if ((rc = make_map(&tmA, A, M, K, lda, BM)) || (rc = make_map(&tmBh, Bt_head, N, K, ldb, a.n_pad)) ||
-            (rc = make_map(&tmBt, Bt_tail, N, K, ldb, a.n_pad)))
-            return rc;
-        static std::atomic<bool> granted[64];
-        if ((rc = allow_smem((const void*)k_dense_nt, granted))) return rc;
-        k_dense_nt<<<(unsigned)((M + BM - 1) / BM), kThreads, smem, (cudaStream_t)stream>>>(tmA, tmBh, tmBt, a);
-        return (int)cudaGetLastError();
+    return launch_nt(A, lda, Bt_head, Bt_tail, ldb, a, mask ? kMasked : kPlain, (cudaStream_t)stream);
+}
+
+// The fp32 product of dg_linear: panels as above, the epilogue's operands with them.
+int dg_dense_linear(const dg_linear_args* g, cudaStream_t stream)
+{
+    const float* x = static_cast<const float*>(g->x);
+    if (!g->head || !g->tail) return DG_ERR_NULL;
+    if (!dg_dense_supported(g->M, g->N, g->K, g->ldx, g->ldb, x, g->head, g->tail)) return DG_ERR_UNSUPPORTED;
+    for (int32_t n0 = 0; n0 < g->N; n0 += 256) {
+        DenseArgs a{};
+        a.C = static_cast<float*>(g->y) + n0; a.ldc = g->ldy; a.M = g->M; a.N = std::min(256, g->N - n0); a.K = g->K;
+        a.mask = g->residual ? static_cast<const float*>(g->residual) + n0 : nullptr; a.ldm = g->ldr;
+        a.bias = g->bias ? static_cast<const float*>(g->bias) + n0 : nullptr;
+        a.z = g->z ? static_cast<float*>(g->z) + n0 : nullptr; a.ldz = g->ldz;
+        a.bits = g->bits ? g->bits + n0 / 32 : nullptr; a.ldbits = g->ldbits;
+        a.act = g->act;
+        const int rc = launch_nt(x, g->ldx, g->head + (int64_t)n0 * g->ldb, g->tail + (int64_t)n0 * g->ldb, g->ldb, a, kLinear, stream);
+        if (rc) return rc;
     }
-    a.n_pad = (N + 31) / 32 * 32;                                 // both CTAs hold whole groups of 16 of its rows
-    if ((rc = make_map(&tmA, A, M, K, lda, BM, PK)) || (rc = make_map(&tmBh, Bt_head, N, K, ldb, a.n_pad / 2, PK)) ||
-        (rc = make_map(&tmBt, Bt_tail, N, K, ldb, a.n_pad / 2, PK)))
-        return rc;
-    const size_t stage = (size_t)PK * 4 * (2 * BM + a.n_pad), rest = kEpilogueWarps * kPieceBytes + kPairBarBytes + 1024;
-    const int stages = (int)std::min<size_t>(kMaxPairStages, (227 * 1024 - rest) / stage);
-    static std::atomic<bool> granted[64];
-    static std::atomic<bool> granted_masked[64];
-    if ((rc = mask ? allow_smem((const void*)k_dense_nt_pair<true>, granted_masked) : allow_smem((const void*)k_dense_nt_pair<false>, granted))) return rc;
-    const int n_tiles = (int)((M + 2 * BM - 1) / (2 * BM));
-    (mask ? k_dense_nt_pair<true> : k_dense_nt_pair<false>)<<<2u * (unsigned)std::min(n_tiles, sms / 2), kThreadsPair, stages * stage + rest, (cudaStream_t)stream>>>(
-        tmA, tmBh, tmBt, a, n_tiles, stages);
-    return (int)cudaGetLastError();
+    return DG_OK;
 }
 
 extern "C" int dg_dense_status(int* host_status, void* stream)

@@ -1,0 +1,1014 @@
+// Linear layer with bias, activation and residual in the product's epilogue, y = act(x w + b) + r, for 16-bit operands, and what its gradients need.
+//
+// k_linear_pair: x w on the tensor cores (tcgen05 kind::f16, fp32 accumulators in tensor memory) by CTA pairs that walk over tiles of 256 rows x up to 256
+// columns.  w is read as it lies: [N x K] rows are K-major operands, [K x N] rows MN-major ones, both in 128B-swizzled boxes.
+// k_linear_dw: the weight gradient x^T dz, both operands MN-major, rows cut into ranges whose partial results are added in order.
+// k_linear_dz: dz = dy act'(z) and its column sums.
+// k_few_*: products of few rows, bound by latency.
+// The fp32 product is dg_dense.cu's.
+#include <algorithm>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include "dg_act.h"
+#include "dg_internal.h"
+#include "dg_tma.h"
+
+namespace {
+
+using namespace dg;
+
+template <class T> struct Pair;
+template <> struct Pair<__nv_bfloat16> {
+    using Two = __nv_bfloat162;
+    static __device__ __forceinline__ float2 wide(uint32_t v) { return __bfloat1622float2(*reinterpret_cast<const Two*>(&v)); }
+    static __device__ __forceinline__ uint32_t narrow(float a, float b)
+    {
+        const Two t = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&t);
+    }
+    static __device__ __forceinline__ float one(__nv_bfloat16 v) { return __bfloat162float(v); }
+    static __device__ __forceinline__ __nv_bfloat16 round(float v) { return __float2bfloat16_rn(v); }
+    static constexpr uint32_t kFormat = 1;
+};
+template <> struct Pair<__half> {
+    using Two = __half2;
+    static __device__ __forceinline__ float2 wide(uint32_t v) { return __half22float2(*reinterpret_cast<const Two*>(&v)); }
+    static __device__ __forceinline__ uint32_t narrow(float a, float b)
+    {
+        const Two t = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&t);
+    }
+    static __device__ __forceinline__ float one(__half v) { return __half2float(v); }
+    static __device__ __forceinline__ __half round(float v) { return __float2half_rn(v); }
+    static constexpr uint32_t kFormat = 0;
+};
+template <> struct Pair<float> {
+    static __device__ __forceinline__ float one(float v) { return v; }
+    static __device__ __forceinline__ float round(float v) { return v; }
+};
+
+// ---- the product on the tensor cores ------------------------------------------------------------------------------------
+constexpr int BM = 128, BK = 64;                  // rows of a CTA, K-columns of a stage: 128 bytes
+constexpr int kEpilogueWarps = 8, kThreadsPair = 32 * (2 + kEpilogueWarps);
+constexpr int kMaxStages = 8;
+constexpr int kABytes = BM * BK * 2;
+constexpr int kPieceBytes = 32 * 64 * 2;          // an epilogue warp's 32 rows x 64 columns
+constexpr int kBarBytes = 8 * (2 * kMaxStages + 5 + 2 * kEpilogueWarps) + 8;
+
+struct LinearPairArgs {
+    const void* bias;
+    uint32_t* bits;
+    int64_t ldbits;
+    int64_t M;
+    int32_t N, K;
+    int32_t n_tile, n_panels, tiles;
+    int32_t stages;
+    int32_t b_boxes;                              // w MN-major: boxes of 64 columns a CTA loads; 0: K-major
+    int32_t residual, save_z, whole_bias;
+    int* status;
+};
+
+// A load into this CTA whose arrival is counted at a barrier of the pair's even CTA.
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t cluster_bar)
+{
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 ::"r"(dst), "l"(map), "r"(cluster_bar), "r"(c0), "r"(c1) : "memory");
+}
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int c0, int c1, uint32_t src)
+{
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(src), "r"(c0), "r"(c1) : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// MN-major 16-bit tile: boxes of 64 columns x `rows` K-rows of 128 bytes, 128B swizzle; 8-row groups are 1024 bytes apart (stride byte offset), boxes
+// `box_bytes` (leading byte offset).
+__device__ __forceinline__ uint64_t umma_desc_mn16(uint32_t smem_addr, uint32_t box_bytes)
+{
+    return (uint64_t)((smem_addr & 0x3FFFF) >> 4) | (uint64_t)(box_bytes >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// kind::f16: fp32 accumulator, A and B of `format` (0: fp16, 1: bf16)
+__device__ __forceinline__ uint32_t umma_idesc_f16(uint32_t format, int m, int n, bool a_mn, bool b_mn)
+{
+    return 1u << 4 | format << 7 | format << 10 | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24;
+}
+__device__ __forceinline__ void umma_f16_pair(uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+
+// Warps: 0 TMA, 1 MMA issue (even CTA) + tensor-memory allocation, 2-9 epilogue (lane quarter w % 4; two warps a quarter take its 64-column pieces
+// in turn).  A stage is 64 K-columns of the CTA's 128 rows of x and of its half of the panel's columns of w.  Two accumulators (columns 0 / 256).
+// Barriers: full (even CTA, the loads of both), empty and acc_full (both CTAs, by commit), acc_empty (even CTA: the epilogue warps of both), and one an
+// epilogue warp and buffer for its residual's pieces.
+template <class T, int ACT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadsPair, 1)
+k_linear_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmY,
+              const __grid_constant__ CUtensorMap tmR, const __grid_constant__ CUtensorMap tmZ, const LinearPairArgs a)
+{
+    extern __shared__ unsigned char smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t base = (raw + 1023u) & ~1023u;
+    unsigned char* gbase = smem_raw + (base - raw);
+    const int half_n = a.n_tile / 2, b_bytes = a.b_boxes ? a.b_boxes * BK * 128 : half_n * 128;
+    const int stage_bytes = kABytes + b_bytes;
+    const int staging = a.stages * stage_bytes, per_warp = (a.save_z ? 3 : 2) * kPieceBytes;
+    const uint32_t bars = base + staging + kEpilogueWarps * per_warp;
+    const uint32_t full0 = bars, empty0 = bars + 8 * kMaxStages, acc_full0 = bars + 16 * kMaxStages, acc_empty0 = acc_full0 + 16, done = acc_empty0 + 16;
+    const uint32_t res0 = done + 8;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbase + staging + kEpilogueWarps * per_warp + 8 * (2 * kMaxStages + 5 + 2 * kEpilogueWarps));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const int slabs = (a.K + BK - 1) / BK;
+    constexpr int kTmemCols = 512;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < a.stages; ++s) {
+            mbar_init(full0 + 8 * s, 1);
+            mbar_init(empty0 + 8 * s, 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(acc_full0 + 8 * b, 1);
+            mbar_init(acc_empty0 + 8 * b, 2 * kEpilogueWarps);
+        }
+        mbar_init(done, 1);
+        for (int w = 0; w < 2 * kEpilogueWarps; ++w) mbar_init(res0 + 8 * w, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(kTmemCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    cluster_sync();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *tmem_slot;
+    bool ok = true;
+
+    if (warp == 0) {
+        if (lane == 0) {                                          // TMA producer: one ring of stages across all tiles
+            const uint32_t leader_full0 = in_leader(full0);
+            int it = 0, s = 0, phase = 1;
+            for (int tile = pair; tile < a.tiles && ok; tile += pairs) {
+                const int row0 = (int)((int64_t)(tile / a.n_panels) * (2 * BM) + rank * BM);      // rows beyond the matrix arrive as zeros
+                const int n0 = tile % a.n_panels * a.n_tile + rank * half_n;
+                for (int i = 0; i < slabs; ++i, ++it) {
+                    if (it >= a.stages) ok = mbar_wait(empty0 + 8 * s, phase);
+                    if (!ok) break;
+                    const uint32_t st = base + s * stage_bytes, bar = leader_full0 + 8 * s;
+                    if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * stage_bytes);
+                    tma_load_2d_pair(st, &tmA, i * BK, row0, bar);
+                    if (a.b_boxes)
+                        for (int j = 0; j < a.b_boxes; ++j) tma_load_2d_pair(st + kABytes + j * BK * 128, &tmB, n0 + 64 * j, i * BK, bar);
+                    else
+                        tma_load_2d_pair(st + kABytes, &tmB, i * BK, n0, bar);
+                    if (++s == a.stages) s = 0, phase ^= 1;
+                }
+            }
+            if (rank == 0) await_loads(full0, it, a.stages);      // of both CTAs; the odd one leaves after this
+        }
+    } else if (warp == 1) {
+        if (rank == 0) {                                          // MMA issuer: the warp waits and counts together, one lane issues
+            const bool issuer = elect_one();
+            auto wait = [&](uint32_t bar, int parity) { return __any_sync(0xffffffffu, issuer && mbar_wait(bar, parity)) != 0; };
+            const uint32_t idesc = umma_idesc_f16(Pair<T>::kFormat, 2 * BM, a.n_tile, false, a.b_boxes != 0);
+            const uint64_t a0 = umma_desc_sw128(base);
+            const uint64_t b0 = a.b_boxes ? umma_desc_mn16(base + kABytes, BK * 128) : umma_desc_sw128(base + kABytes);
+            const uint32_t next_stage = (uint32_t)stage_bytes >> 4, b_step = a.b_boxes ? 16 * 128 >> 4 : 2;      // 16 K-columns
+            int s = 0, phase = 0, lt = 0;
+            for (int tile = pair; tile < a.tiles && ok; tile += pairs, ++lt) {
+                const int b = lt & 1, v = lt >> 1;
+                if (lt >= 2) ok = wait(acc_empty0 + 8 * b, (v - 1) & 1);     // both epilogues have drained this accumulator
+                const uint32_t acc = tmem + (uint32_t)(b * 256);
+                for (int i = 0; i < slabs && ok; ++i) {
+                    ok = wait(full0 + 8 * s, phase);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (issuer) {
+                        const uint32_t at = (uint32_t)s * next_stage;
+#pragma unroll
+                        for (int k = 0; k < BK / 16; ++k) umma_f16_pair(acc, a0 + at + 2 * k, b0 + at + b_step * k, idesc, i > 0 || k > 0 ? 1u : 0u);
+                        umma_commit_pair(empty0 + 8 * s);
+                    }
+                    __syncwarp();
+                    if (++s == a.stages) s = 0, phase ^= 1;
+                }
+                if (ok && issuer) umma_commit_pair(acc_full0 + 8 * b);
+                __syncwarp();
+            }
+            if (issuer) await_mmas_pair(done);
+            __syncwarp();
+        } else if (lane == 0) {
+            mbar_wait(done, 0);
+        }
+    } else {
+        // A lane holds a row's 64 columns of the accumulator.  Pieces of 32 rows x 128 bytes lie in shared memory with the 128B swizzle (conflict-free by
+        // rows) and are moved by TMA, which leaves out what lies beyond the matrix: the residual arrives where y is then put together.
+        const int w = warp - 2, q = warp & 3, first = w / 4 * 64;      // a warp may only read its own quarter of the TMEM lanes
+        constexpr int step = kEpilogueWarps / 4 * 64;
+        const uint32_t leader_acc_empty0 = in_leader(acc_empty0);
+        const int own = staging + w * per_warp;
+        const uint32_t swizzle = lane & 7;
+        const T* bias = static_cast<const T*>(a.bias);
+        int lt = 0, count = 0;                                    // pieces so far: buffer count & 1
+        auto row_of = [&](int tile) { return (int64_t)(tile / a.n_panels) * (2 * BM) + rank * BM + q * 32; };
+        auto fetch = [&](int tile, int c0, int n) {               // the residual's piece into buffer n & 1, whose last store has been read
+            const int64_t row = row_of(tile);
+            if (row >= a.M || tile % a.n_panels * a.n_tile + c0 >= a.N) return;
+            mbar_expect_tx(res0 + 8 * (2 * w + (n & 1)), kPieceBytes);
+            tma_load_2d(base + own + (n & 1) * kPieceBytes, &tmR, tile % a.n_panels * a.n_tile + c0, (int)row, res0 + 8 * (2 * w + (n & 1)));
+        };
+        int res_uses[2] = {0, 0};
+        if (a.residual && lane == 0 && pair < a.tiles && first < a.n_tile) fetch(pair, first, 0);
+        for (int tile = pair; tile < a.tiles && ok; tile += pairs, ++lt) {
+            const int b = lt & 1, v = lt >> 1;
+            const int n0 = tile % a.n_panels * a.n_tile;
+            const int64_t row0 = row_of(tile);
+            const uint32_t acc = tmem + (uint32_t)(b * 256) + ((uint32_t)(q * 32) << 16);
+            ok = __all_sync(0xffffffffu, mbar_wait(acc_full0 + 8 * b, v & 1));     // tcgen05.ld is warp-collective
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (first >= a.n_tile) {                              // nothing here for this warp
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(leader_acc_empty0 + 8 * b);
+                continue;
+            }
+            for (int c0 = first; c0 < a.n_tile; c0 += step, ++count) {
+                uint32_t r[64];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) tmem_ld16(acc + (uint32_t)(c0 + 16 * j), r + 16 * j);
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                if (c0 + step >= a.n_tile) {                      // the accumulator has been read: its next tile may start
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(leader_acc_empty0 + 8 * b);
+                }
+                const int col0 = n0 + c0, s = count & 1;
+                const bool live = row0 < a.M && col0 < a.N;       // the same for the warp
+                if (lane == 0) {
+                    bulk_wait_read();                             // what the last pieces stored has left the buffers
+                    if (a.residual) {
+                        const bool more = c0 + step < a.n_tile;
+                        if (more || tile + pairs < a.tiles) fetch(more ? tile : tile + pairs, more ? c0 + step : first, count + 1);
+                    }
+                }
+                if (a.residual && live) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(res0 + 8 * (2 * w + s), res_uses[s] & 1));
+                    if (!ok) break;
+                    ++res_uses[s];
+                }
+                __syncwarp();
+                if (!live) continue;
+                unsigned char* y_row = gbase + own + s * kPieceBytes + lane * 128;
+                unsigned char* z_row = gbase + own + 2 * kPieceBytes + lane * 128;
+                uint32_t positive[2] = {0u, 0u};
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {                     // eight columns: 16 bytes
+                    float z[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) z[e] = __uint_as_float(r[8 * j + e]);
+                    if (bias) {
+                        const int c = col0 + 8 * j;
+                        if (a.whole_bias && c + 8 <= a.N) {
+                            const uint4 t = __ldg(reinterpret_cast<const uint4*>(bias + c));
+                            const uint32_t u[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const float2 f = Pair<T>::wide(u[e]);
+                                z[2 * e] += f.x, z[2 * e + 1] += f.y;
+                            }
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                if (c + e < a.N) z[e] += Pair<T>::one(bias[c + e]);
+                        }
+                    }
+                    const uint32_t at = ((uint32_t)j ^ swizzle) * 16;
+                    if (ACT != DG_ACT_NONE && a.save_z)
+                        *reinterpret_cast<uint4*>(z_row + at) = make_uint4(Pair<T>::narrow(z[0], z[1]), Pair<T>::narrow(z[2], z[3]), Pair<T>::narrow(z[4], z[5]),
+                                                                           Pair<T>::narrow(z[6], z[7]));
+                    if (ACT == DG_ACT_RELU && a.bits) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) positive[j / 4] |= (z[e] <= 0.f ? 0u : 1u) << (8 * (j % 4) + e);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) z[e] = act_value<ACT>(z[e]);
+                    uint4* to = reinterpret_cast<uint4*>(y_row + at);
+                    if (a.residual) {
+                        const uint4 t = *to;
+                        const uint32_t u[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float2 f = Pair<T>::wide(u[e]);
+                            z[2 * e] += f.x, z[2 * e + 1] += f.y;
+                        }
+                    }
+                    *to = make_uint4(Pair<T>::narrow(z[0], z[1]), Pair<T>::narrow(z[2], z[3]), Pair<T>::narrow(z[4], z[5]), Pair<T>::narrow(z[6], z[7]));
+                }
+                if (ACT == DG_ACT_RELU && a.bits && row0 + lane < a.M) {      // words beyond the row's are left alone
+                    uint32_t* to = a.bits + (row0 + lane) * a.ldbits + col0 / 32;
+                    *reinterpret_cast<uint2*>(to) = make_uint2(positive[0], positive[1]);
+                }
+                fence_async();
+                __syncwarp();
+                if (lane == 0) {
+                    tma_store_2d(&tmY, col0, (int)row0, base + own + s * kPieceBytes);
+                    if (ACT != DG_ACT_NONE && a.save_z) tma_store_2d(&tmZ, col0, (int)row0, base + own + 2 * kPieceBytes);
+                    bulk_commit();
+                }
+            }
+        }
+        if (lane == 0) bulk_wait();
+        __syncwarp();
+    }
+    if (!ok) atomicExch(a.status, 1);
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    cluster_sync();                                               // no CTA leaves while the other's MMAs read its operands or arrive at its barriers
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (warp == 1)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+}
+
+// ---- the weight gradient --------------------------------------------------------------------------------------------------
+// A CTA owns a panel of up to 256 x 256 of dw and a range of rows.  Both operands come in boxes of 64 columns x 64 rows (MN-major); x's columns lie along
+// the MMA's 128 rows, so a panel wider than 128 takes two accumulators.  The range's partial goes to scratch, four columns of dz and all of x's side by
+// side; a second kernel adds the ranges in order.
+// A chain of accumulations, which the tensor cores truncate, is as long as the range: 16 rows each, some 1,000 at 2.4 M rows, 3e-5 of the sum at most where
+// bf16 rounds by 4e-3 and fp16 by 5e-4; so no flush in between, which fp32 needs.
+constexpr int kDwRows = 64, kDwBox = kDwRows * 128, kDwThreads = 32 * 6, kDwMaxStages = 8;
+constexpr int kDwBarBytes = 8 * (2 * kDwMaxStages + 2) + 8;
+
+struct LinearDwArgs {
+    float4* partial;                              // [range][panel][q_store / 4][p_store]
+    int64_t M, rows_per_range;
+    int32_t p_cols, q_cols;                       // K, N
+    int32_t p_panels, q_panels, p_store, q_store;
+    int32_t stages, p_boxes, q_boxes;             // of a full panel
+    int* status;
+};
+
+template <class T>
+__global__ void __launch_bounds__(kDwThreads, 1) k_linear_dw(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ CUtensorMap tmQ, const LinearDwArgs a)
+{
+    extern __shared__ unsigned char smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t base = (raw + 1023u) & ~1023u;
+    unsigned char* gbase = smem_raw + (base - raw);
+    const int stage_bytes = (a.p_boxes + a.q_boxes) * kDwBox;
+    const uint32_t bars = base + a.stages * stage_bytes;
+    const uint32_t full0 = bars, empty0 = bars + 8 * kDwMaxStages, acc_full = bars + 16 * kDwMaxStages, done = acc_full + 8;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbase + a.stages * stage_bytes + 8 * (2 * kDwMaxStages + 2));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int panels = a.p_panels * a.q_panels, panel = blockIdx.x % panels, range = blockIdx.x / panels;
+    const int p0 = panel / a.q_panels * 256, q0 = panel % a.q_panels * 256;
+    const int p_here = min(256, a.p_cols - p0), q_here = min(256, a.q_cols - q0);
+    const int p_boxes = (p_here + 63) / 64, q_boxes = (q_here + 63) / 64, halves = (p_here + 127) / 128, q_pad = (q_here + 15) / 16 * 16;
+    const int64_t r0 = range * a.rows_per_range, r1 = min(a.M, r0 + a.rows_per_range);
+    const int slabs = (int)((max((int64_t)0, r1 - r0) + kDwRows - 1) / kDwRows);
+    constexpr int kTmemCols = 512;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < a.stages; ++s) {
+            mbar_init(full0 + 8 * s, 1);
+            mbar_init(empty0 + 8 * s, 1);
+        }
+        mbar_init(acc_full, 1);
+        mbar_init(done, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(kTmemCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *tmem_slot;
+    bool ok = true;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int s = 0, phase = 1, i = 0;
+            for (; i < slabs && ok; ++i) {
+                if (i >= a.stages) ok = mbar_wait(empty0 + 8 * s, phase);
+                if (!ok) break;
+                const uint32_t st = base + s * stage_bytes;
+                const int row = (int)(r0 + (int64_t)i * kDwRows);
+                mbar_expect_tx(full0 + 8 * s, (p_boxes + q_boxes) * kDwBox);
+                for (int j = 0; j < p_boxes; ++j) tma_load_2d(st + j * kDwBox, &tmP, p0 + 64 * j, row, full0 + 8 * s);
+                for (int j = 0; j < q_boxes; ++j) tma_load_2d(st + (a.p_boxes + j) * kDwBox, &tmQ, q0 + 64 * j, row, full0 + 8 * s);
+                if (++s == a.stages) s = 0, phase ^= 1;
+            }
+            await_loads(full0, i, a.stages);
+        }
+    } else if (warp == 1) {
+        const bool issuer = elect_one();
+        auto wait = [&](uint32_t bar, int parity) { return __any_sync(0xffffffffu, issuer && mbar_wait(bar, parity)) != 0; };
+        const uint32_t idesc = umma_idesc_f16(Pair<T>::kFormat, 128, q_pad, true, true);
+        int s = 0, phase = 0;
+        for (int i = 0; i < slabs && ok; ++i) {
+            ok = wait(full0 + 8 * s, phase);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (issuer) {
+                const uint32_t st = base + s * stage_bytes;
+                const uint64_t p = umma_desc_mn16(st, kDwBox), q = umma_desc_mn16(st + a.p_boxes * kDwBox, kDwBox);
+                for (int h = 0; h < halves; ++h)
+#pragma unroll
+                    for (int k = 0; k < kDwRows / 16; ++k)        // 16 rows: 2048 bytes
+                        umma_f16(tmem + (uint32_t)(h * 256), p + (uint32_t)((h * 2 * kDwBox + k * 2048) >> 4), q + (uint32_t)(k * 2048 >> 4), idesc,
+                                 i > 0 || k > 0 ? 1u : 0u);
+                umma_commit(empty0 + 8 * s);
+            }
+            __syncwarp();
+            if (++s == a.stages) s = 0, phase ^= 1;
+        }
+        if (ok && issuer) umma_commit(acc_full);
+        __syncwarp();
+        if (issuer) await_mmas(done);
+        __syncwarp();
+    } else {
+        const int q = warp & 3;
+        ok = __all_sync(0xffffffffu, mbar_wait(acc_full, 0));     // tcgen05.ld is warp-collective
+        if (ok) {
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            for (int h = 0; h < halves; ++h) {
+                const int row = h * 128 + q * 32 + lane;
+                float4* part = a.partial + ((int64_t)range * panels + panel) * (a.q_store / 4) * a.p_store + row;
+                for (int c0 = 0; c0 < q_pad; c0 += 16) {
+                    uint32_t r[16];
+                    tmem_ld16(tmem + (uint32_t)(h * 256 + c0) + ((uint32_t)(q * 32) << 16), r);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (row < a.p_store)
+                            __stcg(part + (int64_t)(c0 / 4 + j) * a.p_store,
+                                   slabs ? make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]), __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3]))
+                                         : make_float4(0.f, 0.f, 0.f, 0.f));
+                }
+            }
+        }
+    }
+    if (!ok) atomicExch(a.status, 1);
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 1)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+}
+
+// dw[p, q] = sum of the ranges' partials, in their order.  A thread takes four columns of a row.
+template <class T>
+__global__ void __launch_bounds__(256) k_linear_dw_reduce(const float4* __restrict__ partial, int ranges, int32_t p_panels, int32_t q_panels, int32_t p_store,
+                                                          int32_t q_store, int32_t p_cols, int32_t q_cols, T* __restrict__ dw, int64_t row_stride, int64_t col_stride)
+{
+    const int panels = p_panels * q_panels, per_panel = q_store / 4 * p_store;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (int64_t)panels * per_panel) return;
+    const int panel = (int)(i / per_panel), in = (int)(i % per_panel);
+    const int p = panel / q_panels * 256 + in % p_store, q = panel % q_panels * 256 + in / p_store * 4;
+    if (p >= p_cols || q >= q_cols) return;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    const float4* from = partial + i;
+    const int64_t stride = (int64_t)panels * per_panel;
+#pragma unroll 8
+    for (int r = 0; r < ranges; ++r) {
+        const float4 v = __ldcg(from + r * stride);
+        sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+    }
+    const float s[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (q + j < q_cols) dw[p * row_stride + (q + j) * col_stride] = Pair<T>::round(s[j]);
+}
+
+// ---- dz = dy act'(z) and its column sums ------------------------------------------------------------------------------------
+// A thread owns eight neighbouring columns and walks over rows; the lanes of a row read neighbouring pieces.  `lanes` threads a row (a power of two), a
+// CTA takes 8 * lanes columns and every (256 / lanes * gridDim.x)-th row.
+constexpr int kDzThreads = 256;
+template <class T> __device__ __forceinline__ void load8(const T* p, int n, bool whole, float* v)
+{
+    if (whole && n >= 8) {
+        if constexpr (sizeof(T) == 4) {
+            const float4 a = __ldcs(reinterpret_cast<const float4*>(p)), b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
+            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        } else {
+            const uint4 t = __ldcs(reinterpret_cast<const uint4*>(p));
+            const uint32_t u[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 f = Pair<T>::wide(u[e]);
+                v[2 * e] = f.x, v[2 * e + 1] = f.y;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = e < n ? Pair<T>::one(p[e]) : 0.f;
+    }
+}
+template <class T> __device__ __forceinline__ void store8(T* p, int n, bool whole, const float* v)
+{
+    if (whole && n >= 8) {
+        if constexpr (sizeof(T) == 4) {
+            reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+            reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+            *reinterpret_cast<uint4*>(p) = make_uint4(Pair<T>::narrow(v[0], v[1]), Pair<T>::narrow(v[2], v[3]), Pair<T>::narrow(v[4], v[5]), Pair<T>::narrow(v[6], v[7]));
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e < n) p[e] = Pair<T>::round(v[e]);
+    }
+}
+
+struct LinearDzArgs {
+    int64_t lddy, ldz, ldbits, lddz, M;
+    const uint32_t* bits;
+    float* partial;                               // [gridDim.x][N], or null
+    int32_t N, lanes, whole_dy, whole_z, whole_dz;
+};
+
+template <class T, int ACT>
+__global__ void __launch_bounds__(kDzThreads) k_linear_dz(const T* __restrict__ dy, const T* __restrict__ z, T* __restrict__ dz, const LinearDzArgs a)
+{
+    __shared__ float sums[kDzThreads][9];
+    const int lane = threadIdx.x & (a.lanes - 1), group = threadIdx.x / a.lanes, groups = kDzThreads / a.lanes;
+    const int c = (blockIdx.y * a.lanes + lane) * 8, n = min(8, a.N - c);
+    float sum[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum[e] = 0.f;
+    if (n > 0) {
+#pragma unroll 2
+        for (int64_t row = (int64_t)blockIdx.x * groups + group; row < a.M; row += (int64_t)gridDim.x * groups) {
+            float g[8];
+            load8(dy + row * a.lddy + c, n, a.whole_dy, g);
+            if constexpr (ACT == DG_ACT_RELU) {
+                const uint32_t word = __ldg(a.bits + row * a.ldbits + c / 32) >> (c % 32);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) g[e] = word >> e & 1 ? g[e] : 0.f;
+            } else if constexpr (ACT != DG_ACT_NONE) {
+                float v[8];
+                load8(z + row * a.ldz + c, n, a.whole_z, v);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) g[e] *= act_slope<ACT>(v[e]);
+            }
+            if (dz) store8(dz + row * a.lddz + c, n, a.whole_dz, g);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum[e] += g[e];
+        }
+    }
+    if (!a.partial) return;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sums[threadIdx.x][e] = sum[e];
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.lanes * 8; i += kDzThreads) {
+        const int l = i / 8, col = blockIdx.y * a.lanes * 8 + i;
+        if (col >= a.N) continue;
+        float s = 0.f;
+        for (int k = 0; k < groups; ++k) s += sums[k * a.lanes + l][i % 8];
+        a.partial[(int64_t)blockIdx.x * a.N + col] = s;
+    }
+}
+
+// db: 32 columns a CTA, eight warps share the parts.
+template <class T> __global__ void __launch_bounds__(256) k_linear_db(const float* __restrict__ partial, int parts, int32_t N, T* __restrict__ db)
+{
+    __shared__ double sums[8][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
+    double s = 0.0;
+    if (col < N)
+        for (int i = warp; i < parts; i += 8) s += __ldg(partial + (int64_t)i * N + col);
+    sums[warp][lane] = s;
+    __syncthreads();
+    if (warp || col >= N) return;
+    for (int w = 1; w < 8; ++w) s += sums[w][lane];
+    db[col] = Pair<T>::round((float)s);
+}
+
+// The CTAs over the rows: enough to fill the device twice over, and at least 16 rows a thread.
+int dz_lanes(int32_t N)
+{
+    int lanes = 1;
+    while (lanes < 32 && lanes * 8 < N) lanes *= 2;
+    return lanes;
+}
+int dz_ctas(int64_t M, int32_t N)
+{
+    const int lanes = dz_lanes(N), columns = (N + lanes * 8 - 1) / (lanes * 8);
+    const int64_t most = std::max(1, 148 * 8 / columns), rows = kDzThreads / lanes * 16;
+    return (int)std::min<int64_t>(most, (M + rows - 1) / rows);
+}
+
+// ---- few rows -----------------------------------------------------------------------------------------------------------------
+// 16 bits: y^T by mma.m16n8k16 with x along the 16 rows.  The order in which k goes through the sum is free as long as both operands agree on it, so a thread
+// takes four neighbouring k's of both: 8 bytes of a row of x, and four rows (w [K x N], four neighbouring columns each, which are then columns of four
+// MMAs) or 8 bytes of a row (w [N x K]) of w.  A CTA makes 32 columns; its warps share K, and their sums meet in shared memory.
+constexpr int kFewRows = 16, kFewWarps = 8, kFewCols = 32;
+
+template <class T> __device__ __forceinline__ uint2 load4(const T* p, int n, bool whole)
+{
+    if (whole && n >= 4) return __ldg(reinterpret_cast<const uint2*>(p));
+    unsigned short v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = e < n ? __ldg(reinterpret_cast<const unsigned short*>(p) + e) : (unsigned short)0;
+    return make_uint2(v[0] | (uint32_t)v[1] << 16, v[2] | (uint32_t)v[3] << 16);
+}
+template <class T> __device__ __forceinline__ void mma16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1)
+{
+    if constexpr (Pair<T>::kFormat == 1)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+struct FewArgs {
+    const void *x, *w, *bias, *residual;
+    void *y, *z;
+    uint32_t* bits;
+    int64_t ldx, ldw, ldr, ldy, ldz, ldbits, M;
+    int32_t N, K, act, whole_x, whole_w;
+};
+
+// One element of the result, from its sum.  Lanes of a warp hold the 32 columns of a row from a multiple of 32 on.
+template <class T> __device__ __forceinline__ void finish(const FewArgs& a, int64_t m, int col, float z)
+{
+    const bool live = col < a.N;
+    if (live && a.bias) z += Pair<T>::one(static_cast<const T*>(a.bias)[col]);
+    if (a.bits) {
+        const uint32_t word = __ballot_sync(0xffffffffu, live && !(z <= 0.f));
+        if (threadIdx.x % 32 == 0) a.bits[m * a.ldbits + col / 32] = word;
+    }
+    if (!live) return;
+    if (a.z) static_cast<T*>(a.z)[m * a.ldz + col] = Pair<T>::round(z);
+    float y = a.act == DG_ACT_RELU ? act_value<DG_ACT_RELU>(z) : a.act == DG_ACT_GELU ? act_value<DG_ACT_GELU>(z) : a.act == DG_ACT_SILU ? act_value<DG_ACT_SILU>(z) : z;
+    if (a.residual) y += Pair<T>::one(static_cast<const T*>(a.residual)[m * a.ldr + col]);
+    static_cast<T*>(a.y)[m * a.ldy + col] = Pair<T>::round(y);
+}
+
+template <class T, bool OUT_IN>
+__global__ void __launch_bounds__(32 * kFewWarps) k_few_rows16(const FewArgs a)
+{
+    __shared__ float sums[kFewWarps][kFewRows][kFewCols + 1];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int64_t m0 = (int64_t)blockIdx.y * kFewRows;
+    const int n0 = blockIdx.x * kFewCols;
+    const T* x = static_cast<const T*>(a.x);
+    const T* w = static_cast<const T*>(a.w);
+    const bool row0 = m0 + g < a.M, row1 = m0 + g + 8 < a.M;
+    float acc[4][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
+    const int steps = (a.K + 15) / 16;
+#pragma unroll 4
+    for (int step = warp; step < steps; step += kFewWarps) {
+        const int k = step * 16 + 4 * t, nk = a.K - k;
+        const uint2 x0 = row0 && nk > 0 ? load4(x + (m0 + g) * a.ldx + k, nk, a.whole_x) : make_uint2(0u, 0u);
+        const uint2 x1 = row1 && nk > 0 ? load4(x + (m0 + g + 8) * a.ldx + k, nk, a.whole_x) : make_uint2(0u, 0u);
+        const uint32_t xa[4] = {x0.x, x1.x, x0.y, x1.y};
+        if constexpr (OUT_IN) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int n = n0 + 8 * j + g;
+                const uint2 b = n < a.N && nk > 0 ? load4(w + n * a.ldw + k, nk, a.whole_w) : make_uint2(0u, 0u);
+                mma16<T>(acc[j], xa, b.x, b.y);
+            }
+        } else {
+            const int n = n0 + 4 * g, nn = a.N - n;
+            uint2 b[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) b[e] = e < nk && nn > 0 ? load4(w + (int64_t)(k + e) * a.ldw + n, nn, a.whole_w) : make_uint2(0u, 0u);
+            mma16<T>(acc[0], xa, __byte_perm(b[0].x, b[1].x, 0x5410), __byte_perm(b[2].x, b[3].x, 0x5410));
+            mma16<T>(acc[1], xa, __byte_perm(b[0].x, b[1].x, 0x7632), __byte_perm(b[2].x, b[3].x, 0x7632));
+            mma16<T>(acc[2], xa, __byte_perm(b[0].y, b[1].y, 0x5410), __byte_perm(b[2].y, b[3].y, 0x5410));
+            mma16<T>(acc[3], xa, __byte_perm(b[0].y, b[1].y, 0x7632), __byte_perm(b[2].y, b[3].y, 0x7632));
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int in_mma = 2 * t + (e & 1), col = OUT_IN ? 8 * j + in_mma : 4 * in_mma + j;
+            sums[warp][g + (e & 2) * 4][col] = acc[j][e];
+        }
+    __syncthreads();
+    for (int m = warp; m < kFewRows && m0 + m < a.M; m += kFewWarps) {
+        float z = 0.f;
+#pragma unroll
+        for (int s = 0; s < kFewWarps; ++s) z += sums[s][m][lane];
+        finish<T>(a, m0 + m, n0 + lane, z);
+    }
+}
+
+// fp32: a lane owns a column of w [K x N] (its warp's share of K), or a warp a row of w [N x K] with K along the lanes; x is read through the L1.
+constexpr int kFewRows32 = 4, kFewWarps32 = 16;
+template <bool OUT_IN> __global__ void __launch_bounds__(32 * kFewWarps32) k_few_rows32(const FewArgs a)
+{
+    __shared__ float sums[kFewWarps32][kFewRows32][33];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t m0 = (int64_t)blockIdx.y * kFewRows32;
+    const int rows = (int)min((int64_t)kFewRows32, a.M - m0), n0 = blockIdx.x * 32;
+    const float* x = static_cast<const float*>(a.x) + m0 * a.ldx;
+    const float* w = static_cast<const float*>(a.w);
+    if constexpr (!OUT_IN) {
+        float acc[kFewRows32] = {};
+        const int col = min(n0 + lane, a.N - 1);
+#pragma unroll 8
+        for (int k = warp; k < a.K; k += kFewWarps32) {
+            const float v = __ldg(w + k * a.ldw + col);
+#pragma unroll
+            for (int m = 0; m < kFewRows32; ++m) acc[m] = fmaf(m < rows ? __ldg(x + m * a.ldx + k) : 0.f, v, acc[m]);
+        }
+#pragma unroll
+        for (int m = 0; m < kFewRows32; ++m) sums[warp][m][lane] = acc[m];
+        __syncthreads();
+        if (warp >= rows) return;
+        float z = 0.f;
+#pragma unroll
+        for (int s = 0; s < kFewWarps32; ++s) z += sums[s][warp][lane];
+        finish<float>(a, m0 + warp, n0 + lane, z);
+    } else {
+        float acc[2][kFewRows32] = {};                            // columns n0 + 2 warp, n0 + 2 warp + 1
+        const int64_t c0 = min(n0 + 2 * warp, a.N - 1), c1 = min(n0 + 2 * warp + 1, a.N - 1);
+#pragma unroll 4
+        for (int k = lane; k < a.K; k += 32) {
+            const float v0 = __ldg(w + c0 * a.ldw + k), v1 = __ldg(w + c1 * a.ldw + k);
+#pragma unroll
+            for (int m = 0; m < kFewRows32; ++m) {
+                const float u = m < rows ? __ldg(x + m * a.ldx + k) : 0.f;
+                acc[0][m] = fmaf(u, v0, acc[0][m]);
+                acc[1][m] = fmaf(u, v1, acc[1][m]);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int m = 0; m < kFewRows32; ++m) {
+                float v = acc[c][m];
+                for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+                if (lane == 0) sums[0][m][2 * warp + c] = v;
+            }
+        __syncthreads();
+        if (warp >= rows) return;
+        finish<float>(a, m0 + warp, n0 + lane, sums[0][warp][lane]);
+    }
+}
+
+// ---- rows of whole 16-byte pieces ------------------------------------------------------------------------------------------------
+__global__ void __launch_bounds__(256) k_pad_rows16(const unsigned short* __restrict__ src, int64_t ld_src, int64_t n, int32_t cols, uint4* __restrict__ dst, int32_t pieces)
+{
+    const int64_t total = n * pieces, stride = (int64_t)gridDim.x * blockDim.x;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += stride) {
+        const int64_t row = i / pieces;
+        const int c = (int)(i - row * pieces) * 8;
+        const unsigned short* s = src + row * ld_src + c;
+        uint32_t v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t low = c + 2 * e < cols ? __ldcs(s + 2 * e) : 0, high = c + 2 * e + 1 < cols ? __ldcs(s + 2 * e + 1) : 0;
+            v[e] = low | high << 16;
+        }
+        dst[i] = make_uint4(v[0], v[1], v[2], v[3]);
+    }
+}
+
+// ---- host side ---------------------------------------------------------------------------------------------------------------------
+bool on_rows(const void* p, int64_t ld, int item) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld * item % 16 == 0; }
+
+// [rows x cols] of 16-bit elements, row-major, boxes of 64 columns x box_rows rows with the 128B swizzle, out-of-range elements read as zero.
+int make_map16(CUtensorMap* map, const void* ptr, int32_t type, int64_t rows, int64_t cols, int64_t ld, int box_rows)
+{
+    EncodeTiledFn fn = encode_tiled();
+    if (!fn) return DG_ERR_UNSUPPORTED;
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+    const cuuint32_t elem[2] = {1, 1};
+    const CUresult r = fn(map, type == DG_BFLOAT16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(ptr), dims, strides, box,
+                          elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? DG_OK : DG_ERR_UNSUPPORTED;
+}
+
+template <class T, int ACT> int launch_pair(const CUtensorMap* maps, const LinearPairArgs& a, unsigned ctas, size_t smem, cudaStream_t stream)
+{
+    static std::atomic<bool> granted[64];
+    const int rc = allow_smem((const void*)k_linear_pair<T, ACT>, granted);
+    if (rc) return rc;
+    k_linear_pair<T, ACT><<<ctas, kThreadsPair, smem, stream>>>(maps[0], maps[1], maps[2], maps[3], maps[4], a);
+    return (int)cudaGetLastError();
+}
+template <class T> int launch_pair(int act, const CUtensorMap* maps, const LinearPairArgs& a, unsigned ctas, size_t smem, cudaStream_t stream)
+{
+    switch (act) {
+        case DG_ACT_RELU: return launch_pair<T, DG_ACT_RELU>(maps, a, ctas, smem, stream);
+        case DG_ACT_GELU: return launch_pair<T, DG_ACT_GELU>(maps, a, ctas, smem, stream);
+        case DG_ACT_SILU: return launch_pair<T, DG_ACT_SILU>(maps, a, ctas, smem, stream);
+        default: return launch_pair<T, DG_ACT_NONE>(maps, a, ctas, smem, stream);
+    }
+}
+
+// The columns of a tile: as many as the result has, up to 256, in fewer while that leaves pairs without a tile.
+int tile_columns(int64_t m_tiles, int32_t N, int pairs)
+{
+    if (N <= 64) return (N + 31) / 32 * 32;
+    int cols = std::min(256, (N + 63) / 64 * 64);
+    while (cols > 64 && m_tiles * ((N + cols - 1) / cols) < pairs) cols -= 64;
+    return cols;
+}
+
+int linear16(const dg_linear_args* g, cudaStream_t stream)
+{
+    if (!on_rows(g->x, g->ldx, 2) || !on_rows(g->w, g->ldw, 2) || !on_rows(g->y, g->ldy, 2) || (g->residual && !on_rows(g->residual, g->ldr, 2)) ||
+        (g->z && !on_rows(g->z, g->ldz, 2)))
+        return DG_ERR_UNSUPPORTED;
+    LinearPairArgs a{};
+    const int sms = sm_count();
+    if (sms < 2) return DG_ERR_STATE;
+    a.bias = g->bias, a.bits = g->bits, a.ldbits = g->ldbits, a.M = g->M, a.N = g->N, a.K = g->K;
+    const int64_t m_tiles = (g->M + 2 * BM - 1) / (2 * BM);
+    a.n_tile = tile_columns(m_tiles, g->N, sms / 2);
+    a.n_panels = (g->N + a.n_tile - 1) / a.n_tile;
+    if (m_tiles * a.n_panels >= (int64_t)1 << 30) return DG_ERR_UNSUPPORTED;
+    a.tiles = (int)(m_tiles * a.n_panels);
+    a.b_boxes = g->out_in ? 0 : (a.n_tile / 2 + 63) / 64;
+    a.residual = g->residual != nullptr, a.save_z = g->z != nullptr, a.whole_bias = (reinterpret_cast<uintptr_t>(g->bias) & 15) == 0;
+    a.status = dg_status_word();
+    if (!a.status) return DG_ERR_STATE;
+    CUtensorMap maps[5];
+    int rc;
+    if ((rc = make_map16(&maps[0], g->x, g->type, g->M, g->K, g->ldx, BM)) ||
+        (rc = g->out_in ? make_map16(&maps[1], g->w, g->type, g->N, g->K, g->ldw, a.n_tile / 2) : make_map16(&maps[1], g->w, g->type, g->K, g->N, g->ldw, BK)) ||
+        (rc = make_map16(&maps[2], g->y, g->type, g->M, g->N, g->ldy, 32)))
+        return rc;
+    maps[3] = maps[4] = maps[2];
+    if (g->residual && (rc = make_map16(&maps[3], g->residual, g->type, g->M, g->N, g->ldr, 32))) return rc;
+    if (g->z && (rc = make_map16(&maps[4], g->z, g->type, g->M, g->N, g->ldz, 32))) return rc;
+    const size_t stage = kABytes + (a.b_boxes ? a.b_boxes * BK * 128 : a.n_tile / 2 * 128);
+    const size_t rest = (size_t)kEpilogueWarps * (a.save_z ? 3 : 2) * kPieceBytes + kBarBytes + 1024;
+    a.stages = (int)std::min<size_t>(kMaxStages, (227 * 1024 - rest) / stage);
+    const unsigned ctas = 2u * (unsigned)std::min(a.tiles, sms / 2);
+    const size_t smem = a.stages * stage + rest;
+    return g->type == DG_BFLOAT16 ? launch_pair<__nv_bfloat16>(g->act, maps, a, ctas, smem, stream) : launch_pair<__half>(g->act, maps, a, ctas, smem, stream);
+}
+
+int linear_few(const dg_linear_args* g, cudaStream_t stream)
+{
+    FewArgs a{g->x, g->w, g->bias, g->residual, g->y, g->z, g->bits, g->ldx, g->ldw, g->ldr, g->ldy, g->ldz, g->ldbits, g->M, g->N, g->K, g->act, 0, 0};
+    if (g->type == DG_FLOAT32) {
+        const dim3 grid((unsigned)((g->N + 31) / 32), (unsigned)((g->M + kFewRows32 - 1) / kFewRows32));
+        if (g->out_in) k_few_rows32<true><<<grid, 32 * kFewWarps32, 0, stream>>>(a);
+        else k_few_rows32<false><<<grid, 32 * kFewWarps32, 0, stream>>>(a);
+        return (int)cudaGetLastError();
+    }
+    auto on_8 = [](const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 7) == 0 && ld % 4 == 0; };
+    a.whole_x = on_8(g->x, g->ldx), a.whole_w = on_8(g->w, g->ldw);
+    const dim3 grid((unsigned)((g->N + kFewCols - 1) / kFewCols), (unsigned)((g->M + kFewRows - 1) / kFewRows));
+    auto run = [&](auto value) {
+        using T = decltype(value);
+        if (g->out_in) k_few_rows16<T, true><<<grid, 32 * kFewWarps, 0, stream>>>(a);
+        else k_few_rows16<T, false><<<grid, 32 * kFewWarps, 0, stream>>>(a);
+    };
+    if (g->type == DG_BFLOAT16) run(__nv_bfloat16{});
+    else run(__half{});
+    return (int)cudaGetLastError();
+}
+
+bool aligned(const void* p, int item) { return reinterpret_cast<uintptr_t>(p) % item == 0; }
+
+// Ranges of rows: a CTA for every range and panel, as many as the device has, at least four stages each.
+struct DwShape {
+    int32_t p_panels, q_panels, p_store, q_store, ranges;
+    int64_t rows_per_range, floats;
+};
+DwShape dw_shape(int64_t M, int32_t N, int32_t K)
+{
+    DwShape s{};
+    s.p_panels = (K + 255) / 256, s.q_panels = (N + 255) / 256;
+    s.p_store = (std::min(K, 256) + 15) / 16 * 16, s.q_store = (std::min(N, 256) + 15) / 16 * 16;
+    const int64_t panels = (int64_t)s.p_panels * s.q_panels, slabs = (M + kDwRows - 1) / kDwRows;
+    const int64_t ranges = std::max<int64_t>(1, std::min<int64_t>(148 / panels, slabs / 4));
+    s.rows_per_range = (slabs + ranges - 1) / ranges * kDwRows;
+    s.ranges = (int)((M + s.rows_per_range - 1) / s.rows_per_range);
+    s.floats = s.ranges * panels * s.p_store * s.q_store;
+    return s;
+}
+
+}  // namespace
+
+extern "C" int64_t dg_linear_few(int32_t, int32_t, int32_t type) { return type == DG_FLOAT32 ? 16 : 32; }
+
+extern "C" int dg_linear(const dg_linear_args* g, void* stream)
+{
+    if (!g || !g->x || !g->w || !g->y) return DG_ERR_NULL;
+    if (g->M < 0 || g->M >= (int64_t)1 << 31 || g->N < 1 || g->K < 1 || g->type < 0 || g->type > 2 || g->act < 0 || g->act > 3) return DG_ERR_DIMS;
+    if (g->ldx < g->K || g->ldw < (g->out_in ? g->K : g->N) || g->ldy < g->N || (g->residual && g->ldr < g->N) || (g->z && g->ldz < g->N)) return DG_ERR_DIMS;
+    if (g->bits && (g->act != DG_ACT_RELU || g->ldbits % 2 || g->ldbits * 32 < g->N || !aligned(g->bits, 8))) return DG_ERR_DIMS;
+    const int item = g->type == DG_FLOAT32 ? 4 : 2;
+    if (!aligned(g->x, item) || !aligned(g->w, item) || !aligned(g->y, item) || !aligned(g->bias, item) || !aligned(g->residual, item) || !aligned(g->z, item)) return DG_ERR_DIMS;
+    if (g->M == 0) return DG_OK;
+    if (g->M <= dg_linear_few(g->N, g->K, g->type)) return linear_few(g, (cudaStream_t)stream);
+    return g->type == DG_FLOAT32 ? dg_dense_linear(g, (cudaStream_t)stream) : linear16(g, (cudaStream_t)stream);
+}
+
+extern "C" int64_t dg_linear_dz_scratch(int64_t M, int32_t N) { return M < 1 || N < 1 ? 0 : (int64_t)dz_ctas(M, N) * N; }
+
+extern "C" int dg_linear_dz(const void* dy, int64_t lddy, const void* z, int64_t ldz, const uint32_t* bits, int64_t ldbits, int32_t act, void* dz, int64_t lddz,
+                            void* db, int64_t M, int32_t N, int32_t type, float* scratch, void* stream)
+{
+    if (!dy || (!dz && !db) || (db && !scratch)) return DG_ERR_NULL;
+    if (M < 1 || N < 1 || type < 0 || type > 2 || act < 0 || act > 3 || lddy < N || (dz && lddz < N)) return DG_ERR_DIMS;
+    if (act == DG_ACT_RELU ? !bits || ldbits * 32 < N : act != DG_ACT_NONE && (!z || ldz < N)) return DG_ERR_NULL;
+    const int item = type == DG_FLOAT32 ? 4 : 2;
+    if (!aligned(dy, item) || !aligned(z, item) || !aligned(dz, item) || !aligned(db, item)) return DG_ERR_DIMS;
+    LinearDzArgs a{};
+    a.lddy = lddy, a.ldz = ldz, a.ldbits = ldbits, a.lddz = lddz, a.M = M, a.N = N, a.bits = bits, a.partial = db ? scratch : nullptr;
+    a.lanes = dz_lanes(N);
+    a.whole_dy = on_rows(dy, lddy, item), a.whole_z = on_rows(z, ldz, item), a.whole_dz = on_rows(dz, lddz, item);
+    const dim3 grid((unsigned)dz_ctas(M, N), (unsigned)((N + a.lanes * 8 - 1) / (a.lanes * 8)));
+    cudaStream_t s = (cudaStream_t)stream;
+    auto run = [&](auto value) {
+        using T = decltype(value);
+        const T *from = static_cast<const T*>(dy), *pre = static_cast<const T*>(z);
+        T* to = static_cast<T*>(dz);
+        switch (act) {
+            case DG_ACT_RELU: k_linear_dz<T, DG_ACT_RELU><<<grid, kDzThreads, 0, s>>>(from, pre, to, a); break;
+            case DG_ACT_GELU: k_linear_dz<T, DG_ACT_GELU><<<grid, kDzThreads, 0, s>>>(from, pre, to, a); break;
+            case DG_ACT_SILU: k_linear_dz<T, DG_ACT_SILU><<<grid, kDzThreads, 0, s>>>(from, pre, to, a); break;
+            default: k_linear_dz<T, DG_ACT_NONE><<<grid, kDzThreads, 0, s>>>(from, pre, to, a);
+        }
+        if (db) k_linear_db<T><<<(unsigned)((N + 31) / 32), 256, 0, s>>>(scratch, (int)grid.x, N, static_cast<T*>(db));
+    };
+    if (type == DG_FLOAT32) run(float{});
+    else if (type == DG_BFLOAT16) run(__nv_bfloat16{});
+    else run(__half{});
+    return (int)cudaGetLastError();
+}
+
+extern "C" int64_t dg_linear_dw_scratch(int64_t M, int32_t N, int32_t K) { return M < 1 || N < 1 || K < 1 ? 0 : dw_shape(M, N, K).floats; }
+
+extern "C" int dg_linear_dw(const void* x, int64_t ldx, const void* dz, int64_t lddz, void* dw, int64_t row_stride, int64_t col_stride, int64_t M, int32_t N, int32_t K,
+                            int32_t type, float* scratch, int64_t scratch_floats, void* stream)
+{
+    if (!x || !dz || !dw || !scratch) return DG_ERR_NULL;
+    if (M < 1 || M >= (int64_t)1 << 31 || N < 1 || K < 1 || ldx < K || lddz < N || (type != DG_BFLOAT16 && type != DG_FLOAT16) || !aligned(dw, 2) || !aligned(scratch, 16))
+        return DG_ERR_DIMS;
+    if (!on_rows(x, ldx, 2) || !on_rows(dz, lddz, 2)) return DG_ERR_UNSUPPORTED;
+    const DwShape shape = dw_shape(M, N, K);
+    if (scratch_floats < shape.floats) return DG_ERR_SCRATCH;
+    LinearDwArgs a{};
+    a.partial = reinterpret_cast<float4*>(scratch);
+    a.M = M, a.rows_per_range = shape.rows_per_range, a.p_cols = K, a.q_cols = N;
+    a.p_panels = shape.p_panels, a.q_panels = shape.q_panels, a.p_store = shape.p_store, a.q_store = shape.q_store;
+    a.p_boxes = (std::min(K, 256) + 63) / 64, a.q_boxes = (std::min(N, 256) + 63) / 64;
+    if (K > 64) a.p_boxes = (a.p_boxes + 1) / 2 * 2;              // an MMA reads 128 columns; what lies beyond x's reaches rows that are not stored
+    a.status = dg_status_word();
+    if (!a.status) return DG_ERR_STATE;
+    CUtensorMap tmP, tmQ;
+    int rc;
+    if ((rc = make_map16(&tmP, x, type, M, K, ldx, kDwRows)) || (rc = make_map16(&tmQ, dz, type, M, N, lddz, kDwRows))) return rc;
+    const size_t stage = (size_t)(a.p_boxes + a.q_boxes) * kDwBox;
+    a.stages = (int)std::min<size_t>(kDwMaxStages, (227 * 1024 - kDwBarBytes - 1024) / stage);
+    const size_t smem = a.stages * stage + kDwBarBytes + 1024;
+    const unsigned ctas = (unsigned)(shape.ranges * shape.p_panels * shape.q_panels);
+    const int64_t slots = (int64_t)shape.p_panels * shape.q_panels * (shape.p_store * shape.q_store / 4);
+    auto run = [&](auto value) {
+        using T = decltype(value);
+        static std::atomic<bool> granted[64];
+        const int code = allow_smem((const void*)k_linear_dw<T>, granted);
+        if (code) return code;
+        k_linear_dw<T><<<ctas, kDwThreads, smem, (cudaStream_t)stream>>>(tmP, tmQ, a);
+        k_linear_dw_reduce<T><<<(unsigned)((slots + 255) / 256), 256, 0, (cudaStream_t)stream>>>(a.partial, shape.ranges, a.p_panels, a.q_panels, a.p_store, a.q_store, K, N,
+                                                                                              static_cast<T*>(dw), row_stride, col_stride);
+        return (int)cudaGetLastError();
+    };
+    return type == DG_BFLOAT16 ? run(__nv_bfloat16{}) : run(__half{});
+}
+
+extern "C" int dg_pad_rows16(const void* src, int64_t ld_src, int64_t n, int32_t cols, void* dst, int64_t ld_dst, void* stream)
+{
+    if (n < 0 || cols < 0 || ld_src < cols || ld_dst < cols || ld_dst % 8 || ld_dst >= ((int64_t)1 << 31)) return DG_ERR_DIMS;
+    if (n == 0 || ld_dst == 0) return DG_OK;
+    if (!src || !dst) return DG_ERR_NULL;
+    if (!aligned(src, 2) || !aligned(dst, 16)) return DG_ERR_DIMS;
+    const int64_t blocks = (n * (ld_dst / 8) + 255) / 256;
+    k_pad_rows16<<<(unsigned)std::min<int64_t>(blocks, 148 * 32), 256, 0, (cudaStream_t)stream>>>(static_cast<const unsigned short*>(src), ld_src, n, cols,
+                                                                                                static_cast<uint4*>(dst), (int32_t)(ld_dst / 8));
+    return (int)cudaGetLastError();
+}

@@ -392,15 +392,6 @@ Tensor row_cross_entropy(const Tensor& x, const Tensor& targets, int64_t count)
     return loss;
 }
 
-// ---- AdamW over all tensors of an optimiser ----------------------------------------------------------------------------------
-// What spmm_cpp.AdamW steps: its parameters and their state, group after group.  A step takes the gradients' addresses anew; whether the optimiser's state
-// is still the one this was made from is asked by identity (same_state), without hashing a parameter.
-struct AdamwEntry {
-    Tensor p, m, v, m_scale, v_scale, step;
-    int64_t place;
-    int32_t group;
-};
-
 int32_t type_of(const Tensor& t)
 {
     switch (t.scalar_type()) {
@@ -410,6 +401,228 @@ int32_t type_of(const Tensor& t)
         default: return -1;
     }
 }
+
+// ---- linear layer with bias, activation and residual --------------------------------------------------------------------------------
+int64_t item_of(const Tensor& t) { return t.scalar_type() == at::kFloat ? 4 : 2; }
+int64_t pad_row(int64_t w, int64_t item) { return (w * item + 15) / 16 * 16 / item; }
+int64_t ld_of(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : std::max(t.stride(0), t.size(1)); }
+// t itself, or a copy of it, with elements of a row side by side and rows that do not overlap
+Tensor by_rows(const Tensor& t)
+{
+    return (t.size(1) > 1 && t.stride(1) != 1) || (t.size(0) > 1 && t.stride(0) < t.size(1)) ? t.contiguous() : t;
+}
+bool on_rows(const Tensor& t) { return ld_of(t) * item_of(t) % 16 == 0 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
+Tensor whole_rows(int64_t rows, int64_t cols, const Tensor& like)
+{
+    const int64_t width = pad_row(cols, item_of(like));
+    const Tensor t = at::empty({rows, width}, like.options().requires_grad(false));
+    return width == cols ? t : t.narrow(1, 0, cols);
+}
+// by_rows(t), with rows of whole 16-byte pieces
+Tensor to_rows(const Tensor& t, int64_t* launches)
+{
+    const Tensor src = by_rows(t);
+    if (on_rows(src)) return src;
+    const Tensor out = whole_rows(src.size(0), src.size(1), src);
+    check(item_of(src) == 4 ? dg_pad_rows(src.data_ptr<float>(), ld_of(src), src.size(0), (int32_t)src.size(1), out.data_ptr<float>(), out.stride(0), stream_of(src))
+                            : dg_pad_rows16(src.data_ptr(), ld_of(src), src.size(0), (int32_t)src.size(1), out.data_ptr(), out.stride(0), stream_of(src)));
+    ++*launches;
+    return out;
+}
+
+// A weight [K x N] as the matrix that lies in memory: its rows are inputs, or outputs where out_in.
+struct Weight {
+    Tensor t;
+    bool out_in;
+};
+Weight stored(const Tensor& w)
+{
+    const int64_t K = w.size(0), N = w.size(1);
+    const bool in_out = (N == 1 || w.stride(1) == 1) && (K == 1 || w.stride(0) >= N), out_in = (K == 1 || w.stride(0) == 1) && (N == 1 || w.stride(1) >= K);
+    if (out_in && (N == 1 || !in_out)) return {w.t(), true};
+    return {in_out ? w : w.contiguous(), false};
+}
+
+struct LinearNode : public torch::autograd::Node {
+    SavedVariable x_saved, w_saved;       // x and w, to notice that they were changed in place
+    Tensor x, w, splits, z, bits;         // the operands as the product read them; w as it lies in memory
+    int64_t N = 0, K = 0;
+    int32_t act = 0;
+    bool out_in = false;
+
+    std::string name() const override { return "LinearBackward"; }
+    void release_variables() override
+    {
+        x_saved.reset_data(), w_saved.reset_data();
+        x.reset(), w.reset(), splits.reset(), z.reset(), bits.reset();
+    }
+    variable_list apply(variable_list&& grads) override
+    {
+        variable_list out(4);
+        if (!grads[0].defined()) return out;
+        TORCH_CHECK(x.defined(), "Trying to backward through the graph a second time");
+        TORCH_CHECK(!at::GradMode::is_enabled(), "the gradient of linear cannot be differentiated again");
+        x_saved.unpack(), w_saved.unpack();
+        const bool dx = task_should_compute_output(0), dw = task_should_compute_output(1), db = task_should_compute_output(2), dr = task_should_compute_output(3);
+        c10::cuda::CUDAGuard guard(x.device());
+        void* stream = stream_of(x);
+        const int64_t M = x.size(0), item = item_of(x);
+        const int32_t type = type_of(x);
+        const Tensor dy = grads[0].scalar_type() == x.scalar_type() ? grads[0] : grads[0].to(x.scalar_type());
+        if (dr) out[3] = dy;
+        if (M == 0) {
+            if (dx) out[0] = at::empty({M, K}, x.options());
+            if (dw) out[1] = at::zeros({K, N}, x.options());
+            if (db) out[2] = at::zeros({N}, x.options());
+            return out;
+        }
+        int64_t launches = 0;
+        Tensor g = by_rows(dy);
+        if (act != DG_ACT_NONE || db || ((dx || dw) && !on_rows(g))) {
+            const bool make = act != DG_ACT_NONE ? dx || dw || db : (dx || dw) && !on_rows(g);
+            Tensor dz = make && (dx || dw) ? whole_rows(M, N, x) : Tensor(), scratch;
+            if (db) {
+                out[2] = at::empty({N}, x.options());
+                scratch = at::empty({dg_linear_dz_scratch(M, (int32_t)N)}, x.options().dtype(at::kFloat));
+            }
+            if (dz.defined() || db) {
+                check(dg_linear_dz(g.data_ptr(), ld_of(g), z.defined() ? z.data_ptr() : nullptr, z.defined() ? ld_of(z) : 0,
+                                   bits.defined() ? reinterpret_cast<const uint32_t*>(bits.data_ptr<int32_t>()) : nullptr, bits.defined() ? bits.size(1) : 0, act,
+                                   dz.defined() ? dz.data_ptr() : nullptr, dz.defined() ? dz.stride(0) : 0, db ? out[2].data_ptr() : nullptr, M, (int32_t)N, type,
+                                   db ? scratch.data_ptr<float>() : nullptr, stream));
+                launches += db ? 2 : 1;
+            }
+            if (dz.defined()) g = dz;
+        }
+        if (dx) {
+            out[0] = whole_rows(M, K, x);
+            dg_linear_args a{};
+            a.x = g.data_ptr(), a.ldx = ld_of(g), a.w = w.data_ptr(), a.ldw = ld_of(w), a.out_in = !out_in;
+            a.y = out[0].data_ptr(), a.ldy = out[0].stride(0), a.M = M, a.N = (int32_t)K, a.K = (int32_t)N, a.type = type;
+            if (splits.defined()) {
+                a.ldb = pad4(N), a.head = splits.data_ptr<float>(), a.tail = a.head + K * a.ldb;
+            }
+            check(dg_linear(&a, stream));
+            launches += item == 4 ? (K + 255) / 256 : 1;
+        }
+        if (dw) {
+            const Tensor rows = to_rows(x, &launches);
+            const Tensor d = out_in ? at::empty({N, K}, x.options()) : at::empty({K, N}, x.options());
+            if (item == 4) {
+                const Tensor &left = out_in ? g : rows, &right = out_in ? rows : g;
+                const auto [partial, ctas] = tn_scratch(x, d.size(0), d.size(1));
+                check(dg_dense_tn(left.data_ptr<float>(), ld_of(left), right.data_ptr<float>(), ld_of(right), d.data_ptr<float>(), d.size(1), M, (int32_t)d.size(0),
+                                  (int32_t)d.size(1), partial.data_ptr<float>(), partial.numel(), ctas, stream));
+                launches += 2 * ((K + 255) / 256) * ((N + 255) / 256);
+            } else {
+                const Tensor partial = at::empty({dg_linear_dw_scratch(M, (int32_t)N, (int32_t)K)}, x.options().dtype(at::kFloat));
+                check(dg_linear_dw(rows.data_ptr(), ld_of(rows), g.data_ptr(), ld_of(g), d.data_ptr(), out_in ? 1 : N, out_in ? K : 1, M, (int32_t)N, (int32_t)K, type,
+                                   partial.data_ptr<float>(), partial.numel(), stream));
+                launches += 2;
+            }
+            out[1] = out_in ? d.t() : d;
+        }
+        g_launches += launches;
+        return out;
+    }
+};
+
+Tensor linear(const Tensor& x, const Tensor& w, const std::optional<Tensor>& bias, const std::optional<Tensor>& residual, int64_t act)
+{
+    auto refuse = [](const std::string& why) { throw std::runtime_error("linear: " + why); };
+    auto same = [&](const Tensor& t, const char* what) {
+        if (!t.is_cuda()) refuse(std::string(what) + " must be a CUDA tensor: this library has no CPU path");
+        if (t.device() != x.device() || t.scalar_type() != x.scalar_type()) refuse(std::string(what) + " must have the type and device of x");
+    };
+    if (!x.is_cuda()) refuse("x must be a CUDA tensor: this library has no CPU path");
+    if (type_of(x) < 0) refuse("x must be fp32, bf16 or fp16");
+    if (x.dim() != 2 || w.dim() != 2 || x.size(1) != w.size(0)) {
+        std::ostringstream s;
+        s << "x must be [M x K] and weight [K x N], got " << x.sizes() << " and " << w.sizes();
+        refuse(s.str());
+    }
+    same(w, "weight");
+    const int64_t M = x.size(0), K = x.size(1), N = w.size(1);
+    if (K < 1 || N < 1 || K >= (int64_t)1 << 24 || N >= (int64_t)1 << 24 || M >= (int64_t)1 << 31) refuse("sizes out of range");
+    if (bias) {
+        same(*bias, "bias");
+        if (bias->dim() != 1 || bias->size(0) != N) refuse("bias must have one element for every column of weight");
+    }
+    if (residual) {
+        same(*residual, "residual");
+        if (residual->dim() != 2 || residual->size(0) != M || residual->size(1) != N) refuse("residual must have the shape of the result");
+    }
+    const Tensor b = bias.value_or(Tensor()), r = residual.value_or(Tensor());
+    auto wants = [](const Tensor& t) { return t.defined() && t.requires_grad(); };
+    const bool train = at::GradMode::is_enabled() && (wants(x) || wants(w) || wants(b) || wants(r));
+    c10::cuda::CUDAGuard guard(x.device());
+    const int32_t type = type_of(x);
+    Tensor y, x2, splits, z, bits;
+    Weight weight;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        int64_t launches = 0;
+        void* stream = stream_of(x);
+        const bool few = M <= dg_linear_few((int32_t)N, (int32_t)K, type);
+        weight = stored(w);
+        x2 = few ? by_rows(x) : to_rows(x, &launches);
+        if (!few && type != DG_FLOAT32) weight.t = to_rows(weight.t, &launches);
+        y = few ? at::empty({M, N}, x.options().requires_grad(false)) : whole_rows(M, N, x);
+        const bool dz = train && (wants(x) || wants(w) || wants(b));
+        if (dz && (act == DG_ACT_GELU || act == DG_ACT_SILU)) z = few ? at::empty({M, N}, y.options()) : whole_rows(M, N, x);
+        if (dz && act == DG_ACT_RELU) bits = at::empty({M, (N + 63) / 64 * 2}, y.options().dtype(at::kInt));
+        dg_linear_args a{};
+        Tensor split, res;
+        if (!few && type == DG_FLOAT32) {                     // w^T for the product and, where x wants its gradient, w for that: one launch
+            const int64_t forward = 2 * N * pad4(K), backward = train && wants(x) ? 2 * K * pad4(N) : 0;
+            split = at::empty({forward}, y.options());
+            if (backward) splits = at::empty({backward}, y.options());
+            const float* from = weight.t.data_ptr<float>();
+            dg_split_job jobs[2] = {};
+            float* f = split.data_ptr<float>();
+            jobs[0] = {from, ld_of(weight.t), f, f + N * pad4(K), pad4(K), (int32_t)N, (int32_t)K, !weight.out_in, 0};
+            if (backward) {
+                float* h = splits.data_ptr<float>();
+                jobs[1] = {from, ld_of(weight.t), h, h + K * pad4(N), pad4(N), (int32_t)K, (int32_t)N, weight.out_in, 0};
+            }
+            check(dg_dense_split_operands(jobs, backward ? 2 : 1, stream));
+            ++launches;
+            a.head = f, a.tail = f + N * pad4(K), a.ldb = pad4(K);
+        }
+        if (r.defined()) {
+            res = few ? by_rows(r) : to_rows(r, &launches);
+            a.residual = res.data_ptr(), a.ldr = ld_of(res);
+        }
+        const Tensor flat = b.defined() ? b.contiguous() : b;
+        a.x = x2.data_ptr(), a.ldx = ld_of(x2), a.w = weight.t.data_ptr(), a.ldw = ld_of(weight.t), a.out_in = weight.out_in;
+        a.bias = flat.defined() ? flat.data_ptr() : nullptr;
+        a.y = y.data_ptr(), a.ldy = ld_of(y);
+        if (z.defined()) a.z = z.data_ptr(), a.ldz = ld_of(z);
+        if (bits.defined()) a.bits = reinterpret_cast<uint32_t*>(bits.data_ptr<int32_t>()), a.ldbits = bits.size(1);
+        a.M = M, a.N = (int32_t)N, a.K = (int32_t)K, a.type = type, a.act = (int32_t)act;
+        if (M > 0) check(dg_linear(&a, stream));
+        g_launches += launches + (few || type != DG_FLOAT32 ? 1 : (N + 255) / 256);
+    }
+    if (train) {
+        auto node = std::shared_ptr<LinearNode>(new LinearNode(), torch::autograd::deleteNode);
+        node->set_next_edges(torch::autograd::collect_next_edges(x, w, b, r));
+        node->x_saved = SavedVariable(x, false), node->w_saved = SavedVariable(w, false);
+        node->x = x2.detach(), node->w = weight.t.detach();
+        node->splits = splits, node->z = z, node->bits = bits;
+        node->N = N, node->K = K, node->act = (int32_t)act, node->out_in = weight.out_in;
+        torch::autograd::set_history(y, node);
+    }
+    return y;
+}
+
+// ---- AdamW over all tensors of an optimiser ----------------------------------------------------------------------------------
+// What spmm_cpp.AdamW steps: its parameters and their state, group after group.  A step takes the gradients' addresses anew; whether the optimiser's state
+// is still the one this was made from is asked by identity (same_state), without hashing a parameter.
+struct AdamwEntry {
+    Tensor p, m, v, m_scale, v_scale, step;
+    int64_t place;
+    int32_t group;
+};
 
 struct AdamwTable {
     std::vector<AdamwEntry> entries;
@@ -530,6 +743,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
         .def("same_state", &AdamwTable::same_state)
         .def("step", &AdamwTable::step)
         .def_readonly("norm", &AdamwTable::norm);
+    m.def("linear", &linear);
     m.def("spmm", &spmm);
     m.def("gcn", &gcn);
     m.def("readable_padded", &readable_padded);

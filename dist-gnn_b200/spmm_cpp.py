@@ -818,6 +818,26 @@ def dense_tn(x, g):
     return d
 
 
+ACTIVATIONS = {None: 0, 'relu': 1, 'gelu': 2, 'silu': 3}
+
+
+def linear(x, weight, bias=None, residual=None, activation=None):
+    """activation(x @ weight + bias) + residual in one kernel (dg_linear), differentiable in all four: x [M x K], weight [K x N] as the
+    layers here hold it, or the transpose of an [N x K] matrix, bias [N], residual [M x N], all fp32, bf16 or fp16.  activation: None, 'relu', 'gelu'
+    (z Phi(z), not its tanh form) or 'silu'.
+
+    Everything between the operands and the result is in fp32 (fp32 products: three TF32 passes, as dense_nt), rounded once.  For the gradients
+    ReLU keeps a bit an element; GELU and SiLU keep x @ weight + bias in the type of x, and the gradient behind the activation is rounded to
+    that type before it is multiplied.  Operands may have any strides: x, residual and gradients whose rows do not start on 16-byte boundaries are copied
+    once, to padded rows, and the rows of the result and of x's gradient are padded to whole 16-byte pieces (a column slice of a wider buffer)
+    where M exceeds the few rows (fp32 16, else 32) that smaller kernels take."""
+    try:
+        act = ACTIVATIONS[activation]
+    except KeyError:
+        raise ValueError(f"activation must be None, 'relu', 'gelu' or 'silu', got {activation!r}") from None
+    return binding().linear(x, weight, bias, residual, act)
+
+
 def dense_status(reset=False):
     """0, or non-zero if a tensor-core kernel - a dense transform's or a tiled product's - gave up on one of its bounded waits
     since the last reset (its output is then invalid).  Synchronises the current stream.  reset=True clears the word after

@@ -387,6 +387,52 @@ int dg_rows_cross_entropy(const float* x, int64_t ld, int64_t n, int32_t C, cons
 int dg_rows_cross_entropy_grad(const float* x, int64_t ld, int64_t n, int32_t C, const int32_t* target, int64_t count,
                                const float* lse, const float* upstream, float* grad, int64_t ldg, void* stream);
 
+/* ---- linear layer: y = act(x w + b) + r, and its gradients (the reference's layers are torch.mm and F.relu, models/gcn.py:41, :70) ----
+ * Types: fp32 (three TF32 passes, fp32 accuracy), bf16, fp16; every operand of a call is of its type, sums, bias, activation and residual are in fp32,
+ * rounded once.  "On rows" below: the address is a multiple of 16 bytes and so is the row stride.
+ *   x [M x K] ldx, w: [K x N] ldw (out_in == 0) or [N x K] ldw (out_in != 0), bias [N] or NULL, residual [M x N] ldr or NULL, y [M x N] ldy
+ *   z, ldz    NULL, or where z = x w + b goes, rounded to the type, which the gradient of GELU and SiLU reads
+ *   bits      NULL, or with ReLU a bit an element, set where z > 0: ldbits words a row, an even number >= N / 32, 8-byte aligned
+ *   head, tail, ldb   fp32 beyond dg_linear_few rows: w as [N x K], split (dg_dense_split_operands), on rows
+ * dg_linear_few: how many rows, at most, a product of this shape and type takes with the kernels for few rows, which read operands of any stride and
+ * alignment.  Beyond it: 16-bit operands, fp32 x, z and y (16 bits) are on rows (DG_ERR_UNSUPPORTED otherwise); M < 2^31.
+ * The gradient with respect to x is dg_linear with the same w and out_in inverted, N and K exchanged. */
+#define DG_FLOAT32 0
+#define DG_BFLOAT16 1
+#define DG_FLOAT16 2
+#define DG_ACT_NONE 0
+#define DG_ACT_RELU 1
+#define DG_ACT_GELU 2
+#define DG_ACT_SILU 3
+typedef struct dg_linear_args {
+    const void* x;
+    const void* w;
+    const float* head;
+    const float* tail;
+    const void* bias;
+    const void* residual;
+    void* y;
+    void* z;
+    uint32_t* bits;
+    int64_t ldx, ldw, ldb, ldr, ldy, ldz, ldbits;
+    int64_t M;
+    int32_t N, K, type, act, out_in, pad;
+} dg_linear_args;
+int64_t dg_linear_few(int32_t N, int32_t K, int32_t type);
+int dg_linear(const dg_linear_args* args, void* stream);
+/* dz = dy * act'(z) and db = the column sums of dz.  dz == NULL: only db; db == NULL: only dz.  z / bits as dg_linear left them (neither: dz = dy).
+ * scratch: dg_linear_dz_scratch(M, N) floats where db is asked for.  Any strides and alignments; the sums are taken in a fixed order. */
+int64_t dg_linear_dz_scratch(int64_t M, int32_t N);
+int dg_linear_dz(const void* dy, int64_t lddy, const void* z, int64_t ldz, const uint32_t* bits, int64_t ldbits, int32_t act, void* dz, int64_t lddz,
+                 void* db, int64_t M, int32_t N, int32_t type, float* scratch, void* stream);
+/* dw[k * row_stride + n * col_stride] = sum over rows of x[m, k] dz[m, n] for bf16 and fp16 (fp32: dg_dense_tn).  x and dz on rows.  scratch: 16-byte
+ * aligned, dg_linear_dw_scratch floats. */
+int64_t dg_linear_dw_scratch(int64_t M, int32_t N, int32_t K);
+int dg_linear_dw(const void* x, int64_t ldx, const void* dz, int64_t lddz, void* dw, int64_t row_stride, int64_t col_stride, int64_t M, int32_t N, int32_t K,
+                 int32_t type, float* scratch, int64_t scratch_floats, void* stream);
+/* dg_pad_rows for 16-bit elements: ld_dst a multiple of 8. */
+int dg_pad_rows16(const void* src, int64_t ld_src, int64_t n, int32_t cols, void* dst, int64_t ld_dst, void* stream);
+
 /* ---- AdamW over many tensors at once (the reference trains with torch.optim.Adam, light_dist_gnn/dist_train.py:31) ---------------
  * One step of p <- p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps) with the running means m of the gradients
  * and v of their squares, for all tensors of a model in one launch (a launch for every type, and for every 376 tensors).  Arithmetic in fp32; p
@@ -402,9 +448,6 @@ int dg_rows_cross_entropy_grad(const float* x, int64_t ld, int64_t n, int32_t C,
  * dg_grad_norm: result[0] = the 2-norm of all gradients (sums in 64 bits, in a fixed order), result[1] = min(1, max_norm / (norm + 1e-6)); only g, n
  * and type are read.
  * workspace: 16-byte aligned, dg_adamw_workspace bytes, zero before its first use; steps that use one workspace run one after the other. */
-#define DG_FLOAT32 0
-#define DG_BFLOAT16 1
-#define DG_FLOAT16 2
 typedef struct dg_adamw_tensor {
     void* p;
     const void* g;

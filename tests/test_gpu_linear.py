@@ -1,0 +1,278 @@
+"""spmm_cpp.linear - activation(x w + b) + r in one kernel, and its gradients - against float64.  Needs a GPU.
+
+Tolerances.  S = |x| |w| is the sum of the magnitudes that go into an element.  A product's sum in fp32 accumulators that truncate is off by at most one
+step (2^-23) of the running sum for every accumulation, K / 8 of them and fewer, and the fp32 product drops three terms of 2^-22: SUM(K) = (K / 8 + 16) *
+2^-23 * 3 of S.  The result adds half a step of its type.  Behind an activation the slope is at most 1.13.  The gradient rounds z (its slope changes by at
+most 0.8 a unit) and dz to the type before it is multiplied: HALF * (|dz| + 0.8 |z| |dy|) for each, which goes through |w| or |x| like dz itself.
+Inputs that are small whole numbers make all of this exact: then the result is the rounded number itself."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+SHAPES = [(1, 1, 1), (1, 256, 256), (2, 7, 5), (16, 1024, 1024), (17, 64, 64), (31, 100, 47), (32, 33, 130), (33, 8, 8), (100, 602, 41), (127, 256, 16), (128, 128, 48),
+          (129, 100, 256), (255, 48, 300), (256, 256, 256), (257, 300, 512), (1000, 16, 1024), (1500, 1024, 65), (20001, 256, 256), (40000, 64, 10), (38000, 72, 200)]
+
+
+def _acts64(name, z):
+    """(value, slope)"""
+    if name == 'relu':
+        return z.clamp(min=0), (z > 0).double()
+    if name == 'gelu':
+        cdf = 0.5 * torch.erfc(-z * math.sqrt(0.5))
+        return z * cdf, cdf + z * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)
+    if name == 'silu':
+        s = torch.sigmoid(z)
+        return z * s, s * (1 + z * (1 - s))
+    return z, torch.ones_like(z)
+
+
+def _whole(gen, *shape, most=2):
+    return torch.randint(-most, most + 1, shape, device='cuda', generator=gen).float()
+
+
+def _grads(y, dy, *tensors):
+    return torch.autograd.grad(y, [t for t in tensors if t is not None], dy)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('M,K,N', SHAPES)
+@pytest.mark.parametrize('act', [None, 'relu'])
+def test_whole_numbers_are_exact(dtype, M, K, N, act):
+    import spmm_cpp
+    gen = torch.Generator(device='cuda').manual_seed(M + 3 * K + 7 * N)
+    out_in = (M + K) % 2 == 1
+    x = _whole(gen, M, K).to(dtype).requires_grad_()
+    w = _whole(gen, N, K, most=1).to(dtype).t() if out_in else _whole(gen, K, N, most=1).to(dtype)
+    w = w.detach().requires_grad_()
+    b = (_whole(gen, N) + 0.5).to(dtype).requires_grad_()          # no z is zero
+    r = _whole(gen, M, N).to(dtype).requires_grad_()
+    dy = _whole(gen, M, N, most=1).to(dtype)
+    y = spmm_cpp.linear(x, w, b, residual=r, activation=act)
+    z = x.detach().double() @ w.detach().double() + b.detach().double()
+    value, slope = _acts64(act, z)
+    assert y.dtype == dtype and y.shape == (M, N)
+    assert torch.equal(y.detach(), (value + r.detach().double()).to(dtype))
+    dx, dw, db, dr = _grads(y, dy, x, w, b, r)
+    dz = dy.double() * slope
+    assert torch.equal(dx, (dz @ w.detach().double().t()).to(dtype))
+    assert torch.equal(dw, (x.detach().double().t() @ dz).to(dtype)) and dw.shape == w.shape
+    assert torch.equal(db, dz.sum(0).to(dtype)) and torch.equal(dr, dy)
+    with torch.no_grad():
+        assert torch.equal(spmm_cpp.linear(x, w, b, residual=r, activation=act), y)
+        assert torch.equal(spmm_cpp.linear(x, w, activation=act), _acts64(act, z - b.double())[0].to(dtype))
+    assert spmm_cpp.dense_status() == 0
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('M,K,N', SHAPES)
+@pytest.mark.parametrize('act', ['gelu', 'silu'])
+def test_smooth_activations_match_float64(dtype, M, K, N, act):
+    import spmm_cpp
+    gen = torch.Generator(device='cuda').manual_seed(M + 5 * K + 11 * N)
+    x = torch.randn(M, K, device='cuda', generator=gen).to(dtype).requires_grad_()
+    w = (torch.randn(K, N, device='cuda', generator=gen) / K ** 0.5).to(dtype).requires_grad_()
+    b = torch.randn(N, device='cuda', generator=gen).to(dtype).requires_grad_()
+    r = torch.randn(M, N, device='cuda', generator=gen).to(dtype).requires_grad_()
+    dy = torch.randn(M, N, device='cuda', generator=gen).to(dtype)
+    y = spmm_cpp.linear(x, w, b, residual=r, activation=act)
+    got = _grads(y, dy, x, w, b, r)
+    xd, wd, bd, rd, dyd = (t.detach().double() for t in (x, w, b, r, dy))
+    half, sums = HALF[dtype], lambda n: (n / 8 + 16) * 3 * 2.0 ** -23
+    z = xd @ wd + bd
+    value, slope = _acts64(act, z)
+    ez = sums(K) * (xd.abs() @ wd.abs() + bd.abs())
+    want = value + rd
+    small = 2.0 ** -22 * (1 + z.abs())                             # of the activation itself, and of the residual's addition
+    subnormal = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    assert bool(((y.detach().double() - want).abs() <= half * want.abs() + 1.14 * ez + small * (1 + rd.abs()) + subnormal).all())
+    dz = dyd * slope
+    edz = half * (dz.abs() + 0.81 * z.abs() * dyd.abs()) * 1.01 + (ez + 2 * small) * dyd.abs() + subnormal
+    for name, grad, exact, error, terms, count in (('dx', got[0], dz @ wd.t(), edz @ wd.abs().t(), dz.abs() @ wd.abs().t(), N),
+                                                   ('dw', got[1], xd.t() @ dz, xd.abs().t() @ edz, xd.abs().t() @ dz.abs(), min(M, 32768)),
+                                                   ('db', got[2], dz.sum(0), edz.sum(0), dz.abs().sum(0), min(M, 512))):
+        bound = half * exact.abs() + error * 1.01 + sums(count) * terms + subnormal
+        worst = ((grad.double() - exact).abs() / bound.clamp(min=1e-300)).max()
+        assert float(worst) <= 1, f'{name}: {float(worst):.2f} of the bound'
+    assert torch.equal(got[3], dy)
+    again = spmm_cpp.linear(x, w, b, residual=r, activation=act)
+    assert torch.equal(again, y) and all(torch.equal(p, q) for p, q in zip(_grads(again, dy, x, w, b, r), got))
+    assert spmm_cpp.dense_status() == 0
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('M', [5, 700])
+def test_strides_offsets_and_broadcasts(dtype, M):
+    """Operands that are slices, transposes and expansions, every gradient against that of contiguous copies."""
+    import spmm_cpp
+    gen = torch.Generator(device='cuda').manual_seed(M)
+    K, N = 40, 24
+
+    def wide(rows, cols, kind):
+        if kind == 'slice':
+            return _whole(gen, rows, cols + 5).to(dtype)[:, 3:3 + cols]
+        if kind == 'transpose':
+            return _whole(gen, cols, rows).to(dtype).t()
+        if kind == 'rows':
+            return _whole(gen, 2 * rows, cols).to(dtype)[::2]
+        if kind == 'padded':
+            return _whole(gen, rows, cols + 8).to(dtype)[:, :cols]
+        return _whole(gen, 1, cols).to(dtype).expand(rows, cols)
+
+    for kx, kw, kr, kd in (('slice', 'slice', 'slice', 'slice'), ('transpose', 'transpose', 'transpose', 'transpose'), ('rows', 'rows', 'rows', 'rows'),
+                           ('padded', 'padded', 'padded', 'padded'), ('one', 'one', 'one', 'one')):
+        x, w, r, dy = wide(M, K, kx), wide(K, N, kw), wide(M, N, kr), wide(M, N, kd)
+        b = _whole(gen, 2 * N).to(dtype)[::2] + 0.5
+        views = [t.detach().requires_grad_() for t in (x, w, b, r)]
+        plain = [t.detach().clone(memory_format=torch.contiguous_format).requires_grad_() for t in (x, w, b, r)]
+        a = spmm_cpp.linear(views[0], views[1], views[2], residual=views[3], activation='relu')
+        c = spmm_cpp.linear(plain[0], plain[1], plain[2], residual=plain[3], activation='relu')
+        assert torch.equal(a, c), (kx, kw)
+        for p, q in zip(_grads(a, dy, *views), _grads(c, dy.contiguous(), *plain)):
+            assert torch.equal(p, q), (kx, kw)
+        wanted = (x.double() @ w.double() + b.double()).clamp(min=0) + r.double()
+        assert torch.equal(c.detach(), wanted.to(dtype))
+    # a broadcast input's gradient is summed by autograd
+    row = torch.ones(1, K, device='cuda', dtype=dtype, requires_grad=True)
+    w = _whole(gen, K, N).to(dtype)
+    spmm_cpp.linear(row.expand(M, K), w).sum().backward()
+    assert torch.equal(row.grad, (w.double().sum(1) * M).to(dtype)[None]) or dtype != torch.float32
+
+
+def test_only_what_is_asked_for():
+    import spmm_cpp
+    x, w, b, r = (torch.randn(s, device='cuda') for s in ((300, 20), (20, 30), (30,), (300, 30)))
+    for asked in range(1, 16):
+        tensors = [t.clone().requires_grad_(bool(asked >> i & 1)) for i, t in enumerate((x, w, b, r))]
+        y = spmm_cpp.linear(tensors[0], tensors[1], tensors[2], residual=tensors[3], activation='gelu')
+        y.backward(torch.ones_like(y))
+        for i, t in enumerate(tensors):
+            assert (t.grad is not None) == bool(asked >> i & 1)
+    assert not spmm_cpp.linear(x, w).requires_grad
+
+
+def test_gradients_against_differences():
+    """Central differences of f = sum(c y) along random directions in fp32: truncation h^2 / 6 of third derivatives (at most 2 a unit of z) and the
+    rounding of y, 2^-22 (|y| + S) / 2h for each, added as if they were independent, eight deviations."""
+    import spmm_cpp
+    gen = torch.Generator(device='cuda').manual_seed(2)
+    M, K, N, h = 200, 32, 24, 2.0 ** -6
+    base = [torch.randn(M, K, device='cuda', generator=gen), torch.randn(K, N, device='cuda', generator=gen) / K ** 0.5, torch.randn(N, device='cuda', generator=gen),
+            torch.randn(M, N, device='cuda', generator=gen)]
+    c = torch.randn(M, N, device='cuda', generator=gen)
+    for act in ('gelu', 'silu'):
+        leaves = [t.clone().requires_grad_() for t in base]
+        y = spmm_cpp.linear(leaves[0], leaves[1], leaves[2], residual=leaves[3], activation=act)
+        grads = _grads(y, c, *leaves)
+        for i, t in enumerate(base):
+            v = torch.randn(t.shape, device='cuda', generator=gen)
+            v /= max(1.0, float(v.norm()) / math.sqrt(M))           # a change of z of order one
+            f = []
+            for sign in (1, -1):
+                moved = [u + sign * h * v if j == i else u for j, u in enumerate(base)]
+                f.append(float((spmm_cpp.linear(moved[0], moved[1], moved[2], residual=moved[3], activation=act).double() * c.double()).sum()))
+            slope = (f[0] - f[1]) / (2 * h)
+            want = float((grads[i].double() * v.double()).sum())
+            moved_z = (v @ base[1] if i == 0 else base[0] @ v if i == 1 else v.expand(M, N)).double().abs() if i < 3 else torch.zeros(M, N, device='cuda', dtype=torch.float64)
+            truncation = float((c.abs().double() * 2 * moved_z ** 3).sum()) * h * h / 6
+            rounding = 8 * float((c.abs() * (y.detach().abs() + 4) * 2.0 ** -22).norm()) / (2 * h)
+            assert abs(slope - want) <= truncation + rounding, (act, i, slope, want)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('M', [8, 500])
+def test_what_is_not_finite_stays_in_its_row(dtype, M):
+    import spmm_cpp
+    for act in (None, 'relu', 'gelu', 'silu'):
+        x, w = torch.ones(M, 64, device='cuda', dtype=dtype), torch.full((64, 40), 0.125, device='cuda', dtype=dtype)
+        x[3, 5], x[6, 7] = float('nan'), float('inf')
+        y = spmm_cpp.linear(x, w, activation=act)
+        assert bool(torch.isnan(y[3]).all()) and not bool(torch.isfinite(y[6]).any())
+        rest = [i for i in range(M) if i not in (3, 6)]
+        assert bool(torch.isfinite(y[rest]).all())
+
+
+def test_rows_behind_the_result_are_left_alone():
+    """The padded rows' columns aside, nothing but the result is written: results of many shapes in one buffer's neighbourhood."""
+    import ctypes
+    import spmm_cpp
+    L = spmm_cpp.lib()
+
+    class Args(ctypes.Structure):
+        _fields_ = [(n, ctypes.c_void_p) for n in ('x', 'w', 'head', 'tail', 'bias', 'residual', 'y', 'z', 'bits')] + \
+                   [(n, ctypes.c_int64) for n in ('ldx', 'ldw', 'ldb', 'ldr', 'ldy', 'ldz', 'ldbits', 'M')] + \
+                   [(n, ctypes.c_int32) for n in ('N', 'K', 'type', 'act', 'out_in', 'pad')]
+
+    for M, K, N in ((5, 16, 40), (300, 64, 40), (129, 8, 200), (1, 8, 8), (511, 128, 264)):
+        x, w = torch.ones(M, K, device='cuda', dtype=torch.bfloat16), torch.ones(K, N, device='cuda', dtype=torch.bfloat16)
+        y = torch.full((M + 2, N + 8), 7.0, device='cuda', dtype=torch.bfloat16)
+        z = y.clone()
+        a = Args(x=x.data_ptr(), w=w.data_ptr(), y=y[1:].data_ptr(), z=z[1:].data_ptr(), ldx=K, ldw=N, ldy=N + 8, ldz=N + 8, M=M, N=N, K=K, type=1, act=2)
+        assert L.dg_linear(ctypes.byref(a), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)) == 0
+        torch.cuda.synchronize()
+        assert bool((z[1:-1, :N] == K).all())
+        for t in (y, z):
+            assert bool((t[0] == 7).all()) and bool((t[-1] == 7).all()) and bool((t[:, N:] == 7).all())
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_captured_and_on_two_streams(dtype):
+    import spmm_cpp
+    gen = torch.Generator(device='cuda').manual_seed(1)
+    x, w, b, r, dy = (_whole(gen, *s).to(dtype) for s in ((900, 64), (64, 72), (72,), (900, 72), (900, 72)))
+    leaves = [t.clone().requires_grad_() for t in (x, w, b, r)]
+
+    def both(ts):
+        y = spmm_cpp.linear(ts[0], ts[1], ts[2], residual=ts[3], activation='silu')
+        return (y.detach(), *_grads(y, dy, *ts))
+
+    want = both(leaves)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):                                             # the same weight on two streams at once
+        with torch.cuda.stream(side):
+            there = both(leaves)
+        here = both(leaves)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(p, q) for p, q in zip(want, there)) and all(torch.equal(p, q) for p, q in zip(want, here))
+    torch.cuda.synchronize()
+    fresh = [t.detach().clone().requires_grad_() for t in leaves]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = both(fresh)
+    with torch.no_grad():
+        fresh[0].copy_(_whole(gen, 900, 64))
+    graph.replay()
+    torch.cuda.synchronize()
+    eager = [t.detach().clone().requires_grad_() for t in fresh]
+    assert all(torch.equal(p, q) for p, q in zip(got, both(eager)))
+
+
+def test_refusals():
+    import spmm_cpp
+    x, w = torch.ones(4, 6, device='cuda'), torch.ones(6, 5, device='cuda')
+    for args, kw in (((x, w.t()), {}), ((x.cpu(), w), {}), ((x, w.cpu()), {}), ((x, w.bfloat16()), {}), ((x.double(), w.double()), {}), ((x[0], w), {}),
+                     ((x, w, torch.ones(6, device='cuda')), {}), ((x, w, torch.ones(5)), {}), ((x, w), dict(residual=torch.ones(1, 5, device='cuda'))),
+                     ((x, w), dict(residual=torch.ones(4, 5, device='cuda').half())), ((x[:, :0], w[:0]), {}), ((x, w[:, :0]), {})):
+        with pytest.raises(RuntimeError, match='linear'):
+            spmm_cpp.linear(*args, **kw)
+    with pytest.raises(ValueError):
+        spmm_cpp.linear(x, w, activation='tanh')
+    y = spmm_cpp.linear(x[:0], w.requires_grad_())
+    assert y.shape == (0, 5)
+    y.sum().backward()
+    assert bool((w.grad == 0).all())
+    y = spmm_cpp.linear(x, w, activation='gelu')
+    with torch.no_grad():
+        w.add_(1)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        y.sum().backward()
+    y = spmm_cpp.linear(x, w, activation='gelu')
+    with pytest.raises(RuntimeError, match='differentiated again'):
+        torch.autograd.grad(y.sum(), w, create_graph=True)
+    y.sum().backward()
+    with pytest.raises(RuntimeError, match='second time'):
+        y.sum().backward()
