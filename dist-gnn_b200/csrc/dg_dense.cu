@@ -47,12 +47,12 @@ struct DenseArgs {
     float* z;                       // x w + b, or nullptr
     uint32_t* bits;                 // a bit an element where that is above zero, or nullptr
     int64_t ldz, ldbits;
-    int32_t act;
 };
+// What a kernel's epilogue does; from kLinear on: the linear layer's, with activation EPI - kLinear.
 constexpr int kPlain = 0, kMasked = 1, kLinear = 2;
 
 // A lane's 32 columns of its row: the bias is added, and where asked the signs are kept.
-__device__ __forceinline__ void add_bias(const DenseArgs& a, uint32_t* r, int c0, int64_t row)
+template <int EPI> __device__ __forceinline__ void add_bias(const DenseArgs& a, uint32_t* r, int c0, int64_t row)
 {
     if (a.bias) {
         if (c0 + 32 <= a.N && (reinterpret_cast<uintptr_t>(a.bias) & 15) == 0) {
@@ -70,16 +70,12 @@ __device__ __forceinline__ void add_bias(const DenseArgs& a, uint32_t* r, int c0
                 if (c0 + j < a.N) r[j] = __float_as_uint(__uint_as_float(r[j]) + __ldg(a.bias + c0 + j));
         }
     }
-    if (a.bits && row < a.M) {
+    if (EPI == kLinear + DG_ACT_RELU && a.bits && row < a.M) {
         uint32_t word = 0;
 #pragma unroll
         for (int j = 0; j < 32; ++j) word |= (__uint_as_float(r[j]) <= 0.f ? 0u : 1u) << j;
         a.bits[row * a.ldbits + c0 / 32] = word;
     }
-}
-__device__ __forceinline__ float activate(int act, float z)
-{
-    return act == DG_ACT_RELU ? act_value<DG_ACT_RELU>(z) : act == DG_ACT_GELU ? act_value<DG_ACT_GELU>(z) : act == DG_ACT_SILU ? act_value<DG_ACT_SILU>(z) : z;
 }
 
 // umma_desc_sw128 for rows of 64 bytes with the 64B swizzle: 8-row groups are 512 bytes apart.
@@ -115,11 +111,11 @@ namespace {
 // registers touch 32 cache lines an instruction (and so do the mask's loads); the piece goes through `stage` in shared memory
 // (32 rows of 36 floats, conflict-free both ways) and leaves as whole 128-byte row pieces, four rows an instruction.
 constexpr int kStagePitch = 36, kStageBytes = 32 * kStagePitch * 4;
-template <bool LINEAR> __device__ __forceinline__ void store_rows(const DenseArgs& a, uint32_t acc, float* stage, int64_t row0, int lane)
+template <int EPI> __device__ __forceinline__ void store_rows(const DenseArgs& a, uint32_t acc, float* stage, int64_t row0, int lane)
 {
     const bool vec = a.ldc % 4 == 0 && (reinterpret_cast<uintptr_t>(a.C) & 15) == 0 &&
                      (!a.mask || (a.ldm % 4 == 0 && (reinterpret_cast<uintptr_t>(a.mask) & 15) == 0)) &&
-                     (!LINEAR || !a.z || (a.ldz % 4 == 0 && (reinterpret_cast<uintptr_t>(a.z) & 15) == 0));
+                     (EPI < kLinear || !a.z || (a.ldz % 4 == 0 && (reinterpret_cast<uintptr_t>(a.z) & 15) == 0));
     const int rows = (int)min((int64_t)32, a.M - row0);
     for (int c0 = 0; c0 < a.n_pad; c0 += 32) {
         const bool pieces = vec && c0 + 32 <= a.N;                // whole 128-byte pieces of every row
@@ -134,7 +130,7 @@ template <bool LINEAR> __device__ __forceinline__ void store_rows(const DenseArg
         tmem_ld16(acc + (uint32_t)c0, r);
         if (c0 + 16 < a.n_pad) tmem_ld16(acc + (uint32_t)c0 + 16, r + 16);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-        if constexpr (LINEAR) add_bias(a, r, c0, row0 + lane);
+        if constexpr (EPI >= kLinear) add_bias<EPI>(a, r, c0, row0 + lane);
         float4* mine = reinterpret_cast<float4*>(stage + lane * kStagePitch);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
@@ -145,9 +141,9 @@ template <bool LINEAR> __device__ __forceinline__ void store_rows(const DenseArg
             for (int i = 0; i < 8; ++i) {
                 if (i * 4 + r4 >= rows) continue;
                 float4 v = *reinterpret_cast<const float4*>(stage + (i * 4 + r4) * kStagePitch + (lane & 7) * 4);
-                if constexpr (LINEAR) {
+                if constexpr (EPI >= kLinear) {
                     if (a.z) __stcs(reinterpret_cast<float4*>(a.z + (row0 + i * 4 + r4) * a.ldz + col4), v);
-                    v = make_float4(activate(a.act, v.x), activate(a.act, v.y), activate(a.act, v.z), activate(a.act, v.w));
+                    v = make_float4(act_value<EPI - kLinear>(v.x), act_value<EPI - kLinear>(v.y), act_value<EPI - kLinear>(v.z), act_value<EPI - kLinear>(v.w));
                     if (a.mask) v = make_float4(v.x + mk[i].x, v.y + mk[i].y, v.z + mk[i].z, v.w + mk[i].w);
                     __stcs(reinterpret_cast<float4*>(a.C + (row0 + i * 4 + r4) * a.ldc + col4), v);
                     continue;
@@ -174,9 +170,9 @@ template <bool LINEAR> __device__ __forceinline__ void store_rows(const DenseArg
                 for (int i = 0; i < 8; ++i) {
                     if (i0 + i >= rows) break;
                     float v = stage[(i0 + i) * kStagePitch + lane];
-                    if constexpr (LINEAR) {
+                    if constexpr (EPI >= kLinear) {
                         if (a.z) a.z[(row0 + i0 + i) * a.ldz + c] = v;
-                        v = activate(a.act, v);
+                        v = act_value<EPI - kLinear>(v);
                         if (a.mask) v += mrow[i];
                         __stcs(a.C + (row0 + i0 + i) * a.ldc + c, v);
                         continue;
@@ -191,7 +187,7 @@ template <bool LINEAR> __device__ __forceinline__ void store_rows(const DenseArg
     }
 }
 
-template <bool LINEAR>
+template <int EPI>
 __global__ void __launch_bounds__(kThreads, 1)
 k_dense_nt(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmBh,
            const __grid_constant__ CUtensorMap tmBt, const DenseArgs a)
@@ -295,7 +291,7 @@ k_dense_nt(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
             const int q = warp & 3;                               // a warp may only read its own quarter of the TMEM lanes
             // every load has landed and every MMA has read its operands: the stages are free for the staging of the rows
             if (m0 + q * 32 < a.M)
-                store_rows<LINEAR>(a, tmem + ((uint32_t)(q * 32) << 16), reinterpret_cast<float*>(gbase + q * kStageBytes), m0 + q * 32, lane);
+                store_rows<EPI>(a, tmem + ((uint32_t)(q * 32) << 16), reinterpret_cast<float*>(gbase + q * kStageBytes), m0 + q * 32, lane);
         }
     }
     if (!ok) atomicExch(a.status, 1);
@@ -491,8 +487,8 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         float4* stage = reinterpret_cast<float4*>(gbase + staging + (warp - 2 - kSplitWarps) * kPieceBytes);
         const bool vec = a.ldc % 4 == 0 && (reinterpret_cast<uintptr_t>(a.C) & 15) == 0 &&
                          (EPI == kPlain || !a.mask || (a.ldm % 4 == 0 && (reinterpret_cast<uintptr_t>(a.mask) & 15) == 0)) &&
-                         (EPI != kLinear || !a.z || (a.ldz % 4 == 0 && (reinterpret_cast<uintptr_t>(a.z) & 15) == 0));
-        const bool side = EPI == kMasked || (EPI == kLinear && a.mask);
+                         (EPI < kLinear || !a.z || (a.ldz % 4 == 0 && (reinterpret_cast<uintptr_t>(a.z) & 15) == 0));
+        const bool side = EPI == kMasked || (EPI >= kLinear && a.mask);
         const int r4 = lane >> 3, piece = lane & 7;
         int lt = 0;
         for (int tile = pair; tile < n_tiles; tile += pairs, ++lt) {
@@ -524,7 +520,7 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                         __syncwarp();
                         if (lane == 0) mbar_arrive_cluster(leader_acc_empty0 + 8 * b);
                     }
-                    if constexpr (EPI == kLinear) add_bias(a, r, c0, row0 + lane);
+                    if constexpr (EPI >= kLinear) add_bias<EPI>(a, r, c0, row0 + lane);
 #pragma unroll
                     for (int j = 0; j < 8; ++j)                   // a lane holds one row: through shared memory, conflict-free both ways
                         stage[lane * 8 + (j ^ (lane & 7))] = make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]), __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3]));
@@ -537,10 +533,10 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                     float* c = a.C + (row0 + r4) * a.ldc + c0 + piece * 4;
 #pragma unroll
                     for (int i = 0; i < 8; ++i, c += 4 * a.ldc) {
-                        if constexpr (EPI == kLinear) {
+                        if constexpr (EPI >= kLinear) {
                             if (i * 4 + r4 >= rows) continue;
                             if (a.z) __stcs(reinterpret_cast<float4*>(a.z + (row0 + i * 4 + r4) * a.ldz + c0 + piece * 4), x[i]);
-                            x[i] = make_float4(activate(a.act, x[i].x), activate(a.act, x[i].y), activate(a.act, x[i].z), activate(a.act, x[i].w));
+                            x[i] = make_float4(act_value<EPI - kLinear>(x[i].x), act_value<EPI - kLinear>(x[i].y), act_value<EPI - kLinear>(x[i].z), act_value<EPI - kLinear>(x[i].w));
                             if (a.mask) x[i] = make_float4(x[i].x + mk[i].x, x[i].y + mk[i].y, x[i].z + mk[i].z, x[i].w + mk[i].w);
                             __stcs(reinterpret_cast<float4*>(c), x[i]);
                             continue;
@@ -567,9 +563,9 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                         for (int i = 0; i < 8; ++i) {
                             if (i0 + i >= rows) break;
                             float x = flat[((i0 + i) * 8 + ((lane >> 2) ^ ((i0 + i) & 7))) * 4 + (lane & 3)];
-                            if constexpr (EPI == kLinear) {
+                            if constexpr (EPI >= kLinear) {
                                 if (a.z) a.z[(row0 + i0 + i) * a.ldz + c0 + lane] = x;
-                                x = activate(a.act, x);
+                                x = act_value<EPI - kLinear>(x);
                                 if (a.mask) x += mrow[i];
                                 __stcs(a.C + (row0 + i0 + i) * a.ldc + c0 + lane, x);
                                 continue;
@@ -673,6 +669,18 @@ bool by_pairs(int64_t M, int n_pad, int K, bool masked, int sms)
     return n_pad > 80 || (tiles > 2 * sms && (!masked || K > 64));
 }
 
+template <class Use> int by_epilogue(int epilogue, Use use)
+{
+    switch (epilogue) {
+        case kMasked: return use(std::integral_constant<int, kMasked>{});
+        case kLinear + DG_ACT_NONE: return use(std::integral_constant<int, kLinear + DG_ACT_NONE>{});
+        case kLinear + DG_ACT_RELU: return use(std::integral_constant<int, kLinear + DG_ACT_RELU>{});
+        case kLinear + DG_ACT_GELU: return use(std::integral_constant<int, kLinear + DG_ACT_GELU>{});
+        case kLinear + DG_ACT_SILU: return use(std::integral_constant<int, kLinear + DG_ACT_SILU>{});
+        default: return use(std::integral_constant<int, kPlain>{});
+    }
+}
+
 // One panel (up to 256 columns) of a product with the epilogue that `a` describes.
 int launch_nt(const float* A, int64_t lda, const float* Bt_head, const float* Bt_tail, int64_t ldb, DenseArgs a, int epilogue, cudaStream_t stream)
 {
@@ -695,8 +703,10 @@ int launch_nt(const float* A, int64_t lda, const float* Bt_head, const float* Bt
             kernel<<<(unsigned)((a.M + BM - 1) / BM), kThreads, smem, stream>>>(tmA, tmBh, tmBt, a);
             return (int)cudaGetLastError();
         };
-        static std::atomic<bool> granted[64], granted_linear[64];
-        return epilogue == kLinear ? run(k_dense_nt<true>, granted_linear) : run(k_dense_nt<false>, granted);
+        return by_epilogue(epilogue, [&](auto e) {
+            static std::atomic<bool> granted[64];
+            return run(k_dense_nt<decltype(e)::value == kMasked ? kPlain : decltype(e)::value>, granted);      // it asks for the mask itself
+        });
     }
     a.n_pad = (a.N + 31) / 32 * 32;                               // both CTAs hold whole groups of 16 of its rows
     if ((rc = make_map(&tmA, A, a.M, a.K, lda, BM, PK)) || (rc = make_map(&tmBh, Bt_head, a.N, a.K, ldb, a.n_pad / 2, PK)) ||
@@ -711,9 +721,10 @@ int launch_nt(const float* A, int64_t lda, const float* Bt_head, const float* Bt
         kernel<<<2u * (unsigned)std::min(n_tiles, sms / 2), kThreadsPair, stages * stage + rest, stream>>>(tmA, tmBh, tmBt, a, n_tiles, stages);
         return (int)cudaGetLastError();
     };
-    static std::atomic<bool> granted[64], granted_masked[64], granted_linear[64];
-    return epilogue == kLinear ? run(k_dense_nt_pair<kLinear>, granted_linear) : epilogue == kMasked ? run(k_dense_nt_pair<kMasked>, granted_masked)
-                                                                                               : run(k_dense_nt_pair<kPlain>, granted);
+    return by_epilogue(epilogue, [&](auto e) {
+        static std::atomic<bool> granted[64];
+        return run(k_dense_nt_pair<decltype(e)::value>, granted);
+    });
 }
 
 }  // namespace
@@ -800,8 +811,7 @@ int dg_dense_linear(const dg_linear_args* g, cudaStream_t stream)
         a.bias = g->bias ? static_cast<const float*>(g->bias) + n0 : nullptr;
         a.z = g->z ? static_cast<float*>(g->z) + n0 : nullptr; a.ldz = g->ldz;
         a.bits = g->bits ? g->bits + n0 / 32 : nullptr; a.ldbits = g->ldbits;
-        a.act = g->act;
-        const int rc = launch_nt(x, g->ldx, g->head + (int64_t)n0 * g->ldb, g->tail + (int64_t)n0 * g->ldb, g->ldb, a, kLinear, stream);
+        const int rc = launch_nt(x, g->ldx, g->head + (int64_t)n0 * g->ldb, g->tail + (int64_t)n0 * g->ldb, g->ldb, a, kLinear + g->act, stream);
         if (rc) return rc;
     }
     return DG_OK;

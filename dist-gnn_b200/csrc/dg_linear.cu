@@ -232,7 +232,7 @@ k_linear_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
             mbar_expect_tx(res0 + 8 * (2 * w + (n & 1)), kPieceBytes);
             tma_load_2d(base + own + (n & 1) * kPieceBytes, &tmR, tile % a.n_panels * a.n_tile + c0, (int)row, res0 + 8 * (2 * w + (n & 1)));
         };
-        int res_uses[2] = {0, 0};
+        uint32_t res_phase = 0;                                   // a bit a buffer
         if (a.residual && lane == 0 && pair < a.tiles && first < a.n_tile) fetch(pair, first, 0);
         for (int tile = pair; tile < a.tiles && ok; tile += pairs, ++lt) {
             const int b = lt & 1, v = lt >> 1;
@@ -267,9 +267,9 @@ k_linear_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
                     }
                 }
                 if (a.residual && live) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(res0 + 8 * (2 * w + s), res_uses[s] & 1));
+                    ok = __all_sync(0xffffffffu, mbar_wait(res0 + 8 * (2 * w + s), res_phase >> s & 1));
                     if (!ok) break;
-                    ++res_uses[s];
+                    res_phase ^= 1u << s;
                 }
                 __syncwarp();
                 if (!live) continue;
@@ -470,25 +470,34 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_linear_dw(const __grid_consta
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
 }
 
-// dw[p, q] = sum of the ranges' partials, in their order.  A thread takes four columns of a row.
+// dw[p, q] = sum of the ranges' partials: a thread takes four columns of a row and an eighth of the ranges, in their order; the eighths are added in theirs.
 template <class T>
 __global__ void __launch_bounds__(256) k_linear_dw_reduce(const float4* __restrict__ partial, int ranges, int32_t p_panels, int32_t q_panels, int32_t p_store,
                                                           int32_t q_store, int32_t p_cols, int32_t q_cols, T* __restrict__ dw, int64_t row_stride, int64_t col_stride)
 {
-    const int panels = p_panels * q_panels, per_panel = q_store / 4 * p_store;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (int64_t)panels * per_panel) return;
-    const int panel = (int)(i / per_panel), in = (int)(i % per_panel);
-    const int p = panel / q_panels * 256 + in % p_store, q = panel % q_panels * 256 + in / p_store * 4;
-    if (p >= p_cols || q >= q_cols) return;
+    __shared__ float4 part[8][32];
+    const int panels = p_panels * q_panels, per_panel = q_store / 4 * p_store, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t i = (int64_t)blockIdx.x * 32 + lane, stride = (int64_t)panels * per_panel;
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    const float4* from = partial + i;
-    const int64_t stride = (int64_t)panels * per_panel;
+    if (i < stride) {
+        const int each = (ranges + 7) / 8, end = min(ranges, (warp + 1) * each);
+        const float4* from = partial + i;
 #pragma unroll 8
-    for (int r = 0; r < ranges; ++r) {
-        const float4 v = __ldcg(from + r * stride);
+        for (int r = warp * each; r < end; ++r) {
+            const float4 v = __ldcg(from + r * stride);
+            sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+        }
+    }
+    part[warp][lane] = sum;
+    __syncthreads();
+    if (warp || i >= stride) return;
+    for (int w = 1; w < 8; ++w) {
+        const float4 v = part[w][lane];
         sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
     }
+    const int panel = (int)(i / per_panel), in = (int)(i % per_panel);
+    const int p = panel / q_panels * 256 + in % p_store, q = panel % q_panels * 256 + in / p_store * 4;
+    if (p >= p_cols) return;
     const float s[4] = {sum.x, sum.y, sum.z, sum.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -499,26 +508,35 @@ __global__ void __launch_bounds__(256) k_linear_dw_reduce(const float4* __restri
 // A thread owns eight neighbouring columns and walks over rows; the lanes of a row read neighbouring pieces.  `lanes` threads a row (a power of two), a
 // CTA takes 8 * lanes columns and every (256 / lanes * gridDim.x)-th row.
 constexpr int kDzThreads = 256;
-template <class T> __device__ __forceinline__ void load8(const T* p, int n, bool whole, float* v)
-{
-    if (whole && n >= 8) {
+// Eight neighbouring elements as they lie in memory.
+template <class T> struct Raw {
+    uint4 v[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T* p)
+    {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+    }
+    __device__ __forceinline__ void load(const T* p, int n)
+    {
+        T* e = reinterpret_cast<T*>(v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = i < n ? p[i] : Pair<T>::round(0.f);
+    }
+    __device__ __forceinline__ void wide(float* to) const
+    {
         if constexpr (sizeof(T) == 4) {
-            const float4 a = __ldcs(reinterpret_cast<const float4*>(p)), b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) to[i] = reinterpret_cast<const float*>(v)[i];
         } else {
-            const uint4 t = __ldcs(reinterpret_cast<const uint4*>(p));
-            const uint32_t u[4] = {t.x, t.y, t.z, t.w};
+            const uint32_t u[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float2 f = Pair<T>::wide(u[e]);
-                v[2 * e] = f.x, v[2 * e + 1] = f.y;
+                to[2 * e] = f.x, to[2 * e + 1] = f.y;
             }
         }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = e < n ? Pair<T>::one(p[e]) : 0.f;
     }
-}
+};
 template <class T> __device__ __forceinline__ void store8(T* p, int n, bool whole, const float* v)
 {
     if (whole && n >= 8) {
@@ -543,7 +561,7 @@ struct LinearDzArgs {
 };
 
 template <class T, int ACT>
-__global__ void __launch_bounds__(kDzThreads) k_linear_dz(const T* __restrict__ dy, const T* __restrict__ z, T* __restrict__ dz, const LinearDzArgs a)
+__global__ void __launch_bounds__(kDzThreads, 3) k_linear_dz(const T* __restrict__ dy, const T* __restrict__ z, T* __restrict__ dz, const LinearDzArgs a)
 {
     __shared__ float sums[kDzThreads][9];
     const int lane = threadIdx.x & (a.lanes - 1), group = threadIdx.x / a.lanes, groups = kDzThreads / a.lanes;
@@ -551,26 +569,48 @@ __global__ void __launch_bounds__(kDzThreads) k_linear_dz(const T* __restrict__ 
     float sum[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) sum[e] = 0.f;
-    if (n > 0) {
-#pragma unroll 2
-        for (int64_t row = (int64_t)blockIdx.x * groups + group; row < a.M; row += (int64_t)gridDim.x * groups) {
-            float g[8];
-            load8(dy + row * a.lddy + c, n, a.whole_dy, g);
-            if constexpr (ACT == DG_ACT_RELU) {
-                const uint32_t word = __ldg(a.bits + row * a.ldbits + c / 32) >> (c % 32);
+    const int64_t step = (int64_t)gridDim.x * groups;
+    auto work = [&](int64_t row, const Raw<T>& from, const Raw<T>& pre, uint32_t word) {
+        float g[8];
+        from.wide(g);
+        if constexpr (ACT == DG_ACT_RELU) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) g[e] = word >> e & 1 ? g[e] : 0.f;
-            } else if constexpr (ACT != DG_ACT_NONE) {
-                float v[8];
-                load8(z + row * a.ldz + c, n, a.whole_z, v);
+            for (int e = 0; e < 8; ++e) g[e] = word >> e & 1 ? g[e] : 0.f;
+        } else if constexpr (ACT != DG_ACT_NONE) {
+            float v[8];
+            pre.wide(v);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) g[e] *= act_slope<ACT>(v[e]);
+            for (int e = 0; e < 8; ++e) g[e] *= act_slope<ACT>(v[e]);
+        }
+        if (dz) store8(dz + row * a.lddz + c, n, a.whole_dz, g);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] += g[e];
+    };
+    auto bits_of = [&](int64_t row) { return ACT == DG_ACT_RELU ? __ldg(a.bits + row * a.ldbits + c / 32) >> (c % 32) : 0u; };
+    int64_t row = (int64_t)blockIdx.x * groups + group;
+    constexpr bool smooth = ACT == DG_ACT_GELU || ACT == DG_ACT_SILU;
+    if (n == 8 && a.whole_dy && (!smooth || a.whole_z)) {
+        constexpr int U = sizeof(T) == 4 ? 2 : 4;                 // rows in flight
+        for (; row + (U - 1) * step < a.M; row += U * step) {
+            Raw<T> from[U], pre[U];
+            uint32_t word[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                from[u].load(dy + (row + u * step) * a.lddy + c);
+                if constexpr (smooth) pre[u].load(z + (row + u * step) * a.ldz + c);
+                word[u] = bits_of(row + u * step);
             }
-            if (dz) store8(dz + row * a.lddz + c, n, a.whole_dz, g);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) sum[e] += g[e];
+            for (int u = 0; u < U; ++u) work(row + u * step, from[u], pre[u], word[u]);
         }
     }
+    if (n > 0)
+        for (; row < a.M; row += step) {
+            Raw<T> from, pre;
+            from.load(dy + row * a.lddy + c, n);
+            if constexpr (smooth) pre.load(z + row * a.ldz + c, n);
+            work(row, from, pre, bits_of(row));
+        }
     if (!a.partial) return;
 #pragma unroll
     for (int e = 0; e < 8; ++e) sums[threadIdx.x][e] = sum[e];
@@ -584,18 +624,19 @@ __global__ void __launch_bounds__(kDzThreads) k_linear_dz(const T* __restrict__ 
     }
 }
 
-// db: 32 columns a CTA, eight warps share the parts.
-template <class T> __global__ void __launch_bounds__(256) k_linear_db(const float* __restrict__ partial, int parts, int32_t N, T* __restrict__ db)
+// db: 32 columns a CTA, 32 warps share the parts.
+template <class T> __global__ void __launch_bounds__(1024) k_linear_db(const float* __restrict__ partial, int parts, int32_t N, T* __restrict__ db)
 {
-    __shared__ double sums[8][33];
+    __shared__ double sums[32][33];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
     double s = 0.0;
     if (col < N)
-        for (int i = warp; i < parts; i += 8) s += __ldg(partial + (int64_t)i * N + col);
+#pragma unroll 8
+        for (int i = warp; i < parts; i += 32) s += __ldg(partial + (int64_t)i * N + col);
     sums[warp][lane] = s;
     __syncthreads();
     if (warp || col >= N) return;
-    for (int w = 1; w < 8; ++w) s += sums[w][lane];
+    for (int w = 1; w < 32; ++w) s += sums[w][lane];
     db[col] = Pair<T>::round((float)s);
 }
 
@@ -609,7 +650,7 @@ int dz_lanes(int32_t N)
 int dz_ctas(int64_t M, int32_t N)
 {
     const int lanes = dz_lanes(N), columns = (N + lanes * 8 - 1) / (lanes * 8);
-    const int64_t most = std::max(1, 148 * 8 / columns), rows = kDzThreads / lanes * 16;
+    const int64_t most = std::max(1, 148 * 6 / columns), rows = kDzThreads / lanes * 16;
     return (int)std::min<int64_t>(most, (M + rows - 1) / rows);
 }
 
@@ -953,7 +994,7 @@ extern "C" int dg_linear_dz(const void* dy, int64_t lddy, const void* z, int64_t
             case DG_ACT_SILU: k_linear_dz<T, DG_ACT_SILU><<<grid, kDzThreads, 0, s>>>(from, pre, to, a); break;
             default: k_linear_dz<T, DG_ACT_NONE><<<grid, kDzThreads, 0, s>>>(from, pre, to, a);
         }
-        if (db) k_linear_db<T><<<(unsigned)((N + 31) / 32), 256, 0, s>>>(scratch, (int)grid.x, N, static_cast<T*>(db));
+        if (db) k_linear_db<T><<<(unsigned)((N + 31) / 32), 1024, 0, s>>>(scratch, (int)grid.x, N, static_cast<T*>(db));
     };
     if (type == DG_FLOAT32) run(float{});
     else if (type == DG_BFLOAT16) run(__nv_bfloat16{});
@@ -994,7 +1035,7 @@ extern "C" int dg_linear_dw(const void* x, int64_t ldx, const void* dz, int64_t 
         const int code = allow_smem((const void*)k_linear_dw<T>, granted);
         if (code) return code;
         k_linear_dw<T><<<ctas, kDwThreads, smem, (cudaStream_t)stream>>>(tmP, tmQ, a);
-        k_linear_dw_reduce<T><<<(unsigned)((slots + 255) / 256), 256, 0, (cudaStream_t)stream>>>(a.partial, shape.ranges, a.p_panels, a.q_panels, a.p_store, a.q_store, K, N,
+        k_linear_dw_reduce<T><<<(unsigned)((slots + 31) / 32), 256, 0, (cudaStream_t)stream>>>(a.partial, shape.ranges, a.p_panels, a.q_panels, a.p_store, a.q_store, K, N,
                                                                                               static_cast<T*>(dw), row_stride, col_stride);
         return (int)cudaGetLastError();
     };
