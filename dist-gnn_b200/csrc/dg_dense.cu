@@ -51,34 +51,28 @@ struct DenseArgs {
 // What a kernel's epilogue does; from kLinear on: the linear layer's, with activation EPI - kLinear.
 constexpr int kPlain = 0, kMasked = 1, kLinear = 2;
 
-// A lane's 32 columns of its row: the bias is added, and where asked the signs are kept.
-template <int EPI> __device__ __forceinline__ void add_bias(const DenseArgs& a, uint32_t* r, int c0, int64_t row)
+// A lane's 32 columns of its row: a bit each where x w + b is above zero.
+__device__ __forceinline__ void keep_signs(const DenseArgs& a, const uint32_t* r, int c0, int64_t row)
 {
-    if (a.bias) {
-        if (c0 + 32 <= a.N && (reinterpret_cast<uintptr_t>(a.bias) & 15) == 0) {
+    if (row >= a.M) return;
+    uint32_t word = 0;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float4 b = __ldg(reinterpret_cast<const float4*>(a.bias + c0) + j);
-                r[4 * j] = __float_as_uint(__uint_as_float(r[4 * j]) + b.x);
-                r[4 * j + 1] = __float_as_uint(__uint_as_float(r[4 * j + 1]) + b.y);
-                r[4 * j + 2] = __float_as_uint(__uint_as_float(r[4 * j + 2]) + b.z);
-                r[4 * j + 3] = __float_as_uint(__uint_as_float(r[4 * j + 3]) + b.w);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-                if (c0 + j < a.N) r[j] = __float_as_uint(__uint_as_float(r[j]) + __ldg(a.bias + c0 + j));
-        }
+    for (int j = 0; j < 32; ++j) {
+        const float b = a.bias && c0 + j < a.N ? __ldg(a.bias + c0 + j) : 0.f;
+        word |= (__uint_as_float(r[j]) + b <= 0.f ? 0u : 1u) << j;
     }
-    if (EPI == kLinear + DG_ACT_RELU && a.bits && row < a.M) {
-        uint32_t word = 0;
-#pragma unroll
-        for (int j = 0; j < 32; ++j) word |= (__uint_as_float(r[j]) <= 0.f ? 0u : 1u) << j;
-        a.bits[row * a.ldbits + c0 / 32] = word;
-    }
+    a.bits[row * a.ldbits + c0 / 32] = word;
 }
+__device__ __forceinline__ float4 bias_piece(const DenseArgs& a, int c)      // four columns of which all are the result's
+{
+    return a.bias ? make_float4(__ldg(a.bias + c), __ldg(a.bias + c + 1), __ldg(a.bias + c + 2), __ldg(a.bias + c + 3)) : make_float4(0.f, 0.f, 0.f, 0.f);
+}
+template <int ACT> __device__ __forceinline__ float4 activate(float4 v)
+{
+    return make_float4(act_value<ACT>(v.x), act_value<ACT>(v.y), act_value<ACT>(v.z), act_value<ACT>(v.w));
+}
+__device__ __forceinline__ float4 operator+(float4 a, float4 b) { return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); }
 
-// umma_desc_sw128 for rows of 64 bytes with the 64B swizzle: 8-row groups are 512 bytes apart.
 __device__ __forceinline__ uint64_t umma_desc_sw64(uint32_t smem_addr)
 {
     return (uint64_t)((smem_addr & 0x3FFFF) >> 4) | (uint64_t)1 << 16 | (uint64_t)(512 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)4 << 61;
@@ -126,11 +120,13 @@ template <int EPI> __device__ __forceinline__ void store_rows(const DenseArgs& a
             for (int i = 0; i < 8; ++i)
                 if (i * 4 + r4 < rows) mk[i] = __ldg(reinterpret_cast<const float4*>(a.mask + (row0 + i * 4 + r4) * a.ldm + col4));
         }
+        [[maybe_unused]] float4 shift;
+        if (EPI >= kLinear && pieces) shift = bias_piece(a, col4);
         uint32_t r[32];
         tmem_ld16(acc + (uint32_t)c0, r);
         if (c0 + 16 < a.n_pad) tmem_ld16(acc + (uint32_t)c0 + 16, r + 16);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-        if constexpr (EPI >= kLinear) add_bias<EPI>(a, r, c0, row0 + lane);
+        if (EPI == kLinear + DG_ACT_RELU && a.bits) keep_signs(a, r, c0, row0 + lane);
         float4* mine = reinterpret_cast<float4*>(stage + lane * kStagePitch);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
@@ -142,9 +138,10 @@ template <int EPI> __device__ __forceinline__ void store_rows(const DenseArgs& a
                 if (i * 4 + r4 >= rows) continue;
                 float4 v = *reinterpret_cast<const float4*>(stage + (i * 4 + r4) * kStagePitch + (lane & 7) * 4);
                 if constexpr (EPI >= kLinear) {
+                    v = v + shift;
                     if (a.z) __stcs(reinterpret_cast<float4*>(a.z + (row0 + i * 4 + r4) * a.ldz + col4), v);
-                    v = make_float4(act_value<EPI - kLinear>(v.x), act_value<EPI - kLinear>(v.y), act_value<EPI - kLinear>(v.z), act_value<EPI - kLinear>(v.w));
-                    if (a.mask) v = make_float4(v.x + mk[i].x, v.y + mk[i].y, v.z + mk[i].z, v.w + mk[i].w);
+                    v = activate<EPI - kLinear>(v);
+                    if (a.mask) v = v + mk[i];
                     __stcs(reinterpret_cast<float4*>(a.C + (row0 + i * 4 + r4) * a.ldc + col4), v);
                     continue;
                 }
@@ -171,6 +168,7 @@ template <int EPI> __device__ __forceinline__ void store_rows(const DenseArgs& a
                     if (i0 + i >= rows) break;
                     float v = stage[(i0 + i) * kStagePitch + lane];
                     if constexpr (EPI >= kLinear) {
+                        if (a.bias) v += __ldg(a.bias + c);
                         if (a.z) a.z[(row0 + i0 + i) * a.ldz + c] = v;
                         v = act_value<EPI - kLinear>(v);
                         if (a.mask) v += mrow[i];
@@ -505,6 +503,8 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                     for (int i = 0; i < 8; ++i, m += 4 * a.ldm)
                         if (i * 4 + r4 < rows) mk[i] = __ldg(reinterpret_cast<const float4*>(m));
                 }
+                [[maybe_unused]] float4 shift;
+                if (EPI >= kLinear && whole) shift = bias_piece(a, c0 + piece * 4);
                 if (c0 == first) {
                     ok = __all_sync(0xffffffffu, mbar_wait(acc_full0 + 8 * b, v & 1));     // tcgen05.ld is warp-collective
                     if (!ok) break;
@@ -520,7 +520,7 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                         __syncwarp();
                         if (lane == 0) mbar_arrive_cluster(leader_acc_empty0 + 8 * b);
                     }
-                    if constexpr (EPI >= kLinear) add_bias<EPI>(a, r, c0, row0 + lane);
+                    if (EPI == kLinear + DG_ACT_RELU && a.bits) keep_signs(a, r, c0, row0 + lane);
 #pragma unroll
                     for (int j = 0; j < 8; ++j)                   // a lane holds one row: through shared memory, conflict-free both ways
                         stage[lane * 8 + (j ^ (lane & 7))] = make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]), __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3]));
@@ -535,9 +535,10 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                     for (int i = 0; i < 8; ++i, c += 4 * a.ldc) {
                         if constexpr (EPI >= kLinear) {
                             if (i * 4 + r4 >= rows) continue;
+                            x[i] = x[i] + shift;
                             if (a.z) __stcs(reinterpret_cast<float4*>(a.z + (row0 + i * 4 + r4) * a.ldz + c0 + piece * 4), x[i]);
-                            x[i] = make_float4(act_value<EPI - kLinear>(x[i].x), act_value<EPI - kLinear>(x[i].y), act_value<EPI - kLinear>(x[i].z), act_value<EPI - kLinear>(x[i].w));
-                            if (a.mask) x[i] = make_float4(x[i].x + mk[i].x, x[i].y + mk[i].y, x[i].z + mk[i].z, x[i].w + mk[i].w);
+                            x[i] = activate<EPI - kLinear>(x[i]);
+                            if (a.mask) x[i] = x[i] + mk[i];
                             __stcs(reinterpret_cast<float4*>(c), x[i]);
                             continue;
                         }
@@ -564,6 +565,7 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                             if (i0 + i >= rows) break;
                             float x = flat[((i0 + i) * 8 + ((lane >> 2) ^ ((i0 + i) & 7))) * 4 + (lane & 3)];
                             if constexpr (EPI >= kLinear) {
+                                if (a.bias) x += __ldg(a.bias + c0 + lane);
                                 if (a.z) a.z[(row0 + i0 + i) * a.ldz + c0 + lane] = x;
                                 x = act_value<EPI - kLinear>(x);
                                 if (a.mask) x += mrow[i];
