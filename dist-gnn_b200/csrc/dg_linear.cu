@@ -26,6 +26,12 @@ template <> struct Pair<__nv_bfloat16> {
         const Two t = __floats2bfloat162_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&t);
     }
+    static __device__ __forceinline__ float_pair two(uint32_t v) { return pair_of(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u)); }
+    static __device__ __forceinline__ uint32_t narrow(float_pair v)
+    {
+        const float2 f = halves(v);
+        return narrow(f.x, f.y);
+    }
     static __device__ __forceinline__ float one(__nv_bfloat16 v) { return __bfloat162float(v); }
     static __device__ __forceinline__ __nv_bfloat16 round(float v) { return __float2bfloat16_rn(v); }
     static constexpr uint32_t kFormat = 1;
@@ -38,6 +44,16 @@ template <> struct Pair<__half> {
         const Two t = __floats2half2_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&t);
     }
+    static __device__ __forceinline__ float_pair two(uint32_t v)
+    {
+        const float2 f = wide(v);
+        return pair_of(f.x, f.y);
+    }
+    static __device__ __forceinline__ uint32_t narrow(float_pair v)
+    {
+        const float2 f = halves(v);
+        return narrow(f.x, f.y);
+    }
     static __device__ __forceinline__ float one(__half v) { return __half2float(v); }
     static __device__ __forceinline__ __half round(float v) { return __float2half_rn(v); }
     static constexpr uint32_t kFormat = 0;
@@ -49,10 +65,10 @@ template <> struct Pair<float> {
 
 // ---- the product on the tensor cores ------------------------------------------------------------------------------------
 constexpr int BM = 128, BK = 64;                  // rows of a CTA, K-columns of a stage: 128 bytes
-constexpr int kEpilogueWarps = 8, kThreadsPair = 32 * (2 + kEpilogueWarps);
+constexpr int kEpilogueWarps = 16, kThreadsPair = 32 * (2 + kEpilogueWarps);
 constexpr int kMaxStages = 8;
 constexpr int kABytes = BM * BK * 2;
-constexpr int kPieceBytes = 32 * 64 * 2;          // an epilogue warp's 32 rows x 64 columns
+constexpr int kPiece = 32, kPieceBytes = 32 * kPiece * 2;      // an epilogue warp's 32 rows x 32 columns
 constexpr int kBarBytes = 8 * (2 * kMaxStages + 5 + 2 * kEpilogueWarps) + 8;
 
 struct LinearPairArgs {
@@ -111,7 +127,7 @@ __device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t a_desc, uint6
         ::"r"(tmem_d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
 }
 
-// Warps: 0 TMA, 1 MMA issue (even CTA) + tensor-memory allocation, 2-9 epilogue (lane quarter w % 4; two warps a quarter take its 64-column pieces
+// Warps: 0 TMA, 1 MMA issue (even CTA) + tensor-memory allocation, 2-17 epilogue (lane quarter w % 4; four warps a quarter take its 32-column pieces
 // in turn).  A stage is 64 K-columns of the CTA's 128 rows of x and of its half of the panel's columns of w.  Two accumulators (columns 0 / 256).
 // Barriers: full (even CTA, the loads of both), empty and acc_full (both CTAs, by commit), acc_empty (even CTA: the epilogue warps of both), and one an
 // epilogue warp and buffer for its residual's pieces.
@@ -216,23 +232,24 @@ k_linear_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
             mbar_wait(done, 0);
         }
     } else {
-        // A lane holds a row's 64 columns of the accumulator.  Pieces of 32 rows x 128 bytes lie in shared memory with the 128B swizzle (conflict-free by
+        // A lane holds a row's 32 columns of the accumulator.  Pieces of 32 rows x 64 bytes lie in shared memory with the 64B swizzle (conflict-free by
         // rows) and are moved by TMA, which leaves out what lies beyond the matrix: the residual arrives where y is then put together.
-        const int w = warp - 2, q = warp & 3, first = w / 4 * 64;      // a warp may only read its own quarter of the TMEM lanes
-        constexpr int step = kEpilogueWarps / 4 * 64;
+        const int w = warp - 2, q = warp & 3, first = w / 4 * kPiece;      // a warp may only read its own quarter of the TMEM lanes
+        constexpr int step = kEpilogueWarps / 4 * kPiece;
         const uint32_t leader_acc_empty0 = in_leader(acc_empty0);
         const int own = staging + w * per_warp;
-        const uint32_t swizzle = lane & 7;
+        const uint32_t swizzle = lane >> 1 & 3, my_res0 = res0 + 16 * w;
         const T* bias = static_cast<const T*>(a.bias);
-        int lt = 0, count = 0;                                    // pieces so far: buffer count & 1
         auto row_of = [&](int tile) { return (int64_t)(tile / a.n_panels) * (2 * BM) + rank * BM + q * 32; };
-        auto fetch = [&](int tile, int c0, int n) {               // the residual's piece into buffer n & 1, whose last store has been read
+        auto fetch = [&](int tile, int c0, int s) {               // the residual's piece into buffer s, whose last store has been read
             const int64_t row = row_of(tile);
-            if (row >= a.M || tile % a.n_panels * a.n_tile + c0 >= a.N) return;
-            mbar_expect_tx(res0 + 8 * (2 * w + (n & 1)), kPieceBytes);
-            tma_load_2d(base + own + (n & 1) * kPieceBytes, &tmR, tile % a.n_panels * a.n_tile + c0, (int)row, res0 + 8 * (2 * w + (n & 1)));
+            const int col = tile % a.n_panels * a.n_tile + c0;
+            if (row >= a.M || col >= a.N) return;
+            mbar_expect_tx(my_res0 + 8 * s, kPieceBytes);
+            tma_load_2d(base + own + s * kPieceBytes, &tmR, col, (int)row, my_res0 + 8 * s);
         };
         uint32_t res_phase = 0;                                   // a bit a buffer
+        int lt = 0, s = 0;
         if (a.residual && lane == 0 && pair < a.tiles && first < a.n_tile) fetch(pair, first, 0);
         for (int tile = pair; tile < a.tiles && ok; tile += pairs, ++lt) {
             const int b = lt & 1, v = lt >> 1;
@@ -247,82 +264,75 @@ k_linear_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
                 if (lane == 0) mbar_arrive_cluster(leader_acc_empty0 + 8 * b);
                 continue;
             }
-            for (int c0 = first; c0 < a.n_tile; c0 += step, ++count) {
-                uint32_t r[64];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) tmem_ld16(acc + (uint32_t)(c0 + 16 * j), r + 16 * j);
+            for (int c0 = first; c0 < a.n_tile; c0 += step, s ^= 1) {
+                uint32_t r[kPiece];
+                tmem_ld16(acc + (uint32_t)c0, r);
+                tmem_ld16(acc + (uint32_t)c0 + 16, r + 16);
+                const int col0 = n0 + c0;
+                const bool live = row0 < a.M && col0 < a.N;       // the same for the warp
+                if (lane == 0) {
+                    bulk_wait_read();                             // what the last piece stored has left the buffers
+                    if (a.residual) {
+                        const bool more = c0 + step < a.n_tile;
+                        if (more || tile + pairs < a.tiles) fetch(more ? tile : tile + pairs, more ? c0 + step : first, s ^ 1);
+                    }
+                }
+                __syncwarp();
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                 if (c0 + step >= a.n_tile) {                      // the accumulator has been read: its next tile may start
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                     __syncwarp();
                     if (lane == 0) mbar_arrive_cluster(leader_acc_empty0 + 8 * b);
                 }
-                const int col0 = n0 + c0, s = count & 1;
-                const bool live = row0 < a.M && col0 < a.N;       // the same for the warp
-                if (lane == 0) {
-                    bulk_wait_read();                             // what the last pieces stored has left the buffers
-                    if (a.residual) {
-                        const bool more = c0 + step < a.n_tile;
-                        if (more || tile + pairs < a.tiles) fetch(more ? tile : tile + pairs, more ? c0 + step : first, count + 1);
-                    }
-                }
-                if (a.residual && live) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(res0 + 8 * (2 * w + s), res_phase >> s & 1));
+                if (!live) continue;
+                if (a.residual) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(my_res0 + 8 * s, res_phase >> s & 1));
                     if (!ok) break;
                     res_phase ^= 1u << s;
                 }
-                __syncwarp();
-                if (!live) continue;
-                unsigned char* y_row = gbase + own + s * kPieceBytes + lane * 128;
-                unsigned char* z_row = gbase + own + 2 * kPieceBytes + lane * 128;
-                uint32_t positive[2] = {0u, 0u};
+                unsigned char* y_row = gbase + own + s * kPieceBytes + lane * 64;
+                unsigned char* z_row = gbase + own + 2 * kPieceBytes + lane * 64;
+                uint32_t positive = 0u;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {                     // eight columns: 16 bytes
-                    float z[8];
+                for (int j = 0; j < kPiece / 8; ++j) {            // eight columns: 16 bytes
+                    float_pair z[4];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) z[e] = __uint_as_float(r[8 * j + e]);
+                    for (int e = 0; e < 4; ++e) z[e] = pair_of(__uint_as_float(r[8 * j + 2 * e]), __uint_as_float(r[8 * j + 2 * e + 1]));
                     if (bias) {
                         const int c = col0 + 8 * j;
                         if (a.whole_bias && c + 8 <= a.N) {
                             const uint4 t = __ldg(reinterpret_cast<const uint4*>(bias + c));
                             const uint32_t u[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const float2 f = Pair<T>::wide(u[e]);
-                                z[2 * e] += f.x, z[2 * e + 1] += f.y;
-                            }
+                            for (int e = 0; e < 4; ++e) z[e] = add2(z[e], Pair<T>::two(u[e]));
                         } else {
 #pragma unroll
-                            for (int e = 0; e < 8; ++e)
-                                if (c + e < a.N) z[e] += Pair<T>::one(bias[c + e]);
+                            for (int e = 0; e < 4; ++e)
+                                z[e] = add2(z[e], pair_of(c + 2 * e < a.N ? Pair<T>::one(bias[c + 2 * e]) : 0.f, c + 2 * e + 1 < a.N ? Pair<T>::one(bias[c + 2 * e + 1]) : 0.f));
                         }
                     }
                     const uint32_t at = ((uint32_t)j ^ swizzle) * 16;
                     if (ACT != DG_ACT_NONE && a.save_z)
-                        *reinterpret_cast<uint4*>(z_row + at) = make_uint4(Pair<T>::narrow(z[0], z[1]), Pair<T>::narrow(z[2], z[3]), Pair<T>::narrow(z[4], z[5]),
-                                                                           Pair<T>::narrow(z[6], z[7]));
+                        *reinterpret_cast<uint4*>(z_row + at) = make_uint4(Pair<T>::narrow(z[0]), Pair<T>::narrow(z[1]), Pair<T>::narrow(z[2]), Pair<T>::narrow(z[3]));
                     if (ACT == DG_ACT_RELU && a.bits) {
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) positive[j / 4] |= (z[e] <= 0.f ? 0u : 1u) << (8 * (j % 4) + e);
+                        for (int e = 0; e < 4; ++e) {
+                            const float2 f = halves(z[e]);
+                            positive |= ((f.x <= 0.f ? 0u : 1u) | (f.y <= 0.f ? 0u : 2u)) << (8 * j + 2 * e);
+                        }
                     }
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) z[e] = act_value<ACT>(z[e]);
+                    for (int e = 0; e < 4; ++e) z[e] = act_value2<ACT>(z[e]);
                     uint4* to = reinterpret_cast<uint4*>(y_row + at);
                     if (a.residual) {
                         const uint4 t = *to;
                         const uint32_t u[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float2 f = Pair<T>::wide(u[e]);
-                            z[2 * e] += f.x, z[2 * e + 1] += f.y;
-                        }
+                        for (int e = 0; e < 4; ++e) z[e] = add2(z[e], Pair<T>::two(u[e]));
                     }
-                    *to = make_uint4(Pair<T>::narrow(z[0], z[1]), Pair<T>::narrow(z[2], z[3]), Pair<T>::narrow(z[4], z[5]), Pair<T>::narrow(z[6], z[7]));
+                    *to = make_uint4(Pair<T>::narrow(z[0]), Pair<T>::narrow(z[1]), Pair<T>::narrow(z[2]), Pair<T>::narrow(z[3]));
                 }
-                if (ACT == DG_ACT_RELU && a.bits && row0 + lane < a.M) {      // words beyond the row's are left alone
-                    uint32_t* to = a.bits + (row0 + lane) * a.ldbits + col0 / 32;
-                    *reinterpret_cast<uint2*>(to) = make_uint2(positive[0], positive[1]);
-                }
+                if (ACT == DG_ACT_RELU && a.bits && row0 + lane < a.M) a.bits[(row0 + lane) * a.ldbits + col0 / 32] = positive;
                 fence_async();
                 __syncwarp();
                 if (lane == 0) {
@@ -580,7 +590,14 @@ __global__ void __launch_bounds__(kDzThreads, 3) k_linear_dz(const T* __restrict
             float v[8];
             pre.wide(v);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) g[e] *= act_slope<ACT>(v[e]);
+            for (int e = 0; e < 8; e += 2) {
+                if constexpr (sizeof(T) == 4) {
+                    g[e] *= act_slope<ACT>(v[e]), g[e + 1] *= act_slope<ACT>(v[e + 1]);
+                } else {
+                    const float2 f = halves(mul2(pair_of(g[e], g[e + 1]), act_slope2<ACT>(pair_of(v[e], v[e + 1]))));
+                    g[e] = f.x, g[e + 1] = f.y;
+                }
+            }
         }
         if (dz) store8(dz + row * a.lddz + c, n, a.whole_dz, g);
 #pragma unroll
@@ -833,17 +850,17 @@ __global__ void __launch_bounds__(256) k_pad_rows16(const unsigned short* __rest
 // ---- host side ---------------------------------------------------------------------------------------------------------------------
 bool on_rows(const void* p, int64_t ld, int item) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld * item % 16 == 0; }
 
-// [rows x cols] of 16-bit elements, row-major, boxes of 64 columns x box_rows rows with the 128B swizzle, out-of-range elements read as zero.
-int make_map16(CUtensorMap* map, const void* ptr, int32_t type, int64_t rows, int64_t cols, int64_t ld, int box_rows)
+// [rows x cols] of 16-bit elements, row-major, boxes of 64 columns (128B swizzle; 32: 64B swizzle) x box_rows rows, out-of-range elements read as zero.
+int make_map16(CUtensorMap* map, const void* ptr, int32_t type, int64_t rows, int64_t cols, int64_t ld, int box_rows, int box_cols = 64)
 {
     EncodeTiledFn fn = encode_tiled();
     if (!fn) return DG_ERR_UNSUPPORTED;
     const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
     const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
-    const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+    const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
     const cuuint32_t elem[2] = {1, 1};
     const CUresult r = fn(map, type == DG_BFLOAT16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(ptr), dims, strides, box,
-                          elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                          elem, CU_TENSOR_MAP_INTERLEAVE_NONE, box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? DG_OK : DG_ERR_UNSUPPORTED;
 }
 
@@ -896,11 +913,11 @@ int linear16(const dg_linear_args* g, cudaStream_t stream)
     int rc;
     if ((rc = make_map16(&maps[0], g->x, g->type, g->M, g->K, g->ldx, BM)) ||
         (rc = g->out_in ? make_map16(&maps[1], g->w, g->type, g->N, g->K, g->ldw, a.n_tile / 2) : make_map16(&maps[1], g->w, g->type, g->K, g->N, g->ldw, BK)) ||
-        (rc = make_map16(&maps[2], g->y, g->type, g->M, g->N, g->ldy, 32)))
+        (rc = make_map16(&maps[2], g->y, g->type, g->M, g->N, g->ldy, 32, kPiece)))
         return rc;
     maps[3] = maps[4] = maps[2];
-    if (g->residual && (rc = make_map16(&maps[3], g->residual, g->type, g->M, g->N, g->ldr, 32))) return rc;
-    if (g->z && (rc = make_map16(&maps[4], g->z, g->type, g->M, g->N, g->ldz, 32))) return rc;
+    if (g->residual && (rc = make_map16(&maps[3], g->residual, g->type, g->M, g->N, g->ldr, 32, kPiece))) return rc;
+    if (g->z && (rc = make_map16(&maps[4], g->z, g->type, g->M, g->N, g->ldz, 32, kPiece))) return rc;
     const size_t stage = kABytes + (a.b_boxes ? a.b_boxes * BK * 128 : a.n_tile / 2 * 128);
     const size_t rest = (size_t)kEpilogueWarps * (a.save_z ? 3 : 2) * kPieceBytes + kBarBytes + 1024;
     a.stages = (int)std::min<size_t>(kMaxStages, (227 * 1024 - rest) / stage);
