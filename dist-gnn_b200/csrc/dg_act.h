@@ -1,16 +1,10 @@
 // Activations of the linear layer and their derivatives, in fp32.
 #pragma once
-#include <cstdint>
 #include "dist_gnn_b200.h"
+#include "dg_pair.h"
 
 namespace dg {
 
-__device__ __forceinline__ float reciprocal(float v)      // within a unit in the last place
-{
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-    return r;
-}
 // Phi(z) and e = exp(-z^2 / 2) by Hastings' formula (Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26): Phi(-|z|) = t (a1 + t (a2 + ... a5)) e / 2
 // with t = 1 / (1 + p |z| / sqrt 2), off by at most 7.5e-8.  No branches, and the density that the derivative needs comes with it: against erff, whose two
 // branches diverge, the forward pass of 2,449,029 x 256 -> 256 bf16 went from 1,329 us to FWD and the gradient's pass from 1,101 to DZ.
@@ -21,17 +15,13 @@ __device__ __forceinline__ float normal_cdf(float z, float* e)
     p = fmaf(t, p, 0.5f * 1.421413741f);
     p = fmaf(t, p, 0.5f * -0.284496736f);
     p = fmaf(t, p, 0.5f * 0.254829592f);
-    float x;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(x) : "f"(z * z * -0.72134752f));
-    *e = x;
-    const float tail = p * t * x;
+    *e = exp2_approx(z * z * -0.72134752f);
+    const float tail = p * t * *e;
     return z > 0.f ? 1.f - tail : tail;
 }
 __device__ __forceinline__ float sigmoid(float z)
 {
-    float x;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(x) : "f"(z * -1.44269504f));
-    return reciprocal(1.f + x);
+    return reciprocal(1.f + exp2_approx(z * -1.44269504f));
 }
 
 // gelu(z) = z Phi(z) with the distribution function of the normal distribution, silu(z) = z / (1 + exp(-z)).
@@ -66,44 +56,6 @@ template <int ACT> __device__ __forceinline__ float act_slope(float z)
 // where R(a) = Phi(-a) / e is a polynomial, fitted on [0, 5.6] for the least largest max(1, a) |e R - Phi(-a)|: 1.8e-6, a 250th of half a step of fp16.
 // Beyond 16 the polynomial is held and e is zero.  SiLU takes one reciprocal for a pair: 1 / u = v / (u v).
 // 2,449,029 x 256 -> 256 bf16, forward: GELU PAIR_GELU, SiLU PAIR_SILU.
-using float_pair = unsigned long long;
-__device__ __forceinline__ float_pair pair_of(float a, float b)
-{
-    float_pair r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float2 halves(float_pair v)
-{
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-__device__ __forceinline__ float_pair fma2(float_pair a, float_pair b, float_pair c)
-{
-    float_pair r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ float_pair mul2(float_pair a, float_pair b)
-{
-    float_pair r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ float_pair add2(float_pair a, float_pair b)
-{
-    float_pair r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ float_pair both(float v) { return pair_of(v, v); }
-__device__ __forceinline__ float exp2_approx(float v)
-{
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-    return r;
-}
 // -e R(a), or with SLOPE  e (a / sqrt(2 pi) - R(a))
 template <bool SLOPE> __device__ __forceinline__ float_pair normal_tail(float_pair z, float_pair a)
 {

@@ -11,17 +11,21 @@
 //
 // What bounds it: HBM for tables (28 bytes an element with 32-bit states, 10 with bf16 and 8), the launch for small models.
 #include <algorithm>
+#include <cmath>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include "dg_internal.h"
+#include "dg_pair.h"
 
 namespace {
 
+using namespace dg;
+
 constexpr int kThreads = 256, kEach = 8, kChunk = kThreads * kEach;      // a lane takes 8 neighbouring elements, a warp one block of 256
 constexpr int kBlock = 256;
-constexpr int kNormCtas = 148 * 4;
-constexpr float kLargest = 448.f, kSmallestNormal = 0.015625f, kSmallest = 0.001953125f;
+constexpr int kNormCtas = 148 * 8;
+constexpr float kLargest = 448.f;
 
 // Tensors of one launch.  Their table travels with the launch, so that a captured graph holds it and nothing has to be copied ahead: 40 entries
 // are 3.4 KB of arguments, 376 the 32 KB that a launch can have.
@@ -34,8 +38,9 @@ template <int CAP> struct Table {
 constexpr int kFew = 40, kMany = 376;
 
 struct Factors {
-    double lr, beta1, beta2;
-    float b1, a1, b2, a2, eps, keep;      // a = 1 - b; keep = 1 - lr wd
+    double log_beta1, log_beta2;
+    float lr, b1, a1, b2, a2, eps, keep;  // a = 1 - b; keep = 1 - lr wd
+    float one;
     uint32_t seed;
 };
 
@@ -100,14 +105,13 @@ __device__ __forceinline__ void store_codes(uint8_t* p, int n, bool wide, uint2 
     }
     for (int i = 0; i < 8 && i < n; ++i) p[i] = (uint8_t)((i < 4 ? c.x : c.y) >> (i % 4 * 8));
 }
-__device__ __forceinline__ void decode(uint2 c, float scale, float* v)
+__device__ __forceinline__ void decode(uint2 c, float scale, float_pair* v)
 {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const uint32_t w = i < 2 ? c.x : c.y;
         const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> (i % 2 * 16)), __NV_E4M3)));
-        v[2 * i] = __fmul_rn(f.x, scale);
-        v[2 * i + 1] = __fmul_rn(f.y, scale);
+        v[i] = mul2(pair_of(f.x, f.y), both(scale));
     }
 }
 
@@ -121,42 +125,44 @@ __device__ __forceinline__ uint32_t mix(uint32_t h)
 }
 __device__ __forceinline__ uint32_t key_of(uint32_t seed, int64_t step) { return mix(seed + (uint32_t)step * 0x3C6EF373u); }
 
-// A block's values, eight a lane, as codes and a scale.  q = |x| 448 / largest; below 2^-6, where e4m3 steps by 2^-9, 2^-6 more gives a number that steps
-// by as much in its third mantissa bit: the noise is added below that bit, which is then the last one kept.
-template <bool POSITIVE> __device__ __forceinline__ uint2 encode(const float* x, const uint32_t* noise, float* scale)
+// A block's values, eight a lane, as codes and a scale.  q = |x| 448 / largest; times 2^-120 the smallest normal number of e4m3 is the smallest one of fp32, so
+// that an fp32 number's leading bits are the code, below 2^-6 too where both step evenly.  The noise is added below the code's last bit.
+// (q times 2^-120 in one factor would leave fp32's range where the block's largest is beyond 28,672.)
+template <bool POSITIVE> __device__ __forceinline__ uint2 encode(const float_pair* x, const uint32_t* noise, float* scale)
 {
-    uint32_t top = 0;
+    float most = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
-    const float most = __uint_as_float(__reduce_max_sync(0xffffffffu, top));            // magnitudes are ordered as their bits, NaN above all
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = halves(x[i]);
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(most) : "f"(fabsf(f.x)));
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(most) : "f"(fabsf(f.y)));
+    }
+    most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most) & 0x7FFFFFFFu));      // magnitudes are ordered as their bits, NaN above all
     const bool none = most < 1e-30f;
     const float factor = none ? 0.f : __fmul_rn(__frcp_rn(most), kLargest);
     *scale = none ? 0.f : __fmul_rn(most, 1.f / kLargest);
-    uint32_t c[4];
+    uint32_t c[2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        float y[2];
+    for (int i = 0; i < 2; ++i) {
+        uint32_t t[4];                                            // the code in the leading byte; the sign is shifted out
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const float v = x[2 * i + j], q = fminf(__fmul_rn(fabsf(v), factor), kLargest);
-            const float lift = q < kSmallestNormal ? kSmallestNormal : 0.f;
-            const uint32_t bits = (__float_as_uint(__fadd_rn(q, lift)) + ((j ? noise[i] >> 16 : noise[i] & 0xFFFFu) << 4)) & 0xFFF00000u;
-            y[j] = __fsub_rn(__uint_as_float(bits), lift);
-            if (POSITIVE) y[j] = q > 0.f ? fmaxf(y[j], kSmallest) : y[j];
-            else y[j] = v < 0.f ? -y[j] : y[j];
+            const float_pair q = mul2(x[2 * i + j], both(factor));
+            const float2 f = halves(x[2 * i + j]), l = halves(mul2(q, both(0x1p-120f)));
+            const uint32_t n = noise[2 * i + j];
+            t[2 * j] = (__float_as_uint(l.x) << 4) + __byte_perm(n, 0, 0x4104);
+            t[2 * j + 1] = (__float_as_uint(l.y) << 4) + __byte_perm(n, 0, 0x4324);
+            if (POSITIVE) {
+                t[2 * j] = max(t[2 * j], f.x > 0.f ? 0x01000000u : 0u);
+                t[2 * j + 1] = max(t[2 * j + 1], f.y > 0.f ? 0x01000000u : 0u);
+            } else {
+                t[2 * j] |= __float_as_uint(f.x) & 0x80000000u;
+                t[2 * j + 1] |= __float_as_uint(f.y) & 0x80000000u;
+            }
         }
-        c[i] = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
+        c[i] = __byte_perm(__byte_perm(t[0], t[1], 0x0073), __byte_perm(t[2], t[3], 0x0073), 0x5410);
     }
-    return make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
-}
-
-// b^t by squaring: log2(t) dependent products.
-__device__ __forceinline__ void powers(double b1, double b2, int64_t t, double* p1, double* p2)
-{
-    double x = 1.0, y = 1.0;
-    for (; t > 0; t >>= 1, b1 *= b1, b2 *= b2)
-        if (t & 1) x *= b1, y *= b2;
-    *p1 = x, *p2 = y;
+    return make_uint2(c[0], c[1]);
 }
 
 template <int CAP> __device__ __forceinline__ int find(const Table<CAP>& tab, int chunk)
@@ -171,10 +177,9 @@ template <int CAP> __device__ __forceinline__ int find(const Table<CAP>& tab, in
 }
 
 template <class T, bool SMALL, int CAP>
-__global__ void __launch_bounds__(kThreads) k_adamw(const __grid_constant__ Table<CAP> tab, const Factors f, const float* __restrict__ clip, int* __restrict__ arrived)
+__global__ void __launch_bounds__(kThreads, SMALL ? 4 : 3) k_adamw(const __grid_constant__ Table<CAP> tab, const Factors f, const float* __restrict__ clip,
+                                                                  int* __restrict__ arrived)
 {
-    __shared__ float shared_factor[2];
-    __shared__ uint32_t shared_key;
     __shared__ int last;
     const int chunks = tab.first[tab.count];
     int at = -1;
@@ -190,50 +195,54 @@ __global__ void __launch_bounds__(kThreads) k_adamw(const __grid_constant__ Tabl
         const bool wide = tab.wide[i / 32] >> (i % 32) & 1;
         const int64_t e0 = (int64_t)(chunk - tab.first[i]) * kChunk + threadIdx.x * kEach;
         const int n = (int)max((int64_t)0, min((int64_t)kEach, t.n - e0));
-        float p[8], g[8], m[8], v[8], r[8];
-        uint2 cm, cr;
+        float pf[8], gf[8];
+        [[maybe_unused]] float mf[8], vf[8];
+        [[maybe_unused]] uint2 cm, cr;
         float sm = 0.f, sr = 0.f;
         const int64_t block = e0 / kBlock;
-        load8(reinterpret_cast<const T*>(t.p) + e0, n, wide, p);
-        load8(reinterpret_cast<const T*>(t.g) + e0, n, wide, g);
+        load8(reinterpret_cast<const T*>(t.g) + e0, n, wide, gf);
         if constexpr (SMALL) {
             cm = load_codes(reinterpret_cast<const uint8_t*>(t.m) + e0, n, wide);
             cr = load_codes(reinterpret_cast<const uint8_t*>(t.v) + e0, n, wide);
             if (block * kBlock < t.n) sm = t.m_scale[block], sr = t.v_scale[block];
         } else {
-            load8(reinterpret_cast<const float*>(t.m) + e0, n, wide, m);
-            load8(reinterpret_cast<const float*>(t.v) + e0, n, wide, v);
+            load8(reinterpret_cast<const float*>(t.m) + e0, n, wide, mf);
+            load8(reinterpret_cast<const float*>(t.v) + e0, n, wide, vf);
         }
-        if (i != at) {                                            // the same for all threads
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                const int64_t step = *t.step + 1;
-                double p1, p2;
-                powers(f.beta1, f.beta2, step, &p1, &p2);
-                shared_factor[0] = (float)(f.lr / (1.0 - p1));
-                shared_factor[1] = (float)(1.0 / sqrt(1.0 - p2));
-                shared_key = key_of(f.seed, step);
-            }
-            __syncthreads();
-            rate = shared_factor[0], correction = shared_factor[1], key = shared_key;
+        load8(reinterpret_cast<const T*>(t.p) + e0, n, wide, pf);
+        if (i != at) {                                            // 1 - b^t = -expm1(t log b)
+            const int64_t step = *t.step + 1;
+            rate = __fdividef(f.lr, -expm1f((float)((double)step * f.log_beta1)));
+            correction = rsqrtf(-expm1f((float)((double)step * f.log_beta2)));
+            key = key_of(f.seed, step);
             at = i;
         }
+        float_pair m[4], v[4], r[4];
         if constexpr (SMALL) {
             decode(cm, sm, m);
             decode(cr, sr, r);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = __fmul_rn(r[j], r[j]);
-        }
+            for (int j = 0; j < 4; ++j) v[j] = mul2(r[j], r[j]);
+        } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float h = clip ? __fmul_rn(g[j], coef) : g[j];
-            m[j] = __fadd_rn(__fmul_rn(m[j], f.b1), __fmul_rn(h, f.a1));
-            v[j] = __fadd_rn(__fmul_rn(v[j], f.b2), __fmul_rn(__fmul_rn(h, h), f.a2));
-            r[j] = __fsqrt_rn(v[j]);
-            const float u = __fdiv_rn(m[j], __fadd_rn(__fmul_rn(r[j], correction), f.eps));
-            p[j] = __fsub_rn(__fmul_rn(p[j], f.keep), __fmul_rn(u, rate));
+            for (int j = 0; j < 4; ++j) m[j] = pair_of(mf[2 * j], mf[2 * j + 1]), v[j] = pair_of(vf[2 * j], vf[2 * j + 1]);
         }
-        store8(reinterpret_cast<T*>(t.p) + e0, n, wide, p);
+        // What the means are made of is rounded operation by operation, so that the codes are those of the definition (the assembler would join a packed
+        // product and sum, but not a product by a number that it does not know to be one); the update takes what is fastest.
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float_pair h = pair_of(gf[2 * j], gf[2 * j + 1]);
+            if (clip) h = mul2(h, both(coef));
+            m[j] = fma2(mul2(m[j], both(f.b1)), both(f.one), mul2(h, both(f.a1)));
+            v[j] = fma2(mul2(v[j], both(f.b2)), both(f.one), mul2(mul2(h, h), both(f.a2)));
+            const float2 w = halves(v[j]);
+            r[j] = pair_of(__fsqrt_rn(w.x), __fsqrt_rn(w.y));
+            const float2 d = halves(fma2(r[j], both(correction), both(f.eps)));
+            const float_pair u = mul2(m[j], pair_of(reciprocal(d.x), reciprocal(d.y)));
+            const float2 p = halves(fma2(u, both(-rate), mul2(pair_of(pf[2 * j], pf[2 * j + 1]), both(f.keep))));
+            pf[2 * j] = p.x, pf[2 * j + 1] = p.y;
+        }
+        store8(reinterpret_cast<T*>(t.p) + e0, n, wide, pf);
         if constexpr (SMALL) {
             uint32_t noise[4];
             const uint32_t place = (uint32_t)((t.place + e0) >> 1);
@@ -241,8 +250,11 @@ __global__ void __launch_bounds__(kThreads) k_adamw(const __grid_constant__ Tabl
             for (int j = 0; j < 4; ++j) noise[j] = mix((place + j) * 0x9E3779B1u + key);
             if (n < kEach)                                        // what lies beyond the tensor is no part of its block
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (j >= n) m[j] = r[j] = 0.f;
+                for (int j = 0; j < 4; ++j) {
+                    const float2 a = halves(m[j]), b = halves(r[j]);
+                    m[j] = pair_of(2 * j < n ? a.x : 0.f, 2 * j + 1 < n ? a.y : 0.f);
+                    r[j] = pair_of(2 * j < n ? b.x : 0.f, 2 * j + 1 < n ? b.y : 0.f);
+                }
             float scale_m, scale_r;
             cm = encode<false>(m, noise, &scale_m);
             cr = encode<true>(r, noise, &scale_r);
@@ -250,8 +262,13 @@ __global__ void __launch_bounds__(kThreads) k_adamw(const __grid_constant__ Tabl
             store_codes(reinterpret_cast<uint8_t*>(t.v) + e0, n, wide, cr);
             if (threadIdx.x % 32 == 0 && block * kBlock < t.n) t.m_scale[block] = scale_m, t.v_scale[block] = scale_r;
         } else {
-            store8(reinterpret_cast<float*>(t.m) + e0, n, wide, m);
-            store8(reinterpret_cast<float*>(t.v) + e0, n, wide, v);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 a = halves(m[j]), b = halves(v[j]);
+                mf[2 * j] = a.x, mf[2 * j + 1] = a.y, vf[2 * j] = b.x, vf[2 * j + 1] = b.y;
+            }
+            store8(reinterpret_cast<float*>(t.m) + e0, n, wide, mf);
+            store8(reinterpret_cast<float*>(t.v) + e0, n, wide, vf);
         }
     }
     // The steps are counted by the CTA that comes last: all others have read them.
@@ -442,9 +459,9 @@ extern "C" int dg_adamw_step(const dg_adamw_tensor* host_tensors, int32_t count,
         return DG_ERR_DIMS;
     if (workspace_bytes < 16) return DG_ERR_SCRATCH;
     Factors f{};
-    f.lr = options->lr, f.beta1 = options->beta1, f.beta2 = options->beta2;
+    f.lr = (float)options->lr, f.log_beta1 = log(options->beta1), f.log_beta2 = log(options->beta2);
     f.b1 = (float)options->beta1, f.a1 = (float)(1.0 - options->beta1), f.b2 = (float)options->beta2, f.a2 = (float)(1.0 - options->beta2);
-    f.eps = (float)options->eps, f.keep = (float)(1.0 - options->lr * options->weight_decay), f.seed = options->seed;
+    f.one = 1.f, f.eps = (float)options->eps, f.keep = (float)(1.0 - options->lr * options->weight_decay), f.seed = options->seed;
     int* arrived = reinterpret_cast<int*>(workspace) + 1;
     const bool small = options->bits == 8;
     return each_table(host_tensors, count, false, options->bits, [&](auto& tab, auto value) {
