@@ -12,6 +12,7 @@
 // What bounds it: HBM for tables (28 bytes an element with 32-bit states, 10 with bf16 and 8), the launch for small models.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -22,20 +23,25 @@ namespace {
 
 using namespace dg;
 
-constexpr int kThreads = 256, kEach = 8, kChunk = kThreads * kEach;      // a lane takes 8 neighbouring elements, a warp one block of 256
+// A lane takes 8 neighbouring elements, a warp one block of 256; a thread works on two such pieces of a chunk at once.
+constexpr int kThreads = 256, kEach = 8, kHalf = kThreads * kEach, kChunk = 2 * kHalf;
 constexpr int kBlock = 256;
-constexpr int kNormCtas = 148 * 8;
+constexpr int kNormCtas = 148 * 8, kStepCtas = 148 * 8;
 constexpr float kLargest = 448.f;
 
-// Tensors of one launch.  Their table travels with the launch, so that a captured graph holds it and nothing has to be copied ahead: 40 entries
-// are 3.4 KB of arguments, 376 the 32 KB that a launch can have.
-template <int CAP> struct Table {
-    dg_adamw_tensor t[CAP];
+// Tensors of one launch.  Their table travels with the launch, so that a captured graph holds it and nothing has to be copied ahead; a launch takes 32 KB of
+// arguments at most, and the more of them the longer: three sizes.
+struct Gradient {
+    const void* g;
+    int64_t n;
+};
+template <class Entry, int CAP> struct Table {
+    Entry t[CAP];
     int32_t first[CAP + 1];               // running count of chunks
     int32_t count;
     uint32_t wide[(CAP + 31) / 32];       // bit: every address on the boundary that whole loads want
 };
-constexpr int kFew = 40, kMany = 376;
+constexpr int kFew = 40, kSome = 136, kMany = 376;
 
 struct Factors {
     double log_beta1, log_beta2;
@@ -44,35 +50,47 @@ struct Factors {
     uint32_t seed;
 };
 
-template <class T> __device__ __forceinline__ float to_float(T v);
-template <> __device__ __forceinline__ float to_float(float v) { return v; }
-template <> __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <> __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
 template <class T> __device__ __forceinline__ T from_float(float v);
 template <> __device__ __forceinline__ float from_float(float v) { return v; }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
 
 // Eight neighbouring elements, as whole 16-byte pieces (8 bytes for codes) or one by one; elements from n on are zero and not stored.
-template <class T> __device__ __forceinline__ void load8(const T* p, int n, bool wide, float* v)
-{
-    if (wide && n >= 8) {
-        if constexpr (sizeof(T) == 4) {
-            const float4 a = __ldcs(reinterpret_cast<const float4*>(p)), b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+template <class T> struct Eight {
+    uint4 raw[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T* p, int n, bool wide)
+    {
+        if (wide && n >= 8) {
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
         } else {
-            const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p));
-            const T* e = reinterpret_cast<const T*>(&a);
+            T* e = reinterpret_cast<T*>(raw);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = to_float(e[i]);
+            for (int i = 0; i < 8; ++i) e[i] = i < n ? p[i] : from_float<T>(0.f);
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < n ? to_float(p[i]) : 0.f;
     }
-}
-template <class T> __device__ __forceinline__ void store8(T* p, int n, bool wide, const float* v)
+    __device__ __forceinline__ float_pair pair(int i) const
+    {
+        const uint32_t w[4] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w};
+        if constexpr (sizeof(T) == 4) {
+            const float* f = reinterpret_cast<const float*>(raw);
+            return pair_of(f[2 * i], f[2 * i + 1]);
+        } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+            return pair_of(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
+        } else {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            return pair_of(f.x, f.y);
+        }
+    }
+};
+template <class T> __device__ __forceinline__ void store8(T* p, int n, bool wide, const float_pair* pairs)
 {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = halves(pairs[i]);
+        v[2 * i] = f.x, v[2 * i + 1] = f.y;
+    }
     if (wide && n >= 8) {
         if constexpr (sizeof(T) == 4) {
             __stcs(reinterpret_cast<float4*>(p), make_float4(v[0], v[1], v[2], v[3]));
@@ -113,6 +131,18 @@ __device__ __forceinline__ void decode(uint2 c, float scale, float_pair* v)
         const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> (i % 2 * 16)), __NV_E4M3)));
         v[i] = mul2(pair_of(f.x, f.y), both(scale));
     }
+}
+
+// The square root, by Newton's step with the remainder from a fused product (Markstein, IBM Journal of Research and Development, 1990): the correctly
+// rounded one but for a few arguments in a million, where it is the neighbour.  Below fp32's smallest normal number it is too small by up to a third.
+__device__ __forceinline__ float_pair square_root(float_pair v)
+{
+    const float2 f = halves(v);
+    float a, b;
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(fmaxf(f.x, 0x1p-126f)));
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(fmaxf(f.y, 0x1p-126f)));
+    const float_pair y = pair_of(a, b), s = mul2(v, y);
+    return fma2(fma2(mul2(s, both(-1.f)), s, v), mul2(y, both(0.5f)), s);
 }
 
 // Random numbers: xor-shift and product, twice, for a pair of neighbours, 16 bits for each.  The odd factors are the leading bits of the golden
@@ -165,7 +195,7 @@ template <bool POSITIVE> __device__ __forceinline__ uint2 encode(const float_pai
     return make_uint2(c[0], c[1]);
 }
 
-template <int CAP> __device__ __forceinline__ int find(const Table<CAP>& tab, int chunk)
+template <class Tab> __device__ __forceinline__ int find(const Tab& tab, int chunk)
 {
     int lo = 0, hi = tab.count - 1;
     while (lo < hi) {
@@ -177,15 +207,15 @@ template <int CAP> __device__ __forceinline__ int find(const Table<CAP>& tab, in
 }
 
 template <class T, bool SMALL, int CAP>
-__global__ void __launch_bounds__(kThreads, SMALL ? 4 : 3) k_adamw(const __grid_constant__ Table<CAP> tab, const Factors f, const float* __restrict__ clip,
+__global__ void __launch_bounds__(kThreads, SMALL ? 3 : 2) k_adamw(const __grid_constant__ Table<dg_adamw_tensor, CAP> tab, const Factors f, const float* __restrict__ clip,
                                                                   int* __restrict__ arrived)
 {
-    __shared__ int last;
     const int chunks = tab.first[tab.count];
     int at = -1;
     float rate = 0.f, correction = 0.f;
     uint32_t key = 0;
     const float coef = clip ? __ldg(clip) : 1.f;
+    int before = 0;
     for (int chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
         int i = at;
         if (at < 0) i = find(tab, chunk);
@@ -193,23 +223,31 @@ __global__ void __launch_bounds__(kThreads, SMALL ? 4 : 3) k_adamw(const __grid_
             while (tab.first[i + 1] <= chunk) ++i;
         const dg_adamw_tensor& t = tab.t[i];
         const bool wide = tab.wide[i / 32] >> (i % 32) & 1;
-        const int64_t e0 = (int64_t)(chunk - tab.first[i]) * kChunk + threadIdx.x * kEach;
-        const int n = (int)max((int64_t)0, min((int64_t)kEach, t.n - e0));
-        float pf[8], gf[8];
-        [[maybe_unused]] float mf[8], vf[8];
-        [[maybe_unused]] uint2 cm, cr;
-        float sm = 0.f, sr = 0.f;
-        const int64_t block = e0 / kBlock;
-        load8(reinterpret_cast<const T*>(t.g) + e0, n, wide, gf);
-        if constexpr (SMALL) {
-            cm = load_codes(reinterpret_cast<const uint8_t*>(t.m) + e0, n, wide);
-            cr = load_codes(reinterpret_cast<const uint8_t*>(t.v) + e0, n, wide);
-            if (block * kBlock < t.n) sm = t.m_scale[block], sr = t.v_scale[block];
-        } else {
-            load8(reinterpret_cast<const float*>(t.m) + e0, n, wide, mf);
-            load8(reinterpret_cast<const float*>(t.v) + e0, n, wide, vf);
+        const int64_t e0 = (int64_t)(chunk - tab.first[i]) * kChunk + threadIdx.x * kEach, left = t.n - e0;
+        using State = std::conditional_t<SMALL, uint8_t, float>;
+        T* const p_at = reinterpret_cast<T*>(t.p) + e0;
+        const T* const g_at = reinterpret_cast<const T*>(t.g) + e0;
+        State *const m_at = reinterpret_cast<State*>(t.m) + e0, *const v_at = reinterpret_cast<State*>(t.v) + e0;
+        float *const sm_at = SMALL ? t.m_scale + e0 / kBlock : nullptr, *const sv_at = SMALL ? t.v_scale + e0 / kBlock : nullptr;
+        int n[2];
+        Eight<T> p_in[2], g_in[2];
+        [[maybe_unused]] Eight<float> m_in[2], v_in[2];
+        [[maybe_unused]] uint2 cm[2], cv[2];
+        float sm[2] = {0.f, 0.f}, sv[2] = {0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            n[u] = (int)max((int64_t)0, min((int64_t)kEach, left - u * kHalf));
+            g_in[u].load(g_at + u * kHalf, n[u], wide);
+            if constexpr (SMALL) {
+                cm[u] = load_codes(m_at + u * kHalf, n[u], wide);
+                cv[u] = load_codes(v_at + u * kHalf, n[u], wide);
+                if (n[u] > 0) sm[u] = sm_at[u * (kHalf / kBlock)], sv[u] = sv_at[u * (kHalf / kBlock)];
+            } else {
+                m_in[u].load(m_at + u * kHalf, n[u], wide);
+                v_in[u].load(v_at + u * kHalf, n[u], wide);
+            }
+            p_in[u].load(p_at + u * kHalf, n[u], wide);
         }
-        load8(reinterpret_cast<const T*>(t.p) + e0, n, wide, pf);
         if (i != at) {                                            // 1 - b^t = -expm1(t log b)
             const int64_t step = *t.step + 1;
             rate = __fdividef(f.lr, -expm1f((float)((double)step * f.log_beta1)));
@@ -217,75 +255,71 @@ __global__ void __launch_bounds__(kThreads, SMALL ? 4 : 3) k_adamw(const __grid_
             key = key_of(f.seed, step);
             at = i;
         }
-        float_pair m[4], v[4], r[4];
-        if constexpr (SMALL) {
-            decode(cm, sm, m);
-            decode(cr, sr, r);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = mul2(r[j], r[j]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) m[j] = pair_of(mf[2 * j], mf[2 * j + 1]), v[j] = pair_of(vf[2 * j], vf[2 * j + 1]);
+        if (chunk + (int)gridDim.x >= chunks) {                   // no more steps to read here
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                __threadfence();
+                before = atomicAdd(arrived, 1);
+            }
         }
-        // What the means are made of is rounded operation by operation, so that the codes are those of the definition (the assembler would join a packed
-        // product and sum, but not a product by a number that it does not know to be one); the update takes what is fastest.
+        const uint32_t place = (uint32_t)((t.place + e0) >> 1);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            float_pair h = pair_of(gf[2 * j], gf[2 * j + 1]);
-            if (clip) h = mul2(h, both(coef));
-            m[j] = fma2(mul2(m[j], both(f.b1)), both(f.one), mul2(h, both(f.a1)));
-            v[j] = fma2(mul2(v[j], both(f.b2)), both(f.one), mul2(mul2(h, h), both(f.a2)));
-            const float2 w = halves(v[j]);
-            r[j] = pair_of(__fsqrt_rn(w.x), __fsqrt_rn(w.y));
-            const float2 d = halves(fma2(r[j], both(correction), both(f.eps)));
-            const float_pair u = mul2(m[j], pair_of(reciprocal(d.x), reciprocal(d.y)));
-            const float2 p = halves(fma2(u, both(-rate), mul2(pair_of(pf[2 * j], pf[2 * j + 1]), both(f.keep))));
-            pf[2 * j] = p.x, pf[2 * j + 1] = p.y;
-        }
-        store8(reinterpret_cast<T*>(t.p) + e0, n, wide, pf);
-        if constexpr (SMALL) {
-            uint32_t noise[4];
-            const uint32_t place = (uint32_t)((t.place + e0) >> 1);
+        for (int u = 0; u < 2; ++u) {
+            float_pair p[4], m[4], v[4], r[4];
+            if constexpr (SMALL) {
+                decode(cm[u], sm[u], m);
+                decode(cv[u], sv[u], r);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) noise[j] = mix((place + j) * 0x9E3779B1u + key);
-            if (n < kEach)                                        // what lies beyond the tensor is no part of its block
+                for (int j = 0; j < 4; ++j) v[j] = mul2(r[j], r[j]);
+            } else {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float2 a = halves(m[j]), b = halves(r[j]);
-                    m[j] = pair_of(2 * j < n ? a.x : 0.f, 2 * j + 1 < n ? a.y : 0.f);
-                    r[j] = pair_of(2 * j < n ? b.x : 0.f, 2 * j + 1 < n ? b.y : 0.f);
-                }
-            float scale_m, scale_r;
-            cm = encode<false>(m, noise, &scale_m);
-            cr = encode<true>(r, noise, &scale_r);
-            store_codes(reinterpret_cast<uint8_t*>(t.m) + e0, n, wide, cm);
-            store_codes(reinterpret_cast<uint8_t*>(t.v) + e0, n, wide, cr);
-            if (threadIdx.x % 32 == 0 && block * kBlock < t.n) t.m_scale[block] = scale_m, t.v_scale[block] = scale_r;
-        } else {
+                for (int j = 0; j < 4; ++j) m[j] = m_in[u].pair(j), v[j] = v_in[u].pair(j);
+            }
+            // What the means are made of is rounded operation by operation, so that the codes are those of the definition (the assembler would join a
+            // packed product and sum, but not a product by a number that it does not know to be one); the update takes what is fastest.
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float2 a = halves(m[j]), b = halves(v[j]);
-                mf[2 * j] = a.x, mf[2 * j + 1] = a.y, vf[2 * j] = b.x, vf[2 * j + 1] = b.y;
+                float_pair h = g_in[u].pair(j);
+                if (clip) h = mul2(h, both(coef));
+                m[j] = fma2(mul2(m[j], both(f.b1)), both(f.one), mul2(h, both(f.a1)));
+                v[j] = fma2(mul2(v[j], both(f.b2)), both(f.one), mul2(mul2(h, h), both(f.a2)));
+                r[j] = square_root(v[j]);
+                const float2 d = halves(fma2(r[j], both(correction), both(f.eps)));
+                const float_pair x = mul2(m[j], pair_of(reciprocal(d.x), reciprocal(d.y)));
+                p[j] = fma2(x, both(-rate), mul2(p_in[u].pair(j), both(f.keep)));
             }
-            store8(reinterpret_cast<float*>(t.m) + e0, n, wide, mf);
-            store8(reinterpret_cast<float*>(t.v) + e0, n, wide, vf);
+            store8(p_at + u * kHalf, n[u], wide, p);
+            if constexpr (SMALL) {
+                uint32_t noise[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) noise[j] = mix((place + u * (kHalf / 2) + j) * 0x9E3779B1u + key);
+                if (n[u] < kEach)                                 // what lies beyond the tensor is no part of its block
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 a = halves(m[j]), b = halves(r[j]);
+                        m[j] = pair_of(2 * j < n[u] ? a.x : 0.f, 2 * j + 1 < n[u] ? a.y : 0.f);
+                        r[j] = pair_of(2 * j < n[u] ? b.x : 0.f, 2 * j + 1 < n[u] ? b.y : 0.f);
+                    }
+                float scale_m, scale_v;
+                const uint2 to_m = encode<false>(m, noise, &scale_m), to_v = encode<true>(r, noise, &scale_v);
+                store_codes(m_at + u * kHalf, n[u], wide, to_m);
+                store_codes(v_at + u * kHalf, n[u], wide, to_v);
+                if (threadIdx.x % 32 == 0 && n[u] > 0) sm_at[u * (kHalf / kBlock)] = scale_m, sv_at[u * (kHalf / kBlock)] = scale_v;
+            } else {
+                store8(m_at + u * kHalf, n[u], wide, m);
+                store8(v_at + u * kHalf, n[u], wide, v);
+            }
         }
     }
-    // The steps are counted by the CTA that comes last: all others have read them.
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        __threadfence();
-        last = atomicAdd(arrived, 1) == (int)gridDim.x - 1;
-    }
-    __syncthreads();
-    if (!last) return;
-    for (int i = threadIdx.x; i < tab.count; i += kThreads) ++*tab.t[i].step;
+    // The CTA that was last to have read its steps counts them all up.
+    if (threadIdx.x >= 32 || __shfl_sync(0xffffffffu, before, 0) != (int)gridDim.x - 1) return;
+    for (int k = threadIdx.x; k < tab.count; k += 32) ++*tab.t[k].step;
     if (threadIdx.x == 0) *arrived = 0;
 }
 
 // Sum of squares in 64 bits, every CTA's in its own place; the CTA that comes last of the last launch adds them in order.
 template <class T, int CAP>
-__global__ void __launch_bounds__(kThreads) k_grad_norm(const __grid_constant__ Table<CAP> tab, double* __restrict__ partial, int total, double max_norm,
+__global__ void __launch_bounds__(kThreads) k_grad_norm(const __grid_constant__ Table<Gradient, CAP> tab, double* __restrict__ partial, int total, double max_norm,
                                                         float* __restrict__ result, int* __restrict__ arrived)
 {
     __shared__ double warp_sum[kThreads / 32];
@@ -306,13 +340,21 @@ __global__ void __launch_bounds__(kThreads) k_grad_norm(const __grid_constant__ 
         if (i < 0) i = find(tab, chunk);
         else
             while (tab.first[i + 1] <= chunk) ++i;
-        const dg_adamw_tensor& t = tab.t[i];
+        const Gradient& t = tab.t[i];
         const int64_t e0 = (int64_t)(chunk - tab.first[i]) * kChunk + threadIdx.x * kEach;
-        const int n = (int)max((int64_t)0, min((int64_t)kEach, t.n - e0));
-        float g[8];
-        load8(reinterpret_cast<const T*>(t.g) + e0, n, tab.wide[i / 32] >> (i % 32) & 1, g);
+        const bool wide = tab.wide[i / 32] >> (i % 32) & 1;
+        Eight<T> g[2];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sum += (double)g[j] * (double)g[j];
+        for (int u = 0; u < 2; ++u)
+            g[u].load(reinterpret_cast<const T*>(t.g) + e0 + u * kHalf, (int)max((int64_t)0, min((int64_t)kEach, t.n - e0 - u * kHalf)), wide);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 f = halves(g[u].pair(j));
+                sum += (double)f.x * (double)f.x;
+                sum += (double)f.y * (double)f.y;
+            }
     }
     sum = sum_of_cta(sum);
     if (threadIdx.x == 0) partial[blockIdx.x] = sum;
@@ -340,7 +382,14 @@ bool aligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) %
 int64_t chunks_of(int64_t n) { return (n + kChunk - 1) / kChunk; }
 
 // Fills a table with as many of the tensors [at, count) of `type` as it holds; returns where the next one starts.
-template <int CAP> int fill(Table<CAP>* tab, const dg_adamw_tensor* t, int at, int count, int32_t type, bool norm, int32_t bits)
+void entry(dg_adamw_tensor* to, const dg_adamw_tensor& t) { *to = t; }
+void entry(Gradient* to, const dg_adamw_tensor& t) { *to = {t.g, t.n}; }
+bool whole(const dg_adamw_tensor*, const dg_adamw_tensor& t, int32_t bits)
+{
+    return aligned(t.g, 16) && aligned(t.p, 16) && aligned(t.m, bits == 8 ? 8 : 16) && aligned(t.v, bits == 8 ? 8 : 16);
+}
+bool whole(const Gradient*, const dg_adamw_tensor& t, int32_t) { return aligned(t.g, 16); }
+template <class Entry, int CAP> int fill(Table<Entry, CAP>* tab, const dg_adamw_tensor* t, int at, int count, int32_t type, int32_t bits)
 {
     int64_t chunks = 0;
     tab->count = 0;
@@ -350,12 +399,10 @@ template <int CAP> int fill(Table<CAP>* tab, const dg_adamw_tensor* t, int at, i
         const int64_t more = chunks_of(t[at].n);
         if (chunks + more >= (int64_t)1 << 30) break;             // chunk numbers, with a stride added, stay within 31 bits
         const int k = tab->count++;
-        tab->t[k] = t[at];
+        entry(&tab->t[k], t[at]);
         tab->first[k] = (int32_t)chunks;
         chunks += more;
-        bool wide = aligned(t[at].g, 16);
-        if (!norm) wide = wide && aligned(t[at].p, 16) && aligned(t[at].m, bits == 8 ? 8 : 16) && aligned(t[at].v, bits == 8 ? 8 : 16);
-        if (wide) tab->wide[k / 32] |= 1u << (k % 32);
+        if (whole(tab->t, t[at], bits)) tab->wide[k / 32] |= 1u << (k % 32);
     }
     tab->first[tab->count] = (int32_t)chunks;
     return at;
@@ -380,26 +427,31 @@ int check(const dg_adamw_tensor* t, int32_t count, int32_t bits, bool norm)
     return DG_OK;
 }
 
-// `use(table, type constant, first?)` for as many tables as the tensors need; the form by how many there are.
-template <class Use> int each_table(const dg_adamw_tensor* t, int32_t count, bool norm, int32_t bits, Use use)
+// `use(table, type constant, last)` for as many tables as the tensors need, in the smallest size that holds them, or the largest.
+template <class Entry, class Use> int each_table(const dg_adamw_tensor* t, int32_t count, int32_t bits, Use use)
 {
-    auto run = [&](auto* tab, int32_t type, auto value) {
-        for (int at = 0; at < count;) {
-            at = fill(tab, t, at, count, type, norm, bits);
-            if (tab->count == 0) continue;
-            const int rc = use(*tab, value);
-            if (rc) return rc;
-        }
-        return (int)DG_OK;
-    };
-    Table<kFew> few;
-    Table<kMany> many;
+    int have[3] = {0, 0, 0};
+    for (int32_t i = 0; i < count; ++i) have[t[i].type] += t[i].n > 0;
     for (int32_t type = 0; type < 3; ++type) {
-        int have = 0;
-        for (int32_t i = 0; i < count; ++i) have += t[i].type == type && t[i].n > 0;
-        if (have == 0) continue;
-        auto with = [&](auto value) { return have <= kFew ? run(&few, type, value) : run(&many, type, value); };
-        const int rc = type == DG_FLOAT32 ? with(float{}) : type == DG_BFLOAT16 ? with(__nv_bfloat16{}) : with(__half{});
+        if (have[type] == 0) continue;
+        const bool more_types = (type < 1 && have[1]) || (type < 2 && have[2]);
+        auto with = [&](auto cap, auto value) {
+            Table<Entry, decltype(cap)::value> tab;
+            int left = have[type];
+            for (int at = 0; left > 0;) {
+                at = fill(&tab, t, at, count, type, bits);
+                left -= tab.count;
+                const int rc = use(tab, value, left == 0 && !more_types);
+                if (rc) return rc;
+            }
+            return (int)DG_OK;
+        };
+        auto sized = [&](auto value) {
+            if (have[type] <= kFew) return with(std::integral_constant<int, kFew>{}, value);
+            if (have[type] <= kSome) return with(std::integral_constant<int, kSome>{}, value);
+            return with(std::integral_constant<int, kMany>{}, value);
+        };
+        const int rc = type == DG_FLOAT32 ? sized(float{}) : type == DG_BFLOAT16 ? sized(__nv_bfloat16{}) : sized(__half{});
         if (rc) return rc;
     }
     return DG_OK;
@@ -428,24 +480,18 @@ extern "C" int dg_grad_norm(const dg_adamw_tensor* host_tensors, int32_t count, 
     if (!result || !workspace) return DG_ERR_NULL;
     if (!(max_norm > 0.0) || !aligned(workspace, 16)) return DG_ERR_DIMS;
     if (workspace_bytes < dg_adamw_workspace(host_tensors, count)) return DG_ERR_SCRATCH;
-    // every launch's CTAs first, then the last launch once more with the result: so the tables are counted ahead
-    int launches = 0;
-    rc = each_table(host_tensors, count, true, 32, [&](auto&, auto) { return ++launches, (int)DG_OK; });
-    if (rc) return rc;
     int* arrived = reinterpret_cast<int*>(workspace);
     double* partial = reinterpret_cast<double*>(reinterpret_cast<char*>(workspace) + 16);
-    if (launches == 0) {
-        const float none[2] = {0.f, 1.f};
-        return (int)cudaMemcpyAsync(result, none, sizeof none, cudaMemcpyHostToDevice, (cudaStream_t)stream);
-    }
-    int total = 0, done = 0;
-    return each_table(host_tensors, count, true, 32, [&](auto& tab, auto value) {
+    int total = 0;
+    rc = each_table<Gradient>(host_tensors, count, 32, [&](auto& tab, auto value, bool last) {
         const int grid = std::min(kNormCtas, (int)tab.first[tab.count]);
-        const bool end = ++done == launches;
-        k_grad_norm<decltype(value)><<<grid, kThreads, 0, (cudaStream_t)stream>>>(tab, partial + total, total + grid, max_norm, end ? result : nullptr, arrived);
         total += grid;
+        k_grad_norm<decltype(value)><<<grid, kThreads, 0, (cudaStream_t)stream>>>(tab, partial + total - grid, total, max_norm, last ? result : nullptr, arrived);
         return (int)cudaGetLastError();
     });
+    if (rc || total > 0) return rc;
+    const float none[2] = {0.f, 1.f};
+    return (int)cudaMemcpyAsync(result, none, sizeof none, cudaMemcpyHostToDevice, (cudaStream_t)stream);
 }
 
 extern "C" int dg_adamw_step(const dg_adamw_tensor* host_tensors, int32_t count, const dg_adamw_options* options, const float* clip, void* workspace,
@@ -464,9 +510,9 @@ extern "C" int dg_adamw_step(const dg_adamw_tensor* host_tensors, int32_t count,
     f.one = 1.f, f.eps = (float)options->eps, f.keep = (float)(1.0 - options->lr * options->weight_decay), f.seed = options->seed;
     int* arrived = reinterpret_cast<int*>(workspace) + 1;
     const bool small = options->bits == 8;
-    return each_table(host_tensors, count, false, options->bits, [&](auto& tab, auto value) {
+    return each_table<dg_adamw_tensor>(host_tensors, count, options->bits, [&](auto& tab, auto value, bool) {
         using T = decltype(value);
-        const int grid = std::min(148 * 8, (int)tab.first[tab.count]);
+        const int grid = std::min(kStepCtas, (int)tab.first[tab.count]);
         if (small) k_adamw<T, true><<<grid, kThreads, 0, (cudaStream_t)stream>>>(tab, f, clip, arrived);
         else k_adamw<T, false><<<grid, kThreads, 0, (cudaStream_t)stream>>>(tab, f, clip, arrived);
         return (int)cudaGetLastError();
