@@ -58,11 +58,15 @@ template <> __device__ __forceinline__ __half from_float(float v) { return __flo
 // Eight neighbouring elements, as whole 16-byte pieces (8 bytes for codes) or one by one; elements from n on are zero and not stored.
 template <class T> struct Eight {
     uint4 raw[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T* p)
+    {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+    }
     __device__ __forceinline__ void load(const T* p, int n, bool wide)
     {
         if (wide && n >= 8) {
-#pragma unroll
-            for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+            load(p);
         } else {
             T* e = reinterpret_cast<T*>(raw);
 #pragma unroll
@@ -158,7 +162,7 @@ __device__ __forceinline__ uint32_t key_of(uint32_t seed, int64_t step) { return
 // A block's values, eight a lane, as codes and a scale.  q = |x| 448 / largest; times 2^-120 the smallest normal number of e4m3 is the smallest one of fp32, so
 // that an fp32 number's leading bits are the code, below 2^-6 too where both step evenly.  The noise is added below the code's last bit.
 // (q times 2^-120 in one factor would leave fp32's range where the block's largest is beyond 28,672.)
-template <bool POSITIVE> __device__ __forceinline__ uint2 encode(const float_pair* x, const uint32_t* noise, float* scale)
+__device__ __forceinline__ float largest(const float_pair* x)
 {
     float most = 0.f;
 #pragma unroll
@@ -167,24 +171,23 @@ template <bool POSITIVE> __device__ __forceinline__ uint2 encode(const float_pai
         asm("max.NaN.f32 %0, %0, %1;" : "+f"(most) : "f"(fabsf(f.x)));
         asm("max.NaN.f32 %0, %0, %1;" : "+f"(most) : "f"(fabsf(f.y)));
     }
-    most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most) & 0x7FFFFFFFu));      // magnitudes are ordered as their bits, NaN above all
-    const bool none = most < 1e-30f;
-    const float factor = none ? 0.f : __fmul_rn(__frcp_rn(most), kLargest);
-    *scale = none ? 0.f : __fmul_rn(most, 1.f / kLargest);
+    return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most) & 0x7FFFFFFFu));      // magnitudes are ordered as their bits, NaN above all
+}
+template <bool ROOT> __device__ __forceinline__ uint2 codes(const float_pair* x, const uint32_t* noise, float factor)
+{
     uint32_t c[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         uint32_t t[4];                                            // the code in the leading byte; the sign is shifted out
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const float_pair q = mul2(x[2 * i + j], both(factor));
-            const float2 f = halves(x[2 * i + j]), l = halves(mul2(q, both(0x1p-120f)));
+            const float2 f = halves(x[2 * i + j]), l = halves(mul2(mul2(x[2 * i + j], both(factor)), both(0x1p-120f)));
             const uint32_t n = noise[2 * i + j];
             t[2 * j] = (__float_as_uint(l.x) << 4) + __byte_perm(n, 0, 0x4104);
             t[2 * j + 1] = (__float_as_uint(l.y) << 4) + __byte_perm(n, 0, 0x4324);
-            if (POSITIVE) {
-                t[2 * j] = max(t[2 * j], f.x > 0.f ? 0x01000000u : 0u);
-                t[2 * j + 1] = max(t[2 * j + 1], f.y > 0.f ? 0x01000000u : 0u);
+            if (ROOT) {                                           // code 1 for what is above zero: the bits of 2^-125 and more reach that far
+                t[2 * j] = max(t[2 * j], min(__float_as_uint(f.x), 0x01000000u));
+                t[2 * j + 1] = max(t[2 * j + 1], min(__float_as_uint(f.y), 0x01000000u));
             } else {
                 t[2 * j] |= __float_as_uint(f.x) & 0x80000000u;
                 t[2 * j + 1] |= __float_as_uint(f.y) & 0x80000000u;
@@ -194,16 +197,25 @@ template <bool POSITIVE> __device__ __forceinline__ uint2 encode(const float_pai
     }
     return make_uint2(c[0], c[1]);
 }
+// 448 / largest as the product of 448 and the reciprocal, which Newton's step with fused products rounds correctly (Markstein, as above).  Blocks whose largest
+// is beyond 2^125, where the reciprocal leaves fp32's normal range, or below 1e-30, are zero.
+__device__ __forceinline__ void encode(const float_pair* m, const float_pair* r, const uint32_t* noise, uint2* to_m, uint2* to_r, float* scale_m, float* scale_r)
+{
+    const float top_m = largest(m), top_r = largest(r);
+    const float_pair top = pair_of(top_m, top_r), y = pair_of(reciprocal(top_m), reciprocal(top_r));
+    const float2 f = halves(mul2(fma2(fma2(mul2(top, both(-1.f)), y, both(1.f)), y, y), both(kLargest))), s = halves(mul2(top, both(1.f / kLargest)));
+    const bool none_m = top_m < 1e-30f, none_r = top_r < 1e-30f;
+    *scale_m = none_m ? 0.f : s.x, *scale_r = none_r ? 0.f : s.y;
+    *to_m = codes<false>(m, noise, none_m ? 0.f : f.x);
+    *to_r = codes<true>(r, noise, none_r ? 0.f : f.y);
+}
 
+// The tensor that a chunk belongs to, by all threads of the CTA.
 template <class Tab> __device__ __forceinline__ int find(const Tab& tab, int chunk)
 {
-    int lo = 0, hi = tab.count - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (tab.first[mid] <= chunk) lo = mid;
-        else hi = mid - 1;
-    }
-    return lo;
+    int before = 0;
+    for (int k = 0; k < tab.count; k += kThreads) before += __syncthreads_count(k + (int)threadIdx.x < tab.count && tab.first[k + threadIdx.x] <= chunk);
+    return before - 1;
 }
 
 template <class T, bool SMALL, int CAP>
@@ -229,24 +241,38 @@ __global__ void __launch_bounds__(kThreads, SMALL ? 3 : 2) k_adamw(const __grid_
         const T* const g_at = reinterpret_cast<const T*>(t.g) + e0;
         State *const m_at = reinterpret_cast<State*>(t.m) + e0, *const v_at = reinterpret_cast<State*>(t.v) + e0;
         float *const sm_at = SMALL ? t.m_scale + e0 / kBlock : nullptr, *const sv_at = SMALL ? t.v_scale + e0 / kBlock : nullptr;
-        int n[2];
+        const bool full = wide && left >= kHalf + kEach;          // nothing of this thread's lies beyond the tensor
         Eight<T> p_in[2], g_in[2];
         [[maybe_unused]] Eight<float> m_in[2], v_in[2];
         [[maybe_unused]] uint2 cm[2], cv[2];
         float sm[2] = {0.f, 0.f}, sv[2] = {0.f, 0.f};
+        auto count = [&](int u) { return (int)max((int64_t)0, min((int64_t)kEach, left - u * kHalf)); };
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            n[u] = (int)max((int64_t)0, min((int64_t)kEach, left - u * kHalf));
-            g_in[u].load(g_at + u * kHalf, n[u], wide);
-            if constexpr (SMALL) {
-                cm[u] = load_codes(m_at + u * kHalf, n[u], wide);
-                cv[u] = load_codes(v_at + u * kHalf, n[u], wide);
-                if (n[u] > 0) sm[u] = sm_at[u * (kHalf / kBlock)], sv[u] = sv_at[u * (kHalf / kBlock)];
+            if (full) {
+                g_in[u].load(g_at + u * kHalf);
+                if constexpr (SMALL) {
+                    cm[u] = __ldcs(reinterpret_cast<const uint2*>(m_at + u * kHalf));
+                    cv[u] = __ldcs(reinterpret_cast<const uint2*>(v_at + u * kHalf));
+                    sm[u] = sm_at[u * (kHalf / kBlock)], sv[u] = sv_at[u * (kHalf / kBlock)];
+                } else {
+                    m_in[u].load(m_at + u * kHalf);
+                    v_in[u].load(v_at + u * kHalf);
+                }
+                p_in[u].load(p_at + u * kHalf);
             } else {
-                m_in[u].load(m_at + u * kHalf, n[u], wide);
-                v_in[u].load(v_at + u * kHalf, n[u], wide);
+                const int n = count(u);
+                g_in[u].load(g_at + u * kHalf, n, wide);
+                if constexpr (SMALL) {
+                    cm[u] = load_codes(m_at + u * kHalf, n, wide);
+                    cv[u] = load_codes(v_at + u * kHalf, n, wide);
+                    if (n > 0) sm[u] = sm_at[u * (kHalf / kBlock)], sv[u] = sv_at[u * (kHalf / kBlock)];
+                } else {
+                    m_in[u].load(m_at + u * kHalf, n, wide);
+                    v_in[u].load(v_at + u * kHalf, n, wide);
+                }
+                p_in[u].load(p_at + u * kHalf, n, wide);
             }
-            p_in[u].load(p_at + u * kHalf, n[u], wide);
         }
         if (i != at) {                                            // 1 - b^t = -expm1(t log b)
             const int64_t step = *t.step + 1;
@@ -288,26 +314,28 @@ __global__ void __launch_bounds__(kThreads, SMALL ? 3 : 2) k_adamw(const __grid_
                 const float_pair x = mul2(m[j], pair_of(reciprocal(d.x), reciprocal(d.y)));
                 p[j] = fma2(x, both(-rate), mul2(p_in[u].pair(j), both(f.keep)));
             }
-            store8(p_at + u * kHalf, n[u], wide, p);
+            const int n = full ? kEach : count(u);
+            store8(p_at + u * kHalf, n, wide, p);
             if constexpr (SMALL) {
                 uint32_t noise[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) noise[j] = mix((place + u * (kHalf / 2) + j) * 0x9E3779B1u + key);
-                if (n[u] < kEach)                                 // what lies beyond the tensor is no part of its block
+                if (n < kEach)                                    // what lies beyond the tensor is no part of its block
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const float2 a = halves(m[j]), b = halves(r[j]);
-                        m[j] = pair_of(2 * j < n[u] ? a.x : 0.f, 2 * j + 1 < n[u] ? a.y : 0.f);
-                        r[j] = pair_of(2 * j < n[u] ? b.x : 0.f, 2 * j + 1 < n[u] ? b.y : 0.f);
+                        m[j] = pair_of(2 * j < n ? a.x : 0.f, 2 * j + 1 < n ? a.y : 0.f);
+                        r[j] = pair_of(2 * j < n ? b.x : 0.f, 2 * j + 1 < n ? b.y : 0.f);
                     }
                 float scale_m, scale_v;
-                const uint2 to_m = encode<false>(m, noise, &scale_m), to_v = encode<true>(r, noise, &scale_v);
-                store_codes(m_at + u * kHalf, n[u], wide, to_m);
-                store_codes(v_at + u * kHalf, n[u], wide, to_v);
-                if (threadIdx.x % 32 == 0 && n[u] > 0) sm_at[u * (kHalf / kBlock)] = scale_m, sv_at[u * (kHalf / kBlock)] = scale_v;
+                uint2 to_m, to_v;
+                encode(m, r, noise, &to_m, &to_v, &scale_m, &scale_v);
+                store_codes(m_at + u * kHalf, n, wide, to_m);
+                store_codes(v_at + u * kHalf, n, wide, to_v);
+                if (threadIdx.x % 32 == 0 && n > 0) sm_at[u * (kHalf / kBlock)] = scale_m, sv_at[u * (kHalf / kBlock)] = scale_v;
             } else {
-                store8(m_at + u * kHalf, n[u], wide, m);
-                store8(v_at + u * kHalf, n[u], wide, v);
+                store8(m_at + u * kHalf, n, wide, m);
+                store8(v_at + u * kHalf, n, wide, v);
             }
         }
     }
