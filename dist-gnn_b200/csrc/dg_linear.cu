@@ -674,8 +674,10 @@ int dz_ctas(int64_t M, int32_t N)
 // ---- few rows -----------------------------------------------------------------------------------------------------------------
 // 16 bits: y^T by mma.m16n8k16 with x along the 16 rows.  The order in which k goes through the sum is free as long as both operands agree on it, so a thread
 // takes four neighbouring k's of both: 8 bytes of a row of x, and four rows (w [K x N], four neighbouring columns each, which are then columns of four
-// MMAs) or 8 bytes of a row (w [N x K]) of w.  A CTA makes 32 columns; its warps share K, and their sums meet in shared memory.
-constexpr int kFewRows = 16, kFewWarps = 8, kFewCols = 32;
+// MMAs) or 8 bytes of a row (w [N x K]) of w.  A CTA makes 32 columns, or 16; its warps share K, and their sums meet in shared memory.  Rows and columns
+// beyond the matrix are read as the last ones, so that the loads of four steps go out together: with a question at each, 16 x 1024 -> 1024 took 10.3 us.
+constexpr int kFewRows = 16, kFewWarps = 16;
+template <bool OUT_IN> constexpr int kFewCols = OUT_IN ? 16 : 32;
 
 template <class T> __device__ __forceinline__ uint2 load4(const T* p, int n, bool whole)
 {
@@ -703,14 +705,15 @@ struct FewArgs {
     int32_t N, K, act, whole_x, whole_w;
 };
 
-// One element of the result, from its sum.  Lanes of a warp hold the 32 columns of a row from a multiple of 32 on.
+// One element of the result, from its sum.  Lanes of a warp, or of half a warp, hold as many neighbouring columns of a row, the first a multiple of their number;
+// elements beyond the matrix are not written.
 template <class T> __device__ __forceinline__ void finish(const FewArgs& a, int64_t m, int col, float z)
 {
-    const bool live = col < a.N;
+    const bool live = col < a.N && m < a.M;
     if (live && a.bias) z += Pair<T>::one(static_cast<const T*>(a.bias)[col]);
-    if (a.bits) {
-        const uint32_t word = __ballot_sync(0xffffffffu, live && !(z <= 0.f));
-        if (threadIdx.x % 32 == 0) a.bits[m * a.ldbits + col / 32] = word;
+    if (a.bits) {                                                 // 16 columns a half warp
+        const uint32_t word = __ballot_sync(0xffffffffu, live && !(z <= 0.f)) >> (threadIdx.x & 16);
+        if (threadIdx.x % 16 == 0 && m < a.M) reinterpret_cast<unsigned short*>(a.bits + m * a.ldbits)[col / 16] = (unsigned short)word;
     }
     if (!live) return;
     if (a.z) static_cast<T*>(a.z)[m * a.ldz + col] = Pair<T>::round(z);
@@ -722,95 +725,111 @@ template <class T> __device__ __forceinline__ void finish(const FewArgs& a, int6
 template <class T, bool OUT_IN>
 __global__ void __launch_bounds__(32 * kFewWarps) k_few_rows16(const FewArgs a)
 {
-    __shared__ float sums[kFewWarps][kFewRows][kFewCols + 1];
+    constexpr int kCols = kFewCols<OUT_IN>, kMmas = kCols / 8;
+    __shared__ float sums[kFewWarps][kFewRows][kCols + 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int64_t m0 = (int64_t)blockIdx.y * kFewRows;
-    const int n0 = blockIdx.x * kFewCols;
-    const T* x = static_cast<const T*>(a.x);
+    const int n0 = blockIdx.x * kCols;
+    const T* x0 = static_cast<const T*>(a.x) + min(m0 + g, a.M - 1) * a.ldx;
+    const T* x1 = static_cast<const T*>(a.x) + min(m0 + g + 8, a.M - 1) * a.ldx;
     const T* w = static_cast<const T*>(a.w);
-    const bool row0 = m0 + g < a.M, row1 = m0 + g + 8 < a.M;
-    float acc[4][4];
+    float acc[kMmas][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < kMmas; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
-    const int steps = (a.K + 15) / 16;
-#pragma unroll 4
-    for (int step = warp; step < steps; step += kFewWarps) {
-        const int k = step * 16 + 4 * t, nk = a.K - k;
-        const uint2 x0 = row0 && nk > 0 ? load4(x + (m0 + g) * a.ldx + k, nk, a.whole_x) : make_uint2(0u, 0u);
-        const uint2 x1 = row1 && nk > 0 ? load4(x + (m0 + g + 8) * a.ldx + k, nk, a.whole_x) : make_uint2(0u, 0u);
-        const uint32_t xa[4] = {x0.x, x1.x, x0.y, x1.y};
+    auto multiply = [&](const uint2& u0, const uint2& u1, const uint2* b) {
+        const uint32_t xa[4] = {u0.x, u1.x, u0.y, u1.y};
         if constexpr (OUT_IN) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int n = n0 + 8 * j + g;
-                const uint2 b = n < a.N && nk > 0 ? load4(w + n * a.ldw + k, nk, a.whole_w) : make_uint2(0u, 0u);
-                mma16<T>(acc[j], xa, b.x, b.y);
-            }
+            for (int j = 0; j < kMmas; ++j) mma16<T>(acc[j], xa, b[j].x, b[j].y);
         } else {
-            const int n = n0 + 4 * g, nn = a.N - n;
-            uint2 b[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) b[e] = e < nk && nn > 0 ? load4(w + (int64_t)(k + e) * a.ldw + n, nn, a.whole_w) : make_uint2(0u, 0u);
             mma16<T>(acc[0], xa, __byte_perm(b[0].x, b[1].x, 0x5410), __byte_perm(b[2].x, b[3].x, 0x5410));
             mma16<T>(acc[1], xa, __byte_perm(b[0].x, b[1].x, 0x7632), __byte_perm(b[2].x, b[3].x, 0x7632));
             mma16<T>(acc[2], xa, __byte_perm(b[0].y, b[1].y, 0x5410), __byte_perm(b[2].y, b[3].y, 0x5410));
             mma16<T>(acc[3], xa, __byte_perm(b[0].y, b[1].y, 0x7632), __byte_perm(b[2].y, b[3].y, 0x7632));
         }
+    };
+    constexpr int kLoads = OUT_IN ? kMmas : 4;
+    const T* from[kLoads];                                        // of w, for k = 4 t
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j)
+        from[j] = OUT_IN ? w + (int64_t)min(n0 + 8 * j + g, a.N - 1) * a.ldw : w + (int64_t)j * a.ldw + min(n0 + 4 * g, (a.N - 1) / 4 * 4);
+    int step = warp;
+    if (a.whole_x && a.whole_w) {
+        const int whole_steps = a.K / 16;
+#pragma unroll 4
+        for (; step < whole_steps; step += kFewWarps) {
+            const int k = step * 16 + 4 * t;
+            const uint2 u0 = __ldg(reinterpret_cast<const uint2*>(x0 + k)), u1 = __ldg(reinterpret_cast<const uint2*>(x1 + k));
+            uint2 b[kLoads];
+#pragma unroll
+            for (int j = 0; j < kLoads; ++j) b[j] = __ldg(reinterpret_cast<const uint2*>(from[j] + (OUT_IN ? (int64_t)k : k * a.ldw)));
+            multiply(u0, u1, b);
+        }
+    }
+    for (; step * 16 < a.K; step += kFewWarps) {                  // other alignments, and the last step of an odd K
+        const int k = step * 16 + 4 * t, nk = a.K - k, nn = a.N - min(n0 + 4 * g, (a.N - 1) / 4 * 4);
+        uint2 b[kLoads];
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j)
+            b[j] = OUT_IN ? load4(from[j] + k, nk, a.whole_w) : j < nk ? load4(from[j] + k * a.ldw, nn, a.whole_w) : make_uint2(0u, 0u);
+        multiply(load4(x0 + k, nk, a.whole_x), load4(x1 + k, nk, a.whole_x), b);
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < kMmas; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int in_mma = 2 * t + (e & 1), col = OUT_IN ? 8 * j + in_mma : 4 * in_mma + j;
             sums[warp][g + (e & 2) * 4][col] = acc[j][e];
         }
     __syncthreads();
-    for (int m = warp; m < kFewRows && m0 + m < a.M; m += kFewWarps) {
-        float z = 0.f;
+    const int m = threadIdx.x / kCols, col = threadIdx.x % kCols;      // a warp has 32 columns of a row, or 16 of two
+    if (m >= kFewRows) return;
+    float z = 0.f;
 #pragma unroll
-        for (int s = 0; s < kFewWarps; ++s) z += sums[s][m][lane];
-        finish<T>(a, m0 + m, n0 + lane, z);
-    }
+    for (int s = 0; s < kFewWarps; ++s) z += sums[s][m][col];
+    finish<T>(a, m0 + m, n0 + col, z);
 }
 
 // fp32: a lane owns a column of w [K x N] (its warp's share of K), or a warp a row of w [N x K] with K along the lanes; x is read through the L1.
-constexpr int kFewRows32 = 4, kFewWarps32 = 16;
-template <bool OUT_IN> __global__ void __launch_bounds__(32 * kFewWarps32) k_few_rows32(const FewArgs a)
+constexpr int kFewWarps32 = 16;
+template <bool OUT_IN, int ROWS> __global__ void __launch_bounds__(32 * kFewWarps32) k_few_rows32(const FewArgs a)
 {
-    __shared__ float sums[kFewWarps32][kFewRows32][33];
+    __shared__ float sums[kFewWarps32][ROWS][33];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t m0 = (int64_t)blockIdx.y * kFewRows32;
-    const int rows = (int)min((int64_t)kFewRows32, a.M - m0), n0 = blockIdx.x * 32;
-    const float* x = static_cast<const float*>(a.x) + m0 * a.ldx;
+    const int64_t m0 = (int64_t)blockIdx.y * ROWS;
+    const int n0 = blockIdx.x * 32;
+    const float* x[ROWS];
+#pragma unroll
+    for (int m = 0; m < ROWS; ++m) x[m] = static_cast<const float*>(a.x) + min(m0 + m, a.M - 1) * a.ldx;
     const float* w = static_cast<const float*>(a.w);
     if constexpr (!OUT_IN) {
-        float acc[kFewRows32] = {};
-        const int col = min(n0 + lane, a.N - 1);
-#pragma unroll 8
+        float acc[ROWS] = {};
+        const float* from = w + min(n0 + lane, a.N - 1);
+#pragma unroll 16
         for (int k = warp; k < a.K; k += kFewWarps32) {
-            const float v = __ldg(w + k * a.ldw + col);
+            const float v = __ldg(from + k * a.ldw);
 #pragma unroll
-            for (int m = 0; m < kFewRows32; ++m) acc[m] = fmaf(m < rows ? __ldg(x + m * a.ldx + k) : 0.f, v, acc[m]);
+            for (int m = 0; m < ROWS; ++m) acc[m] = fmaf(__ldg(x[m] + k), v, acc[m]);
         }
 #pragma unroll
-        for (int m = 0; m < kFewRows32; ++m) sums[warp][m][lane] = acc[m];
+        for (int m = 0; m < ROWS; ++m) sums[warp][m][lane] = acc[m];
         __syncthreads();
-        if (warp >= rows) return;
+        if (warp >= ROWS) return;
         float z = 0.f;
 #pragma unroll
         for (int s = 0; s < kFewWarps32; ++s) z += sums[s][warp][lane];
         finish<float>(a, m0 + warp, n0 + lane, z);
     } else {
-        float acc[2][kFewRows32] = {};                            // columns n0 + 2 warp, n0 + 2 warp + 1
-        const int64_t c0 = min(n0 + 2 * warp, a.N - 1), c1 = min(n0 + 2 * warp + 1, a.N - 1);
-#pragma unroll 4
+        float acc[2][ROWS] = {};                                  // columns n0 + 2 warp, n0 + 2 warp + 1
+        const float *from0 = w + (int64_t)min(n0 + 2 * warp, a.N - 1) * a.ldw, *from1 = w + (int64_t)min(n0 + 2 * warp + 1, a.N - 1) * a.ldw;
+#pragma unroll 8
         for (int k = lane; k < a.K; k += 32) {
-            const float v0 = __ldg(w + c0 * a.ldw + k), v1 = __ldg(w + c1 * a.ldw + k);
+            const float v0 = __ldg(from0 + k), v1 = __ldg(from1 + k);
 #pragma unroll
-            for (int m = 0; m < kFewRows32; ++m) {
-                const float u = m < rows ? __ldg(x + m * a.ldx + k) : 0.f;
+            for (int m = 0; m < ROWS; ++m) {
+                const float u = __ldg(x[m] + k);
                 acc[0][m] = fmaf(u, v0, acc[0][m]);
                 acc[1][m] = fmaf(u, v1, acc[1][m]);
             }
@@ -818,30 +837,37 @@ template <bool OUT_IN> __global__ void __launch_bounds__(32 * kFewWarps32) k_few
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
-            for (int m = 0; m < kFewRows32; ++m) {
+            for (int m = 0; m < ROWS; ++m) {
                 float v = acc[c][m];
                 for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
                 if (lane == 0) sums[0][m][2 * warp + c] = v;
             }
         __syncthreads();
-        if (warp >= rows) return;
+        if (warp >= ROWS) return;
         finish<float>(a, m0 + warp, n0 + lane, sums[0][warp][lane]);
     }
 }
 
 // ---- rows of whole 16-byte pieces ------------------------------------------------------------------------------------------------
+// A 16-byte piece of the copy a thread, out of the five 32-bit words that its elements lie in (rows start on any even address; the first and last word may
+// hold a neighbour's element, which is not used), shifted by half a word where the row starts on one.
 __global__ void __launch_bounds__(256) k_pad_rows16(const unsigned short* __restrict__ src, int64_t ld_src, int64_t n, int32_t cols, uint4* __restrict__ dst, int32_t pieces)
 {
     const int64_t total = n * pieces, stride = (int64_t)gridDim.x * blockDim.x;
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += stride) {
         const int64_t row = i / pieces;
-        const int c = (int)(i - row * pieces) * 8;
+        const int c = (int)(i - row * pieces) * 8, left = cols - c;      // elements of the row from here on
         const unsigned short* s = src + row * ld_src + c;
+        const bool odd = reinterpret_cast<uintptr_t>(s) & 2;
+        const uint32_t* words = reinterpret_cast<const uint32_t*>(s - odd);
+        uint32_t w[5];
+#pragma unroll
+        for (int e = 0; e < 5; ++e) w[e] = 2 * e - odd < left && (e < 4 || odd) ? __ldcs(words + e) : 0u;
         uint32_t v[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const uint32_t low = c + 2 * e < cols ? __ldcs(s + 2 * e) : 0, high = c + 2 * e + 1 < cols ? __ldcs(s + 2 * e + 1) : 0;
-            v[e] = low | high << 16;
+            v[e] = odd ? __funnelshift_r(w[e], w[e + 1], 16) : w[e];
+            if (2 * e + 1 >= left) v[e] = 2 * e < left ? v[e] & 0xFFFFu : 0u;
         }
         dst[i] = make_uint4(v[0], v[1], v[2], v[3]);
     }
@@ -930,14 +956,20 @@ int linear_few(const dg_linear_args* g, cudaStream_t stream)
 {
     FewArgs a{g->x, g->w, g->bias, g->residual, g->y, g->z, g->bits, g->ldx, g->ldw, g->ldr, g->ldy, g->ldz, g->ldbits, g->M, g->N, g->K, g->act, 0, 0};
     if (g->type == DG_FLOAT32) {
-        const dim3 grid((unsigned)((g->N + 31) / 32), (unsigned)((g->M + kFewRows32 - 1) / kFewRows32));
-        if (g->out_in) k_few_rows32<true><<<grid, 32 * kFewWarps32, 0, stream>>>(a);
-        else k_few_rows32<false><<<grid, 32 * kFewWarps32, 0, stream>>>(a);
+        auto run = [&](auto out_in, auto rows) {
+            constexpr int ROWS = decltype(rows)::value;
+            const dim3 grid((unsigned)((g->N + 31) / 32), (unsigned)((g->M + ROWS - 1) / ROWS));
+            k_few_rows32<decltype(out_in)::value, ROWS><<<grid, 32 * kFewWarps32, 0, stream>>>(a);
+        };
+        auto sized = [&](auto out_in) { g->M == 1 ? run(out_in, std::integral_constant<int, 1>{}) : run(out_in, std::integral_constant<int, 4>{}); };
+        if (g->out_in) sized(std::true_type{});
+        else sized(std::false_type{});
         return (int)cudaGetLastError();
     }
     auto on_8 = [](const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 7) == 0 && ld % 4 == 0; };
     a.whole_x = on_8(g->x, g->ldx), a.whole_w = on_8(g->w, g->ldw);
-    const dim3 grid((unsigned)((g->N + kFewCols - 1) / kFewCols), (unsigned)((g->M + kFewRows - 1) / kFewRows));
+    const int cols = g->out_in ? kFewCols<true> : kFewCols<false>;
+    const dim3 grid((unsigned)((g->N + cols - 1) / cols), (unsigned)((g->M + kFewRows - 1) / kFewRows));
     auto run = [&](auto value) {
         using T = decltype(value);
         if (g->out_in) k_few_rows16<T, true><<<grid, 32 * kFewWarps, 0, stream>>>(a);
