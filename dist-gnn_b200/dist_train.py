@@ -71,7 +71,7 @@ def make_optimizer(name, parameters):
 
 def train(g, env, total_epoch, hidden_dim=256, num_layers=3, weights=None, log_every=10, optimizer='adam', **model_options):
     """The reference's epoch loop (dist_train.py:26-55).  model_options go to GCN (cache_input_product,
-    input_gradient_shortcut); the defaults recompute everything every epoch, as the reference does."""
+    input_gradient_shortcut, bias, residual, activation); the defaults recompute everything every epoch, as the reference does."""
     model = GCN(g, env, hidden_dim=hidden_dim, num_layers=num_layers, weights=weights, **model_options)
     optimizer = make_optimizer(optimizer, model.parameters())
     loss_func = nn.CrossEntropyLoss() if g.labels.dim() == 1 else nn.BCEWithLogitsLoss(reduction='mean')
@@ -107,5 +107,6 @@ def main(env, args):
         g = Parted_COO_Graph(args.dataset, rank=env.rank // env.rep, num_parts=parts, device=env.device)
         env.logger.log('graph loaded', g)
         train(g, env, total_epoch=args.epoch, hidden_dim=getattr(args, 'hidden', 256), num_layers=getattr(args, 'layers', 3),
-              optimizer=getattr(args, 'optimizer', 'adam'))
+              optimizer=getattr(args, 'optimizer', 'adam'), bias=getattr(args, 'bias', False), residual=getattr(args, 'residual', False),
+              activation=getattr(args, 'activation', 'relu'))
     env.logger.log(env.timer.summary_all(), rank=0)

@@ -1,5 +1,5 @@
 """Launcher with the flags of light_dist_gnn/main.py:24-33 (--nprocs --epoch --backend --dataset) plus --layers,
---hidden, --rep (1.5D replication factor) and --optimizer.  One process per GPU, spawned on this host."""
+--hidden, --rep (1.5D replication factor), --optimizer, --bias, --residual and --activation.  One process per GPU, spawned on this host."""
 import argparse
 import os
 
@@ -31,5 +31,8 @@ if __name__ == '__main__':
     parser.add_argument('--hidden', type=int, default=256)
     parser.add_argument('--rep', type=int, default=1)
     parser.add_argument('--optimizer', choices=('adam', 'adamw', 'adamw8'), default='adam')
+    parser.add_argument('--bias', action='store_true')
+    parser.add_argument('--residual', action='store_true')
+    parser.add_argument('--activation', choices=('relu', 'gelu', 'silu'), default='relu')
     args = parser.parse_args()
     torch.multiprocessing.spawn(process_wrapper, (args, dist_train.main), args.nprocs)

@@ -459,6 +459,35 @@ class DistGCNLayer(torch.autograd.Function):
         return (grad_features, grad_weight) + (None,) * 8
 
 
+class Aggregate(torch.autograd.Function):
+    """sum_s A[rank, s] X_s as an operation of its own, for layers whose dense part is spmm_cpp.linear.  Backward multiplies by the same row block, which
+    is the gradient for a symmetric adjacency - what DistGCNLayer assumes too (gcn.py:47)."""
+
+    @staticmethod
+    def forward(ctx, features, adj_parts, tag, constant):
+        ctx.adj_parts, ctx.tag = adj_parts, tag
+        return _distributed_spmm(adj_parts, features, constant)
+
+    @staticmethod
+    def backward(ctx, grad_output):
+        return broadcast(ctx.adj_parts, grad_output, 'Backward' + ctx.tag), None, None, None
+
+
+class SumOverRanks(torch.autograd.Function):
+    """A weight that every rank holds and uses on rows of its own: itself, with the sum of all ranks' gradients (gcn.py:51)."""
+
+    @staticmethod
+    def forward(ctx, weight):
+        return weight.view_as(weight)
+
+    @staticmethod
+    def backward(ctx, grad_output):
+        if DistEnv.env.world_size > 1:
+            grad_output = grad_output.contiguous().clone()      # the sum is taken in place
+        _all_reduce(grad_output)
+        return grad_output
+
+
 class GCN(nn.Module):
     """num_layers DistGCNLayers with ReLU between them, no bias (gcn.py:56-72).  Weights are drawn as the reference
     draws them - torch.rand on the host after manual_seed(0), layer by layer - unless `weights` injects them.
@@ -474,11 +503,20 @@ class GCN(nn.Module):
                             gradient for a symmetric adjacency up to rounding, not bit for bit.
     transform_first         the last layer multiplies by its weight before the stage loop when that is the narrower side
                             (DistGCNLayer `transform_first`): a 47-wide distributed SpMM instead of a 256-wide one.
+    bias, residual, activation
+                            layers of the form  h' = act(A h W + b) + h  (spmm_cpp.linear behind Aggregate): a bias a layer (`bias1..L`, zero at
+                            first), the layer's input added where it is as wide as the output (every hidden layer but the first), and 'gelu' or
+                            'silu' in the place of ReLU.  The last layer has neither activation nor residual.  Not with the options above.
     All are off by default: the like-for-like epoch computes what the reference computes, in its order."""
 
     def __init__(self, g, env, hidden_dim=16, num_layers=3, weights=None, cache_input_product=False, input_gradient_shortcut=False,
-                 transform_first=False):
+                 transform_first=False, bias=False, residual=False, activation='relu'):
         super().__init__()
+        if activation not in ('relu', 'gelu', 'silu'):
+            raise ValueError(f"activation must be 'relu', 'gelu' or 'silu', got {activation!r}")
+        self.bias, self.residual, self.activation = bool(bias), bool(residual), activation
+        if self.with_linear and (cache_input_product or input_gradient_shortcut or transform_first):
+            raise ValueError('bias, residual and other activations do not go together with cache_input_product, input_gradient_shortcut or transform_first')
         self.g, self.env, self.num_layers = g, env, num_layers
         self.cache_input_product = bool(cache_input_product or input_gradient_shortcut)
         self.input_gradient_shortcut = bool(input_gradient_shortcut)
@@ -491,9 +529,25 @@ class GCN(nn.Module):
             w = torch.rand(dims[l], dims[l + 1]) if weights is None else weights[l].detach().clone().float()
             assert tuple(w.shape) == (dims[l], dims[l + 1])
             setattr(self, f'weight{l + 1}', nn.Parameter(w.to(env.device)))
+            if self.bias:
+                setattr(self, f'bias{l + 1}', nn.Parameter(torch.zeros(dims[l + 1], device=env.device)))
+
+    @property
+    def with_linear(self):
+        return self.bias or self.residual or self.activation != 'relu'
 
     def weights(self):
         return [getattr(self, f'weight{l + 1}') for l in range(self.num_layers)]
+
+    def _linear_forward(self, h):
+        last = self.num_layers - 1
+        for l, w in enumerate(self.weights()):
+            b = SumOverRanks.apply(getattr(self, f'bias{l + 1}')) if self.bias else None
+            z = Aggregate.apply(h, self.g.adj_parts, f'L{l + 1}', l == 0)
+            with DistEnv.env.timer.timing_cuda('mm'):
+                h = spmm_cpp.linear(z, SumOverRanks.apply(w), b, residual=h if self.residual and 0 < l < last else None,
+                                    activation=self.activation if l < last else None)
+        return h
 
     def input_product(self, features):
         """The cached first-layer product for `features`, computed on first use (None when caching is off or the features
@@ -539,6 +593,8 @@ class GCN(nn.Module):
     def forward(self, features):
         h = features
         last = self.num_layers - 1
+        if self.with_linear:
+            return self._linear_forward(features)
         weights = self.weights()
         plan = self._one_rank_plan(features, weights)
         if plan is not None:
