@@ -662,10 +662,10 @@ int make_map(CUtensorMap* map, const float* ptr, int64_t rows, int64_t cols, int
 // With more rows the pair wins (150,001 rows 100 -> 72 40.6 and 31.7, 256 -> 80 58 and 53, 256 -> 128 96 and 59) but for shallow products up to 80
 // columns with the mask, which wait for its rows and have more warps to do so as two CTAs (150,001 rows 64 -> 65 57 and 61, 100,000 rows
 // 64 -> 80 26.8 and 30.7).  Up to 64 columns the line was drawn when a pair issued its MMAs more slowly (256 -> 47 860 and 895; now 830 and 701).
-bool by_pairs(int64_t M, int n_pad, int K, bool masked, int sms)
+bool by_pairs(int64_t M, int n_pad, int K, bool masked, int sms, bool linear)
 {
-    if (n_pad <= 64) return false;
     const int64_t tiles = (M + BM - 1) / BM;
+    if (n_pad <= 64) return linear && n_pad > 32 && tiles > 2 * sms;      // half of a pair's epilogue warps have no piece of 32 columns
     const bool half_slab = (K - 1) % BK < BK / 2;
     if (tiles <= sms) return n_pad > 128 || half_slab || K > (n_pad > 80 ? 96 : 128);
     return n_pad > 80 || (tiles > 2 * sms && (!masked || K > 64));
@@ -691,7 +691,7 @@ int launch_nt(const float* A, int64_t lda, const float* Bt_head, const float* Bt
     if (!a.status) return DG_ERR_STATE;
     const int sms = sm_count();
     if (sms <= 0) return DG_ERR_STATE;
-    const bool pair = by_pairs(a.M, a.n_pad, a.K, a.mask != nullptr, sms);
+    const bool pair = by_pairs(a.M, a.n_pad, a.K, a.mask != nullptr, sms, epilogue >= kLinear);
     CUtensorMap tmA, tmBh, tmBt;
     int rc;
     if (!pair) {

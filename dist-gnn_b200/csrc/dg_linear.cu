@@ -357,13 +357,16 @@ k_linear_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
 // A CTA owns a panel of up to 256 x 256 of dw and a range of rows.  Both operands come in boxes of 64 columns x 64 rows (MN-major); x's columns lie along
 // the MMA's 128 rows, so a panel wider than 128 takes two accumulators.  The range's partial goes to scratch, four columns of dz and all of x's side by
 // side; a second kernel adds the ranges in order.
+// One range (fewer than 512 rows) is written as it is.
 // A chain of accumulations, which the tensor cores truncate, is as long as the range: 16 rows each, some 1,000 at 2.4 M rows, 3e-5 of the sum at most where
 // bf16 rounds by 4e-3 and fp16 by 5e-4; so no flush in between, which fp32 needs.
 constexpr int kDwRows = 64, kDwBox = kDwRows * 128, kDwThreads = 32 * 6, kDwMaxStages = 8;
 constexpr int kDwBarBytes = 8 * (2 * kDwMaxStages + 2) + 8;
 
 struct LinearDwArgs {
-    float4* partial;                              // [range][panel][q_store / 4][p_store]
+    float4* partial;                              // [range][panel][q_store / 4][p_store]; null: the one range's sums are the result
+    void* dw;
+    int64_t row_stride, col_stride;
     int64_t M, rows_per_range;
     int32_t p_cols, q_cols;                       // K, N
     int32_t p_panels, q_panels, p_store, q_store;
@@ -458,6 +461,29 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_linear_dw(const __grid_consta
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             for (int h = 0; h < halves; ++h) {
                 const int row = h * 128 + q * 32 + lane;
+                if (!a.partial) {
+                    const int p = p0 + row;
+                    const bool whole = a.col_stride == 1 && a.row_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(a.dw) & 15) == 0;
+                    for (int c0 = 0; c0 < q_pad; c0 += 16) {
+                        uint32_t r[16];
+                        tmem_ld16(tmem + (uint32_t)(h * 256 + c0) + ((uint32_t)(q * 32) << 16), r);
+                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                        if (p >= a.p_cols) continue;
+                        T* to = static_cast<T*>(a.dw) + p * a.row_stride + (q0 + c0) * a.col_stride;
+                        if (whole && q0 + c0 + 16 <= a.q_cols) {
+                            uint32_t v[8];
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) v[j] = Pair<T>::narrow(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+                            reinterpret_cast<uint4*>(to)[0] = make_uint4(v[0], v[1], v[2], v[3]);
+                            reinterpret_cast<uint4*>(to)[1] = make_uint4(v[4], v[5], v[6], v[7]);
+                            continue;
+                        }
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            if (q0 + c0 + j < a.q_cols) to[j * a.col_stride] = Pair<T>::round(__uint_as_float(r[j]));
+                    }
+                    continue;
+                }
                 float4* part = a.partial + ((int64_t)range * panels + panel) * (a.q_store / 4) * a.p_store + row;
                 for (int c0 = 0; c0 < q_pad; c0 += 16) {
                     uint32_t r[16];
@@ -567,6 +593,7 @@ struct LinearDzArgs {
     int64_t lddy, ldz, ldbits, lddz, M;
     const uint32_t* bits;
     float* partial;                               // [gridDim.x][N], or null
+    void* db;                                     // one CTA over the rows: its sums are the result
     int32_t N, lanes, whole_dy, whole_z, whole_dz;
 };
 
@@ -628,7 +655,7 @@ __global__ void __launch_bounds__(kDzThreads, 3) k_linear_dz(const T* __restrict
             if constexpr (smooth) pre.load(z + row * a.ldz + c, n);
             work(row, from, pre, bits_of(row));
         }
-    if (!a.partial) return;
+    if (!a.partial && !a.db) return;
 #pragma unroll
     for (int e = 0; e < 8; ++e) sums[threadIdx.x][e] = sum[e];
     __syncthreads();
@@ -637,7 +664,8 @@ __global__ void __launch_bounds__(kDzThreads, 3) k_linear_dz(const T* __restrict
         if (col >= a.N) continue;
         float s = 0.f;
         for (int k = 0; k < groups; ++k) s += sums[k * a.lanes + l][i % 8];
-        a.partial[(int64_t)blockIdx.x * a.N + col] = s;
+        if (a.db) static_cast<T*>(a.db)[col] = Pair<T>::round(s);
+        else a.partial[(int64_t)blockIdx.x * a.N + col] = s;
     }
 }
 
@@ -657,7 +685,7 @@ template <class T> __global__ void __launch_bounds__(1024) k_linear_db(const flo
     db[col] = Pair<T>::round((float)s);
 }
 
-// The CTAs over the rows: enough to fill the device twice over, and at least 16 rows a thread.
+// The CTAs over the rows: enough to fill the device twice over, and at least 32 rows a thread.
 int dz_lanes(int32_t N)
 {
     int lanes = 1;
@@ -667,7 +695,7 @@ int dz_lanes(int32_t N)
 int dz_ctas(int64_t M, int32_t N)
 {
     const int lanes = dz_lanes(N), columns = (N + lanes * 8 - 1) / (lanes * 8);
-    const int64_t most = std::max(1, 148 * 6 / columns), rows = kDzThreads / lanes * 16;
+    const int64_t most = std::max(1, 148 * 6 / columns), rows = kDzThreads / lanes * 32;
     return (int)std::min<int64_t>(most, (M + rows - 1) / rows);
 }
 
@@ -996,7 +1024,7 @@ DwShape dw_shape(int64_t M, int32_t N, int32_t K)
     const int64_t ranges = std::max<int64_t>(1, std::min<int64_t>(148 / panels, slabs / 4));
     s.rows_per_range = (slabs + ranges - 1) / ranges * kDwRows;
     s.ranges = (int)((M + s.rows_per_range - 1) / s.rows_per_range);
-    s.floats = s.ranges * panels * s.p_store * s.q_store;
+    s.floats = s.ranges > 1 ? s.ranges * panels * s.p_store * s.q_store : 0;
     return s;
 }
 
@@ -1017,18 +1045,21 @@ extern "C" int dg_linear(const dg_linear_args* g, void* stream)
     return g->type == DG_FLOAT32 ? dg_dense_linear(g, (cudaStream_t)stream) : linear16(g, (cudaStream_t)stream);
 }
 
-extern "C" int64_t dg_linear_dz_scratch(int64_t M, int32_t N) { return M < 1 || N < 1 ? 0 : (int64_t)dz_ctas(M, N) * N; }
+extern "C" int64_t dg_linear_dz_scratch(int64_t M, int32_t N) { return M < 1 || N < 1 || dz_ctas(M, N) == 1 ? 0 : (int64_t)dz_ctas(M, N) * N; }
 
 extern "C" int dg_linear_dz(const void* dy, int64_t lddy, const void* z, int64_t ldz, const uint32_t* bits, int64_t ldbits, int32_t act, void* dz, int64_t lddz,
                             void* db, int64_t M, int32_t N, int32_t type, float* scratch, void* stream)
 {
-    if (!dy || (!dz && !db) || (db && !scratch)) return DG_ERR_NULL;
+    if (!dy || (!dz && !db)) return DG_ERR_NULL;
     if (M < 1 || N < 1 || type < 0 || type > 2 || act < 0 || act > 3 || lddy < N || (dz && lddz < N)) return DG_ERR_DIMS;
     if (act == DG_ACT_RELU ? !bits || ldbits * 32 < N : act != DG_ACT_NONE && (!z || ldz < N)) return DG_ERR_NULL;
     const int item = type == DG_FLOAT32 ? 4 : 2;
     if (!aligned(dy, item) || !aligned(z, item) || !aligned(dz, item) || !aligned(db, item)) return DG_ERR_DIMS;
     LinearDzArgs a{};
-    a.lddy = lddy, a.ldz = ldz, a.ldbits = ldbits, a.lddz = lddz, a.M = M, a.N = N, a.bits = bits, a.partial = db ? scratch : nullptr;
+    a.lddy = lddy, a.ldz = ldz, a.ldbits = ldbits, a.lddz = lddz, a.M = M, a.N = N, a.bits = bits;
+    const bool direct = dg_linear_dz_scratch(M, N) == 0;
+    if (db && !direct && !scratch) return DG_ERR_NULL;
+    a.partial = db && !direct ? scratch : nullptr, a.db = direct ? db : nullptr;
     a.lanes = dz_lanes(N);
     a.whole_dy = on_rows(dy, lddy, item), a.whole_z = on_rows(z, ldz, item), a.whole_dz = on_rows(dz, lddz, item);
     const dim3 grid((unsigned)dz_ctas(M, N), (unsigned)((N + a.lanes * 8 - 1) / (a.lanes * 8)));
@@ -1043,7 +1074,7 @@ extern "C" int dg_linear_dz(const void* dy, int64_t lddy, const void* z, int64_t
             case DG_ACT_SILU: k_linear_dz<T, DG_ACT_SILU><<<grid, kDzThreads, 0, s>>>(from, pre, to, a); break;
             default: k_linear_dz<T, DG_ACT_NONE><<<grid, kDzThreads, 0, s>>>(from, pre, to, a);
         }
-        if (db) k_linear_db<T><<<(unsigned)((N + 31) / 32), 1024, 0, s>>>(scratch, (int)grid.x, N, static_cast<T*>(db));
+        if (a.partial) k_linear_db<T><<<(unsigned)((N + 31) / 32), 1024, 0, s>>>(scratch, (int)grid.x, N, static_cast<T*>(db));
     };
     if (type == DG_FLOAT32) run(float{});
     else if (type == DG_BFLOAT16) run(__nv_bfloat16{});
@@ -1056,14 +1087,16 @@ extern "C" int64_t dg_linear_dw_scratch(int64_t M, int32_t N, int32_t K) { retur
 extern "C" int dg_linear_dw(const void* x, int64_t ldx, const void* dz, int64_t lddz, void* dw, int64_t row_stride, int64_t col_stride, int64_t M, int32_t N, int32_t K,
                             int32_t type, float* scratch, int64_t scratch_floats, void* stream)
 {
-    if (!x || !dz || !dw || !scratch) return DG_ERR_NULL;
+    if (!x || !dz || !dw) return DG_ERR_NULL;
     if (M < 1 || M >= (int64_t)1 << 31 || N < 1 || K < 1 || ldx < K || lddz < N || (type != DG_BFLOAT16 && type != DG_FLOAT16) || !aligned(dw, 2) || !aligned(scratch, 16))
         return DG_ERR_DIMS;
     if (!on_rows(x, ldx, 2) || !on_rows(dz, lddz, 2)) return DG_ERR_UNSUPPORTED;
     const DwShape shape = dw_shape(M, N, K);
+    if (shape.floats > 0 && !scratch) return DG_ERR_NULL;
     if (scratch_floats < shape.floats) return DG_ERR_SCRATCH;
     LinearDwArgs a{};
-    a.partial = reinterpret_cast<float4*>(scratch);
+    a.partial = shape.floats > 0 ? reinterpret_cast<float4*>(scratch) : nullptr;
+    a.dw = dw, a.row_stride = row_stride, a.col_stride = col_stride;
     a.M = M, a.rows_per_range = shape.rows_per_range, a.p_cols = K, a.q_cols = N;
     a.p_panels = shape.p_panels, a.q_panels = shape.q_panels, a.p_store = shape.p_store, a.q_store = shape.q_store;
     a.p_boxes = (std::min(K, 256) + 63) / 64, a.q_boxes = (std::min(N, 256) + 63) / 64;
@@ -1084,7 +1117,8 @@ extern "C" int dg_linear_dw(const void* x, int64_t ldx, const void* dz, int64_t 
         const int code = allow_smem((const void*)k_linear_dw<T>, granted);
         if (code) return code;
         k_linear_dw<T><<<ctas, kDwThreads, smem, (cudaStream_t)stream>>>(tmP, tmQ, a);
-        k_linear_dw_reduce<T><<<(unsigned)((slots + 31) / 32), 256, 0, (cudaStream_t)stream>>>(a.partial, shape.ranges, a.p_panels, a.q_panels, a.p_store, a.q_store, K, N,
+        if (a.partial)
+            k_linear_dw_reduce<T><<<(unsigned)((slots + 31) / 32), 256, 0, (cudaStream_t)stream>>>(a.partial, shape.ranges, a.p_panels, a.q_panels, a.p_store, a.q_store, K, N,
                                                                                               static_cast<T*>(dw), row_stride, col_stride);
         return (int)cudaGetLastError();
     };

@@ -490,7 +490,7 @@ struct LinearNode : public torch::autograd::Node {
                                    bits.defined() ? reinterpret_cast<const uint32_t*>(bits.data_ptr<int32_t>()) : nullptr, bits.defined() ? bits.size(1) : 0, act,
                                    dz.defined() ? dz.data_ptr() : nullptr, dz.defined() ? dz.stride(0) : 0, db ? out[2].data_ptr() : nullptr, M, (int32_t)N, type,
                                    db ? scratch.data_ptr<float>() : nullptr, stream));
-                launches += db ? 2 : 1;
+                launches += db && scratch.numel() > 0 ? 2 : 1;
             }
             if (dz.defined()) g = dz;
         }
@@ -518,7 +518,7 @@ struct LinearNode : public torch::autograd::Node {
                 const Tensor partial = at::empty({dg_linear_dw_scratch(M, (int32_t)N, (int32_t)K)}, x.options().dtype(at::kFloat));
                 check(dg_linear_dw(rows.data_ptr(), ld_of(rows), g.data_ptr(), ld_of(g), d.data_ptr(), out_in ? 1 : N, out_in ? K : 1, M, (int32_t)N, (int32_t)K, type,
                                    partial.data_ptr<float>(), partial.numel(), stream));
-                launches += 2;
+                launches += partial.numel() > 0 ? 2 : 1;
             }
             out[1] = out_in ? d.t() : d;
         }

@@ -421,12 +421,12 @@ typedef struct dg_linear_args {
 int64_t dg_linear_few(int32_t N, int32_t K, int32_t type);
 int dg_linear(const dg_linear_args* args, void* stream);
 /* dz = dy * act'(z) and db = the column sums of dz.  dz == NULL: only db; db == NULL: only dz.  z / bits as dg_linear left them (neither: dz = dy).
- * scratch: dg_linear_dz_scratch(M, N) floats where db is asked for.  Any strides and alignments; the sums are taken in a fixed order. */
+ * scratch: dg_linear_dz_scratch(M, N) floats (0 for few rows) where db is asked for.  Any strides and alignments; the sums are taken in a fixed order. */
 int64_t dg_linear_dz_scratch(int64_t M, int32_t N);
 int dg_linear_dz(const void* dy, int64_t lddy, const void* z, int64_t ldz, const uint32_t* bits, int64_t ldbits, int32_t act, void* dz, int64_t lddz,
                  void* db, int64_t M, int32_t N, int32_t type, float* scratch, void* stream);
 /* dw[k * row_stride + n * col_stride] = sum over rows of x[m, k] dz[m, n] for bf16 and fp16 (fp32: dg_dense_tn).  x and dz on rows.  scratch: 16-byte
- * aligned, dg_linear_dw_scratch floats. */
+ * aligned, dg_linear_dw_scratch floats (0 for few rows). */
 int64_t dg_linear_dw_scratch(int64_t M, int32_t N, int32_t K);
 int dg_linear_dw(const void* x, int64_t ldx, const void* dz, int64_t lddz, void* dw, int64_t row_stride, int64_t col_stride, int64_t M, int32_t N, int32_t K,
                  int32_t type, float* scratch, int64_t scratch_floats, void* stream);
