@@ -3,7 +3,8 @@
 // k_linear_pair: x w on the tensor cores (tcgen05 kind::f16, fp32 accumulators in tensor memory) by CTA pairs that walk over tiles of 256 rows x up to 256
 // columns.  w is read as it lies: [N x K] rows are K-major operands, [K x N] rows MN-major ones, both in 128B-swizzled boxes.
 // k_linear_dw: the weight gradient x^T dz, both operands MN-major, rows cut into ranges whose partial results are added in order.
-// k_linear_dz: dz = dy act'(z) and its column sums.
+// k_linear_back: the same with dz = dy act'(z), its column sums and, where asked, dz itself made on the way.
+// k_linear_dz: dz and its column sums alone.
 // k_few_*: products of few rows, bound by latency.
 // The fp32 product is dg_dense.cu's.
 #include <algorithm>
@@ -372,7 +373,65 @@ struct LinearDwArgs {
     int32_t p_panels, q_panels, p_store, q_store;
     int32_t stages, p_boxes, q_boxes;             // of a full panel
     int* status;
+    // k_linear_back
+    const uint32_t* bits;
+    int64_t ldbits;
+    void* db;                                     // or null
+    float* db_partial;                            // [range][N]; null: the one range's sums are the result
+    int32_t store;                                // dz is kept
 };
+
+// What a CTA does: its panel and range.
+struct DwPart {
+    int panels, panel, range, p0, q0, p_boxes, q_boxes, halves, q_pad, slabs;
+    int64_t r0;
+    __device__ __forceinline__ DwPart(const LinearDwArgs& a, int rows)
+    {
+        panels = a.p_panels * a.q_panels, panel = blockIdx.x % panels, range = blockIdx.x / panels;
+        p0 = panel / a.q_panels * 256, q0 = panel % a.q_panels * 256;
+        const int p_here = min(256, a.p_cols - p0), q_here = min(256, a.q_cols - q0);
+        p_boxes = (p_here + 63) / 64, q_boxes = (q_here + 63) / 64, halves = (p_here + 127) / 128, q_pad = (q_here + 15) / 16 * 16;
+        r0 = range * a.rows_per_range;
+        slabs = (int)((max((int64_t)0, min(a.M, r0 + a.rows_per_range) - r0) + rows - 1) / rows);
+    }
+};
+
+// The accumulators of a CTA, by four warps: to its place among the partial results, or where it has the only range rounded to dw.
+template <class T> __device__ __forceinline__ void flush_dw(const LinearDwArgs& a, const DwPart& part, uint32_t tmem, int warp, int lane)
+{
+    const int q = warp & 3;                                       // a warp may only read its own quarter of the TMEM lanes
+    const bool whole = a.col_stride == 1 && a.row_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(a.dw) & 15) == 0;
+    for (int h = 0; h < part.halves; ++h) {
+        const int row = h * 128 + q * 32 + lane, p = part.p0 + row;
+        float4* to_part = a.partial + ((int64_t)part.range * part.panels + part.panel) * (a.q_store / 4) * a.p_store + row;
+        for (int c0 = 0; c0 < part.q_pad; c0 += 16) {
+            uint32_t r[16];
+            tmem_ld16(tmem + (uint32_t)(h * 256 + c0) + ((uint32_t)(q * 32) << 16), r);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            if (a.partial) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (row < a.p_store)
+                        __stcg(to_part + (int64_t)(c0 / 4 + j) * a.p_store, make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]), __uint_as_float(r[4 * j + 2]),
+                                                                                          __uint_as_float(r[4 * j + 3])));
+                continue;
+            }
+            if (p >= a.p_cols) continue;
+            T* to = static_cast<T*>(a.dw) + p * a.row_stride + (part.q0 + c0) * a.col_stride;
+            if (whole && part.q0 + c0 + 16 <= a.q_cols) {
+                uint32_t v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = Pair<T>::narrow(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+                reinterpret_cast<uint4*>(to)[0] = make_uint4(v[0], v[1], v[2], v[3]);
+                reinterpret_cast<uint4*>(to)[1] = make_uint4(v[4], v[5], v[6], v[7]);
+                continue;
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                if (part.q0 + c0 + j < a.q_cols) to[j * a.col_stride] = Pair<T>::round(__uint_as_float(r[j]));
+        }
+    }
+}
 
 template <class T>
 __global__ void __launch_bounds__(kDwThreads, 1) k_linear_dw(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ CUtensorMap tmQ, const LinearDwArgs a)
@@ -386,12 +445,7 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_linear_dw(const __grid_consta
     const uint32_t full0 = bars, empty0 = bars + 8 * kDwMaxStages, acc_full = bars + 16 * kDwMaxStages, done = acc_full + 8;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbase + a.stages * stage_bytes + 8 * (2 * kDwMaxStages + 2));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int panels = a.p_panels * a.q_panels, panel = blockIdx.x % panels, range = blockIdx.x / panels;
-    const int p0 = panel / a.q_panels * 256, q0 = panel % a.q_panels * 256;
-    const int p_here = min(256, a.p_cols - p0), q_here = min(256, a.q_cols - q0);
-    const int p_boxes = (p_here + 63) / 64, q_boxes = (q_here + 63) / 64, halves = (p_here + 127) / 128, q_pad = (q_here + 15) / 16 * 16;
-    const int64_t r0 = range * a.rows_per_range, r1 = min(a.M, r0 + a.rows_per_range);
-    const int slabs = (int)((max((int64_t)0, r1 - r0) + kDwRows - 1) / kDwRows);
+    const DwPart part(a, kDwRows);
     constexpr int kTmemCols = 512;
 
     if (threadIdx.x == 0) {
@@ -416,14 +470,14 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_linear_dw(const __grid_consta
     if (warp == 0) {
         if (lane == 0) {
             int s = 0, phase = 1, i = 0;
-            for (; i < slabs && ok; ++i) {
+            for (; i < part.slabs && ok; ++i) {
                 if (i >= a.stages) ok = mbar_wait(empty0 + 8 * s, phase);
                 if (!ok) break;
                 const uint32_t st = base + s * stage_bytes;
-                const int row = (int)(r0 + (int64_t)i * kDwRows);
-                mbar_expect_tx(full0 + 8 * s, (p_boxes + q_boxes) * kDwBox);
-                for (int j = 0; j < p_boxes; ++j) tma_load_2d(st + j * kDwBox, &tmP, p0 + 64 * j, row, full0 + 8 * s);
-                for (int j = 0; j < q_boxes; ++j) tma_load_2d(st + (a.p_boxes + j) * kDwBox, &tmQ, q0 + 64 * j, row, full0 + 8 * s);
+                const int row = (int)(part.r0 + (int64_t)i * kDwRows);
+                mbar_expect_tx(full0 + 8 * s, (part.p_boxes + part.q_boxes) * kDwBox);
+                for (int j = 0; j < part.p_boxes; ++j) tma_load_2d(st + j * kDwBox, &tmP, part.p0 + 64 * j, row, full0 + 8 * s);
+                for (int j = 0; j < part.q_boxes; ++j) tma_load_2d(st + (a.p_boxes + j) * kDwBox, &tmQ, part.q0 + 64 * j, row, full0 + 8 * s);
                 if (++s == a.stages) s = 0, phase ^= 1;
             }
             await_loads(full0, i, a.stages);
@@ -431,16 +485,16 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_linear_dw(const __grid_consta
     } else if (warp == 1) {
         const bool issuer = elect_one();
         auto wait = [&](uint32_t bar, int parity) { return __any_sync(0xffffffffu, issuer && mbar_wait(bar, parity)) != 0; };
-        const uint32_t idesc = umma_idesc_f16(Pair<T>::kFormat, 128, q_pad, true, true);
+        const uint32_t idesc = umma_idesc_f16(Pair<T>::kFormat, 128, part.q_pad, true, true);
         int s = 0, phase = 0;
-        for (int i = 0; i < slabs && ok; ++i) {
+        for (int i = 0; i < part.slabs && ok; ++i) {
             ok = wait(full0 + 8 * s, phase);
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (issuer) {
                 const uint32_t st = base + s * stage_bytes;
                 const uint64_t p = umma_desc_mn16(st, kDwBox), q = umma_desc_mn16(st + a.p_boxes * kDwBox, kDwBox);
-                for (int h = 0; h < halves; ++h)
+                for (int h = 0; h < part.halves; ++h)
 #pragma unroll
                     for (int k = 0; k < kDwRows / 16; ++k)        // 16 rows: 2048 bytes
                         umma_f16(tmem + (uint32_t)(h * 256), p + (uint32_t)((h * 2 * kDwBox + k * 2048) >> 4), q + (uint32_t)(k * 2048 >> 4), idesc,
@@ -455,49 +509,199 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_linear_dw(const __grid_consta
         if (issuer) await_mmas(done);
         __syncwarp();
     } else {
-        const int q = warp & 3;
         ok = __all_sync(0xffffffffu, mbar_wait(acc_full, 0));     // tcgen05.ld is warp-collective
         if (ok) {
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            for (int h = 0; h < halves; ++h) {
-                const int row = h * 128 + q * 32 + lane;
-                if (!a.partial) {
-                    const int p = p0 + row;
-                    const bool whole = a.col_stride == 1 && a.row_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(a.dw) & 15) == 0;
-                    for (int c0 = 0; c0 < q_pad; c0 += 16) {
-                        uint32_t r[16];
-                        tmem_ld16(tmem + (uint32_t)(h * 256 + c0) + ((uint32_t)(q * 32) << 16), r);
-                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                        if (p >= a.p_cols) continue;
-                        T* to = static_cast<T*>(a.dw) + p * a.row_stride + (q0 + c0) * a.col_stride;
-                        if (whole && q0 + c0 + 16 <= a.q_cols) {
-                            uint32_t v[8];
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) v[j] = Pair<T>::narrow(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
-                            reinterpret_cast<uint4*>(to)[0] = make_uint4(v[0], v[1], v[2], v[3]);
-                            reinterpret_cast<uint4*>(to)[1] = make_uint4(v[4], v[5], v[6], v[7]);
-                            continue;
-                        }
-#pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            if (q0 + c0 + j < a.q_cols) to[j * a.col_stride] = Pair<T>::round(__uint_as_float(r[j]));
-                    }
-                    continue;
+            flush_dw<T>(a, part, tmem, warp, lane);
+        }
+    }
+    if (!ok) atomicExch(a.status, 1);
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 1)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+}
+
+// The same product with dz made on the way, for x of up to 256 columns: dy arrives where dz is put together, z beside it; the operand that the tensor cores
+// then read is also what TMA stores, and its column sums are taken by the threads that make it.  So the gradients of w and b and dz itself, which x's
+// gradient needs, take one pass over x, dy and z; dz by a pass of its own reads and writes as much again (2,449,029 x 256, 256 bf16: 617 + 384 us, 725 this way).
+// Warps: 0 TMA, 1 MMA issue + tensor-memory allocation, 2-9 dz (a row's 16-byte piece a thread and box of 32 rows x 64 columns), of which 2-5 flush, 10 stores dz.
+constexpr int kBackRows = 32, kBackBox = kBackRows * 128, kBackMakers = 8, kBackThreads = 32 * (3 + kBackMakers), kBackMaxStages = 8;
+constexpr int kBackBarBytes = 8 * (4 * kBackMaxStages + 2) + 8, kBackSumPitch = 9, kBackSumBytes = 32 * kBackMakers * kBackSumPitch * 4;
+
+template <class T, int ACT>
+__global__ void __launch_bounds__(kBackThreads, 1)
+k_linear_back(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmZ,
+              const __grid_constant__ CUtensorMap tmS, const LinearDwArgs a)
+{
+    constexpr bool kSmooth = ACT == DG_ACT_GELU || ACT == DG_ACT_SILU;
+    extern __shared__ unsigned char smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t base = (raw + 1023u) & ~1023u;
+    unsigned char* gbase = smem_raw + (base - raw);
+    const int q_at = a.p_boxes * kBackBox, z_at = q_at + a.q_boxes * kBackBox, stage_bytes = z_at + (kSmooth ? a.q_boxes * kBackBox : 0);
+    float* sums = reinterpret_cast<float*>(gbase + a.stages * stage_bytes);
+    const uint32_t bars = base + a.stages * stage_bytes + kBackSumBytes;
+    const uint32_t full0 = bars, ready0 = bars + 8 * kBackMaxStages, empty0 = bars + 16 * kBackMaxStages, stored0 = bars + 24 * kBackMaxStages;
+    const uint32_t acc_full = bars + 32 * kBackMaxStages, done = acc_full + 8;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbase + a.stages * stage_bytes + kBackSumBytes + 8 * (4 * kBackMaxStages + 2));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const DwPart part(a, kBackRows);
+    constexpr int kTmemCols = 512;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < a.stages; ++s) {
+            mbar_init(full0 + 8 * s, 1);
+            mbar_init(ready0 + 8 * s, kBackMakers);
+            mbar_init(empty0 + 8 * s, 1);
+            mbar_init(stored0 + 8 * s, 1);
+        }
+        mbar_init(acc_full, 1);
+        mbar_init(done, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(kTmemCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *tmem_slot;
+    bool ok = true;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int s = 0, phase = 1, i = 0;
+            for (; i < part.slabs && ok; ++i) {
+                if (i >= a.stages) ok = mbar_wait(empty0 + 8 * s, phase) && (!a.store || mbar_wait(stored0 + 8 * s, phase));
+                if (!ok) break;
+                const uint32_t st = base + s * stage_bytes;
+                const int row = (int)(part.r0 + (int64_t)i * kBackRows);
+                mbar_expect_tx(full0 + 8 * s, (part.p_boxes + (kSmooth ? 2 : 1) * part.q_boxes) * kBackBox);
+                for (int j = 0; j < part.q_boxes; ++j) {
+                    tma_load_2d(st + q_at + j * kBackBox, &tmQ, part.q0 + 64 * j, row, full0 + 8 * s);
+                    if (kSmooth) tma_load_2d(st + z_at + j * kBackBox, &tmZ, part.q0 + 64 * j, row, full0 + 8 * s);
                 }
-                float4* part = a.partial + ((int64_t)range * panels + panel) * (a.q_store / 4) * a.p_store + row;
-                for (int c0 = 0; c0 < q_pad; c0 += 16) {
-                    uint32_t r[16];
-                    tmem_ld16(tmem + (uint32_t)(h * 256 + c0) + ((uint32_t)(q * 32) << 16), r);
-                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                for (int j = 0; j < part.p_boxes; ++j) tma_load_2d(st + j * kBackBox, &tmP, part.p0 + 64 * j, row, full0 + 8 * s);
+                if (++s == a.stages) s = 0, phase ^= 1;
+            }
+            await_loads(full0, i, a.stages);
+        }
+    } else if (warp == 1) {
+        const bool issuer = elect_one();
+        auto wait = [&](uint32_t bar, int parity) { return __any_sync(0xffffffffu, issuer && mbar_wait(bar, parity)) != 0; };
+        const uint32_t idesc = umma_idesc_f16(Pair<T>::kFormat, 128, part.q_pad, true, true);
+        int s = 0, phase = 0;
+        for (int i = 0; i < part.slabs && ok; ++i) {
+            ok = wait(ready0 + 8 * s, phase);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (issuer) {
+                const uint32_t st = base + s * stage_bytes;
+                const uint64_t p = umma_desc_mn16(st, kBackBox), q = umma_desc_mn16(st + q_at, kBackBox);
+                for (int h = 0; h < part.halves; ++h)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (row < a.p_store)
-                            __stcg(part + (int64_t)(c0 / 4 + j) * a.p_store,
-                                   slabs ? make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]), __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3]))
-                                         : make_float4(0.f, 0.f, 0.f, 0.f));
+                    for (int k = 0; k < kBackRows / 16; ++k)      // 16 rows: 2048 bytes
+                        umma_f16(tmem + (uint32_t)(h * 256), p + (uint32_t)((h * 2 * kBackBox + k * 2048) >> 4), q + (uint32_t)(k * 2048 >> 4), idesc,
+                                 i > 0 || k > 0 ? 1u : 0u);
+                umma_commit(empty0 + 8 * s);
+            }
+            __syncwarp();
+            if (++s == a.stages) s = 0, phase ^= 1;
+        }
+        if (ok && issuer) umma_commit(acc_full);
+        __syncwarp();
+        if (issuer) await_mmas(done);
+        __syncwarp();
+    } else if (warp < 2 + kBackMakers) {
+        const int t = threadIdx.x - 64, row = t >> 3, piece = (t & 7) ^ (row & 7);      // the swizzle: which eight columns of a box lie here
+        float_pair sum[4][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[j][e] = both(0.f);
+        int s = 0, phase = 0;
+        for (int i = 0; i < part.slabs; ++i) {
+            uint32_t above[4] = {0u, 0u, 0u, 0u};
+            if constexpr (ACT == DG_ACT_RELU) {                   // on their way while the stage is waited for
+                const int64_t at = part.r0 + (int64_t)i * kBackRows + row;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int c = part.q0 + 64 * j + 8 * piece;
+                    if (at < a.M && c < a.q_cols) above[j] = __ldg(reinterpret_cast<const unsigned char*>(a.bits + at * a.ldbits) + c / 8);
                 }
             }
+            ok = __all_sync(0xffffffffu, mbar_wait(full0 + 8 * s, phase));
+            if (!ok) break;
+            unsigned char* st = gbase + (size_t)s * stage_bytes + t * 16;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (j >= part.q_boxes) break;
+                uint4* at = reinterpret_cast<uint4*>(st + q_at + j * kBackBox);
+                uint4 v = *at;
+                float_pair g[4] = {Pair<T>::two(v.x), Pair<T>::two(v.y), Pair<T>::two(v.z), Pair<T>::two(v.w)};
+                if constexpr (ACT == DG_ACT_RELU) {
+                    const uint32_t m = above[j];
+                    auto keep = [](uint32_t two) { return (two & 1 ? 0xFFFFu : 0u) | (two & 2 ? 0xFFFF0000u : 0u); };
+                    v = make_uint4(v.x & keep(m), v.y & keep(m >> 2), v.z & keep(m >> 4), v.w & keep(m >> 6));
+                    g[0] = Pair<T>::two(v.x), g[1] = Pair<T>::two(v.y), g[2] = Pair<T>::two(v.z), g[3] = Pair<T>::two(v.w);
+                    *at = v;
+                } else if constexpr (kSmooth) {
+                    const uint4 u = *reinterpret_cast<const uint4*>(st + z_at + j * kBackBox);
+                    g[0] = mul2(g[0], act_slope2<ACT>(Pair<T>::two(u.x))), g[1] = mul2(g[1], act_slope2<ACT>(Pair<T>::two(u.y)));
+                    g[2] = mul2(g[2], act_slope2<ACT>(Pair<T>::two(u.z))), g[3] = mul2(g[3], act_slope2<ACT>(Pair<T>::two(u.w)));
+                    *at = make_uint4(Pair<T>::narrow(g[0]), Pair<T>::narrow(g[1]), Pair<T>::narrow(g[2]), Pair<T>::narrow(g[3]));
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum[j][e] = add2(sum[j][e], g[e]);
+            }
+            if (ACT != DG_ACT_NONE) fence_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(ready0 + 8 * s);
+            if (++s == a.stages) s = 0, phase ^= 1;
         }
+        if (a.db) {                                               // box by box: the 32 rows of a column, in order
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (j >= part.q_boxes) break;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 f = halves(sum[j][e]);
+                    sums[t * kBackSumPitch + 2 * e] = f.x, sums[t * kBackSumPitch + 2 * e + 1] = f.y;
+                }
+                asm volatile("bar.sync 1, %0;" ::"n"(32 * kBackMakers) : "memory");
+                const int c = part.q0 + 64 * j + t;
+                if (t < 64 && c < a.q_cols) {
+                    float total = 0.f;
+#pragma unroll 8
+                    for (int r = 0; r < 32; ++r) total += sums[(r * 8 + (t >> 3 ^ (r & 7))) * kBackSumPitch + (t & 7)];
+                    if (a.db_partial) a.db_partial[(int64_t)part.range * a.q_cols + c] = total;
+                    else static_cast<T*>(a.db)[c] = Pair<T>::round(total);
+                }
+                asm volatile("bar.sync 1, %0;" ::"n"(32 * kBackMakers) : "memory");
+            }
+        }
+        if (warp < 6) {
+            ok = ok && __all_sync(0xffffffffu, mbar_wait(acc_full, 0));     // tcgen05.ld is warp-collective
+            if (ok) {
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                flush_dw<T>(a, part, tmem, warp, lane);
+            }
+        }
+    } else if (lane == 0 && a.store) {
+        int s = 0, phase = 0;
+        for (int i = 0; i < part.slabs; ++i) {
+            ok = mbar_wait(ready0 + 8 * s, phase);
+            if (!ok) break;
+            const int row = (int)(part.r0 + (int64_t)i * kBackRows);
+            for (int j = 0; j < part.q_boxes; ++j) tma_store_2d(&tmS, part.q0 + 64 * j, row, base + s * stage_bytes + q_at + j * kBackBox);
+            bulk_commit();
+            bulk_wait_read();
+            mbar_arrive(stored0 + 8 * s);
+            if (++s == a.stages) s = 0, phase ^= 1;
+        }
+        bulk_wait();
     }
     if (!ok) atomicExch(a.status, 1);
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -1082,44 +1286,81 @@ extern "C" int dg_linear_dz(const void* dy, int64_t lddy, const void* z, int64_t
     return (int)cudaGetLastError();
 }
 
-extern "C" int64_t dg_linear_dw_scratch(int64_t M, int32_t N, int32_t K) { return M < 1 || N < 1 || K < 1 ? 0 : dw_shape(M, N, K).floats; }
-
-extern "C" int dg_linear_dw(const void* x, int64_t ldx, const void* dz, int64_t lddz, void* dw, int64_t row_stride, int64_t col_stride, int64_t M, int32_t N, int32_t K,
-                            int32_t type, float* scratch, int64_t scratch_floats, void* stream)
+extern "C" int64_t dg_linear_dw_scratch(int64_t M, int32_t N, int32_t K)
 {
-    if (!x || !dz || !dw) return DG_ERR_NULL;
-    if (M < 1 || M >= (int64_t)1 << 31 || N < 1 || K < 1 || ldx < K || lddz < N || (type != DG_BFLOAT16 && type != DG_FLOAT16) || !aligned(dw, 2) || !aligned(scratch, 16))
-        return DG_ERR_DIMS;
-    if (!on_rows(x, ldx, 2) || !on_rows(dz, lddz, 2)) return DG_ERR_UNSUPPORTED;
+    if (M < 1 || N < 1 || K < 1) return 0;
     const DwShape shape = dw_shape(M, N, K);
-    if (shape.floats > 0 && !scratch) return DG_ERR_NULL;
-    if (scratch_floats < shape.floats) return DG_ERR_SCRATCH;
+    return shape.floats ? shape.floats + (int64_t)shape.ranges * N : 0;
+}
+
+extern "C" int dg_linear_dw(const dg_linear_dw_args* g, void* stream)
+{
+    if (!g || !g->x || !g->dy || !g->dw) return DG_ERR_NULL;
+    const int64_t M = g->M;
+    const int32_t N = g->N, K = g->K, type = g->type, act = g->act;
+    if (M < 1 || M >= (int64_t)1 << 31 || N < 1 || K < 1 || g->ldx < K || g->lddy < N || (type != DG_BFLOAT16 && type != DG_FLOAT16) || act < 0 || act > 3) return DG_ERR_DIMS;
+    const bool smooth = act == DG_ACT_GELU || act == DG_ACT_SILU, fused = act != DG_ACT_NONE || g->db;
+    if ((smooth && !g->z) || (act == DG_ACT_RELU && !g->bits)) return DG_ERR_NULL;
+    if ((smooth && g->ldz < N) || (act == DG_ACT_RELU && g->ldbits * 32 < N) || (g->dz && (act == DG_ACT_NONE || g->lddz < N))) return DG_ERR_DIMS;
+    if (!aligned(g->dw, 2) || !aligned(g->db, 2) || !aligned(g->scratch, 16)) return DG_ERR_DIMS;
+    if (!on_rows(g->x, g->ldx, 2) || !on_rows(g->dy, g->lddy, 2) || (smooth && !on_rows(g->z, g->ldz, 2)) || (g->dz && !on_rows(g->dz, g->lddz, 2)) || (fused && K > 256))
+        return DG_ERR_UNSUPPORTED;
+    const DwShape shape = dw_shape(M, N, K);
+    const int64_t floats = dg_linear_dw_scratch(M, N, K);
+    if (floats > 0 && !g->scratch) return DG_ERR_NULL;
+    if (g->scratch_floats < floats) return DG_ERR_SCRATCH;
     LinearDwArgs a{};
-    a.partial = shape.floats > 0 ? reinterpret_cast<float4*>(scratch) : nullptr;
-    a.dw = dw, a.row_stride = row_stride, a.col_stride = col_stride;
+    a.partial = floats > 0 ? reinterpret_cast<float4*>(g->scratch) : nullptr;
+    a.dw = g->dw, a.row_stride = g->row_stride, a.col_stride = g->col_stride;
     a.M = M, a.rows_per_range = shape.rows_per_range, a.p_cols = K, a.q_cols = N;
     a.p_panels = shape.p_panels, a.q_panels = shape.q_panels, a.p_store = shape.p_store, a.q_store = shape.q_store;
     a.p_boxes = (std::min(K, 256) + 63) / 64, a.q_boxes = (std::min(N, 256) + 63) / 64;
     if (K > 64) a.p_boxes = (a.p_boxes + 1) / 2 * 2;              // an MMA reads 128 columns; what lies beyond x's reaches rows that are not stored
+    a.bits = g->bits, a.ldbits = g->ldbits, a.db = g->db, a.db_partial = floats > 0 ? g->scratch + shape.floats : nullptr, a.store = g->dz != nullptr;
     a.status = dg_status_word();
     if (!a.status) return DG_ERR_STATE;
-    CUtensorMap tmP, tmQ;
+    CUtensorMap maps[4];
     int rc;
-    if ((rc = make_map16(&tmP, x, type, M, K, ldx, kDwRows)) || (rc = make_map16(&tmQ, dz, type, M, N, lddz, kDwRows))) return rc;
-    const size_t stage = (size_t)(a.p_boxes + a.q_boxes) * kDwBox;
-    a.stages = (int)std::min<size_t>(kDwMaxStages, (227 * 1024 - kDwBarBytes - 1024) / stage);
-    const size_t smem = a.stages * stage + kDwBarBytes + 1024;
+    const int rows = fused ? kBackRows : kDwRows;
+    if ((rc = make_map16(&maps[0], g->x, type, M, K, g->ldx, rows)) || (rc = make_map16(&maps[1], g->dy, type, M, N, g->lddy, rows))) return rc;
+    maps[2] = maps[3] = maps[1];
+    if (smooth && (rc = make_map16(&maps[2], g->z, type, M, N, g->ldz, rows))) return rc;
+    if (g->dz && (rc = make_map16(&maps[3], g->dz, type, M, N, g->lddz, rows))) return rc;
     const unsigned ctas = (unsigned)(shape.ranges * shape.p_panels * shape.q_panels);
     const int64_t slots = (int64_t)shape.p_panels * shape.q_panels * (shape.p_store * shape.q_store / 4);
-    auto run = [&](auto value) {
+    cudaStream_t s = (cudaStream_t)stream;
+    auto product = [&](auto value) {
         using T = decltype(value);
+        const size_t stage = (size_t)(a.p_boxes + a.q_boxes) * kDwBox;
+        a.stages = (int)std::min<size_t>(kDwMaxStages, (227 * 1024 - kDwBarBytes - 1024) / stage);
         static std::atomic<bool> granted[64];
         const int code = allow_smem((const void*)k_linear_dw<T>, granted);
         if (code) return code;
-        k_linear_dw<T><<<ctas, kDwThreads, smem, (cudaStream_t)stream>>>(tmP, tmQ, a);
-        if (a.partial)
-            k_linear_dw_reduce<T><<<(unsigned)((slots + 31) / 32), 256, 0, (cudaStream_t)stream>>>(a.partial, shape.ranges, a.p_panels, a.q_panels, a.p_store, a.q_store, K, N,
-                                                                                              static_cast<T*>(dw), row_stride, col_stride);
+        k_linear_dw<T><<<ctas, kDwThreads, a.stages * stage + kDwBarBytes + 1024, s>>>(maps[0], maps[1], a);
+        return (int)cudaGetLastError();
+    };
+    auto product_with = [&](auto value, auto activation) {
+        using T = decltype(value);
+        constexpr int ACT = decltype(activation)::value;
+        const size_t stage = (size_t)(a.p_boxes + (smooth ? 2 : 1) * a.q_boxes) * kBackBox, rest = kBackSumBytes + kBackBarBytes + 1024;
+        a.stages = (int)std::min<size_t>(kBackMaxStages, (227 * 1024 - rest) / stage);
+        static std::atomic<bool> granted[64];
+        const int code = allow_smem((const void*)k_linear_back<T, ACT>, granted);
+        if (code) return code;
+        k_linear_back<T, ACT><<<ctas, kBackThreads, a.stages * stage + rest, s>>>(maps[0], maps[1], maps[2], maps[3], a);
+        return (int)cudaGetLastError();
+    };
+    auto run = [&](auto value) {
+        using T = decltype(value);
+        const int code = !fused                  ? product(value)
+                         : act == DG_ACT_RELU    ? product_with(value, std::integral_constant<int, DG_ACT_RELU>{})
+                         : act == DG_ACT_GELU    ? product_with(value, std::integral_constant<int, DG_ACT_GELU>{})
+                         : act == DG_ACT_SILU    ? product_with(value, std::integral_constant<int, DG_ACT_SILU>{})
+                                                 : product_with(value, std::integral_constant<int, DG_ACT_NONE>{});
+        if (code || !a.partial) return code;
+        k_linear_dw_reduce<T><<<(unsigned)((slots + 31) / 32), 256, 0, s>>>(a.partial, shape.ranges, a.p_panels, a.q_panels, a.p_store, a.q_store, K, N, static_cast<T*>(g->dw),
+                                                                        g->row_stride, g->col_stride);
+        if (g->db) k_linear_db<T><<<(unsigned)((N + 31) / 32), 1024, 0, s>>>(a.db_partial, shape.ranges, N, static_cast<T*>(g->db));
         return (int)cudaGetLastError();
     };
     return type == DG_BFLOAT16 ? run(__nv_bfloat16{}) : run(__half{});

@@ -478,16 +478,36 @@ struct LinearNode : public torch::autograd::Node {
         }
         int64_t launches = 0;
         Tensor g = by_rows(dy);
-        if (act != DG_ACT_NONE || db || ((dx || dw) && !on_rows(g))) {
-            const bool make = act != DG_ACT_NONE ? dx || dw || db : (dx || dw) && !on_rows(g);
-            Tensor dz = make && (dx || dw) ? whole_rows(M, N, x) : Tensor(), scratch;
-            if (db) {
-                out[2] = at::empty({N}, x.options());
-                scratch = at::empty({dg_linear_dz_scratch(M, (int32_t)N)}, x.options().dtype(at::kFloat));
+        if (db) out[2] = at::empty({N}, x.options());
+        const uint32_t* signs = bits.defined() ? reinterpret_cast<const uint32_t*>(bits.data_ptr<int32_t>()) : nullptr;
+        const int64_t ldbits = bits.defined() ? bits.size(1) : 0;
+        auto weight_gradient = [&](const Tensor& from, int32_t with, const Tensor* dz) {      // 16 bits
+            const Tensor rows = to_rows(x, &launches), d = out_in ? at::empty({N, K}, x.options()) : at::empty({K, N}, x.options());
+            const Tensor partial = at::empty({dg_linear_dw_scratch(M, (int32_t)N, (int32_t)K)}, x.options().dtype(at::kFloat));
+            dg_linear_dw_args a{};
+            a.x = rows.data_ptr(), a.ldx = ld_of(rows), a.dy = from.data_ptr(), a.lddy = ld_of(from), a.dw = d.data_ptr();
+            a.row_stride = out_in ? 1 : N, a.col_stride = out_in ? K : 1, a.M = M, a.N = (int32_t)N, a.K = (int32_t)K, a.type = type, a.act = with;
+            a.scratch = partial.data_ptr<float>(), a.scratch_floats = partial.numel();
+            if (dz) {
+                if (z.defined()) a.z = z.data_ptr(), a.ldz = ld_of(z);
+                a.bits = signs, a.ldbits = ldbits, a.db = db ? out[2].data_ptr() : nullptr;
+                if (dz->defined()) a.dz = dz->data_ptr(), a.lddz = dz->stride(0);
             }
+            check(dg_linear_dw(&a, stream));
+            launches += partial.numel() == 0 ? 1 : a.db ? 3 : 2;
+            out[1] = out_in ? d.t() : d;
+        };
+        // 16 bits, x of up to 256 columns: dz and its sums on the way to the weight gradient
+        const bool together = item == 2 && dw && K <= 256 && (act != DG_ACT_NONE || db) && on_rows(g) && (!z.defined() || on_rows(z));
+        if (together) {
+            const Tensor dz = dx && act != DG_ACT_NONE ? whole_rows(M, N, x) : Tensor();
+            weight_gradient(g, act, &dz);
+            if (dz.defined()) g = dz;
+        } else if (act != DG_ACT_NONE || db || ((dx || dw) && !on_rows(g))) {
+            const Tensor dz = (dx || dw) && (act != DG_ACT_NONE || !on_rows(g)) ? whole_rows(M, N, x) : Tensor();
+            const Tensor scratch = db ? at::empty({dg_linear_dz_scratch(M, (int32_t)N)}, x.options().dtype(at::kFloat)) : Tensor();
             if (dz.defined() || db) {
-                check(dg_linear_dz(g.data_ptr(), ld_of(g), z.defined() ? z.data_ptr() : nullptr, z.defined() ? ld_of(z) : 0,
-                                   bits.defined() ? reinterpret_cast<const uint32_t*>(bits.data_ptr<int32_t>()) : nullptr, bits.defined() ? bits.size(1) : 0, act,
+                check(dg_linear_dz(g.data_ptr(), ld_of(g), z.defined() ? z.data_ptr() : nullptr, z.defined() ? ld_of(z) : 0, signs, ldbits, act,
                                    dz.defined() ? dz.data_ptr() : nullptr, dz.defined() ? dz.stride(0) : 0, db ? out[2].data_ptr() : nullptr, M, (int32_t)N, type,
                                    db ? scratch.data_ptr<float>() : nullptr, stream));
                 launches += db && scratch.numel() > 0 ? 2 : 1;
@@ -505,21 +525,15 @@ struct LinearNode : public torch::autograd::Node {
             check(dg_linear(&a, stream));
             launches += item == 4 ? (K + 255) / 256 : 1;
         }
-        if (dw) {
+        if (dw && item == 2 && !together) weight_gradient(g, DG_ACT_NONE, nullptr);
+        if (dw && item == 4) {
             const Tensor rows = to_rows(x, &launches);
             const Tensor d = out_in ? at::empty({N, K}, x.options()) : at::empty({K, N}, x.options());
-            if (item == 4) {
-                const Tensor &left = out_in ? g : rows, &right = out_in ? rows : g;
-                const auto [partial, ctas] = tn_scratch(x, d.size(0), d.size(1));
-                check(dg_dense_tn(left.data_ptr<float>(), ld_of(left), right.data_ptr<float>(), ld_of(right), d.data_ptr<float>(), d.size(1), M, (int32_t)d.size(0),
-                                  (int32_t)d.size(1), partial.data_ptr<float>(), partial.numel(), ctas, stream));
-                launches += 2 * ((K + 255) / 256) * ((N + 255) / 256);
-            } else {
-                const Tensor partial = at::empty({dg_linear_dw_scratch(M, (int32_t)N, (int32_t)K)}, x.options().dtype(at::kFloat));
-                check(dg_linear_dw(rows.data_ptr(), ld_of(rows), g.data_ptr(), ld_of(g), d.data_ptr(), out_in ? 1 : N, out_in ? K : 1, M, (int32_t)N, (int32_t)K, type,
-                                   partial.data_ptr<float>(), partial.numel(), stream));
-                launches += partial.numel() > 0 ? 2 : 1;
-            }
+            const Tensor &left = out_in ? g : rows, &right = out_in ? rows : g;
+            const auto [partial, ctas] = tn_scratch(x, d.size(0), d.size(1));
+            check(dg_dense_tn(left.data_ptr<float>(), ld_of(left), right.data_ptr<float>(), ld_of(right), d.data_ptr<float>(), d.size(1), M, (int32_t)d.size(0),
+                              (int32_t)d.size(1), partial.data_ptr<float>(), partial.numel(), ctas, stream));
+            launches += 2 * ((K + 255) / 256) * ((N + 255) / 256);
             out[1] = out_in ? d.t() : d;
         }
         g_launches += launches;

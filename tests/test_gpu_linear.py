@@ -154,6 +154,31 @@ def test_only_what_is_asked_for():
     assert not spmm_cpp.linear(x, w).requires_grad
 
 
+@pytest.mark.parametrize('M,K,N', [(40, 24, 16), (700, 256, 264), (700, 300, 40), (20000, 64, 96), (900, 40, 41)])
+@pytest.mark.parametrize('act', [None, 'relu', 'gelu', 'silu'])
+def test_every_subset_of_gradients_is_the_same(M, K, N, act):
+    """Which gradients are asked for decides which kernels run (dz on the way to the weight gradient, by itself, kept or not): the numbers are those of all of them, but
+    for sums that a kernel of its own takes in another order."""
+    import spmm_cpp
+    gen = torch.Generator(device='cuda').manual_seed(M + N)
+    base = [torch.randn(*s, device='cuda', generator=gen).bfloat16() for s in ((M, K), (K, N), (N,), (M, N))]
+    dy = torch.randn(M, N, device='cuda', generator=gen).bfloat16()
+    all_leaves = [t.clone().requires_grad_() for t in base]
+    want = _grads(spmm_cpp.linear(*all_leaves[:3], residual=all_leaves[3], activation=act), dy, *all_leaves)
+    for asked in range(1, 16):
+        leaves = [t.clone().requires_grad_(bool(asked >> i & 1)) for i, t in enumerate(base)]
+        y = spmm_cpp.linear(*leaves[:3], residual=leaves[3], activation=act)
+        got = iter(_grads(y, dy, *[t for t in leaves if t.requires_grad]))
+        for i in range(4):
+            if asked >> i & 1:
+                g = next(got)
+                if i == 2:                                         # one step of the result, and the order of M sums
+                    assert float((g.double() - want[i].double()).abs().max()) <= (2.0 ** -7 + M * 2.0 ** -24) * float(want[i].abs().max())
+                else:
+                    assert torch.equal(g, want[i]), (asked, i)
+    assert spmm_cpp.dense_status() == 0
+
+
 def test_gradients_against_differences():
     """Central differences of f = sum(c y) along random directions in fp32: truncation h^2 / 6 of third derivatives (at most 2 a unit of z) and the
     rounding of y, 2^-22 (|y| + S) / 2h for each, added as if they were independent, eight deviations."""
@@ -249,6 +274,31 @@ def test_captured_and_on_two_streams(dtype):
     torch.cuda.synchronize()
     eager = [t.detach().clone().requires_grad_() for t in fresh]
     assert all(torch.equal(p, q) for p, q in zip(got, both(eager)))
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_first_call_of_a_thread(dtype):
+    """A thread whose first use of the device is one of these calls, memory for them lying ready."""
+    import threading
+    import spmm_cpp
+    x, w, dy = torch.ones(300, 64, device='cuda', dtype=dtype), torch.ones(64, 40, device='cuda', dtype=dtype, requires_grad=True), torch.ones(300, 40, device='cuda', dtype=dtype)
+    want = spmm_cpp.linear(x, w)
+    del want
+    out = []
+
+    def call():
+        try:
+            out.append(spmm_cpp.linear(x, w).detach().float().mean())
+            out.append(spmm_cpp.dense_nt(x, w.detach(), transposed=True) if dtype == torch.float32 else out[0])
+        except Exception as e:
+            out.append(e)
+    for _ in range(3):
+        thread = threading.Thread(target=call)
+        thread.start(), thread.join()
+    assert not [v for v in out if isinstance(v, Exception)], out
+    assert all(float(v.mean()) == 64 for v in out)
+    y = spmm_cpp.linear(x, w)
+    assert float(torch.autograd.grad(y, w, dy)[0].float().mean()) == 300
 
 
 def test_refusals():
