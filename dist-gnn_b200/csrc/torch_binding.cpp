@@ -10,6 +10,7 @@
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <algorithm>
 #include <atomic>
 #include <functional>
 #include <mutex>
@@ -418,6 +419,13 @@ Tensor whole_rows(int64_t rows, int64_t cols, const Tensor& like)
     const Tensor t = at::empty({rows, width}, like.options().requires_grad(false));
     return width == cols ? t : t.narrow(1, 0, cols);
 }
+// whole_rows that go to the caller.  Products of this library read padded rows of fp32 operands whole: what they find there is zero.
+Tensor result_rows(int64_t rows, int64_t cols, const Tensor& like)
+{
+    const Tensor t = whole_rows(rows, cols, like);
+    if (item_of(like) == 4 && t.stride(0) != cols && rows > 0) t.as_strided({rows, t.stride(0) - cols}, {t.stride(0), 1}, t.storage_offset() + cols).zero_();
+    return t;
+}
 // by_rows(t), with rows of whole 16-byte pieces
 Tensor to_rows(const Tensor& t, int64_t* launches)
 {
@@ -515,7 +523,7 @@ struct LinearNode : public torch::autograd::Node {
             if (dz.defined()) g = dz;
         }
         if (dx) {
-            out[0] = whole_rows(M, K, x);
+            out[0] = result_rows(M, K, x);
             dg_linear_args a{};
             a.x = g.data_ptr(), a.ldx = ld_of(g), a.w = w.data_ptr(), a.ldw = ld_of(w), a.out_in = !out_in;
             a.y = out[0].data_ptr(), a.ldy = out[0].stride(0), a.M = M, a.N = (int32_t)K, a.K = (int32_t)N, a.type = type;
@@ -581,7 +589,7 @@ Tensor linear(const Tensor& x, const Tensor& w, const std::optional<Tensor>& bia
         weight = stored(w);
         x2 = few ? by_rows(x) : to_rows(x, &launches);
         if (!few && type != DG_FLOAT32) weight.t = to_rows(weight.t, &launches);
-        y = few ? at::empty({M, N}, x.options().requires_grad(false)) : whole_rows(M, N, x);
+        y = few ? at::empty({M, N}, x.options().requires_grad(false)) : result_rows(M, N, x);
         const bool dz = train && (wants(x) || wants(w) || wants(b));
         if (dz && (act == DG_ACT_GELU || act == DG_ACT_SILU)) z = few ? at::empty({M, N}, y.options()) : whole_rows(M, N, x);
         if (dz && act == DG_ACT_RELU) bits = at::empty({M, (N + 63) / 64 * 2}, y.options().dtype(at::kInt));
@@ -678,6 +686,12 @@ struct AdamwTable {
             entries.push_back({p, m, v, ms.value_or(Tensor()), vs.value_or(Tensor()), step, place, group});
         }
         if (entries.empty()) return;
+        std::vector<std::pair<uintptr_t, uintptr_t>> spans;        // all tensors are stepped at once: none may share elements with another
+        for (const AdamwEntry& e : entries)
+            if (e.p.numel() > 0) spans.emplace_back(reinterpret_cast<uintptr_t>(e.p.data_ptr()), reinterpret_cast<uintptr_t>(e.p.data_ptr()) + e.p.nbytes());
+        std::sort(spans.begin(), spans.end());
+        for (size_t i = 1; i < spans.size(); ++i)
+            if (spans[i].first < spans[i - 1].second) throw std::runtime_error("parameters must not share memory");
         c10::cuda::CUDAGuard guard(entries[0].p.device());
         std::vector<dg_adamw_tensor> all;
         for (const AdamwEntry& e : entries) {

@@ -917,7 +917,8 @@ class AdamW(torch.optim.Optimizer):
         own = [p for group in self.param_groups for p in group['params']]
         for i, p in zip(saved, own):
             if i in state_dict['state']:
-                self.state[p] = {name: torch.as_tensor(value, device=p.device).clone() for name, value in state_dict['state'][i].items()}
+                self.state[p] = {name: torch.as_tensor(value, device=p.device, dtype=torch.int64 if name == 'step' else None).clone()
+                                 for name, value in state_dict['state'][i].items()}
         self._table = None
 
     def _new_state(self, p):
@@ -930,6 +931,8 @@ class AdamW(torch.optim.Optimizer):
                     root=torch.zeros(p.shape, dtype=torch.float8_e4m3fn, **options), root_scale=torch.zeros(blocks, **options, dtype=torch.float32))
 
     def _make_table(self):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError('AdamW: take a step before capturing one, or every replay would start from the state that the capture made')
         rows, place = [], 0
         names = ('exp_avg', 'exp_avg_sq', None, None) if self.state_bits == 32 else ('exp_avg', 'root', 'exp_avg_scale', 'root_scale')
         for k, group in enumerate(self.param_groups):
@@ -948,7 +951,7 @@ class AdamW(torch.optim.Optimizer):
 
     @property
     def grad_norm(self):
-        """Norm of all gradients in the last step, before they were scaled (None without max_norm, or before the first step)."""
+        """Norm of all gradients in the last step, before they were scaled (None without max_norm, or before the first step); the next step overwrites it."""
         return self._table.norm[0] if self.max_norm is not None and self._table is not None else None
 
     def step(self, closure=None):

@@ -301,6 +301,19 @@ def test_first_call_of_a_thread(dtype):
     assert float(torch.autograd.grad(y, w, dy)[0].float().mean()) == 300
 
 
+def test_padding_of_fp32_rows_is_zero():
+    """Products read padded rows of fp32 operands whole; results and x's gradients of odd widths have zeros there, whatever the memory held."""
+    import spmm_cpp
+    junk = torch.full((64, 1 << 16), float('nan'), device='cuda')
+    del junk
+    for M in (40, 5000):
+        x, w = torch.ones(M, 33, device='cuda', requires_grad=True), torch.ones(33, 41, device='cuda')
+        y = spmm_cpp.linear(x, w, activation='gelu')
+        dx, = torch.autograd.grad(y, x, torch.ones_like(y))
+        for t, cols, width in ((y.detach(), 41, 44), (dx, 33, 36)):
+            assert t.stride(0) == width and bool((t.as_strided((M, width - cols), (width, 1), cols) == 0).all())
+
+
 def test_refusals():
     import spmm_cpp
     x, w = torch.ones(4, 6, device='cuda'), torch.ones(6, 5, device='cuda')

@@ -296,3 +296,54 @@ def test_refusals():
     empty = torch.nn.Parameter(torch.empty(0, device='cuda'))
     empty.grad = torch.empty(0, device='cuda')
     spmm_cpp.AdamW([empty], max_norm=1.0).step()
+
+
+def test_calls_that_would_go_wrong_are_refused():
+    """Parameters that share elements (all are stepped at once), and a first step inside a capture (every replay would start anew)."""
+    import spmm_cpp
+    base = torch.ones(100, device='cuda')
+    a, b = torch.nn.Parameter(base[:60]), torch.nn.Parameter(base[59:])
+    a.grad, b.grad = torch.ones(60, device='cuda'), torch.ones(41, device='cuda')
+    with pytest.raises(RuntimeError, match='share memory'):
+        spmm_cpp.AdamW([a, b]).step()
+    b = torch.nn.Parameter(base[60:])
+    b.grad = torch.ones(40, device='cuda')
+    opt = spmm_cpp.AdamW([a, b])
+    stream = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match='before capturing'):
+        with torch.cuda.graph(graph, stream=stream):
+            opt.step()
+    opt.step()
+    assert float(base.max()) < 1
+
+
+def test_schedulers_hooks_and_foreign_state():
+    """A learning rate that a scheduler sets is the next step's; hooks run; the state of torch.optim.AdamW over fp32 parameters can be taken over."""
+    import spmm_cpp
+    params, g = _params([(300,), (7, 5)], torch.float32, 21)
+    twins = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    opt, ref = spmm_cpp.AdamW(params, **HYPER), torch.optim.AdamW(twins, foreach=False, **HYPER)
+    seen = []
+    handle = opt.register_step_post_hook(lambda *args: seen.append(1))
+    schedulers = [torch.optim.lr_scheduler.StepLR(o, 2, 0.1) for o in (opt, ref)]
+    for t in range(5):
+        for p, q in zip(params, twins):
+            q.grad = p.grad.clone()
+        opt.step(), ref.step()
+        [s.step() for s in schedulers]
+        if t == 2:
+            handle.remove()
+        _regrad(params, g)
+    assert len(seen) == 3 and opt.param_groups[0]['lr'] == ref.param_groups[0]['lr'] < HYPER['lr']
+    for p, q in zip(params, twins):                                # five steps of rates up to 3e-3, each within 2^-19 of itself, on numbers of order one
+        assert float((p - q).abs().max()) <= 5 * (2.0 ** -19 * 40 * HYPER['lr'] + 2.0 ** -23 * float(q.abs().max()))
+    other = spmm_cpp.AdamW([torch.nn.Parameter(q.detach().clone()) for q in twins])
+    other.load_state_dict(ref.state_dict())
+    heirs = other.param_groups[0]['params']
+    for p, q in zip(heirs, twins):
+        p.grad, q.grad = torch.ones_like(p), torch.ones_like(q)
+    other.step(), ref.step()
+    assert int(other.state[heirs[0]]['step']) == 6
+    for p, q in zip(heirs, twins):
+        assert float((p - q).abs().max()) <= 2.0 ** -19 * 40 * HYPER['lr'] + 2.0 ** -22 * float(q.abs().max())
