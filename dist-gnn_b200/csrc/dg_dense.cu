@@ -63,6 +63,17 @@ __device__ __forceinline__ void keep_signs(const DenseArgs& a, const uint32_t* r
     }
     a.bits[row * a.ldbits + c0 / 32] = word;
 }
+// The accumulator of the tail passes, added to the 32 columns of the head passes'.
+__device__ __forceinline__ void add_tails(uint32_t* r, uint32_t at, bool two)
+{
+    uint32_t u[32];
+    tmem_ld16(at, u);
+    if (two) tmem_ld16(at + 16, u + 16);
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+        if (j < 16 || two) r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(u[j]));
+}
 __device__ __forceinline__ float4 bias_piece(const DenseArgs& a, int c)      // four columns of which all are the result's
 {
     return a.bias ? make_float4(__ldg(a.bias + c), __ldg(a.bias + c + 1), __ldg(a.bias + c + 2), __ldg(a.bias + c + 3)) : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -105,28 +116,32 @@ namespace {
 // registers touch 32 cache lines an instruction (and so do the mask's loads); the piece goes through `stage` in shared memory
 // (32 rows of 36 floats, conflict-free both ways) and leaves as whole 128-byte row pieces, four rows an instruction.
 constexpr int kStagePitch = 36, kStageBytes = 32 * kStagePitch * 4;
-template <int EPI> __device__ __forceinline__ void store_rows(const DenseArgs& a, uint32_t acc, float* stage, int64_t row0, int lane)
+template <int EPI> __device__ __forceinline__ void store_rows(const DenseArgs& a, uint32_t acc, uint32_t tails_at, float* stage, int64_t row0, int lane)
 {
     const bool vec = a.ldc % 4 == 0 && (reinterpret_cast<uintptr_t>(a.C) & 15) == 0 &&
                      (!a.mask || (a.ldm % 4 == 0 && (reinterpret_cast<uintptr_t>(a.mask) & 15) == 0)) &&
                      (EPI < kLinear || !a.z || (a.ldz % 4 == 0 && (reinterpret_cast<uintptr_t>(a.z) & 15) == 0));
     const int rows = (int)min((int64_t)32, a.M - row0);
     for (int c0 = 0; c0 < a.n_pad; c0 += 32) {
-        const bool pieces = vec && c0 + 32 <= a.N;                // whole 128-byte pieces of every row
         const int r4 = lane >> 3, col4 = c0 + (lane & 7) * 4;
+        const bool some = EPI >= kLinear && a.N % 4 == 0 && c0 < a.N, mine16 = !some || col4 < a.N;
+        const bool pieces = vec && (c0 + 32 <= a.N || some);      // 128-byte pieces of every row, whole or their first columns
         float4 mk[8];
         if (pieces && a.mask) {                                   // requested before the accumulator read so that both are in flight
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                if (i * 4 + r4 < rows) mk[i] = __ldg(reinterpret_cast<const float4*>(a.mask + (row0 + i * 4 + r4) * a.ldm + col4));
+                if (i * 4 + r4 < rows && mine16) mk[i] = __ldg(reinterpret_cast<const float4*>(a.mask + (row0 + i * 4 + r4) * a.ldm + col4));
         }
         [[maybe_unused]] float4 shift;
-        if (EPI >= kLinear && pieces) shift = bias_piece(a, col4);
+        if (EPI >= kLinear && pieces && mine16) shift = bias_piece(a, col4);
         uint32_t r[32];
         tmem_ld16(acc + (uint32_t)c0, r);
         if (c0 + 16 < a.n_pad) tmem_ld16(acc + (uint32_t)c0 + 16, r + 16);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-        if (EPI == kLinear + DG_ACT_RELU && a.bits) keep_signs(a, r, c0, row0 + lane);
+        if constexpr (EPI >= kLinear) {
+            add_tails(r, acc + tails_at + (uint32_t)c0, c0 + 16 < a.n_pad);
+            if (EPI == kLinear + DG_ACT_RELU && a.bits) keep_signs(a, r, c0, row0 + lane);
+        }
         float4* mine = reinterpret_cast<float4*>(stage + lane * kStagePitch);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
@@ -135,7 +150,7 @@ template <int EPI> __device__ __forceinline__ void store_rows(const DenseArgs& a
         if (pieces) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                if (i * 4 + r4 >= rows) continue;
+                if (i * 4 + r4 >= rows || !mine16) continue;
                 float4 v = *reinterpret_cast<const float4*>(stage + (i * 4 + r4) * kStagePitch + (lane & 7) * 4);
                 if constexpr (EPI >= kLinear) {
                     v = v + shift;
@@ -186,7 +201,7 @@ template <int EPI> __device__ __forceinline__ void store_rows(const DenseArgs& a
 }
 
 template <int EPI>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads, EPI >= kLinear ? 2 : 1)
 k_dense_nt(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmBh,
            const __grid_constant__ CUtensorMap tmBt, const DenseArgs a)
 {
@@ -202,8 +217,11 @@ k_dense_nt(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t m0 = (int64_t)blockIdx.x * BM;
     const int nslabs = (a.K + BK - 1) / BK;
+    constexpr bool kApart = EPI >= kLinear;                       // the tail passes have an accumulator of their own
     int tmem_cols = 32;
     while (tmem_cols < a.n_pad) tmem_cols <<= 1;
+    const uint32_t tails_at = kApart ? (uint32_t)tmem_cols : 0u;
+    if (kApart) tmem_cols <<= 1;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
@@ -253,9 +271,9 @@ k_dense_nt(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
                 const uint64_t b_head = umma_desc_sw128(st + 2 * BM * 128), b_tail = umma_desc_sw128(st + 2 * BM * 128 + b_bytes);
 #pragma unroll
                 for (int k = 0; k < BK / 8; ++k) {               // 8 TF32 columns = 32 bytes per MMA: +2 in 16-byte units
-                    umma_tf32(tmem, a_tail + 2 * k, b_head + 2 * k, idesc, (i > 0 || k > 0) ? 1u : 0u);
-                    umma_tf32(tmem, a_head + 2 * k, b_tail + 2 * k, idesc, 1u);
-                    umma_tf32(tmem, a_head + 2 * k, b_head + 2 * k, idesc, 1u);
+                    umma_tf32(tmem + tails_at, a_tail + 2 * k, b_head + 2 * k, idesc, (i > 0 || k > 0) ? 1u : 0u);
+                    umma_tf32(tmem + tails_at, a_head + 2 * k, b_tail + 2 * k, idesc, 1u);
+                    umma_tf32(tmem, a_head + 2 * k, b_head + 2 * k, idesc, kApart && i == 0 && k == 0 ? 0u : 1u);
                 }
                 umma_commit(empty0 + 8 * s);                      // the stage is free once these MMAs have read it
             }
@@ -289,7 +307,7 @@ k_dense_nt(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
             const int q = warp & 3;                               // a warp may only read its own quarter of the TMEM lanes
             // every load has landed and every MMA has read its operands: the stages are free for the staging of the rows
             if (m0 + q * 32 < a.M)
-                store_rows<EPI>(a, tmem + ((uint32_t)(q * 32) << 16), reinterpret_cast<float*>(gbase + q * kStageBytes), m0 + q * 32, lane);
+                store_rows<EPI>(a, tmem + ((uint32_t)(q * 32) << 16), tails_at, reinterpret_cast<float*>(gbase + q * kStageBytes), m0 + q * 32, lane);
         }
     }
     if (!ok) atomicExch(a.status, 1);
@@ -322,7 +340,7 @@ k_dense_nt(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
 constexpr int PK = 16, kMaxPairStages = 10, kSplitWarps = 4, kEpilogueWarps = 8;
 constexpr int kThreadsPair = 32 * (2 + kSplitWarps + kEpilogueWarps);
 constexpr int kPieceBytes = 32 * 32 * 4;                          // staging of an epilogue warp: 32 rows x 32 columns
-constexpr int kPairBarBytes = 8 * (3 * kMaxPairStages + 5) + 8;
+constexpr int kPairBarBytes = 8 * (4 * kMaxPairStages + 5) + 8;
 
 __device__ __forceinline__ void umma_tf32_pair(uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate)
 {
@@ -348,11 +366,15 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     const int staging = stages * stage_bytes;                     // the epilogue warps' row pieces
     const uint32_t bars = base + staging + kEpilogueWarps * kPieceBytes;
     const uint32_t full0 = bars, ready0 = bars + 8 * kMaxPairStages, empty0 = bars + 16 * kMaxPairStages;
-    const uint32_t acc_full0 = bars + 24 * kMaxPairStages, acc_empty0 = acc_full0 + 16, done = acc_empty0 + 16;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbase + staging + kEpilogueWarps * kPieceBytes + 24 * kMaxPairStages + 40);
+    const uint32_t acc_full0 = bars + 24 * kMaxPairStages, acc_empty0 = acc_full0 + 16, done = acc_empty0 + 16, heads0 = done + 8;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbase + staging + kEpilogueWarps * kPieceBytes + 32 * kMaxPairStages + 40);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     const int nhalves = (a.K + PK - 1) / PK;
+    // The linear layer keeps the tail passes' sums, a 2,048th of the head passes', from being rounded with them: in accumulators of their own (columns 128 / 384)
+    // up to 128 columns, beyond by going through K twice, tails first.
+    const bool apart = EPI >= kLinear && a.n_pad <= 128;
+    const int sweeps = EPI >= kLinear && !apart ? 2 : 1;
     constexpr int kTmemCols = 512;                                // two accumulators of up to 256 columns
 
     if (threadIdx.x == 0) {
@@ -360,6 +382,7 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             mbar_init(full0 + 8 * s, 1);
             mbar_init(ready0 + 8 * s, 2 * kSplitWarps);
             mbar_init(empty0 + 8 * s, 1);
+            mbar_init(heads0 + 8 * s, 1);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(acc_full0 + 8 * b, 1);
@@ -381,20 +404,33 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     if (warp == 0) {
         if (lane == 0) {                                          // TMA producer: one ring of stages across all tiles
             int it = 0, s = 0, phase = 1;
+            StagePhases tails_of, heads_of;
+            const uint32_t leader_heads0 = in_leader(heads0);
             for (int tile = pair; tile < n_tiles && ok; tile += pairs) {
                 const int row0 = (int)((int64_t)tile * (2 * BM) + rank * BM);      // rows beyond the matrix arrive as zeros
-                for (int i = 0; i < nhalves; ++i, ++it) {
+                for (int i = 0; i < sweeps * nhalves; ++i, ++it) {
                     if (it >= stages) ok = mbar_wait(empty0 + 8 * s, phase);
                     if (!ok) break;
                     const uint32_t st = base + s * stage_bytes;
-                    mbar_expect_tx(full0 + 8 * s, a_bytes + 2 * b_bytes);
-                    tma_load_2d(st, &tmA, i * PK, row0, full0 + 8 * s);
-                    tma_load_2d(st + 2 * a_bytes, &tmBh, i * PK, rank * half_n, full0 + 8 * s);
-                    tma_load_2d(st + 2 * a_bytes + b_bytes, &tmBt, i * PK, rank * half_n, full0 + 8 * s);
+                    if (i < nhalves) {
+                        tails_of.take(s);
+                        mbar_expect_tx(full0 + 8 * s, a_bytes + 2 * b_bytes);
+                        tma_load_2d(st, &tmA, i * PK, row0, full0 + 8 * s);
+                        tma_load_2d(st + 2 * a_bytes, &tmBh, i * PK, rank * half_n, full0 + 8 * s);
+                        tma_load_2d(st + 2 * a_bytes + b_bytes, &tmBt, i * PK, rank * half_n, full0 + 8 * s);
+                    } else {                                      // heads alone need no split: the MMAs wait for the loads of both CTAs
+                        if (rank == 0) {
+                            heads_of.take(s);
+                            mbar_expect_tx(heads0 + 8 * s, 2 * (a_bytes + b_bytes));
+                        }
+                        tma_load_2d_pair(st, &tmA, (i - nhalves) * PK, row0, leader_heads0 + 8 * s);
+                        tma_load_2d_pair(st + 2 * a_bytes, &tmBh, (i - nhalves) * PK, rank * half_n, leader_heads0 + 8 * s);
+                    }
                     if (++s == stages) s = 0, phase ^= 1;
                 }
             }
-            await_loads(full0, it, stages);
+            tails_of.await(full0);
+            heads_of.await(heads0);
         }
     } else if (warp == 1) {
         if (rank == 0) {                                          // MMA issuer: the warp waits and counts together, one lane issues
@@ -405,10 +441,33 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             const uint64_t desc0 = umma_desc_sw64(base);
             const uint32_t next_stage = (uint32_t)stage_bytes >> 4, tail = a_bytes >> 4, b_head = 2 * tail, b_tail = b_head + ((uint32_t)b_bytes >> 4);
             int s = 0, phase = 0, lt = 0;
+            [[maybe_unused]] StagePhases tails_of, heads_of;
             for (int tile = pair; tile < n_tiles && ok; tile += pairs, ++lt) {
                 const int b = lt & 1, v = lt >> 1;
                 if (lt >= 2) ok = wait(acc_empty0 + 8 * b, (v - 1) & 1);     // both epilogues have drained this accumulator
                 const uint32_t acc = tmem + (uint32_t)(b * 256);
+                if constexpr (EPI >= kLinear) {
+                    for (int i = 0; i < sweeps * nhalves && ok; ++i) {
+                        ok = i < nhalves ? wait(ready0 + 8 * s, tails_of.take(s)) : wait(heads0 + 8 * s, heads_of.take(s));
+                        if (!ok) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        if (issuer) {
+                            const uint64_t d = desc0 + (uint32_t)s * next_stage;
+#pragma unroll
+                            for (int k = 0; k < PK / 8; ++k) {
+                                const uint32_t tails = apart ? acc + 128 : acc, add = i > 0 || k > 0 ? 1u : 0u;
+                                if (i < nhalves) {
+                                    umma_tf32_pair(tails, d + tail + 2 * k, d + b_head + 2 * k, idesc, add);
+                                    umma_tf32_pair(tails, d + 2 * k, d + b_tail + 2 * k, idesc, 1u);
+                                }
+                                if (apart || i >= nhalves) umma_tf32_pair(acc, d + 2 * k, d + b_head + 2 * k, idesc, add);
+                            }
+                            umma_commit_pair(empty0 + 8 * s);
+                        }
+                        __syncwarp();
+                        if (++s == stages) s = 0;
+                    }
+                } else
                 for (int i = 0; i < nhalves && ok; i += 2) {
                     // The tensor cores read a TF32 operand from a 32-bit container and ignore its low 13 bits (verified: identical
                     // bits with a masked copy), so the tile as TMA delivered it is the head.  The order of the additions decides the last
@@ -455,10 +514,11 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     } else if (warp < 2 + kSplitWarps) {
         const int t = threadIdx.x - 64;                           // split the A half slab of every stage
         const uint32_t leader_ready0 = in_leader(ready0);
-        int s = 0, phase = 0;
+        int s = 0;
+        StagePhases tails_of;
         for (int tile = pair; tile < n_tiles && ok; tile += pairs) {
             for (int i = 0; i < nhalves; ++i) {
-                ok = __all_sync(0xffffffffu, mbar_wait(full0 + 8 * s, phase));
+                ok = __all_sync(0xffffffffu, mbar_wait(full0 + 8 * s, tails_of.take(s)));
                 if (!ok) break;
                 const float4* head = reinterpret_cast<const float4*>(gbase + (size_t)s * stage_bytes) + t;
                 float4* tail = reinterpret_cast<float4*>(gbase + (size_t)s * stage_bytes + a_bytes) + t;
@@ -475,8 +535,9 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive_cluster(leader_ready0 + 8 * s);
-                if (++s == stages) s = 0, phase ^= 1;
+                if (++s == stages) s = 0;
             }
+            if (sweeps == 2) s = (s + nhalves) % stages;          // the heads' stages
         }
     } else {
         const int q = warp & 3, first = (warp - 2 - kSplitWarps) / 4 * 32;      // a warp may only read its own quarter of the TMEM lanes
@@ -495,16 +556,17 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             const int rows = (int)max((int64_t)0, min((int64_t)32, a.M - row0));
             const uint32_t acc = tmem + (uint32_t)(b * 256) + ((uint32_t)(q * 32) << 16);
             for (int c0 = first; c0 < a.n_pad; c0 += step) {
-                const bool whole = vec && c0 + 32 <= a.N;         // 128-byte pieces of every row, four rows an instruction
+                const bool some = EPI >= kLinear && a.N % 4 == 0 && c0 < a.N, mine16 = !some || c0 + piece * 4 < a.N;
+                const bool whole = vec && (c0 + 32 <= a.N || some);      // 128-byte pieces of every row, whole or their first columns, four rows an instruction
                 [[maybe_unused]] float4 mk[8];
                 if (side && whole) {                              // under way while the accumulator is waited for and read
                     const float* m = a.mask + (row0 + r4) * a.ldm + c0 + piece * 4;
 #pragma unroll
                     for (int i = 0; i < 8; ++i, m += 4 * a.ldm)
-                        if (i * 4 + r4 < rows) mk[i] = __ldg(reinterpret_cast<const float4*>(m));
+                        if (i * 4 + r4 < rows && mine16) mk[i] = __ldg(reinterpret_cast<const float4*>(m));
                 }
                 [[maybe_unused]] float4 shift;
-                if (EPI >= kLinear && whole) shift = bias_piece(a, c0 + piece * 4);
+                if (EPI >= kLinear && whole && mine16) shift = bias_piece(a, c0 + piece * 4);
                 if (c0 == first) {
                     ok = __all_sync(0xffffffffu, mbar_wait(acc_full0 + 8 * b, v & 1));     // tcgen05.ld is warp-collective
                     if (!ok) break;
@@ -515,6 +577,8 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                     tmem_ld16(acc + (uint32_t)c0, r);
                     tmem_ld16(acc + (uint32_t)c0 + 16, r + 16);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    if constexpr (EPI >= kLinear)
+                        if (apart) add_tails(r, acc + 128 + (uint32_t)c0, true);
                     if (c0 + step >= a.n_pad) {                   // the accumulator has been read: its next tile may start
                         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                         __syncwarp();
@@ -534,7 +598,7 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
 #pragma unroll
                     for (int i = 0; i < 8; ++i, c += 4 * a.ldc) {
                         if constexpr (EPI >= kLinear) {
-                            if (i * 4 + r4 >= rows) continue;
+                            if (i * 4 + r4 >= rows || !mine16) continue;
                             x[i] = x[i] + shift;
                             if (a.z) __stcs(reinterpret_cast<float4*>(a.z + (row0 + i * 4 + r4) * a.ldz + c0 + piece * 4), x[i]);
                             x[i] = activate<EPI - kLinear>(x[i]);
@@ -665,7 +729,7 @@ int make_map(CUtensorMap* map, const float* ptr, int64_t rows, int64_t cols, int
 bool by_pairs(int64_t M, int n_pad, int K, bool masked, int sms, bool linear)
 {
     const int64_t tiles = (M + BM - 1) / BM;
-    if (n_pad <= 64) return linear && n_pad > 32 && tiles > 2 * sms;      // half of a pair's epilogue warps have no piece of 32 columns
+    if (n_pad <= 64) return linear && tiles > 2 * sms;
     const bool half_slab = (K - 1) % BK < BK / 2;
     if (tiles <= sms) return n_pad > 128 || half_slab || K > (n_pad > 80 ? 96 : 128);
     return n_pad > 80 || (tiles > 2 * sms && (!masked || K > 64));
@@ -710,7 +774,7 @@ int launch_nt(const float* A, int64_t lda, const float* Bt_head, const float* Bt
             return run(k_dense_nt<decltype(e)::value == kMasked ? kPlain : decltype(e)::value>, granted);      // it asks for the mask itself
         });
     }
-    a.n_pad = (a.N + 31) / 32 * 32;                               // both CTAs hold whole groups of 16 of its rows
+    a.n_pad = std::max(64, (a.N + 31) / 32 * 32);                 // both CTAs hold whole groups of 16 of its rows, every epilogue warp has columns
     if ((rc = make_map(&tmA, A, a.M, a.K, lda, BM, PK)) || (rc = make_map(&tmBh, Bt_head, a.N, a.K, ldb, a.n_pad / 2, PK)) ||
         (rc = make_map(&tmBt, Bt_tail, a.N, a.K, ldb, a.n_pad / 2, PK)))
         return rc;
@@ -940,7 +1004,7 @@ __device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t smem_addr)
 // 100 x 256 1,205 -> 940, 256 x 47 1,017 -> 787, 256 x 128 1,280 -> 970; 150,001 rows: 127 -> 120, 91 -> 73, 78 -> 66, 96 -> 71.
 // Warps: 0 TMA, 1 MMA issue + tensor-memory allocation, 2-9 split, 10-13 flush.  Two accumulators (columns 0 / 256): while one is added to
 // the partial result the other takes the next rows.
-template <bool PAIR>
+template <bool PAIR, bool APART>
 __device__ __forceinline__ void dense_tn(const CUtensorMap& tmP, const CUtensorMap& tmQ, const DenseTnArgs& a)
 {
     extern __shared__ unsigned char smem_raw[];
@@ -1033,24 +1097,26 @@ __device__ __forceinline__ void dense_tn(const CUtensorMap& tmP, const CUtensorM
             for (int range = range0; range < range1; ++range) {
                 const int nslabs = slabs_of(range);
                 for (int i = 0; i < nslabs && ok; ++i) {
-                    const int b = group & 1, in_group = i % T;    // the accumulators change, and restart, with every flush group
-                    if (in_group == 0 && group >= 2) ok = mbar_wait(acc_empty0 + 8 * b, ((group >> 1) - 1) & 1);
+                    const int b = APART ? 0 : group & 1, in_group = i % T;      // the accumulators change, and restart, with every flush group
+                    if (in_group == 0 && group >= (APART ? 1 : 2)) ok = mbar_wait(acc_empty0 + 8 * b, (APART ? group - 1 : (group >> 1) - 1) & 1);
                     ok = ok && mbar_wait(ready0 + 8 * s, phase);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint32_t st = base + s * stage_bytes, acc = tmem + (uint32_t)(b * 256);
                     const uint64_t p_head = umma_desc_mn_sw128(st), p_tail = umma_desc_mn_sw128(st + TN_P_BYTES);
                     const uint64_t q_head = umma_desc_mn_sw128(st + 2 * TN_P_BYTES), q_tail = umma_desc_mn_sw128(st + 2 * TN_P_BYTES + q_bytes);
-                    auto multiply = [&](uint64_t p, uint64_t q, uint32_t add) {
-                        if constexpr (PAIR) umma_tf32_pair(acc, p, q, idesc, add);
-                        else umma_tf32(acc, p, q, idesc, add);
+                    auto multiply = [&](uint32_t to, uint64_t p, uint64_t q, uint32_t add) {
+                        if constexpr (PAIR) umma_tf32_pair(to, p, q, idesc, add);
+                        else umma_tf32(to, p, q, idesc, add);
                     };
+                    constexpr uint32_t kTailColumns = APART ? 256 : 0;
 #pragma unroll
                     for (int k = 0; k < TN_ROWS / 8; ++k) {       // one 8-row group (1024 bytes) per MMA; the tail of X comes first
                         const uint64_t adv = (uint64_t)(k * (1024 >> 4));
-                        multiply((a.swapped ? p_head : p_tail) + adv, (a.swapped ? q_tail : q_head) + adv, (in_group > 0 || k > 0) ? 1u : 0u);
-                        multiply((a.swapped ? p_tail : p_head) + adv, (a.swapped ? q_head : q_tail) + adv, 1u);
-                        multiply(p_head + adv, q_head + adv, 1u);
+                        const uint32_t first = (in_group > 0 || k > 0) ? 1u : 0u;
+                        multiply(acc + kTailColumns, (a.swapped ? p_head : p_tail) + adv, (a.swapped ? q_tail : q_head) + adv, APART ? (i > 0 || k > 0 ? 1u : 0u) : first);
+                        multiply(acc + kTailColumns, (a.swapped ? p_tail : p_head) + adv, (a.swapped ? q_head : q_tail) + adv, 1u);
+                        multiply(acc, p_head + adv, q_head + adv, APART ? first : 1u);
                     }
                     commit(empty0 + 8 * s);
                     if (in_group == T - 1 || i == nslabs - 1) {
@@ -1108,8 +1174,8 @@ __device__ __forceinline__ void dense_tn(const CUtensorMap& tmP, const CUtensorM
             float4* part = a.partial + (int64_t)((PAIR ? 2 : 1) * range + rank) * (a.q_store / 4) * a.p_store + row;
             const int groups = (slabs_of(range) + T - 1) / T;
             for (int g = 0; g < groups; ++g, ++group) {
-                const int b = group & 1;
-                ok = __all_sync(0xffffffffu, mbar_wait(acc_full0 + 8 * b, (group >> 1) & 1));        // tcgen05.ld is warp-collective
+                const int b = APART ? 0 : group & 1;
+                ok = __all_sync(0xffffffffu, mbar_wait(acc_full0 + 8 * b, (APART ? group : group >> 1) & 1));        // tcgen05.ld is warp-collective
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 for (int c0 = 0; c0 < a.q_store; c0 += 32) {      // two 16-column reads in flight per wait
@@ -1119,6 +1185,14 @@ __device__ __forceinline__ void dense_tn(const CUtensorMap& tmP, const CUtensorM
                     tmem_ld16(acc, r);
                     if (two) tmem_ld16(acc + 16, r + 16);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    if (APART && g == groups - 1) {               // the range's tails
+                        uint32_t u[32];
+                        tmem_ld16(acc + 256, u);
+                        if (two) tmem_ld16(acc + 256 + 16, u + 16);
+                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(u[j]));
+                    }
                     float4* p = part + (int64_t)(c0 / 4) * a.p_store;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
@@ -1149,15 +1223,17 @@ __device__ __forceinline__ void dense_tn(const CUtensorMap& tmP, const CUtensorM
         else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
     }
 }
+template <bool APART>
 __global__ void __launch_bounds__(kTnThreads, 1)
 k_dense_tn(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ CUtensorMap tmQ, const DenseTnArgs a)
 {
-    dense_tn<false>(tmP, tmQ, a);
+    dense_tn<false, APART>(tmP, tmQ, a);
 }
+template <bool APART>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTnThreads, 1)
 k_dense_tn_pair(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ CUtensorMap tmQ, const DenseTnArgs a)
 {
-    dense_tn<true>(tmP, tmQ, a);
+    dense_tn<true, APART>(tmP, tmQ, a);
 }
 
 // Adds the ranges' partials slot by slot, in order; slots of the padding are skipped.  A CTA takes 128 slots, eight warps fetch 40 ranges'
@@ -1216,8 +1292,10 @@ extern "C" int dg_dense_tn_supported(int64_t n, int32_t Km, int32_t Nn, int64_t 
     return encode_tiled() != nullptr;
 }
 
-extern "C" int dg_dense_tn(const float* X, int64_t ldx, const float* G, int64_t ldg, float* D, int64_t ldd, int64_t n,
-                           int32_t Km, int32_t Nn, float* scratch, int64_t scratch_floats, int32_t max_ctas, void* stream)
+namespace {
+
+int dense_tn_run(const float* X, int64_t ldx, const float* G, int64_t ldg, float* D, int64_t ldd, int64_t n, int32_t Km, int32_t Nn, float* scratch,
+                 int64_t scratch_floats, int32_t max_ctas, bool apart, void* stream)
 {
     if (!X || !G || !D || !scratch) return DG_ERR_NULL;
     if (ldd < Nn || max_ctas < 1 || (reinterpret_cast<uintptr_t>(scratch) & 15)) return DG_ERR_DIMS;
@@ -1225,15 +1303,15 @@ extern "C" int dg_dense_tn(const float* X, int64_t ldx, const float* G, int64_t 
     if (Km > 256 || Nn > 256) {     // wider than two accumulators: 256 x 256 panels of D, one after the other on the stream
         for (int32_t m0 = 0; m0 < Km; m0 += 256)                  // (they share `scratch`; the operands are streamed once per panel)
             for (int32_t c0 = 0; c0 < Nn; c0 += 256) {
-                const int rc = dg_dense_tn(X + m0, ldx, G + c0, ldg, D + (int64_t)m0 * ldd + c0, ldd, n, Km - m0 < 256 ? Km - m0 : 256,
-                                           Nn - c0 < 256 ? Nn - c0 : 256, scratch, scratch_floats, max_ctas, stream);
+                const int rc = dense_tn_run(X + m0, ldx, G + c0, ldg, D + (int64_t)m0 * ldd + c0, ldd, n, Km - m0 < 256 ? Km - m0 : 256,
+                                           Nn - c0 < 256 ? Nn - c0 : 256, scratch, scratch_floats, max_ctas, apart, stream);
                 if (rc) return rc;
             }
         return DG_OK;
     }
     if (max_ctas == 1 && Km > 128 && Nn > 128) {      // no CTA to pair with: both halves of X, one after the other (the same sums in the same order)
-        const int rc = dg_dense_tn(X, ldx, G, ldg, D, ldd, n, 128, Nn, scratch, scratch_floats, 1, stream);
-        return rc ? rc : dg_dense_tn(X + 128, ldx, G, ldg, D + (int64_t)128 * ldd, ldd, n, Km - 128, Nn, scratch, scratch_floats, 1, stream);
+        const int rc = dense_tn_run(X, ldx, G, ldg, D, ldd, n, 128, Nn, scratch, scratch_floats, 1, apart, stream);
+        return rc ? rc : dense_tn_run(X + 128, ldx, G, ldg, D + (int64_t)128 * ldd, ldd, n, Km - 128, Nn, scratch, scratch_floats, 1, apart, stream);
     }
     const bool pair = std::min(Km, Nn) > 128, swapped = !pair && Nn < Km;
     if (pair) max_ctas &= ~1;                                     // whole pairs, and no more CTAs than allowed
@@ -1261,9 +1339,41 @@ extern "C" int dg_dense_tn(const float* X, int64_t ldx, const float* G, int64_t 
     a.stages = (int)std::min<size_t>(kMaxTnStages, (227 * 1024 - kTnBarBytes - 1024) / stage);
     const size_t smem = a.stages * stage + kTnBarBytes + 1024;
     const CUtensorMap &tmP = swapped ? tmG : tmX, &tmQ = swapped ? tmX : tmG;
-    static std::atomic<bool> granted[64], granted_pair[64];
-    if ((rc = pair ? allow_smem((const void*)k_dense_tn_pair, granted_pair) : allow_smem((const void*)k_dense_tn, granted))) return rc;
-    (pair ? k_dense_tn_pair : k_dense_tn)<<<pair ? (a.ranges + 1) / 2 * 2 : a.ranges, kTnThreads, smem, (cudaStream_t)stream>>>(tmP, tmQ, a);
+    auto run = [&](auto* kernel, std::atomic<bool>* granted) {
+        const int code = allow_smem((const void*)kernel, granted);
+        if (code) return code;
+        kernel<<<pair ? (a.ranges + 1) / 2 * 2 : a.ranges, kTnThreads, smem, (cudaStream_t)stream>>>(tmP, tmQ, a);
+        return (int)cudaGetLastError();
+    };
+    static std::atomic<bool> granted[4][64];
+    rc = apart ? (pair ? run(k_dense_tn_pair<true>, granted[0]) : run(k_dense_tn<true>, granted[1])) : (pair ? run(k_dense_tn_pair<false>, granted[2]) : run(k_dense_tn<false>, granted[3]));
+    if (rc) return rc;
     k_dense_tn_reduce<<<(unsigned)(slots / 128), 256, 0, (cudaStream_t)stream>>>(scratch, a.ranges, (int32_t)slots, D, ldd, a.p_cols, a.q_cols, a.p_store, a.q_store, swapped);
     return (int)cudaGetLastError();
+}
+
+}  // namespace
+
+extern "C" int dg_dense_tn(const float* X, int64_t ldx, const float* G, int64_t ldg, float* D, int64_t ldd, int64_t n,
+                           int32_t Km, int32_t Nn, float* scratch, int64_t scratch_floats, int32_t max_ctas, void* stream)
+{
+    return dense_tn_run(X, ldx, G, ldg, D, ldd, n, Km, Nn, scratch, scratch_floats, max_ctas, false, stream);
+}
+
+// The fp32 weight gradient of dg_linear_dw: the same with an accumulator of its own for the tail passes.
+int64_t dg_dense_linear_dw_scratch(int32_t N, int32_t K)
+{
+    const int sms = sm_count();
+    auto roof = [](int32_t v, int32_t to) { return (int64_t)(std::min(v, 256) + to - 1) / to * to; };
+    return sms * std::max(roof(K, 128) * roof(N, 16), roof(N, 128) * roof(K, 16));
+}
+int dg_dense_linear_dw(const dg_linear_dw_args* g, cudaStream_t stream)
+{
+    const float *x = static_cast<const float*>(g->x), *dz = static_cast<const float*>(g->dy);
+    float* dw = static_cast<float*>(g->dw);
+    const int sms = sm_count();
+    if (sms <= 0) return DG_ERR_STATE;
+    if (g->col_stride == 1) return dense_tn_run(x, g->ldx, dz, g->lddy, dw, g->row_stride, g->M, g->K, g->N, g->scratch, g->scratch_floats, sms, true, stream);
+    if (g->row_stride == 1) return dense_tn_run(dz, g->lddy, x, g->ldx, dw, g->col_stride, g->M, g->N, g->K, g->scratch, g->scratch_floats, sms, true, stream);
+    return DG_ERR_UNSUPPORTED;
 }

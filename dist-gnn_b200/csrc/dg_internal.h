@@ -106,3 +106,5 @@ int dg_spmm_prepare(const dg_plan* plan, int32_t F, cudaStream_t stream);
 int dg_check_spmm_args(const dg_plan* plan, const float* val, const float* B, int64_t ldb, const float* C, int64_t ldc,
                        int32_t F, uint32_t flags, const float* row_scale, const float* bias);
 int dg_dense_linear(const dg_linear_args* args, cudaStream_t stream);      // the fp32 product of dg_linear (dg_dense.cu)
+int64_t dg_dense_linear_dw_scratch(int32_t N, int32_t K);                   // and of dg_linear_dw
+int dg_dense_linear_dw(const dg_linear_dw_args* args, cudaStream_t stream);

@@ -85,12 +85,6 @@ struct LinearPairArgs {
     int* status;
 };
 
-// A load into this CTA whose arrival is counted at a barrier of the pair's even CTA.
-__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t cluster_bar)
-{
-    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-                 ::"r"(dst), "l"(map), "r"(cluster_bar), "r"(c0), "r"(c1) : "memory");
-}
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int c0, int c1, uint32_t src)
 {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(src), "r"(c0), "r"(c1) : "memory");
@@ -1286,9 +1280,10 @@ extern "C" int dg_linear_dz(const void* dy, int64_t lddy, const void* z, int64_t
     return (int)cudaGetLastError();
 }
 
-extern "C" int64_t dg_linear_dw_scratch(int64_t M, int32_t N, int32_t K)
+extern "C" int64_t dg_linear_dw_scratch(int64_t M, int32_t N, int32_t K, int32_t type)
 {
     if (M < 1 || N < 1 || K < 1) return 0;
+    if (type == DG_FLOAT32) return dg_dense_linear_dw_scratch(N, K);
     const DwShape shape = dw_shape(M, N, K);
     return shape.floats ? shape.floats + (int64_t)shape.ranges * N : 0;
 }
@@ -1298,15 +1293,17 @@ extern "C" int dg_linear_dw(const dg_linear_dw_args* g, void* stream)
     if (!g || !g->x || !g->dy || !g->dw) return DG_ERR_NULL;
     const int64_t M = g->M;
     const int32_t N = g->N, K = g->K, type = g->type, act = g->act;
-    if (M < 1 || M >= (int64_t)1 << 31 || N < 1 || K < 1 || g->ldx < K || g->lddy < N || (type != DG_BFLOAT16 && type != DG_FLOAT16) || act < 0 || act > 3) return DG_ERR_DIMS;
+    if (M < 1 || M >= (int64_t)1 << 31 || N < 1 || K < 1 || g->ldx < K || g->lddy < N || type < 0 || type > 2 || act < 0 || act > 3) return DG_ERR_DIMS;
     const bool smooth = act == DG_ACT_GELU || act == DG_ACT_SILU, fused = act != DG_ACT_NONE || g->db;
     if ((smooth && !g->z) || (act == DG_ACT_RELU && !g->bits)) return DG_ERR_NULL;
     if ((smooth && g->ldz < N) || (act == DG_ACT_RELU && g->ldbits * 32 < N) || (g->dz && (act == DG_ACT_NONE || g->lddz < N))) return DG_ERR_DIMS;
-    if (!aligned(g->dw, 2) || !aligned(g->db, 2) || !aligned(g->scratch, 16)) return DG_ERR_DIMS;
+    const int item = type == DG_FLOAT32 ? 4 : 2;
+    if (!aligned(g->dw, item) || !aligned(g->db, item) || !aligned(g->scratch, 16)) return DG_ERR_DIMS;
+    if (type == DG_FLOAT32) return fused ? DG_ERR_UNSUPPORTED : dg_dense_linear_dw(g, (cudaStream_t)stream);
     if (!on_rows(g->x, g->ldx, 2) || !on_rows(g->dy, g->lddy, 2) || (smooth && !on_rows(g->z, g->ldz, 2)) || (g->dz && !on_rows(g->dz, g->lddz, 2)) || (fused && K > 256))
         return DG_ERR_UNSUPPORTED;
     const DwShape shape = dw_shape(M, N, K);
-    const int64_t floats = dg_linear_dw_scratch(M, N, K);
+    const int64_t floats = dg_linear_dw_scratch(M, N, K, type);
     if (floats > 0 && !g->scratch) return DG_ERR_NULL;
     if (g->scratch_floats < floats) return DG_ERR_SCRATCH;
     LinearDwArgs a{};

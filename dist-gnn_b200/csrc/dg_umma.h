@@ -83,6 +83,21 @@ __device__ __forceinline__ void await_loads(uint32_t full0, int issued, int stag
 {
     for (int t = issued > stages ? issued - stages : 0; t < issued; ++t) mbar_wait(full0 + 8 * (t % stages), (t / stages) & 1);
 }
+// The stages of a ring whose loads a barrier of its own counts, however often: the phase of each stage's next use, in a bit.
+struct StagePhases {
+    uint32_t next = 0, used = 0;
+    __device__ __forceinline__ uint32_t take(int s)
+    {
+        const uint32_t phase = next >> s & 1;
+        next ^= 1u << s, used |= 1u << s;
+        return phase;
+    }
+    __device__ __forceinline__ void await(uint32_t bar0) const      // the last use of every stage
+    {
+        for (int s = 0; s < 32; ++s)
+            if (used >> s & 1) mbar_wait(bar0 + 8 * s, (next >> s & 1) ^ 1);
+    }
+};
 // All MMAs this thread has issued; `done` is a barrier of its own, with a count of 1.
 __device__ __forceinline__ void await_mmas(uint32_t done)
 {

@@ -489,9 +489,9 @@ struct LinearNode : public torch::autograd::Node {
         if (db) out[2] = at::empty({N}, x.options());
         const uint32_t* signs = bits.defined() ? reinterpret_cast<const uint32_t*>(bits.data_ptr<int32_t>()) : nullptr;
         const int64_t ldbits = bits.defined() ? bits.size(1) : 0;
-        auto weight_gradient = [&](const Tensor& from, int32_t with, const Tensor* dz) {      // 16 bits
+        auto weight_gradient = [&](const Tensor& from, int32_t with, const Tensor* dz) {
             const Tensor rows = to_rows(x, &launches), d = out_in ? at::empty({N, K}, x.options()) : at::empty({K, N}, x.options());
-            const Tensor partial = at::empty({dg_linear_dw_scratch(M, (int32_t)N, (int32_t)K)}, x.options().dtype(at::kFloat));
+            const Tensor partial = at::empty({dg_linear_dw_scratch(M, (int32_t)N, (int32_t)K, type)}, x.options().dtype(at::kFloat));
             dg_linear_dw_args a{};
             a.x = rows.data_ptr(), a.ldx = ld_of(rows), a.dy = from.data_ptr(), a.lddy = ld_of(from), a.dw = d.data_ptr();
             a.row_stride = out_in ? 1 : N, a.col_stride = out_in ? K : 1, a.M = M, a.N = (int32_t)N, a.K = (int32_t)K, a.type = type, a.act = with;
@@ -502,7 +502,7 @@ struct LinearNode : public torch::autograd::Node {
                 if (dz->defined()) a.dz = dz->data_ptr(), a.lddz = dz->stride(0);
             }
             check(dg_linear_dw(&a, stream));
-            launches += partial.numel() == 0 ? 1 : a.db ? 3 : 2;
+            launches += item == 4 ? 2 * ((K + 255) / 256) * ((N + 255) / 256) : partial.numel() == 0 ? 1 : a.db ? 3 : 2;
             out[1] = out_in ? d.t() : d;
         };
         // 16 bits, x of up to 256 columns: dz and its sums on the way to the weight gradient
@@ -533,17 +533,7 @@ struct LinearNode : public torch::autograd::Node {
             check(dg_linear(&a, stream));
             launches += item == 4 ? (K + 255) / 256 : 1;
         }
-        if (dw && item == 2 && !together) weight_gradient(g, DG_ACT_NONE, nullptr);
-        if (dw && item == 4) {
-            const Tensor rows = to_rows(x, &launches);
-            const Tensor d = out_in ? at::empty({N, K}, x.options()) : at::empty({K, N}, x.options());
-            const Tensor &left = out_in ? g : rows, &right = out_in ? rows : g;
-            const auto [partial, ctas] = tn_scratch(x, d.size(0), d.size(1));
-            check(dg_dense_tn(left.data_ptr<float>(), ld_of(left), right.data_ptr<float>(), ld_of(right), d.data_ptr<float>(), d.size(1), M, (int32_t)d.size(0),
-                              (int32_t)d.size(1), partial.data_ptr<float>(), partial.numel(), ctas, stream));
-            launches += 2 * ((K + 255) / 256) * ((N + 255) / 256);
-            out[1] = out_in ? d.t() : d;
-        }
+        if (dw && !together) weight_gradient(g, DG_ACT_NONE, nullptr);
         g_launches += launches;
         return out;
     }

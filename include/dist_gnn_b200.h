@@ -425,10 +425,10 @@ int dg_linear(const dg_linear_args* args, void* stream);
 int64_t dg_linear_dz_scratch(int64_t M, int32_t N);
 int dg_linear_dz(const void* dy, int64_t lddy, const void* z, int64_t ldz, const uint32_t* bits, int64_t ldbits, int32_t act, void* dz, int64_t lddz,
                  void* db, int64_t M, int32_t N, int32_t type, float* scratch, void* stream);
-/* The weight gradient for bf16 and fp16 (fp32: dg_dense_tn): dw[k * row_stride + n * col_stride] = sum over rows of x[m, k] dz[m, n].
- * With act == DG_ACT_NONE and db == NULL dz is dy.  Else, for K <= 256 (DG_ERR_UNSUPPORTED beyond), dz = dy * act'(z) is made on the way from z or bits as
+/* The weight gradient: dw[k * row_stride + n * col_stride] = sum over rows of x[m, k] dz[m, n].
+ * With act == DG_ACT_NONE and db == NULL dz is dy.  Else, for 16 bits and K <= 256 (DG_ERR_UNSUPPORTED beyond), dz = dy * act'(z) is made on the way from z or bits as
  * dg_linear left them, its column sums go to db where that is given, and dz itself where that is (not with DG_ACT_NONE: it is dy).
- * x, dy, z and dz on rows.  scratch: 16-byte aligned, dg_linear_dw_scratch floats (0 for few rows). */
+ * x, dy, z and dz on rows; in fp32 one of the strides of dw is 1.  scratch: 16-byte aligned, dg_linear_dw_scratch floats (0 for few rows of 16 bits). */
 typedef struct dg_linear_dw_args {
     const void* x;
     const void* dy;
@@ -442,7 +442,7 @@ typedef struct dg_linear_dw_args {
     int64_t M;
     int32_t N, K, type, act;
 } dg_linear_dw_args;
-int64_t dg_linear_dw_scratch(int64_t M, int32_t N, int32_t K);
+int64_t dg_linear_dw_scratch(int64_t M, int32_t N, int32_t K, int32_t type);
 int dg_linear_dw(const dg_linear_dw_args* args, void* stream);
 /* dg_pad_rows for 16-bit elements: ld_dst a multiple of 8. */
 int dg_pad_rows16(const void* src, int64_t ld_src, int64_t n, int32_t cols, void* dst, int64_t ld_dst, void* stream);
