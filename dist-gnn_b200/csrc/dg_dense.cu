@@ -47,6 +47,19 @@ struct DenseArgs {
     float* z;                       // x w + b, or nullptr
     uint32_t* bits;                 // a bit an element where that is above zero, or nullptr
     int64_t ldz, ldbits;
+    int32_t panel;                  // columns of a CTA's panel, blockIdx.y's; 0: all of them
+
+    __device__ __forceinline__ int enter_panel()      // returns its first column
+    {
+        if (panel == 0) return 0;
+        const int n0 = blockIdx.y * panel;
+        C += n0, N = min(panel, N - n0);
+        if (mask) mask += n0;
+        if (bias) bias += n0;
+        if (z) z += n0;
+        if (bits) bits += n0 / 32;
+        return n0;
+    }
 };
 // What a kernel's epilogue does; from kLinear on: the linear layer's, with activation EPI - kLinear.
 constexpr int kPlain = 0, kMasked = 1, kLinear = 2;
@@ -203,8 +216,10 @@ template <int EPI> __device__ __forceinline__ void store_rows(const DenseArgs& a
 template <int EPI>
 __global__ void __launch_bounds__(kThreads, EPI >= kLinear ? 2 : 1)
 k_dense_nt(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmBh,
-           const __grid_constant__ CUtensorMap tmBt, const DenseArgs a)
+           const __grid_constant__ CUtensorMap tmBt, const DenseArgs args)
 {
+    DenseArgs a = args;
+    const int n0 = EPI >= kLinear ? a.enter_panel() : 0;
     extern __shared__ unsigned char smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t base = (raw + 1023u) & ~1023u;                 // swizzled tiles need 1024-byte alignment
@@ -253,8 +268,8 @@ k_dense_nt(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
                 const uint32_t st = base + s * stage_bytes;
                 mbar_expect_tx(full0 + 8 * s, BM * 128 + 2 * b_bytes);
                 tma_load_2d(st, &tmA, i * BK, (int)m0, full0 + 8 * s);
-                tma_load_2d(st + 2 * BM * 128, &tmBh, i * BK, 0, full0 + 8 * s);
-                tma_load_2d(st + 2 * BM * 128 + b_bytes, &tmBt, i * BK, 0, full0 + 8 * s);
+                tma_load_2d(st + 2 * BM * 128, &tmBh, i * BK, n0, full0 + 8 * s);
+                tma_load_2d(st + 2 * BM * 128 + b_bytes, &tmBt, i * BK, n0, full0 + 8 * s);
             }
             await_loads(full0, i, STAGES);
         }
@@ -354,8 +369,10 @@ __device__ __forceinline__ void umma_tf32_pair(uint32_t tmem_d, uint64_t a_desc,
 template <int EPI>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadsPair, 1)
 k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmBh,
-                const __grid_constant__ CUtensorMap tmBt, const DenseArgs a, const int n_tiles, const int stages)
+                const __grid_constant__ CUtensorMap tmBt, const DenseArgs args, const int n_tiles, const int stages)
 {
+    DenseArgs a = args;
+    const int n0 = EPI >= kLinear ? a.enter_panel() : 0;
     extern __shared__ unsigned char smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t base = (raw + 1023u) & ~1023u;
@@ -416,15 +433,15 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                         tails_of.take(s);
                         mbar_expect_tx(full0 + 8 * s, a_bytes + 2 * b_bytes);
                         tma_load_2d(st, &tmA, i * PK, row0, full0 + 8 * s);
-                        tma_load_2d(st + 2 * a_bytes, &tmBh, i * PK, rank * half_n, full0 + 8 * s);
-                        tma_load_2d(st + 2 * a_bytes + b_bytes, &tmBt, i * PK, rank * half_n, full0 + 8 * s);
+                        tma_load_2d(st + 2 * a_bytes, &tmBh, i * PK, n0 + rank * half_n, full0 + 8 * s);
+                        tma_load_2d(st + 2 * a_bytes + b_bytes, &tmBt, i * PK, n0 + rank * half_n, full0 + 8 * s);
                     } else {                                      // heads alone need no split: the MMAs wait for the loads of both CTAs
                         if (rank == 0) {
                             heads_of.take(s);
                             mbar_expect_tx(heads0 + 8 * s, 2 * (a_bytes + b_bytes));
                         }
                         tma_load_2d_pair(st, &tmA, (i - nhalves) * PK, row0, leader_heads0 + 8 * s);
-                        tma_load_2d_pair(st + 2 * a_bytes, &tmBh, (i - nhalves) * PK, rank * half_n, leader_heads0 + 8 * s);
+                        tma_load_2d_pair(st + 2 * a_bytes, &tmBh, (i - nhalves) * PK, n0 + rank * half_n, leader_heads0 + 8 * s);
                     }
                     if (++s == stages) s = 0, phase ^= 1;
                 }
@@ -750,7 +767,8 @@ template <class Use> int by_epilogue(int epilogue, Use use)
 // One panel (up to 256 columns) of a product with the epilogue that `a` describes.
 int launch_nt(const float* A, int64_t lda, const float* Bt_head, const float* Bt_tail, int64_t ldb, DenseArgs a, int epilogue, cudaStream_t stream)
 {
-    a.n_pad = (a.N + 15) / 16 * 16;
+    const int cols = a.panel ? std::min(a.panel, a.N) : a.N, panels = a.panel ? (a.N + a.panel - 1) / a.panel : 1;
+    a.n_pad = (cols + 15) / 16 * 16;
     a.status = dg_status_word();
     if (!a.status) return DG_ERR_STATE;
     const int sms = sm_count();
@@ -766,7 +784,7 @@ int launch_nt(const float* A, int64_t lda, const float* Bt_head, const float* Bt
         auto run = [&](auto* kernel, std::atomic<bool>* granted) {
             const int code = allow_smem((const void*)kernel, granted);
             if (code) return code;
-            kernel<<<(unsigned)((a.M + BM - 1) / BM), kThreads, smem, stream>>>(tmA, tmBh, tmBt, a);
+            kernel<<<dim3((unsigned)((a.M + BM - 1) / BM), (unsigned)panels), kThreads, smem, stream>>>(tmA, tmBh, tmBt, a);
             return (int)cudaGetLastError();
         };
         return by_epilogue(epilogue, [&](auto e) {
@@ -774,7 +792,7 @@ int launch_nt(const float* A, int64_t lda, const float* Bt_head, const float* Bt
             return run(k_dense_nt<decltype(e)::value == kMasked ? kPlain : decltype(e)::value>, granted);      // it asks for the mask itself
         });
     }
-    a.n_pad = std::max(64, (a.N + 31) / 32 * 32);                 // both CTAs hold whole groups of 16 of its rows, every epilogue warp has columns
+    a.n_pad = std::max(64, (cols + 31) / 32 * 32);                // both CTAs hold whole groups of 16 of its rows, every epilogue warp has columns
     if ((rc = make_map(&tmA, A, a.M, a.K, lda, BM, PK)) || (rc = make_map(&tmBh, Bt_head, a.N, a.K, ldb, a.n_pad / 2, PK)) ||
         (rc = make_map(&tmBt, Bt_tail, a.N, a.K, ldb, a.n_pad / 2, PK)))
         return rc;
@@ -784,7 +802,7 @@ int launch_nt(const float* A, int64_t lda, const float* Bt_head, const float* Bt
     auto run = [&](auto* kernel, std::atomic<bool>* granted) {
         const int code = allow_smem((const void*)kernel, granted);
         if (code) return code;
-        kernel<<<2u * (unsigned)std::min(n_tiles, sms / 2), kThreadsPair, stages * stage + rest, stream>>>(tmA, tmBh, tmBt, a, n_tiles, stages);
+        kernel<<<dim3(2u * (unsigned)std::min(n_tiles, sms / 2), (unsigned)panels), kThreadsPair, stages * stage + rest, stream>>>(tmA, tmBh, tmBt, a, n_tiles, stages);
         return (int)cudaGetLastError();
     };
     return by_epilogue(epilogue, [&](auto e) {
@@ -864,23 +882,24 @@ extern "C" int dg_dense_nt_masked(const float* A, int64_t lda, const float* Bt_h
     return launch_nt(A, lda, Bt_head, Bt_tail, ldb, a, mask ? kMasked : kPlain, (cudaStream_t)stream);
 }
 
-// The fp32 product of dg_linear: panels as above, the epilogue's operands with them.
+// The fp32 product of dg_linear.
 int dg_dense_linear(const dg_linear_args* g, cudaStream_t stream)
 {
     const float* x = static_cast<const float*>(g->x);
     if (!g->head || !g->tail) return DG_ERR_NULL;
     if (!dg_dense_supported(g->M, g->N, g->K, g->ldx, g->ldb, x, g->head, g->tail)) return DG_ERR_UNSUPPORTED;
-    for (int32_t n0 = 0; n0 < g->N; n0 += 256) {
-        DenseArgs a{};
-        a.C = static_cast<float*>(g->y) + n0; a.ldc = g->ldy; a.M = g->M; a.N = std::min(256, g->N - n0); a.K = g->K;
-        a.mask = g->residual ? static_cast<const float*>(g->residual) + n0 : nullptr; a.ldm = g->ldr;
-        a.bias = g->bias ? static_cast<const float*>(g->bias) + n0 : nullptr;
-        a.z = g->z ? static_cast<float*>(g->z) + n0 : nullptr; a.ldz = g->ldz;
-        a.bits = g->bits ? g->bits + n0 / 32 : nullptr; a.ldbits = g->ldbits;
-        const int rc = launch_nt(x, g->ldx, g->head + (int64_t)n0 * g->ldb, g->tail + (int64_t)n0 * g->ldb, g->ldb, a, kLinear + g->act, stream);
-        if (rc) return rc;
-    }
-    return DG_OK;
+    DenseArgs a{};
+    a.C = static_cast<float*>(g->y); a.ldc = g->ldy; a.M = g->M; a.N = g->N; a.K = g->K;
+    a.mask = static_cast<const float*>(g->residual); a.ldm = g->ldr;
+    a.bias = static_cast<const float*>(g->bias);
+    a.z = static_cast<float*>(g->z); a.ldz = g->ldz;
+    a.bits = g->bits; a.ldbits = g->ldbits;
+    // Panels of 256 columns, one launch for all; of 128 or 64 while that leaves SMs without a tile of 128 rows (600 x 512 -> 512 57.6 us -> 22.9).
+    const int sms = sm_count();
+    a.panel = 256;
+    while (a.panel > 64 && (a.M + BM - 1) / BM * ((a.N + a.panel - 1) / a.panel) < sms) a.panel /= 2;
+    if (a.N / a.panel >= 65535) return DG_ERR_UNSUPPORTED;
+    return launch_nt(x, g->ldx, g->head, g->tail, g->ldb, a, kLinear + g->act, stream);
 }
 
 extern "C" int dg_dense_status(int* host_status, void* stream)
