@@ -5,7 +5,7 @@
 // k_linear_dw: the weight gradient x^T dz, both operands MN-major, rows cut into ranges whose partial results are added in order.
 // k_linear_back: the same with dz = dy act'(z), its column sums and, where asked, dz itself made on the way.
 // k_linear_dz: dz and its column sums alone.
-// k_few_*: products of few rows, bound by latency.
+// k_few_*: products of few rows, bound by latency.  k_thin, k_thin_grad: narrow layers.
 // The fp32 product is dg_dense.cu's.
 #include <algorithm>
 #include <cuda_bf16.h>
@@ -1074,6 +1074,213 @@ template <bool OUT_IN, int ROWS> __global__ void __launch_bounds__(32 * kFewWarp
     }
 }
 
+// ---- narrow layers ------------------------------------------------------------------------------------------------------------------
+// Up to 32 inputs and 32 outputs: a tile of the tensor cores' kernels costs some 2 us whatever its width, and rows that are no whole 16-byte pieces have to be
+// copied for them (1,611,877 x 7 -> 11 fp32 SiLU took 321 us, a sixteenth of it for the bytes, and takes 66), so these multiply on the CUDA cores, a row a thread, any strides, sums in fp32: K N products a row, for 32 x 32 about as long as the
+// bytes take.  Rows travel through shared memory, so that both ways are whole lines whatever the width; the place of an element by a product and a
+// shift instead of a division.
+constexpr int kThinRows = 128, kThinMost = 32, kThinPitch = 36;      // pitch: rows on 16 bytes, eight of them on all banks
+
+struct Divide {                                   // e / d for e < 4,096 and d <= 32
+    uint32_t factor, d;
+    __device__ __forceinline__ explicit Divide(int by) : factor(((1u << 20) + by - 1) / by), d(by) {}
+    __device__ __forceinline__ int rows(int e) const { return (int)((uint32_t)e * factor >> 20); }
+};
+// rows x cols elements of a matrix to or from shared memory, by all threads; use(value as fp32, row, column, place in shared memory)
+template <class T, class Use> __device__ __forceinline__ void thin_load(const T* p, int64_t ld, int rows, int cols, const Divide& by, Use use)
+{
+#pragma unroll 4
+    for (int e = threadIdx.x; e < rows * cols; e += kThinRows) {
+        const int r = by.rows(e), c = e - r * cols;
+        use(Pair<T>::one(p[r * ld + c]), r, c, r * kThinPitch + c);
+    }
+}
+template <class T> __device__ __forceinline__ void thin_store(T* p, int64_t ld, int rows, int cols, const Divide& by, const float* from)
+{
+#pragma unroll 4
+    for (int e = threadIdx.x; e < rows * cols; e += kThinRows) {
+        const int r = by.rows(e), c = e - r * cols;
+        p[r * ld + c] = Pair<T>::round(from[r * kThinPitch + c]);
+    }
+}
+// acc[n] = sum over k < K of row[k] w[k][n], w in rows of kThinMost.
+template <int NMAX> __device__ __forceinline__ void thin_product(float* acc, const float* row, const float* w, int K)
+{
+#pragma unroll
+    for (int n = 0; n < NMAX; ++n) acc[n] = 0.f;
+    for (int k0 = 0; k0 < K; k0 += 4) {                           // rows are zero up to a multiple of four
+        const float4 four = *reinterpret_cast<const float4*>(row + k0);
+        const float u[4] = {four.x, four.y, four.z, four.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int n = 0; n < NMAX; n += 4) {
+                const float4 v = *reinterpret_cast<const float4*>(w + (k0 + k) * kThinMost + n);
+                acc[n] = fmaf(u[k], v.x, acc[n]), acc[n + 1] = fmaf(u[k], v.y, acc[n + 1]);
+                acc[n + 2] = fmaf(u[k], v.z, acc[n + 2]), acc[n + 3] = fmaf(u[k], v.w, acc[n + 3]);
+            }
+    }
+}
+// w [K x N] as fp32, [k][n] or transposed, zero beyond the matrix.
+template <class T> __device__ __forceinline__ void thin_weight(float* to, const T* w, int64_t ldw, bool out_in, int K, int N, bool transposed)
+{
+    for (int e = threadIdx.x; e < kThinMost * kThinMost; e += kThinRows) {
+        const int a = e / kThinMost, b = e % kThinMost, k = transposed ? b : a, n = transposed ? a : b;
+        to[e] = k < K && n < N ? Pair<T>::one(out_in ? w[n * ldw + k] : w[k * ldw + n]) : 0.f;
+    }
+}
+
+template <class T, int ACT, int NMAX>
+__global__ void __launch_bounds__(kThinRows) k_thin(const FewArgs a, const int out_in)
+{
+    __shared__ __align__(16) float w[kThinMost * kThinMost], rows_in[kThinRows * kThinPitch], rows_out[kThinRows * kThinPitch], shift[kThinMost];
+    const T *x = static_cast<const T*>(a.x), *r = static_cast<const T*>(a.residual);
+    T *y = static_cast<T*>(a.y), *z = static_cast<T*>(a.z);
+    const Divide by_k(a.K), by_n(a.N);
+    thin_weight(w, static_cast<const T*>(a.w), a.ldw, out_in != 0, a.K, a.N, false);
+    if (threadIdx.x < kThinMost) shift[threadIdx.x] = a.bias && threadIdx.x < a.N ? Pair<T>::one(static_cast<const T*>(a.bias)[threadIdx.x]) : 0.f;
+    for (int i = threadIdx.x; i < kThinRows * kThinPitch; i += kThinRows) rows_in[i] = 0.f;
+    float* const mine = rows_out + threadIdx.x * kThinPitch;
+    for (int64_t m0 = (int64_t)blockIdx.x * kThinRows; m0 < a.M; m0 += (int64_t)gridDim.x * kThinRows) {
+        const int rows = (int)min((int64_t)kThinRows, a.M - m0);
+        __syncthreads();
+        thin_load(x + m0 * a.ldx, a.ldx, rows, a.K, by_k, [&](float v, int, int, int at) { rows_in[at] = v; });
+        if (r && !z) thin_load(r + m0 * a.ldr, a.ldr, rows, a.N, by_n, [&](float v, int, int, int at) { rows_out[at] = v; });
+        __syncthreads();
+        float acc[NMAX];
+        thin_product<NMAX>(acc, rows_in + threadIdx.x * kThinPitch, w, a.K);
+#pragma unroll
+        for (int n = 0; n < NMAX; ++n) acc[n] += shift[n];
+        if (ACT == DG_ACT_RELU && a.bits && (int)threadIdx.x < rows) {
+            uint32_t word = 0;
+#pragma unroll
+            for (int n = 0; n < NMAX; ++n) word |= (acc[n] <= 0.f ? 0u : 1u) << n;
+            a.bits[(m0 + threadIdx.x) * a.ldbits] = word;
+        }
+        if (z) {                                                  // z and y go out one after the other through the same rows
+#pragma unroll
+            for (int n = 0; n < NMAX; ++n) mine[n] = acc[n];
+            __syncthreads();
+            thin_store(z + m0 * a.ldz, a.ldz, rows, a.N, by_n, rows_out);
+            __syncthreads();
+            if (r) {
+                thin_load(r + m0 * a.ldr, a.ldr, rows, a.N, by_n, [&](float v, int, int, int at) { rows_out[at] = v; });
+                __syncthreads();
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NMAX; ++n) mine[n] = act_value<ACT>(acc[n]) + (r ? mine[n] : 0.f);
+        __syncthreads();
+        thin_store(y + m0 * a.ldy, a.ldy, rows, a.N, by_n, rows_out);
+    }
+}
+
+// All gradients in one pass over x, dy and z: dz goes to shared memory and stays in fp32, a thread makes a row of dx, and every thread of the dw part four by
+// four of its elements (a row of ones below x makes db the last row of dw) over a share of the tile's rows, tile after tile; the CTAs' sums are added in order.
+struct ThinGradArgs {
+    const void *x, *w, *dy, *z;
+    const uint32_t* bits;
+    void *dx, *dw, *db;
+    float* partial;                               // [CTA][(K + 1) N], or null: the one CTA's sums are the result
+    int64_t ldx, ldw, lddy, ldz, ldbits, lddx, row_stride, col_stride, M;
+    int32_t N, K, out_in;
+};
+
+template <class T, int ACT>
+__global__ void __launch_bounds__(kThinRows) k_thin_grad(const ThinGradArgs a)
+{
+    __shared__ __align__(16) float w[kThinMost * kThinMost], xs[kThinRows * kThinPitch], ds[kThinRows * kThinPitch];
+    const T *x = static_cast<const T*>(a.x), *dy = static_cast<const T*>(a.dy), *z = static_cast<const T*>(a.z);
+    const Divide by_k(a.K), by_n(a.N);
+    const bool sums = a.dw || a.db;
+    if (a.dx) thin_weight(w, static_cast<const T*>(a.w), a.ldw, a.out_in != 0, a.K, a.N, true);      // [n][k]
+    for (int i = threadIdx.x; i < kThinRows * kThinPitch; i += kThinRows) xs[i] = ds[i] = 0.f;
+    __syncthreads();
+    // x's row of ones (column K); rows beyond the matrix have dz = 0
+    xs[threadIdx.x * kThinPitch + a.K] = 1.f;
+    const int k_blocks = a.K / 4 + 1, blocks = k_blocks * ((a.N + 3) / 4), groups = kThinRows / blocks;      // 9 x 8 blocks at most
+    const int block = threadIdx.x % blocks, group = threadIdx.x / blocks, k0 = block % k_blocks * 4, n0 = block / k_blocks * 4;
+    float acc[4][4] = {};
+    for (int64_t m0 = (int64_t)blockIdx.x * kThinRows; m0 < a.M; m0 += (int64_t)gridDim.x * kThinRows) {
+        const int rows = (int)min((int64_t)kThinRows, a.M - m0);
+        __syncthreads();
+        if (a.dw) thin_load(x + m0 * a.ldx, a.ldx, rows, a.K, by_k, [&](float v, int, int, int at) { xs[at] = v; });
+        thin_load(dy + m0 * a.lddy, a.lddy, rows, a.N, by_n, [&](float v, int row, int c, int at) {
+            if constexpr (ACT == DG_ACT_RELU) v = a.bits[(m0 + row) * a.ldbits] >> c & 1 ? v : 0.f;
+            else if constexpr (ACT != DG_ACT_NONE) v *= act_slope<ACT>(Pair<T>::one(z[(m0 + row) * a.ldz + c]));
+            ds[at] = v;
+        });
+        if (rows < kThinRows)                                     // a last tile: what the one before left
+            for (int e = threadIdx.x + rows * kThinPitch; e < kThinRows * kThinPitch; e += kThinRows) ds[e] = 0.f;
+        __syncthreads();
+        if (sums && group < groups)
+            for (int row = group; row < rows; row += groups) {
+                const float4 u = *reinterpret_cast<const float4*>(xs + row * kThinPitch + k0), v = *reinterpret_cast<const float4*>(ds + row * kThinPitch + n0);
+                const float p[4] = {u.x, u.y, u.z, u.w}, q[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(p[i], q[j], acc[i][j]);
+            }
+        if (a.dx) {
+            float out[kThinMost];
+            if (a.K <= 8) thin_product<8>(out, ds + threadIdx.x * kThinPitch, w, a.N);
+            else if (a.K <= 16) thin_product<16>(out, ds + threadIdx.x * kThinPitch, w, a.N);
+            else thin_product<32>(out, ds + threadIdx.x * kThinPitch, w, a.N);
+            __syncthreads();                                      // dz has been read
+            const int most = a.K <= 8 ? 8 : a.K <= 16 ? 16 : 32;
+#pragma unroll
+            for (int k = 0; k < kThinMost; ++k)
+                if (k < most) ds[threadIdx.x * kThinPitch + k] = out[k];
+            __syncthreads();
+            thin_store(static_cast<T*>(a.dx) + m0 * a.lddx, a.lddx, rows, a.K, by_k, ds);
+            __syncthreads();
+            // columns of dx beyond dz's are dz's padding, which the sums read as zero
+            if (a.K > a.N)
+                for (int c = a.N; c < kThinPitch; ++c) ds[threadIdx.x * kThinPitch + c] = 0.f;
+        }
+    }
+    if (!sums) return;
+    __syncthreads();
+    float* total = xs;                                            // [group][4 x 4 blocks]: 128 threads x 16 numbers
+    if (group < groups)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) total[threadIdx.x * 16 + i * 4 + j] = acc[i][j];
+    __syncthreads();
+    for (int e = threadIdx.x; e < (a.K + 1) * a.N; e += kThinRows) {
+        const int k = by_n.rows(e), n = e - k * a.N, b = n / 4 * k_blocks + k / 4, in = k % 4 * 4 + n % 4;
+        float s = 0.f;
+        for (int g = 0; g < groups; ++g) s += total[(g * blocks + b) * 16 + in];
+        if (a.partial) a.partial[(int64_t)blockIdx.x * (a.K + 1) * a.N + e] = s;
+        else if (k == a.K) {
+            if (a.db) static_cast<T*>(a.db)[n] = Pair<T>::round(s);
+        } else if (a.dw) static_cast<T*>(a.dw)[k * a.row_stride + n * a.col_stride] = Pair<T>::round(s);
+    }
+}
+
+// 32 elements of dw and db a CTA, 32 warps share the parts.
+template <class T> __global__ void __launch_bounds__(1024) k_thin_sums(const ThinGradArgs a, const int parts)
+{
+    __shared__ double sums[32][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e = blockIdx.x * 32 + lane, count = (a.K + 1) * a.N;
+    double s = 0.0;
+    if (e < count)
+#pragma unroll 8
+        for (int i = warp; i < parts; i += 32) s += __ldg(a.partial + (int64_t)i * count + e);
+    sums[warp][lane] = s;
+    __syncthreads();
+    if (warp || e >= count) return;
+    for (int v = 1; v < 32; ++v) s += sums[v][lane];
+    const int k = e / a.N, n = e % a.N;
+    if (k == a.K) {
+        if (a.db) static_cast<T*>(a.db)[n] = Pair<T>::round((float)s);
+    } else if (a.dw) {
+        static_cast<T*>(a.dw)[k * a.row_stride + n * a.col_stride] = Pair<T>::round((float)s);
+    }
+}
+
 // ---- rows of whole 16-byte pieces ------------------------------------------------------------------------------------------------
 // A 16-byte piece of the copy a thread, out of the five 32-bit words that its elements lie in (rows start on any even address; the first and last word may
 // hold a neighbour's element, which is not used), shifted by half a word where the row starts on one.
@@ -1228,7 +1435,79 @@ DwShape dw_shape(int64_t M, int32_t N, int32_t K)
 
 }  // namespace
 
-extern "C" int64_t dg_linear_few(int32_t, int32_t, int32_t type) { return type == DG_FLOAT32 ? 16 : 32; }
+namespace {
+
+bool thin(int32_t N, int32_t K) { return N <= kThinMost && K <= kThinMost; }
+unsigned thin_ctas(int64_t M, int each_sm) { return (unsigned)std::min<int64_t>((M + kThinRows - 1) / kThinRows, 148 * each_sm); }
+
+template <class T, class Use> int with_act(int act, Use use)
+{
+    switch (act) {
+        case DG_ACT_RELU: return use(T{}, std::integral_constant<int, DG_ACT_RELU>{});
+        case DG_ACT_GELU: return use(T{}, std::integral_constant<int, DG_ACT_GELU>{});
+        case DG_ACT_SILU: return use(T{}, std::integral_constant<int, DG_ACT_SILU>{});
+        default: return use(T{}, std::integral_constant<int, DG_ACT_NONE>{});
+    }
+}
+template <class Use> int with_type(int type, int act, Use use)
+{
+    return type == DG_FLOAT32 ? with_act<float>(act, use) : type == DG_BFLOAT16 ? with_act<__nv_bfloat16>(act, use) : with_act<__half>(act, use);
+}
+
+int linear_thin(const dg_linear_args* g, cudaStream_t stream)
+{
+    const FewArgs a{g->x, g->w, g->bias, g->residual, g->y, g->z, g->bits, g->ldx, g->ldw, g->ldr, g->ldy, g->ldz, g->ldbits, g->M, g->N, g->K, g->act, 0, 0};
+    const unsigned ctas = thin_ctas(g->M, 5);
+    return with_type(g->type, g->act, [&](auto value, auto act) {
+        using T = decltype(value);
+        constexpr int ACT = decltype(act)::value;
+        if (g->N <= 8) k_thin<T, ACT, 8><<<ctas, kThinRows, 0, stream>>>(a, g->out_in);
+        else if (g->N <= 16) k_thin<T, ACT, 16><<<ctas, kThinRows, 0, stream>>>(a, g->out_in);
+        else k_thin<T, ACT, 32><<<ctas, kThinRows, 0, stream>>>(a, g->out_in);
+        return (int)cudaGetLastError();
+    });
+}
+
+}  // namespace
+
+extern "C" int64_t dg_linear_few(int32_t N, int32_t K, int32_t type) { return thin(N, K) ? ((int64_t)1 << 31) - 1 : type == DG_FLOAT32 ? 16 : 32; }
+
+extern "C" int64_t dg_linear_grad_scratch(int64_t M, int32_t N, int32_t K)
+{
+    if (M < 1 || N < 1 || K < 1 || !thin(N, K)) return 0;
+    const int64_t ctas = thin_ctas(M, 4);
+    return ctas > 1 ? ctas * (K + 1) * N : 0;
+}
+
+extern "C" int dg_linear_grad(const dg_linear_grad_args* g, void* stream)
+{
+    if (!g || !g->dy || (!g->dx && !g->dw && !g->db)) return DG_ERR_NULL;
+    const int64_t M = g->M;
+    const int32_t N = g->N, K = g->K, act = g->act;
+    if (M < 1 || M >= (int64_t)1 << 31 || N < 1 || K < 1 || g->type < 0 || g->type > 2 || act < 0 || act > 3) return DG_ERR_DIMS;
+    if (!thin(N, K)) return DG_ERR_UNSUPPORTED;
+    const bool smooth = act == DG_ACT_GELU || act == DG_ACT_SILU;
+    if ((g->dx && !g->w) || (g->dw && !g->x) || (smooth && !g->z) || (act == DG_ACT_RELU && !g->bits)) return DG_ERR_NULL;
+    if (g->lddy < N || (g->dx && (g->lddx < K || g->ldw < (g->out_in ? K : N))) || (g->dw && g->ldx < K) || (smooth && g->ldz < N) ||
+        (act == DG_ACT_RELU && g->ldbits < 1))
+        return DG_ERR_DIMS;
+    const int item = g->type == DG_FLOAT32 ? 4 : 2;
+    for (const void* p : {g->x, g->w, g->dy, g->z, (const void*)g->dx, (const void*)g->dw, (const void*)g->db})
+        if (!aligned(p, item)) return DG_ERR_DIMS;
+    const int64_t floats = g->dw || g->db ? dg_linear_grad_scratch(M, N, K) : 0;
+    if (floats > 0 && !g->scratch) return DG_ERR_NULL;
+    if (g->scratch_floats < floats) return DG_ERR_SCRATCH;
+    ThinGradArgs a{g->x, g->w, g->dy, g->z, g->bits, g->dx, g->dw, g->db, floats > 0 ? g->scratch : nullptr, g->ldx, g->ldw, g->lddy, g->ldz, g->ldbits, g->lddx,
+                   g->row_stride, g->col_stride, M, N, K, g->out_in};
+    cudaStream_t s = (cudaStream_t)stream;
+    const unsigned ctas = thin_ctas(M, 4);
+    return with_type(g->type, act, [&](auto value, auto activation) {
+        using T = decltype(value);
+        k_thin_grad<T, decltype(activation)::value><<<ctas, kThinRows, 0, s>>>(a);
+        if (a.partial) k_thin_sums<T><<<(unsigned)(((K + 1) * N + 31) / 32), 1024, 0, s>>>(a, (int)ctas);
+        return (int)cudaGetLastError();
+    });
+}
 
 extern "C" int dg_linear(const dg_linear_args* g, void* stream)
 {
@@ -1239,6 +1518,7 @@ extern "C" int dg_linear(const dg_linear_args* g, void* stream)
     const int item = g->type == DG_FLOAT32 ? 4 : 2;
     if (!aligned(g->x, item) || !aligned(g->w, item) || !aligned(g->y, item) || !aligned(g->bias, item) || !aligned(g->residual, item) || !aligned(g->z, item)) return DG_ERR_DIMS;
     if (g->M == 0) return DG_OK;
+    if (thin(g->N, g->K)) return linear_thin(g, (cudaStream_t)stream);
     if (g->M <= dg_linear_few(g->N, g->K, g->type)) return linear_few(g, (cudaStream_t)stream);
     return g->type == DG_FLOAT32 ? dg_dense_linear(g, (cudaStream_t)stream) : linear16(g, (cudaStream_t)stream);
 }

@@ -489,6 +489,21 @@ struct LinearNode : public torch::autograd::Node {
         if (db) out[2] = at::empty({N}, x.options());
         const uint32_t* signs = bits.defined() ? reinterpret_cast<const uint32_t*>(bits.data_ptr<int32_t>()) : nullptr;
         const int64_t ldbits = bits.defined() ? bits.size(1) : 0;
+        if (N <= 32 && K <= 32) {                                 // narrow: all of them in one pass
+            const Tensor d = !dw ? Tensor() : out_in ? at::empty({N, K}, x.options()) : at::empty({K, N}, x.options());
+            const Tensor scratch = dw || db ? at::empty({dg_linear_grad_scratch(M, (int32_t)N, (int32_t)K)}, x.options().dtype(at::kFloat)) : Tensor();
+            dg_linear_grad_args a{};
+            a.x = x.data_ptr(), a.ldx = ld_of(x), a.w = w.data_ptr(), a.ldw = ld_of(w), a.dy = g.data_ptr(), a.lddy = ld_of(g), a.bits = signs, a.ldbits = ldbits;
+            if (z.defined()) a.z = z.data_ptr(), a.ldz = ld_of(z);
+            if (dx) out[0] = at::empty({M, K}, x.options()), a.dx = out[0].data_ptr(), a.lddx = K;
+            if (dw) a.dw = d.data_ptr(), a.row_stride = out_in ? 1 : N, a.col_stride = out_in ? K : 1, out[1] = out_in ? d.t() : d;
+            if (db) a.db = out[2].data_ptr();
+            if (scratch.defined()) a.scratch = scratch.data_ptr<float>(), a.scratch_floats = scratch.numel();
+            a.M = M, a.N = (int32_t)N, a.K = (int32_t)K, a.type = type, a.act = act, a.out_in = out_in;
+            if (dx || dw || db) check(dg_linear_grad(&a, stream));
+            g_launches += (dx || dw || db) + (a.scratch_floats > 0);
+            return out;
+        }
         auto weight_gradient = [&](const Tensor& from, int32_t with, const Tensor* dz) {
             const Tensor rows = to_rows(x, &launches), d = out_in ? at::empty({N, K}, x.options()) : at::empty({K, N}, x.options());
             const Tensor partial = at::empty({dg_linear_dw_scratch(M, (int32_t)N, (int32_t)K, type)}, x.options().dtype(at::kFloat));

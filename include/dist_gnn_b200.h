@@ -394,7 +394,7 @@ int dg_rows_cross_entropy_grad(const float* x, int64_t ld, int64_t n, int32_t C,
  *   z, ldz    NULL, or where z = x w + b goes, rounded to the type, which the gradient of GELU and SiLU reads
  *   bits      NULL, or with ReLU a bit an element, set where z > 0: ldbits words a row, an even number >= N / 32, 8-byte aligned
  *   head, tail, ldb   fp32 beyond dg_linear_few rows: w as [N x K], split (dg_dense_split_operands), on rows
- * dg_linear_few: how many rows, at most, a product of this shape and type takes with the kernels for few rows, which read operands of any stride and
+ * dg_linear_few: how many rows, at most, a product of this shape and type takes with the kernels for few rows or narrow layers, which read operands of any stride and
  * alignment.  Beyond it: 16-bit operands, fp32 x, z and y (16 bits) are on rows (DG_ERR_UNSUPPORTED otherwise); M < 2^31.
  * The gradient with respect to x is dg_linear with the same w and out_in inverted, N and K exchanged. */
 #define DG_FLOAT32 0
@@ -420,6 +420,25 @@ typedef struct dg_linear_args {
 } dg_linear_args;
 int64_t dg_linear_few(int32_t N, int32_t K, int32_t type);
 int dg_linear(const dg_linear_args* args, void* stream);
+/* All gradients of a layer of up to 32 inputs and 32 outputs (DG_ERR_UNSUPPORTED beyond) in one pass, those whose address is given: dx [M x K],
+ * dw[k * row_stride + n * col_stride], db [N].  z / bits as dg_linear left them.  Any strides and alignments.  scratch: dg_linear_grad_scratch floats (0 for
+ * few rows) where dw or db is asked for. */
+typedef struct dg_linear_grad_args {
+    const void* x;
+    const void* w;
+    const void* dy;
+    const void* z;
+    const uint32_t* bits;
+    void* dx;
+    void* dw;
+    void* db;
+    float* scratch;
+    int64_t ldx, ldw, lddy, ldz, ldbits, lddx, row_stride, col_stride, scratch_floats;
+    int64_t M;
+    int32_t N, K, type, act, out_in, pad;
+} dg_linear_grad_args;
+int64_t dg_linear_grad_scratch(int64_t M, int32_t N, int32_t K);
+int dg_linear_grad(const dg_linear_grad_args* args, void* stream);
 /* dz = dy * act'(z) and db = the column sums of dz.  dz == NULL: only db; db == NULL: only dz.  z / bits as dg_linear left them (neither: dz = dy).
  * scratch: dg_linear_dz_scratch(M, N) floats (0 for few rows) where db is asked for.  Any strides and alignments; the sums are taken in a fixed order. */
 int64_t dg_linear_dz_scratch(int64_t M, int32_t N);

@@ -14,7 +14,8 @@ pytestmark = pytest.mark.gpu
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
 HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
 SHAPES = [(1, 1, 1), (1, 256, 256), (2, 7, 5), (16, 1024, 1024), (17, 64, 64), (31, 100, 47), (32, 33, 130), (33, 8, 8), (100, 602, 41), (127, 256, 16), (128, 128, 48),
-          (129, 100, 256), (255, 48, 300), (256, 256, 256), (257, 300, 512), (1000, 16, 1024), (1500, 1024, 65), (20001, 256, 256), (40000, 64, 10), (38000, 72, 200)]
+          (129, 100, 256), (255, 48, 300), (256, 256, 256), (257, 300, 512), (1000, 16, 1024), (1500, 1024, 65), (20001, 256, 256), (40000, 64, 10), (38000, 72, 200),
+          (5, 32, 32), (127, 7, 11), (129, 1, 3), (3000, 32, 16), (9999, 31, 29), (150000, 7, 11), (4096, 4, 4)]
 
 
 def _acts64(name, z):
@@ -154,7 +155,7 @@ def test_only_what_is_asked_for():
     assert not spmm_cpp.linear(x, w).requires_grad
 
 
-@pytest.mark.parametrize('M,K,N', [(40, 24, 16), (700, 256, 264), (700, 300, 40), (20000, 64, 96), (900, 40, 41)])
+@pytest.mark.parametrize('M,K,N', [(40, 24, 16), (5000, 24, 16), (1000, 9, 32), (700, 256, 264), (700, 300, 40), (20000, 64, 96), (900, 40, 41)])
 @pytest.mark.parametrize('act', [None, 'relu', 'gelu', 'silu'])
 def test_every_subset_of_gradients_is_the_same(M, K, N, act):
     """Which gradients are asked for decides which kernels run (dz on the way to the weight gradient, by itself, kept or not): the numbers are those of all of them, but
@@ -231,7 +232,7 @@ def test_rows_behind_the_result_are_left_alone():
                    [(n, ctypes.c_int64) for n in ('ldx', 'ldw', 'ldb', 'ldr', 'ldy', 'ldz', 'ldbits', 'M')] + \
                    [(n, ctypes.c_int32) for n in ('N', 'K', 'type', 'act', 'out_in', 'pad')]
 
-    for M, K, N in ((5, 16, 40), (300, 64, 40), (129, 8, 200), (1, 8, 8), (511, 128, 264)):
+    for M, K, N in ((5, 16, 40), (300, 16, 24), (300, 64, 40), (129, 8, 200), (1, 8, 8), (511, 128, 264)):
         x, w = torch.ones(M, K, device='cuda', dtype=torch.bfloat16), torch.ones(K, N, device='cuda', dtype=torch.bfloat16)
         y = torch.full((M + 2, N + 8), 7.0, device='cuda', dtype=torch.bfloat16)
         z = y.clone()
