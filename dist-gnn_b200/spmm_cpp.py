@@ -931,14 +931,14 @@ class AdamW(torch.optim.Optimizer):
                     root=torch.zeros(p.shape, dtype=torch.float8_e4m3fn, **options), root_scale=torch.zeros(blocks, **options, dtype=torch.float32))
 
     def _make_table(self):
+        if not all(p.is_cuda for group in self.param_groups for p in group['params']):
+            raise RuntimeError('parameters must be CUDA tensors: this library has no CPU path')
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError('AdamW: take a step before capturing one, or every replay would start from the state that the capture made')
         rows, place = [], 0
         names = ('exp_avg', 'exp_avg_sq', None, None) if self.state_bits == 32 else ('exp_avg', 'root', 'exp_avg_scale', 'root_scale')
         for k, group in enumerate(self.param_groups):
             for p in group['params']:
-                if not p.is_cuda:
-                    raise RuntimeError('parameters must be CUDA tensors: this library has no CPU path')
                 if not self.state[p]:
                     self.state[p].update(self._new_state(p))
                 s = self.state[p]
