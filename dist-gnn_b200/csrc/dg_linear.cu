@@ -1228,16 +1228,13 @@ __global__ void __launch_bounds__(kThinRows) k_thin_grad(const ThinGradArgs a)
             else if (a.K <= 16) thin_product<16>(out, ds + threadIdx.x * kThinPitch, w, a.N);
             else thin_product<32>(out, ds + threadIdx.x * kThinPitch, w, a.N);
             __syncthreads();                                      // dz has been read
-            const int most = a.K <= 8 ? 8 : a.K <= 16 ? 16 : 32;
 #pragma unroll
             for (int k = 0; k < kThinMost; ++k)
-                if (k < most) ds[threadIdx.x * kThinPitch + k] = out[k];
+                if (k < a.K) ds[threadIdx.x * kThinPitch + k] = out[k];
             __syncthreads();
             thin_store(static_cast<T*>(a.dx) + m0 * a.lddx, a.lddx, rows, a.K, by_k, ds);
             __syncthreads();
-            // columns of dx beyond dz's are dz's padding, which the sums read as zero
-            if (a.K > a.N)
-                for (int c = a.N; c < kThinPitch; ++c) ds[threadIdx.x * kThinPitch + c] = 0.f;
+            for (int c = a.N; c < a.K; ++c) ds[threadIdx.x * kThinPitch + c] = 0.f;      // dz's padding, which products read as zero
         }
     }
     if (!sums) return;

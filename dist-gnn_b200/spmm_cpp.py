@@ -831,7 +831,9 @@ def linear(x, weight, bias=None, residual=None, activation=None):
     ReLU keeps a bit an element; GELU and SiLU keep x @ weight + bias in the type of x, and the gradient behind the activation is rounded to
     that type before it is multiplied.  Operands may have any strides: x, residual and gradients whose rows do not start on 16-byte boundaries are copied
     once, to padded rows, and the rows of the result and of x's gradient are padded to whole 16-byte pieces (a column slice of a wider buffer)
-    where M exceeds the few rows (fp32 16, else 32) that smaller kernels take."""
+    where M exceeds the few rows (fp32 16, else 32) that smaller kernels take, but for layers of up to 32 inputs and outputs.  What is not finite in a row
+    of x, of the residual or of a gradient stays in that row (and in the weight's and bias's gradients); an infinity among fp32 operands of the
+    three-pass product comes out as a NaN."""
     try:
         act = ACTIVATIONS[activation]
     except KeyError:

@@ -221,6 +221,21 @@ def test_what_is_not_finite_stays_in_its_row(dtype, M):
         assert bool(torch.isfinite(y[rest]).all())
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('M,K,N', [(100_000, 5, 6), (100_000, 30, 7), (100_000, 3, 32), (3000, 64, 40), (20, 64, 40)])
+def test_gradients_that_are_not_finite_stay_in_their_rows(dtype, M, K, N):
+    """A NaN or an infinity in a row of the incoming gradient reaches that row of x's gradient, and no other, whichever rows share its place in a tile."""
+    import spmm_cpp
+    for act in (None, 'relu', 'gelu'):
+        x = torch.ones(M, K, device='cuda', dtype=dtype, requires_grad=True)
+        w = torch.full((K, N), 0.125, device='cuda', dtype=dtype)
+        dy = torch.ones(M, N, device='cuda', dtype=dtype)
+        dy[3, N - 1], dy[7, 0], dy[M - 5, 0] = float('nan'), float('inf'), float('nan')
+        dx, = torch.autograd.grad(spmm_cpp.linear(x, w, activation=act), x, dy)
+        bad = sorted(set((~torch.isfinite(dx)).any(1).nonzero().view(-1).tolist()))
+        assert bad == sorted({3, 7, M - 5}), (act, bad[:10])
+
+
 def test_rows_behind_the_result_are_left_alone():
     """The padded rows' columns aside, nothing but the result is written: results of many shapes in one buffer's neighbourhood."""
     import ctypes
