@@ -26,7 +26,8 @@ using namespace dg;
 // A lane takes 8 neighbouring elements, a warp one block of 256; a thread works on two such pieces of a chunk at once.
 constexpr int kThreads = 256, kEach = 8, kHalf = kThreads * kEach, kChunk = 2 * kHalf;
 constexpr int kBlock = 256;
-constexpr int kNormCtas = 148 * 8, kStepCtas = 148 * 8;
+constexpr int kNormCtas = 148 * 8;
+template <bool SMALL> constexpr int kStepCtas = SMALL ? 3 : 2;      // of a step, that an SM holds
 constexpr float kLargest = 448.f;
 
 // Tensors of one launch.  Their table travels with the launch, so that a captured graph holds it and nothing has to be copied ahead; a launch takes 32 KB of
@@ -219,15 +220,18 @@ template <class Tab> __device__ __forceinline__ int find(const Tab& tab, int chu
 }
 
 template <class T, bool SMALL, int CAP>
-__global__ void __launch_bounds__(kThreads, SMALL ? 3 : 2) k_adamw(const __grid_constant__ Table<dg_adamw_tensor, CAP> tab, const Factors f, const float* __restrict__ clip,
+__global__ void __launch_bounds__(kThreads, kStepCtas<SMALL>) k_adamw(const __grid_constant__ Table<dg_adamw_tensor, CAP> tab, const Factors f, const float* __restrict__ clip,
                                                                   int* __restrict__ arrived)
 {
+    __shared__ int warps_done;
+    if (threadIdx.x == 0) warps_done = 0;                         // find() below is a barrier
     const int chunks = tab.first[tab.count];
     int at = -1;
     float rate = 0.f, correction = 0.f;
     uint32_t key = 0;
     const float coef = clip ? __ldg(clip) : 1.f;
-    int before = 0;
+    int before = -1;
+    int64_t step = 0;
     for (int chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
         int i = at;
         if (at < 0) i = find(tab, chunk);
@@ -275,15 +279,14 @@ __global__ void __launch_bounds__(kThreads, SMALL ? 3 : 2) k_adamw(const __grid_
             }
         }
         if (i != at) {                                            // 1 - b^t = -expm1(t log b)
-            const int64_t step = *t.step + 1;
+            step = *t.step + 1;
             rate = __fdividef(f.lr, -expm1f((float)((double)step * f.log_beta1)));
             correction = rsqrtf(-expm1f((float)((double)step * f.log_beta2)));
             key = key_of(f.seed, step);
             at = i;
         }
-        if (chunk + (int)gridDim.x >= chunks) {                   // no more steps to read here
-            __syncthreads();
-            if (threadIdx.x == 0) {
+        if (chunk + (int)gridDim.x >= chunks) {                   // no more steps to read here: the warp that is last to say so here says it for the CTA
+            if (threadIdx.x % 32 == 0 && atomicAdd(&warps_done, step < 0 ? 0 : 1) == kThreads / 32 - 1) {      // (its step has arrived)
                 __threadfence();
                 before = atomicAdd(arrived, 1);
             }
@@ -339,10 +342,10 @@ __global__ void __launch_bounds__(kThreads, SMALL ? 3 : 2) k_adamw(const __grid_
             }
         }
     }
-    // The CTA that was last to have read its steps counts them all up.
-    if (threadIdx.x >= 32 || __shfl_sync(0xffffffffu, before, 0) != (int)gridDim.x - 1) return;
-    for (int k = threadIdx.x; k < tab.count; k += 32) ++*tab.t[k].step;
-    if (threadIdx.x == 0) *arrived = 0;
+    // The warp that was last of all to have read its steps counts them all up.
+    if (__shfl_sync(0xffffffffu, before, 0) != (int)gridDim.x - 1) return;
+    for (int k = threadIdx.x % 32; k < tab.count; k += 32) ++*tab.t[k].step;
+    if (threadIdx.x % 32 == 0) *arrived = 0;
 }
 
 // Sum of squares in 64 bits, every CTA's in its own place; the CTA that comes last of the last launch adds them in order.
@@ -540,7 +543,8 @@ extern "C" int dg_adamw_step(const dg_adamw_tensor* host_tensors, int32_t count,
     const bool small = options->bits == 8;
     return each_table<dg_adamw_tensor>(host_tensors, count, options->bits, [&](auto& tab, auto value, bool) {
         using T = decltype(value);
-        const int grid = std::min(kStepCtas, (int)tab.first[tab.count]);
+        // Whole waves, each CTA with as many chunks: with 3 CTAs an SM 8 of them an SM leave a third of the last wave idle.
+        const int grid = std::min(148 * (small ? 3 * kStepCtas<true> : 4 * kStepCtas<false>), (int)tab.first[tab.count]);
         if (small) k_adamw<T, true><<<grid, kThreads, 0, (cudaStream_t)stream>>>(tab, f, clip, arrived);
         else k_adamw<T, false><<<grid, kThreads, 0, (cudaStream_t)stream>>>(tab, f, clip, arrived);
         return (int)cudaGetLastError();
