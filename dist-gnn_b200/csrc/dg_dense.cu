@@ -47,18 +47,15 @@ struct DenseArgs {
     float* z;                       // x w + b, or nullptr
     uint32_t* bits;                 // a bit an element where that is above zero, or nullptr
     int64_t ldz, ldbits;
-    int32_t panel;                  // columns of a CTA's panel, blockIdx.y's; 0: all of them
+    int32_t panel, panels;          // its columns in panels; one of all columns elsewhere
 
-    __device__ __forceinline__ int enter_panel()      // returns its first column
+    __device__ __forceinline__ void enter_panel(int n0)
     {
-        if (panel == 0) return 0;
-        const int n0 = blockIdx.y * panel;
         C += n0, N = min(panel, N - n0);
         if (mask) mask += n0;
         if (bias) bias += n0;
         if (z) z += n0;
         if (bits) bits += n0 / 32;
-        return n0;
     }
 };
 // What a kernel's epilogue does; from kLinear on: the linear layer's, with activation EPI - kLinear.
@@ -219,7 +216,8 @@ k_dense_nt(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
            const __grid_constant__ CUtensorMap tmBt, const DenseArgs args)
 {
     DenseArgs a = args;
-    const int n0 = EPI >= kLinear ? a.enter_panel() : 0;
+    const int n0 = EPI >= kLinear ? (int)blockIdx.y * args.panel : 0;
+    if (EPI >= kLinear) a.enter_panel(n0);
     extern __shared__ unsigned char smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t base = (raw + 1023u) & ~1023u;                 // swizzled tiles need 1024-byte alignment
@@ -355,7 +353,7 @@ k_dense_nt(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
 constexpr int PK = 16, kMaxPairStages = 10, kSplitWarps = 4, kEpilogueWarps = 8;
 constexpr int kThreadsPair = 32 * (2 + kSplitWarps + kEpilogueWarps);
 constexpr int kPieceBytes = 32 * 32 * 4;                          // staging of an epilogue warp: 32 rows x 32 columns
-constexpr int kPairBarBytes = 8 * (4 * kMaxPairStages + 5) + 8;
+constexpr int kPairBarBytes = 8 * (3 * kMaxPairStages + 5) + 8;
 
 __device__ __forceinline__ void umma_tf32_pair(uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate)
 {
@@ -372,7 +370,8 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                 const __grid_constant__ CUtensorMap tmBt, const DenseArgs args, const int n_tiles, const int stages)
 {
     DenseArgs a = args;
-    const int n0 = EPI >= kLinear ? a.enter_panel() : 0;
+    const int n0 = EPI >= kLinear ? (int)blockIdx.y * args.panel : 0;
+    if (EPI >= kLinear) a.enter_panel(n0);
     extern __shared__ unsigned char smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t base = (raw + 1023u) & ~1023u;
@@ -383,15 +382,12 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     const int staging = stages * stage_bytes;                     // the epilogue warps' row pieces
     const uint32_t bars = base + staging + kEpilogueWarps * kPieceBytes;
     const uint32_t full0 = bars, ready0 = bars + 8 * kMaxPairStages, empty0 = bars + 16 * kMaxPairStages;
-    const uint32_t acc_full0 = bars + 24 * kMaxPairStages, acc_empty0 = acc_full0 + 16, done = acc_empty0 + 16, heads0 = done + 8;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbase + staging + kEpilogueWarps * kPieceBytes + 32 * kMaxPairStages + 40);
+    const uint32_t acc_full0 = bars + 24 * kMaxPairStages, acc_empty0 = acc_full0 + 16, done = acc_empty0 + 16;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbase + staging + kEpilogueWarps * kPieceBytes + 24 * kMaxPairStages + 40);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     const int nhalves = (a.K + PK - 1) / PK;
-    // The linear layer keeps the tail passes' sums, a 2,048th of the head passes', from being rounded with them: in accumulators of their own (columns 128 / 384)
-    // up to 128 columns, beyond by going through K twice, tails first.
-    const bool apart = EPI >= kLinear && a.n_pad <= 128;
-    const int sweeps = EPI >= kLinear && !apart ? 2 : 1;
+    constexpr bool kApart = EPI >= kLinear;      // the tail passes' sums, a 2,048th of the head passes', are not rounded with them: accumulators of their own, columns 128 / 384
     constexpr int kTmemCols = 512;                                // two accumulators of up to 256 columns
 
     if (threadIdx.x == 0) {
@@ -399,7 +395,6 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             mbar_init(full0 + 8 * s, 1);
             mbar_init(ready0 + 8 * s, 2 * kSplitWarps);
             mbar_init(empty0 + 8 * s, 1);
-            mbar_init(heads0 + 8 * s, 1);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(acc_full0 + 8 * b, 1);
@@ -421,33 +416,20 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     if (warp == 0) {
         if (lane == 0) {                                          // TMA producer: one ring of stages across all tiles
             int it = 0, s = 0, phase = 1;
-            StagePhases tails_of, heads_of;
-            const uint32_t leader_heads0 = in_leader(heads0);
             for (int tile = pair; tile < n_tiles && ok; tile += pairs) {
                 const int row0 = (int)((int64_t)tile * (2 * BM) + rank * BM);      // rows beyond the matrix arrive as zeros
-                for (int i = 0; i < sweeps * nhalves; ++i, ++it) {
+                for (int i = 0; i < nhalves; ++i, ++it) {
                     if (it >= stages) ok = mbar_wait(empty0 + 8 * s, phase);
                     if (!ok) break;
                     const uint32_t st = base + s * stage_bytes;
-                    if (i < nhalves) {
-                        tails_of.take(s);
-                        mbar_expect_tx(full0 + 8 * s, a_bytes + 2 * b_bytes);
-                        tma_load_2d(st, &tmA, i * PK, row0, full0 + 8 * s);
-                        tma_load_2d(st + 2 * a_bytes, &tmBh, i * PK, n0 + rank * half_n, full0 + 8 * s);
-                        tma_load_2d(st + 2 * a_bytes + b_bytes, &tmBt, i * PK, n0 + rank * half_n, full0 + 8 * s);
-                    } else {                                      // heads alone need no split: the MMAs wait for the loads of both CTAs
-                        if (rank == 0) {
-                            heads_of.take(s);
-                            mbar_expect_tx(heads0 + 8 * s, 2 * (a_bytes + b_bytes));
-                        }
-                        tma_load_2d_pair(st, &tmA, (i - nhalves) * PK, row0, leader_heads0 + 8 * s);
-                        tma_load_2d_pair(st + 2 * a_bytes, &tmBh, (i - nhalves) * PK, n0 + rank * half_n, leader_heads0 + 8 * s);
-                    }
+                    mbar_expect_tx(full0 + 8 * s, a_bytes + 2 * b_bytes);
+                    tma_load_2d(st, &tmA, i * PK, row0, full0 + 8 * s);
+                    tma_load_2d(st + 2 * a_bytes, &tmBh, i * PK, n0 + rank * half_n, full0 + 8 * s);
+                    tma_load_2d(st + 2 * a_bytes + b_bytes, &tmBt, i * PK, n0 + rank * half_n, full0 + 8 * s);
                     if (++s == stages) s = 0, phase ^= 1;
                 }
             }
-            tails_of.await(full0);
-            heads_of.await(heads0);
+            await_loads(full0, it, stages);
         }
     } else if (warp == 1) {
         if (rank == 0) {                                          // MMA issuer: the warp waits and counts together, one lane issues
@@ -458,31 +440,42 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             const uint64_t desc0 = umma_desc_sw64(base);
             const uint32_t next_stage = (uint32_t)stage_bytes >> 4, tail = a_bytes >> 4, b_head = 2 * tail, b_tail = b_head + ((uint32_t)b_bytes >> 4);
             int s = 0, phase = 0, lt = 0;
-            [[maybe_unused]] StagePhases tails_of, heads_of;
+            [[maybe_unused]] bool early = false;
             for (int tile = pair; tile < n_tiles && ok; tile += pairs, ++lt) {
                 const int b = lt & 1, v = lt >> 1;
                 if (lt >= 2) ok = wait(acc_empty0 + 8 * b, (v - 1) & 1);     // both epilogues have drained this accumulator
                 const uint32_t acc = tmem + (uint32_t)(b * 256);
-                if constexpr (EPI >= kLinear) {
-                    for (int i = 0; i < sweeps * nhalves && ok; ++i) {
-                        ok = i < nhalves ? wait(ready0 + 8 * s, tails_of.take(s)) : wait(heads0 + 8 * s, heads_of.take(s));
+                // What goes around the MMAs costs the issuing warp 500 clocks a turn (200 of them the barrier's answer), six MMAs 90 to issue and 540 to run at 128 columns:
+                // hence two stages a turn, and the next two asked for before these are issued (382,902 rows 488 -> 8 265 us -> 199, 150,001 rows 256 -> 256 127 -> 110).
+                if constexpr (kApart) {
+                    for (int i = 0; i < nhalves && ok; i += 2) {
+                        const bool two = i + 1 < nhalves;
+                        const int s1 = s + 1 == stages ? 0 : s + 1, phase1 = phase ^ (s + 1 == stages);
+                        if (!early) ok = __any_sync(0xffffffffu, issuer && mbar_wait(ready0 + 8 * s, phase) && (!two || mbar_wait(ready0 + 8 * s1, phase1))) != 0;
                         if (!ok) break;
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        const int from = two ? s1 : s, next = from + 1 == stages ? 0 : from + 1, next1 = next + 1 == stages ? 0 : next + 1;
+                        const int phase2 = (two ? phase1 : phase) ^ (next == 0), phase3 = phase2 ^ (next1 == 0);
+                        bool there = false;
                         if (issuer) {
-                            const uint64_t d = desc0 + (uint32_t)s * next_stage;
+                            there = mbar_test(ready0 + 8 * next, phase2);
+                            const bool there1 = mbar_test(ready0 + 8 * next1, phase3);
+                            auto multiply = [&](int stage, uint32_t add) {
+                                const uint64_t d = desc0 + (uint32_t)stage * next_stage;
 #pragma unroll
-                            for (int k = 0; k < PK / 8; ++k) {
-                                const uint32_t tails = apart ? acc + 128 : acc, add = i > 0 || k > 0 ? 1u : 0u;
-                                if (i < nhalves) {
-                                    umma_tf32_pair(tails, d + tail + 2 * k, d + b_head + 2 * k, idesc, add);
-                                    umma_tf32_pair(tails, d + 2 * k, d + b_tail + 2 * k, idesc, 1u);
+                                for (int k = 0; k < PK / 8; ++k) {
+                                    umma_tf32_pair(acc + 128, d + tail + 2 * k, d + b_head + 2 * k, idesc, k > 0 ? 1u : add);
+                                    umma_tf32_pair(acc + 128, d + 2 * k, d + b_tail + 2 * k, idesc, 1u);
+                                    umma_tf32_pair(acc, d + 2 * k, d + b_head + 2 * k, idesc, k > 0 ? 1u : add);
                                 }
-                                if (apart || i >= nhalves) umma_tf32_pair(acc, d + 2 * k, d + b_head + 2 * k, idesc, add);
-                            }
-                            umma_commit_pair(empty0 + 8 * s);
+                                umma_commit_pair(empty0 + 8 * stage);
+                            };
+                            multiply(s, i > 0);
+                            if (two) multiply(s1, 1u);
+                            there = there && there1;
                         }
-                        __syncwarp();
-                        if (++s == stages) s = 0;
+                        early = __any_sync(0xffffffffu, there) != 0;
+                        s = next, phase = phase2;
                     }
                 } else
                 for (int i = 0; i < nhalves && ok; i += 2) {
@@ -531,11 +524,10 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     } else if (warp < 2 + kSplitWarps) {
         const int t = threadIdx.x - 64;                           // split the A half slab of every stage
         const uint32_t leader_ready0 = in_leader(ready0);
-        int s = 0;
-        StagePhases tails_of;
+        int s = 0, phase = 0;
         for (int tile = pair; tile < n_tiles && ok; tile += pairs) {
             for (int i = 0; i < nhalves; ++i) {
-                ok = __all_sync(0xffffffffu, mbar_wait(full0 + 8 * s, tails_of.take(s)));
+                ok = __all_sync(0xffffffffu, mbar_wait(full0 + 8 * s, phase));
                 if (!ok) break;
                 const float4* head = reinterpret_cast<const float4*>(gbase + (size_t)s * stage_bytes) + t;
                 float4* tail = reinterpret_cast<float4*>(gbase + (size_t)s * stage_bytes + a_bytes) + t;
@@ -552,9 +544,8 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive_cluster(leader_ready0 + 8 * s);
-                if (++s == stages) s = 0;
+                if (++s == stages) s = 0, phase ^= 1;
             }
-            if (sweeps == 2) s = (s + nhalves) % stages;          // the heads' stages
         }
     } else {
         const int q = warp & 3, first = (warp - 2 - kSplitWarps) / 4 * 32;      // a warp may only read its own quarter of the TMEM lanes
@@ -594,8 +585,7 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                     tmem_ld16(acc + (uint32_t)c0, r);
                     tmem_ld16(acc + (uint32_t)c0 + 16, r + 16);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                    if constexpr (EPI >= kLinear)
-                        if (apart) add_tails(r, acc + 128 + (uint32_t)c0, true);
+                    if constexpr (kApart) add_tails(r, acc + 128 + (uint32_t)c0, true);
                     if (c0 + step >= a.n_pad) {                   // the accumulator has been read: its next tile may start
                         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                         __syncwarp();
@@ -743,9 +733,8 @@ int make_map(CUtensorMap* map, const float* ptr, int64_t rows, int64_t cols, int
 // With more rows the pair wins (150,001 rows 100 -> 72 40.6 and 31.7, 256 -> 80 58 and 53, 256 -> 128 96 and 59) but for shallow products up to 80
 // columns with the mask, which wait for its rows and have more warps to do so as two CTAs (150,001 rows 64 -> 65 57 and 61, 100,000 rows
 // 64 -> 80 26.8 and 30.7).  Up to 64 columns the line was drawn when a pair issued its MMAs more slowly (256 -> 47 860 and 895; now 830 and 701).
-bool by_pairs(int64_t M, int n_pad, int K, bool masked, int sms, bool linear)
+bool by_pairs(int64_t tiles, int n_pad, int K, bool masked, int sms, bool linear)
 {
-    const int64_t tiles = (M + BM - 1) / BM;
     if (n_pad <= 64) return linear && tiles > 2 * sms;
     const bool half_slab = (K - 1) % BK < BK / 2;
     if (tiles <= sms) return n_pad > 128 || half_slab || K > (n_pad > 80 ? 96 : 128);
@@ -767,13 +756,15 @@ template <class Use> int by_epilogue(int epilogue, Use use)
 // One panel (up to 256 columns) of a product with the epilogue that `a` describes.
 int launch_nt(const float* A, int64_t lda, const float* Bt_head, const float* Bt_tail, int64_t ldb, DenseArgs a, int epilogue, cudaStream_t stream)
 {
-    const int cols = a.panel ? std::min(a.panel, a.N) : a.N, panels = a.panel ? (a.N + a.panel - 1) / a.panel : 1;
+    const bool linear = epilogue >= kLinear;
+    if (!linear) a.panel = a.N, a.panels = 1;
+    const int cols = a.panel;
     a.n_pad = (cols + 15) / 16 * 16;
     a.status = dg_status_word();
     if (!a.status) return DG_ERR_STATE;
     const int sms = sm_count();
     if (sms <= 0) return DG_ERR_STATE;
-    const bool pair = by_pairs(a.M, a.n_pad, a.K, a.mask != nullptr, sms, epilogue >= kLinear);
+    const bool pair = by_pairs((a.M + BM - 1) / BM * a.panels, a.n_pad, a.K, a.mask != nullptr, sms, linear);
     CUtensorMap tmA, tmBh, tmBt;
     int rc;
     if (!pair) {
@@ -784,7 +775,7 @@ int launch_nt(const float* A, int64_t lda, const float* Bt_head, const float* Bt
         auto run = [&](auto* kernel, std::atomic<bool>* granted) {
             const int code = allow_smem((const void*)kernel, granted);
             if (code) return code;
-            kernel<<<dim3((unsigned)((a.M + BM - 1) / BM), (unsigned)panels), kThreads, smem, stream>>>(tmA, tmBh, tmBt, a);
+            kernel<<<dim3((unsigned)((a.M + BM - 1) / BM), (unsigned)a.panels), kThreads, smem, stream>>>(tmA, tmBh, tmBt, a);
             return (int)cudaGetLastError();
         };
         return by_epilogue(epilogue, [&](auto e) {
@@ -799,10 +790,12 @@ int launch_nt(const float* A, int64_t lda, const float* Bt_head, const float* Bt
     const size_t stage = (size_t)PK * 4 * (2 * BM + a.n_pad), rest = kEpilogueWarps * kPieceBytes + kPairBarBytes + 1024;
     const int stages = (int)std::min<size_t>(kMaxPairStages, (227 * 1024 - rest) / stage);
     const int n_tiles = (int)((a.M + 2 * BM - 1) / (2 * BM));
+    // Up to eight panels (which leave at most four of 74 pairs without work) stream A side by side, so that DRAM gives it once; more of them go one after the other.
+    const int pairs = a.panels <= 8 ? sms / 2 / a.panels : sms / 2;
     auto run = [&](auto* kernel, std::atomic<bool>* granted) {
         const int code = allow_smem((const void*)kernel, granted);
         if (code) return code;
-        kernel<<<dim3(2u * (unsigned)std::min(n_tiles, sms / 2), (unsigned)panels), kThreadsPair, stages * stage + rest, stream>>>(tmA, tmBh, tmBt, a, n_tiles, stages);
+        kernel<<<dim3(2u * (unsigned)std::min(n_tiles, pairs), (unsigned)a.panels), kThreadsPair, stages * stage + rest, stream>>>(tmA, tmBh, tmBt, a, n_tiles, stages);
         return (int)cudaGetLastError();
     };
     return by_epilogue(epilogue, [&](auto e) {
@@ -894,11 +887,15 @@ int dg_dense_linear(const dg_linear_args* g, cudaStream_t stream)
     a.bias = static_cast<const float*>(g->bias);
     a.z = static_cast<float*>(g->z); a.ldz = g->ldz;
     a.bits = g->bits; a.ldbits = g->ldbits;
-    // Panels of 256 columns, one launch for all; of 128 or 64 while that leaves SMs without a tile of 128 rows (600 x 512 -> 512 57.6 us -> 22.9).
+    // Panels of up to 128 columns, whose tail passes have accumulators of their own, in one launch; of up to 64 while that leaves SMs without a tile of 128 rows
+    // (600 x 512 -> 512 57.6 us -> 22.9).
     const int sms = sm_count();
-    a.panel = 256;
-    while (a.panel > 64 && (a.M + BM - 1) / BM * ((a.N + a.panel - 1) / a.panel) < sms) a.panel /= 2;
-    if (a.N / a.panel >= 65535) return DG_ERR_UNSUPPORTED;
+    const int64_t tiles = (a.M + BM - 1) / BM;
+    const int width = tiles * ((a.N + 127) / 128) < sms ? 64 : 128;
+    a.panels = (a.N + width - 1) / width;
+    a.panel = ((a.N + a.panels - 1) / a.panels + 31) / 32 * 32;
+    a.panels = (a.N + a.panel - 1) / a.panel;
+    if (a.panels > 65535) return DG_ERR_UNSUPPORTED;
     return launch_nt(x, g->ldx, g->head, g->tail, g->ldb, a, kLinear + g->act, stream);
 }
 

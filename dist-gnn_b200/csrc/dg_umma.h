@@ -32,6 +32,16 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int lim
     }
     return false;
 }
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity)
+{
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
 // 16 consecutive accumulator columns of this warp's 32 tensor-memory lanes (no wait: pair with tcgen05.wait::ld).
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r)
 {
@@ -83,21 +93,6 @@ __device__ __forceinline__ void await_loads(uint32_t full0, int issued, int stag
 {
     for (int t = issued > stages ? issued - stages : 0; t < issued; ++t) mbar_wait(full0 + 8 * (t % stages), (t / stages) & 1);
 }
-// The stages of a ring whose loads a barrier of its own counts, however often: the phase of each stage's next use, in a bit.
-struct StagePhases {
-    uint32_t next = 0, used = 0;
-    __device__ __forceinline__ uint32_t take(int s)
-    {
-        const uint32_t phase = next >> s & 1;
-        next ^= 1u << s, used |= 1u << s;
-        return phase;
-    }
-    __device__ __forceinline__ void await(uint32_t bar0) const      // the last use of every stage
-    {
-        for (int s = 0; s < 32; ++s)
-            if (used >> s & 1) mbar_wait(bar0 + 8 * s, (next >> s & 1) ^ 1);
-    }
-};
 // All MMAs this thread has issued; `done` is a barrier of its own, with a count of 1.
 __device__ __forceinline__ void await_mmas(uint32_t done)
 {
