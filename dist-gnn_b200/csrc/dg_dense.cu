@@ -791,7 +791,7 @@ int launch_nt(const float* A, int64_t lda, const float* Bt_head, const float* Bt
     const int stages = (int)std::min<size_t>(kMaxPairStages, (227 * 1024 - rest) / stage);
     const int n_tiles = (int)((a.M + 2 * BM - 1) / (2 * BM));
     // Up to eight panels (which leave at most four of 74 pairs without work) stream A side by side, so that DRAM gives it once; more of them go one after the other.
-    const int pairs = a.panels <= 8 ? sms / 2 / a.panels : sms / 2;
+    const int pairs = std::max(1, a.panels <= 8 ? sms / 2 / a.panels : sms / 2);
     auto run = [&](auto* kernel, std::atomic<bool>* granted) {
         const int code = allow_smem((const void*)kernel, granted);
         if (code) return code;

@@ -521,8 +521,9 @@ extern "C" int dg_grad_norm(const dg_adamw_tensor* host_tensors, int32_t count, 
         return (int)cudaGetLastError();
     });
     if (rc || total > 0) return rc;
-    const float none[2] = {0.f, 1.f};
-    return (int)cudaMemcpyAsync(result, none, sizeof none, cudaMemcpyHostToDevice, (cudaStream_t)stream);
+    Table<Gradient, kFew> none{};                                 // no gradients: a sum of nothing
+    k_grad_norm<float><<<1, kThreads, 0, (cudaStream_t)stream>>>(none, partial, 1, max_norm, result, arrived);
+    return (int)cudaGetLastError();
 }
 
 extern "C" int dg_adamw_step(const dg_adamw_tensor* host_tensors, int32_t count, const dg_adamw_options* options, const float* clip, void* workspace,

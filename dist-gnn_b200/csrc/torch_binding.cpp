@@ -546,7 +546,7 @@ struct LinearNode : public torch::autograd::Node {
                 a.ldb = pad4(N), a.head = splits.data_ptr<float>(), a.tail = a.head + K * a.ldb;
             }
             check(dg_linear(&a, stream));
-            launches += item == 4 ? (K + 255) / 256 : 1;
+            ++launches;
         }
         if (dw && !together) weight_gradient(g, DG_ACT_NONE, nullptr);
         g_launches += launches;
@@ -628,7 +628,7 @@ Tensor linear(const Tensor& x, const Tensor& w, const std::optional<Tensor>& bia
         if (bits.defined()) a.bits = reinterpret_cast<uint32_t*>(bits.data_ptr<int32_t>()), a.ldbits = bits.size(1);
         a.M = M, a.N = (int32_t)N, a.K = (int32_t)K, a.type = type, a.act = (int32_t)act;
         if (M > 0) check(dg_linear(&a, stream));
-        g_launches += launches + (few || type != DG_FLOAT32 ? 1 : (N + 255) / 256);
+        g_launches += launches + (M > 0);
     }
     if (train) {
         auto node = std::shared_ptr<LinearNode>(new LinearNode(), torch::autograd::deleteNode);

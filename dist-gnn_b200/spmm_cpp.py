@@ -878,8 +878,8 @@ class AdamW(torch.optim.Optimizer):
     max_norm    gradients are scaled by min(1, max_norm / (norm + 1e-6)), norm being the 2-norm of all of them, inside the step (the .grad
                 tensors stay as they are); grad_norm is that norm, a 0-dim CUDA tensor.  None: no clipping.
 
-    Parameters are contiguous CUDA tensors of one device; those without a gradient are left as they are.  An infinity or a NaN
-    in a gradient makes its element's parameter and means non-finite, with 8 bits the means of its block of 256, and with max_norm all of them.
+    Parameters are contiguous CUDA tensors of one device; those without a gradient are left as they are.  An infinity, a NaN or a
+    number whose square leaves fp32's range (1.8e19, after clipping) in a gradient makes its element's parameter and means non-finite, with 8 bits the means of its block of 256, and with max_norm all of them.
     Steps are counted on the device (state 'step', int64), so a step can be captured into a CUDA graph and replayed; the hyperparameters
     are those of the capture.  Steps of one optimiser run one after the other: a graph of it and an eager step, or two graphs, not at once."""
 

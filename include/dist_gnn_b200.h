@@ -477,6 +477,7 @@ int dg_pad_rows16(const void* src, int64_t ld_src, int64_t n, int32_t cols, void
  *                above zero never becomes zero.
  *   step         steps taken so far, on the device; counted up by the call.  One for every tensor.
  *   place        number of the tensor's first element among the optimiser's (8 bits: a multiple of 256, no two tensors' ranges overlapping)
+ * A gradient that is not finite, or whose square is not (beyond 1.8e19, after the factor), makes its element's numbers NaN.
  * clip: NULL, or the second number that dg_grad_norm left (a factor for all gradients), on the device.
  * dg_grad_norm: result[0] = the 2-norm of all gradients (sums in 64 bits, in a fixed order), result[1] = min(1, max_norm / (norm + 1e-6)); only g, n
  * and type are read.

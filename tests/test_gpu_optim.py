@@ -347,3 +347,37 @@ def test_schedulers_hooks_and_foreign_state():
     assert int(other.state[heirs[0]]['step']) == 6
     for p, q in zip(heirs, twins):
         assert float((p - q).abs().max()) <= 2.0 ** -19 * 40 * HYPER['lr'] + 2.0 ** -22 * float(q.abs().max())
+
+
+def test_norm_of_no_gradients_in_a_replayed_graph():
+    """Entries without elements: the norm is 0 and the factor 1, in a graph too, which holds nothing of the call's own stack."""
+    import ctypes
+    import spmm_cpp
+    lib, empty = spmm_cpp.lib(), (ctypes.c_char * 512)()      # zeroed entries: n == 0
+    lib.dg_adamw_workspace.restype = ctypes.c_int64
+    size = lib.dg_adamw_workspace(empty, ctypes.c_int32(1))
+    workspace, result = torch.zeros(size, dtype=torch.uint8, device='cuda'), torch.empty(2, device='cuda')
+
+    def norm():
+        stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+        assert lib.dg_grad_norm(empty, ctypes.c_int32(1), ctypes.c_double(2.0), ctypes.c_void_p(result.data_ptr()), ctypes.c_void_p(workspace.data_ptr()),
+                                ctypes.c_int64(size), stream) == 0
+    norm()
+    assert result.tolist() == [0.0, 1.0]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm()
+    result.fill_(7.0)
+    graph.replay()
+    assert result.tolist() == [0.0, 1.0]
+
+
+@pytest.mark.parametrize('bits', [32, 8])
+def test_gradients_whose_square_overflows_show(bits):
+    import spmm_cpp
+    p = torch.nn.Parameter(torch.ones(600, device='cuda'))
+    p.grad = torch.zeros_like(p)
+    p.grad[300] = 1e20
+    opt = spmm_cpp.AdamW([p], state_bits=bits)
+    opt.step()
+    assert torch.isnan(p[300]) and torch.isfinite(p[:256]).all() and torch.isfinite(p[512:]).all()
