@@ -201,22 +201,28 @@ k_linear_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
             const uint64_t b0 = a.b_boxes ? umma_desc_mn16(base + kABytes, BK * 128) : umma_desc_sw128(base + kABytes);
             const uint32_t next_stage = (uint32_t)stage_bytes >> 4, b_step = a.b_boxes ? 16 * 128 >> 4 : 2;      // 16 K-columns
             int s = 0, phase = 0, lt = 0;
+            bool early = false;
             for (int tile = pair; tile < a.tiles && ok; tile += pairs, ++lt) {
                 const int b = lt & 1, v = lt >> 1;
                 if (lt >= 2) ok = wait(acc_empty0 + 8 * b, (v - 1) & 1);     // both epilogues have drained this accumulator
                 const uint32_t acc = tmem + (uint32_t)(b * 256);
                 for (int i = 0; i < slabs && ok; ++i) {
-                    ok = wait(full0 + 8 * s, phase);
+                    if (!early) ok = wait(full0 + 8 * s, phase);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const int next = s + 1 == a.stages ? 0 : s + 1, next_phase = phase ^ (next == 0);
+                    bool there = false;
                     if (issuer) {
+                        // The next stage is asked for first: its answer, 200 clocks of the 500 that a turn of this warp took beside the MMAs (720 of a slab of 256
+                        // columns), is on its way while these are issued (65,536 rows 1024 -> 1024 126 us -> 100, with SiLU, residual and z 147 -> 137).
+                        there = mbar_test(full0 + 8 * next, next_phase);
                         const uint32_t at = (uint32_t)s * next_stage;
 #pragma unroll
                         for (int k = 0; k < BK / 16; ++k) umma_f16_pair(acc, a0 + at + 2 * k, b0 + at + b_step * k, idesc, i > 0 || k > 0 ? 1u : 0u);
                         umma_commit_pair(empty0 + 8 * s);
                     }
-                    __syncwarp();
-                    if (++s == a.stages) s = 0, phase ^= 1;
+                    early = __any_sync(0xffffffffu, there) != 0;
+                    s = next, phase = next_phase;
                 }
                 if (ok && issuer) umma_commit_pair(acc_full0 + 8 * b);
                 __syncwarp();
