@@ -335,7 +335,7 @@ k_dense_nt(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUte
 // rows of the result.  Two accumulators (columns 0 / 256) and separate warps for the operand split and the epilogue, so that tile t is
 // read out and stored while tile t+1 is loaded, split and multiplied.
 // Warps: 0 TMA, 1 MMA issue (even CTA) + tensor-memory allocation, 2-5 split A, 6-13 epilogue (lane quarter w % 4; two warps a quarter take
-// its 32-column pieces in turn).
+// its 32-column pieces in turn).  The linear layer's panels are of up to 128 columns, blockIdx.y's, with the tail passes at columns 128 / 384.
 // The ring holds half slabs of 16 columns (64-byte rows, 64B swizzle), as many as fit (6 at 256 columns, 10 at most).
 // Barriers: full (own CTA, TMA), ready (even CTA: the split warps of both), empty and acc_full (both CTAs, by commit), acc_empty (even CTA:
 // the epilogue warps of both).
