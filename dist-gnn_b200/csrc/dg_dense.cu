@@ -64,7 +64,7 @@ constexpr int kPlain = 0, kMasked = 1, kLinear = 2;
 // A lane's 32 columns of its row: a bit each where x w + b is above zero.
 __device__ __forceinline__ void keep_signs(const DenseArgs& a, const uint32_t* r, int c0, int64_t row)
 {
-    if (row >= a.M) return;
+    if (row >= a.M || c0 >= a.N) return;                          // a panel's last pieces may lie beyond the result: those words are the next row's
     uint32_t word = 0;
 #pragma unroll
     for (int j = 0; j < 32; ++j) {

@@ -355,3 +355,20 @@ def test_refusals():
     y.sum().backward()
     with pytest.raises(RuntimeError, match='second time'):
         y.sum().backward()
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('M,K,N', [(4804, 34, 539), (3000, 40, 298), (20000, 33, 130), (700, 64, 1100), (300, 48, 65), (40000, 36, 257), (5000, 40, 97)])
+def test_relu_gradients_of_wide_layers_are_exact(M, K, N, dtype):
+    """Results in several panels, the last one with pieces beyond the matrix: what ReLU keeps is every row's own.  Small whole numbers: sums stay below
+    2^24, so that results are the exact ones, rounded once."""
+    import spmm_cpp
+    g = torch.Generator(device='cuda').manual_seed(M + N)
+    x, w, b, dy = (torch.randint(-2, 3, size, device='cuda', generator=g).to(dtype) for size in ((M, K), (K, N), (N,), (M, N)))
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    y = spmm_cpp.linear(x, w, b, activation='relu')
+    grads = torch.autograd.grad(y, leaves, dy)
+    z = x.detach().double() @ w.detach().double() + b.detach().double()
+    dz = dy.double() * (z > 0)
+    for got, want in zip((y, *grads), (z.clamp(min=0), dz @ w.detach().double().t(), x.detach().double().t() @ dz, dz.sum(0))):
+        assert torch.equal(got.detach(), want.float().to(dtype))
