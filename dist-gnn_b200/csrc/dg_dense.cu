@@ -1389,7 +1389,9 @@ int dg_dense_linear_dw(const dg_linear_dw_args* g, cudaStream_t stream)
     float* dw = static_cast<float*>(g->dw);
     const int sms = sm_count();
     if (sms <= 0) return DG_ERR_STATE;
-    if (g->col_stride == 1) return dense_tn_run(x, g->ldx, dz, g->lddy, dw, g->row_stride, g->M, g->K, g->N, g->scratch, g->scratch_floats, sms, true, stream);
+    // a matrix of one row has no use for its row stride
+    if (g->col_stride == 1 && (g->K == 1 || g->row_stride >= g->N))
+        return dense_tn_run(x, g->ldx, dz, g->lddy, dw, std::max<int64_t>(g->row_stride, g->N), g->M, g->K, g->N, g->scratch, g->scratch_floats, sms, true, stream);
     if (g->row_stride == 1) return dense_tn_run(dz, g->lddy, x, g->ldx, dw, g->col_stride, g->M, g->N, g->K, g->scratch, g->scratch_floats, sms, true, stream);
     return DG_ERR_UNSUPPORTED;
 }

@@ -372,3 +372,19 @@ def test_relu_gradients_of_wide_layers_are_exact(M, K, N, dtype):
     dz = dy.double() * (z > 0)
     for got, want in zip((y, *grads), (z.clamp(min=0), dz @ w.detach().double().t(), x.detach().double().t() @ dz, dz.sum(0))):
         assert torch.equal(got.detach(), want.float().to(dtype))
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('M,K,N', [(459, 1, 46), (9, 1, 78), (1, 1, 215), (684, 1, 327), (459, 46, 1), (3, 272, 1), (20, 33, 1)])
+def test_one_input_or_output_with_strides(M, K, N, dtype):
+    """A weight of one row or column, whose stride along it says nothing: every second element of a wider one, and its transpose.  Whole numbers, as above."""
+    import spmm_cpp
+    g = torch.Generator(device='cuda').manual_seed(M + N)
+    x, dy = (torch.randint(-2, 3, size, device='cuda', generator=g).to(dtype) for size in ((M, K), (M, N)))
+    wide = torch.randint(-2, 3, (2 * K, 2 * N), device='cuda', generator=g).to(dtype)
+    for w in (wide[:K, ::2], wide[::2, :N], wide[:K, :N].t().contiguous().t(), wide[:K, :N].contiguous()):
+        leaves = [x.detach().requires_grad_(), w.detach().requires_grad_()]
+        y = spmm_cpp.linear(*leaves)
+        grads = torch.autograd.grad(y, leaves, dy)
+        for got, want in zip((y, *grads), (x.double() @ w.double(), dy.double() @ w.double().t(), x.double().t() @ dy.double())):
+            assert torch.equal(got.detach(), want.float().to(dtype))
