@@ -23,6 +23,18 @@ __device__ __forceinline__ float sigmoid(float z)
 {
     return reciprocal(1.f + exp2_approx(z * -1.44269504f));
 }
+// z within [low, high]; a NaN stays one.  SiLU multiplies its sigmoid by a z so bounded: beyond, an s that is a rounding away from 0 or 1 would count |z| times.
+__device__ __forceinline__ float bounded(float z, float low, float high)
+{
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(z) : "f"(low));
+    asm("min.NaN.f32 %0, %0, %1;" : "+f"(z) : "f"(high));
+    return z;
+}
+__device__ __forceinline__ float at_least(float z, float low)
+{
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(z) : "f"(low));
+    return z;
+}
 
 // gelu(z) = z Phi(z) with the distribution function of the normal distribution, silu(z) = z / (1 + exp(-z)).
 template <int ACT> __device__ __forceinline__ float act_value(float z)
@@ -32,7 +44,7 @@ template <int ACT> __device__ __forceinline__ float act_value(float z)
         float e;
         return z * normal_cdf(z, &e);
     }
-    if (ACT == DG_ACT_SILU) return z * sigmoid(z);
+    if (ACT == DG_ACT_SILU) return at_least(z, -104.f) * sigmoid(z);      // -infinity gives zero, as do numbers from -104 on
     return z;
 }
 // d act / dz:  Phi + z phi,  s (1 + z (1 - s)).
@@ -46,7 +58,7 @@ template <int ACT> __device__ __forceinline__ float act_slope(float z)
     }
     if (ACT == DG_ACT_SILU) {
         const float s = sigmoid(z);
-        return s * fmaf(z, 1.f - s, 1.f);
+        return s * fmaf(bounded(z, -104.f, 60.f), 1.f - s, 1.f);
     }
     return 1.f;
 }
@@ -71,6 +83,7 @@ template <bool SLOPE> __device__ __forceinline__ float_pair normal_tail(float_pa
     p = fma2(a, p, both(-0.49999825f));
     return mul2(p, e);
 }
+// SiLU's sigmoid stands at 2^-60 below z = -41.6 and z at -60, which leaves 6e-17 of the true value.
 __device__ __forceinline__ float_pair sigmoid2(float_pair z)
 {
     const float2 s = halves(mul2(z, both(-1.44269504f)));
@@ -86,7 +99,7 @@ template <int ACT> __device__ __forceinline__ float_pair act_value2(float_pair z
         const float_pair a = pair_of(fminf(fabsf(f.x), 16.f), fminf(fabsf(f.y), 16.f));
         return fma2(a, normal_tail<false>(z, a), pair_of(fmaxf(f.x, 0.f), fmaxf(f.y, 0.f)));
     }
-    if (ACT == DG_ACT_SILU) return mul2(z, sigmoid2(z));
+    if (ACT == DG_ACT_SILU) return mul2(pair_of(at_least(f.x, -60.f), at_least(f.y, -60.f)), sigmoid2(z));
     return z;
 }
 template <int ACT> __device__ __forceinline__ float_pair act_slope2(float_pair z)
@@ -98,8 +111,9 @@ template <int ACT> __device__ __forceinline__ float_pair act_slope2(float_pair z
         return pair_of(f.x > 0.f ? w.x + 1.f : -w.x, f.y > 0.f ? w.y + 1.f : -w.y);
     }
     if (ACT == DG_ACT_SILU) {
-        const float_pair s = sigmoid2(z), rest = fma2(s, both(-1.f), both(1.f));
-        return mul2(s, fma2(z, rest, both(1.f)));
+        const float2 f = halves(z);
+        const float_pair s = sigmoid2(z), rest = fma2(s, both(-1.f), both(1.f)), near = pair_of(bounded(f.x, -60.f, 60.f), bounded(f.y, -60.f, 60.f));
+        return mul2(s, fma2(near, rest, both(1.f)));
     }
     return both(1.f);
 }
