@@ -63,7 +63,7 @@ def _within(got, want, bound, z, what):
 
 
 @pytest.mark.parametrize('dtype', TYPES)
-@pytest.mark.parametrize('act', ['silu'])
+@pytest.mark.parametrize('act', ['gelu', 'silu'])
 @pytest.mark.parametrize('form', ['many', 'panels', 'few', 'narrow'])
 def test_values_over_the_whole_range(form, act, dtype):
     import spmm_cpp
@@ -83,7 +83,7 @@ def test_values_over_the_whole_range(form, act, dtype):
 
 
 @pytest.mark.parametrize('dtype', TYPES)
-@pytest.mark.parametrize('act', ['silu'])
+@pytest.mark.parametrize('act', ['gelu', 'silu'])
 @pytest.mark.parametrize('form', ['back', 'alone', 'few', 'narrow'])
 def test_slopes_over_the_whole_range(form, act, dtype):
     """One column (row) of the incoming gradient is one, the others are zero: x's (w's) gradient is the slope."""
@@ -106,7 +106,7 @@ def test_slopes_over_the_whole_range(form, act, dtype):
 
 
 @pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize('act', ['silu'])
+@pytest.mark.parametrize('act', ['gelu', 'silu'])
 def test_what_is_not_a_number_stays_one(act, dtype):
     """In every form, value and slope, whatever stands beside it."""
     import spmm_cpp
