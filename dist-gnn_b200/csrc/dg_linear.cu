@@ -8,6 +8,7 @@
 // k_few_*: products of few rows, bound by latency.  k_thin, k_thin_grad: narrow layers.
 // The fp32 product is dg_dense.cu's.
 #include <algorithm>
+#include <type_traits>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include "dg_act.h"
@@ -360,12 +361,15 @@ k_linear_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
 // A CTA owns a panel of up to 256 x 256 of dw and a range of rows.  Both operands come in boxes of 64 columns x 64 rows (MN-major); x's columns lie along
 // the MMA's 128 rows, so a panel wider than 128 takes two accumulators.  The range's partial goes to scratch, four columns of dz and all of x's side by
 // side; a second kernel adds the ranges in order.
-// One range (fewer than 512 rows) is written as it is.
+// One range (fewer than 512 rows, or more than 74 panels) of one chain is written as it is.
 // What bounds it: the tensor cores for wide layers (65,536 rows 1024 x 1024 93 us, 1,480 TFLOP/s), HBM for the others (232,965 rows 602 x 41 65 us, 4.6 TB/s).
-// A chain of accumulations, which the tensor cores truncate, is as long as the range: 16 rows each, some 1,000 at 2.4 M rows, 3e-5 of the sum at most where
-// bf16 rounds by 4e-3 and fp16 by 5e-4; so no flush in between, which fp32 needs.
+// The tensor cores truncate when they add into an accumulator: where all terms are of one sign a chain of n accumulations, 16 rows each, is some n 2^-23 too small.  So a
+// chain ends after chain_rows, and the CTA adds the accumulators to its partial result: fp16, which rounds by 2^-11, after 512 accumulations (6e-5), bf16, by 2^-8, after
+// 2,048.  With ranges of one chain each, 300,000 x 264, 2304 fp16 were 2.3e-4 too small and 131,072 x 2304, 2304, whose 81 panels leave one range, 7.8e-4.
 constexpr int kDwRows = 64, kDwBox = kDwRows * 128, kDwThreads = 32 * 6, kDwMaxStages = 8;
-constexpr int kDwBarBytes = 8 * (2 * kDwMaxStages + 2) + 8;
+constexpr int kDwBarBytes = 8 * (2 * kDwMaxStages + 3) + 8;
+constexpr int chain_rows(bool bf16) { return bf16 ? 32768 : 8192; }
+template <class T> constexpr int kChainRows = chain_rows(std::is_same<T, __nv_bfloat16>::value);
 
 struct LinearDwArgs {
     float4* partial;                              // [range][panel][q_store / 4][p_store]; null: the one range's sums are the result
@@ -399,8 +403,9 @@ struct DwPart {
     }
 };
 
-// The accumulators of a CTA, by four warps: to its place among the partial results, or where it has the only range rounded to dw.
-template <class T> __device__ __forceinline__ void flush_dw(const LinearDwArgs& a, const DwPart& part, uint32_t tmem, int warp, int lane)
+// The accumulators of a CTA, by four warps: to its place among the partial results, added to what its earlier chains left there, or where it has the only chain
+// rounded to dw.
+template <class T> __device__ __forceinline__ void flush_dw(const LinearDwArgs& a, const DwPart& part, uint32_t tmem, int warp, int lane, bool add)
 {
     const int q = warp & 3;                                       // a warp may only read its own quarter of the TMEM lanes
     const bool whole = a.col_stride == 1 && a.row_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(a.dw) & 15) == 0;
@@ -414,9 +419,15 @@ template <class T> __device__ __forceinline__ void flush_dw(const LinearDwArgs& 
             if (a.partial) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (row < a.p_store)
-                        __stcg(to_part + (int64_t)(c0 / 4 + j) * a.p_store, make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]), __uint_as_float(r[4 * j + 2]),
-                                                                                          __uint_as_float(r[4 * j + 3])));
+                    if (row < a.p_store) {
+                        float4* const to = to_part + (int64_t)(c0 / 4 + j) * a.p_store;
+                        float4 v = make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]), __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3]));
+                        if (add) {
+                            const float4 u = __ldcg(to);
+                            v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+                        }
+                        __stcg(to, v);
+                    }
                 continue;
             }
             if (p >= a.p_cols) continue;
@@ -445,11 +456,11 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_linear_dw(const __grid_consta
     unsigned char* gbase = smem_raw + (base - raw);
     const int stage_bytes = (a.p_boxes + a.q_boxes) * kDwBox;
     const uint32_t bars = base + a.stages * stage_bytes;
-    const uint32_t full0 = bars, empty0 = bars + 8 * kDwMaxStages, acc_full = bars + 16 * kDwMaxStages, done = acc_full + 8;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbase + a.stages * stage_bytes + 8 * (2 * kDwMaxStages + 2));
+    const uint32_t full0 = bars, empty0 = bars + 8 * kDwMaxStages, acc_full = bars + 16 * kDwMaxStages, acc_empty = acc_full + 8, done = acc_full + 16;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbase + a.stages * stage_bytes + 8 * (2 * kDwMaxStages + 3));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const DwPart part(a, kDwRows);
-    constexpr int kTmemCols = 512;
+    constexpr int kTmemCols = 512, kChain = kChainRows<T> / kDwRows;      // slabs of a chain
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < a.stages; ++s) {
@@ -457,6 +468,7 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_linear_dw(const __grid_consta
             mbar_init(empty0 + 8 * s, 1);
         }
         mbar_init(acc_full, 1);
+        mbar_init(acc_empty, 4);
         mbar_init(done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -489,33 +501,38 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_linear_dw(const __grid_consta
         const bool issuer = elect_one();
         auto wait = [&](uint32_t bar, int parity) { return __any_sync(0xffffffffu, issuer && mbar_wait(bar, parity)) != 0; };
         const uint32_t idesc = umma_idesc_f16(Pair<T>::kFormat, 128, part.q_pad, true, true);
-        int s = 0, phase = 0;
+        int s = 0, phase = 0, in_chain = 0, chain = 0;
         for (int i = 0; i < part.slabs && ok; ++i) {
-            ok = wait(full0 + 8 * s, phase);
+            if (in_chain == kChain) ok = wait(acc_empty, chain++ & 1), in_chain = 0;      // the chain before has left the accumulators
+            ok = ok && wait(full0 + 8 * s, phase);
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (issuer) {
-                const uint32_t st = base + s * stage_bytes;
+                const uint32_t st = base + s * stage_bytes, more = in_chain > 0;
                 const uint64_t p = umma_desc_mn16(st, kDwBox), q = umma_desc_mn16(st + a.p_boxes * kDwBox, kDwBox);
                 for (int h = 0; h < part.halves; ++h)
 #pragma unroll
                     for (int k = 0; k < kDwRows / 16; ++k)        // 16 rows: 2048 bytes
-                        umma_f16(tmem + (uint32_t)(h * 256), p + (uint32_t)((h * 2 * kDwBox + k * 2048) >> 4), q + (uint32_t)(k * 2048 >> 4), idesc,
-                                 i > 0 || k > 0 ? 1u : 0u);
+                        umma_f16(tmem + (uint32_t)(h * 256), p + (uint32_t)((h * 2 * kDwBox + k * 2048) >> 4), q + (uint32_t)(k * 2048 >> 4), idesc, k > 0 ? 1u : more);
                 umma_commit(empty0 + 8 * s);
+                if (in_chain == kChain - 1 || i == part.slabs - 1) umma_commit(acc_full);
             }
+            ++in_chain;
             __syncwarp();
             if (++s == a.stages) s = 0, phase ^= 1;
         }
-        if (ok && issuer) umma_commit(acc_full);
-        __syncwarp();
         if (issuer) await_mmas(done);
         __syncwarp();
     } else {
-        ok = __all_sync(0xffffffffu, mbar_wait(acc_full, 0));     // tcgen05.ld is warp-collective
-        if (ok) {
+        const int chains = (part.slabs + kChain - 1) / kChain;
+        for (int chain = 0; chain < chains; ++chain) {
+            ok = __all_sync(0xffffffffu, mbar_wait(acc_full, chain & 1));      // tcgen05.ld is warp-collective
+            if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            flush_dw<T>(a, part, tmem, warp, lane);
+            flush_dw<T>(a, part, tmem, warp, lane, chain > 0);
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acc_empty);
         }
     }
     if (!ok) atomicExch(a.status, 1);
@@ -530,7 +547,7 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_linear_dw(const __grid_consta
 // gradient needs, take one pass over x, dy and z; dz by a pass of its own reads and writes as much again (2,449,029 x 256, 256 bf16: 617 + 384 us, 725 this way).
 // Warps: 0 TMA, 1 MMA issue + tensor-memory allocation, 2-9 dz (a row's 16-byte piece a thread and box of 32 rows x 64 columns), of which 2-5 flush, 10 stores dz.
 constexpr int kBackRows = 32, kBackBox = kBackRows * 128, kBackMakers = 8, kBackThreads = 32 * (3 + kBackMakers), kBackMaxStages = 8;
-constexpr int kBackBarBytes = 8 * (4 * kBackMaxStages + 2) + 8, kBackSumPitch = 9, kBackSumBytes = 32 * kBackMakers * kBackSumPitch * 4;
+constexpr int kBackBarBytes = 8 * (4 * kBackMaxStages + 3) + 8, kBackSumPitch = 9, kBackSumBytes = 32 * kBackMakers * kBackSumPitch * 4;
 
 template <class T, int ACT>
 __global__ void __launch_bounds__(kBackThreads, 1)
@@ -546,11 +563,11 @@ k_linear_back(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ C
     float* sums = reinterpret_cast<float*>(gbase + a.stages * stage_bytes);
     const uint32_t bars = base + a.stages * stage_bytes + kBackSumBytes;
     const uint32_t full0 = bars, ready0 = bars + 8 * kBackMaxStages, empty0 = bars + 16 * kBackMaxStages, stored0 = bars + 24 * kBackMaxStages;
-    const uint32_t acc_full = bars + 32 * kBackMaxStages, done = acc_full + 8;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbase + a.stages * stage_bytes + kBackSumBytes + 8 * (4 * kBackMaxStages + 2));
+    const uint32_t acc_full = bars + 32 * kBackMaxStages, acc_empty = acc_full + 8, done = acc_full + 16;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbase + a.stages * stage_bytes + kBackSumBytes + 8 * (4 * kBackMaxStages + 3));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const DwPart part(a, kBackRows);
-    constexpr int kTmemCols = 512;
+    constexpr int kTmemCols = 512, kChain = kChainRows<T> / kBackRows;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < a.stages; ++s) {
@@ -560,6 +577,7 @@ k_linear_back(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ C
             mbar_init(stored0 + 8 * s, 1);
         }
         mbar_init(acc_full, 1);
+        mbar_init(acc_empty, 4);
         mbar_init(done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -595,26 +613,26 @@ k_linear_back(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ C
         const bool issuer = elect_one();
         auto wait = [&](uint32_t bar, int parity) { return __any_sync(0xffffffffu, issuer && mbar_wait(bar, parity)) != 0; };
         const uint32_t idesc = umma_idesc_f16(Pair<T>::kFormat, 128, part.q_pad, true, true);
-        int s = 0, phase = 0;
+        int s = 0, phase = 0, in_chain = 0, chain = 0;
         for (int i = 0; i < part.slabs && ok; ++i) {
-            ok = wait(ready0 + 8 * s, phase);
+            if (in_chain == kChain) ok = wait(acc_empty, chain++ & 1), in_chain = 0;
+            ok = ok && wait(ready0 + 8 * s, phase);
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (issuer) {
-                const uint32_t st = base + s * stage_bytes;
+                const uint32_t st = base + s * stage_bytes, more = in_chain > 0;
                 const uint64_t p = umma_desc_mn16(st, kBackBox), q = umma_desc_mn16(st + q_at, kBackBox);
                 for (int h = 0; h < part.halves; ++h)
 #pragma unroll
                     for (int k = 0; k < kBackRows / 16; ++k)      // 16 rows: 2048 bytes
-                        umma_f16(tmem + (uint32_t)(h * 256), p + (uint32_t)((h * 2 * kBackBox + k * 2048) >> 4), q + (uint32_t)(k * 2048 >> 4), idesc,
-                                 i > 0 || k > 0 ? 1u : 0u);
+                        umma_f16(tmem + (uint32_t)(h * 256), p + (uint32_t)((h * 2 * kBackBox + k * 2048) >> 4), q + (uint32_t)(k * 2048 >> 4), idesc, k > 0 ? 1u : more);
                 umma_commit(empty0 + 8 * s);
+                if (in_chain == kChain - 1 || i == part.slabs - 1) umma_commit(acc_full);
             }
+            ++in_chain;
             __syncwarp();
             if (++s == a.stages) s = 0, phase ^= 1;
         }
-        if (ok && issuer) umma_commit(acc_full);
-        __syncwarp();
         if (issuer) await_mmas(done);
         __syncwarp();
     } else if (warp < 2 + kBackMakers) {
@@ -624,6 +642,16 @@ k_linear_back(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ C
         for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e) sum[j][e] = both(0.f);
+        // The accumulators at a chain's end, by the first four of these warps; the others are held up by the barriers of the stages that follow.
+        auto flush = [&](int chain) {
+            ok = __all_sync(0xffffffffu, mbar_wait(acc_full, chain & 1));      // tcgen05.ld is warp-collective
+            if (!ok) return;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            flush_dw<T>(a, part, tmem, warp, lane, chain > 0);
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acc_empty);
+        };
         int s = 0, phase = 0;
         for (int i = 0; i < part.slabs; ++i) {
             uint32_t above[4] = {0u, 0u, 0u, 0u};
@@ -663,6 +691,10 @@ k_linear_back(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ C
             __syncwarp();
             if (lane == 0) mbar_arrive(ready0 + 8 * s);
             if (++s == a.stages) s = 0, phase ^= 1;
+            if (warp < 6 && i % kChain == kChain - 1 && i + 1 < part.slabs) {
+                flush(i / kChain);
+                if (!ok) break;
+            }
         }
         if (a.db) {                                               // box by box: the 32 rows of a column, in order
 #pragma unroll
@@ -685,13 +717,7 @@ k_linear_back(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ C
                 asm volatile("bar.sync 1, %0;" ::"n"(32 * kBackMakers) : "memory");
             }
         }
-        if (warp < 6) {
-            ok = ok && __all_sync(0xffffffffu, mbar_wait(acc_full, 0));     // tcgen05.ld is warp-collective
-            if (ok) {
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                flush_dw<T>(a, part, tmem, warp, lane);
-            }
-        }
+        if (warp < 6 && ok && part.slabs > 0) flush((part.slabs - 1) / kChain);
     } else if (lane == 0 && a.store) {
         int s = 0, phase = 0;
         for (int i = 0; i < part.slabs; ++i) {
@@ -1426,7 +1452,7 @@ struct DwShape {
     int32_t p_panels, q_panels, p_store, q_store, ranges;
     int64_t rows_per_range, floats;
 };
-DwShape dw_shape(int64_t M, int32_t N, int32_t K)
+DwShape dw_shape(int64_t M, int32_t N, int32_t K, int32_t type)
 {
     DwShape s{};
     s.p_panels = (K + 255) / 256, s.q_panels = (N + 255) / 256;
@@ -1435,7 +1461,7 @@ DwShape dw_shape(int64_t M, int32_t N, int32_t K)
     const int64_t ranges = std::max<int64_t>(1, std::min<int64_t>(148 / panels, slabs / 4));
     s.rows_per_range = (slabs + ranges - 1) / ranges * kDwRows;
     s.ranges = (int)((M + s.rows_per_range - 1) / s.rows_per_range);
-    s.floats = s.ranges > 1 ? s.ranges * panels * s.p_store * s.q_store : 0;
+    s.floats = s.ranges > 1 || M > chain_rows(type == DG_BFLOAT16) ? s.ranges * panels * s.p_store * s.q_store : 0;
     return s;
 }
 
@@ -1570,7 +1596,7 @@ extern "C" int64_t dg_linear_dw_scratch(int64_t M, int32_t N, int32_t K, int32_t
 {
     if (M < 1 || N < 1 || K < 1) return 0;
     if (type == DG_FLOAT32) return dg_dense_linear_dw_scratch(N, K);
-    const DwShape shape = dw_shape(M, N, K);
+    const DwShape shape = dw_shape(M, N, K, type);
     return shape.floats ? shape.floats + (int64_t)shape.ranges * N : 0;
 }
 
@@ -1588,7 +1614,7 @@ extern "C" int dg_linear_dw(const dg_linear_dw_args* g, void* stream)
     if (type == DG_FLOAT32) return fused ? DG_ERR_UNSUPPORTED : dg_dense_linear_dw(g, (cudaStream_t)stream);
     if (!on_rows(g->x, g->ldx, 2) || !on_rows(g->dy, g->lddy, 2) || (smooth && !on_rows(g->z, g->ldz, 2)) || (g->dz && !on_rows(g->dz, g->lddz, 2)) || (fused && K > 256))
         return DG_ERR_UNSUPPORTED;
-    const DwShape shape = dw_shape(M, N, K);
+    const DwShape shape = dw_shape(M, N, K, type);
     const int64_t floats = dg_linear_dw_scratch(M, N, K, type);
     if (floats > 0 && !g->scratch) return DG_ERR_NULL;
     if (g->scratch_floats < floats) return DG_ERR_SCRATCH;

@@ -1,0 +1,67 @@
+"""Long sums of spmm_cpp.linear: many rows in the weight gradient, many columns in the product, on operands of one sign, where what an accumulator
+truncates adds up, against float64.  Needs a GPU.
+
+An accumulation into the tensor cores' accumulator is off by up to three steps (2^-23) of the running sum, on average over a sum that grows evenly three halves of a step of
+the whole.  Chains of them end, and their sums are added in fp32: after 512 (fp16), 2,048 (bf16) and 32 (fp32, of 8 columns) accumulations, CHAIN below.  The result
+rounds by half a step of its type, evenly in both directions: over n elements the mean of that is zero within 6 half steps / sqrt(3 n)."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+CHAIN = {torch.float32: 32 * 1.5 * 2.0 ** -23, torch.bfloat16: 2048 * 1.5 * 2.0 ** -23, torch.float16: 512 * 1.5 * 2.0 ** -23}
+
+
+def _positive(gen, *shape, dtype):
+    return torch.rand(shape, device='cuda', generator=gen, dtype=torch.float32).to(dtype)
+
+
+def _check(got, want, dtype, added=0.0):
+    off = got.double() / want - 1
+    bound = CHAIN[dtype] + added
+    assert float(off.abs().max()) <= HALF[dtype] + bound, float(off.abs().max())
+    assert float(off.mean().abs()) <= bound + 6 * HALF[dtype] / (3 * off.numel()) ** 0.5, float(off.mean())
+
+
+@pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize('M,K,N,act', [(300_000, 264, 2304, None), (131_072, 2304, 2304, None), (70_001, 64, 19_200, 'relu'), (70_001, 40, 19_208, 'silu'), (100_003, 72, 200, None),
+                                       (9_000, 2304, 2312, None)])
+def test_weight_gradients_of_many_rows(M, K, N, act, dtype):
+    """Ranges of one chain and of several, one range and many, dz as it comes and made on the way."""
+    import spmm_cpp
+    gen = torch.Generator(device='cuda').manual_seed(M + N)
+    x, w = _positive(gen, M, K, dtype=dtype), (_positive(gen, K, N, dtype=dtype) / K).requires_grad_()
+    dy = _positive(gen, M, N, dtype=dtype) * (64 / M)
+    y = spmm_cpp.linear(x, w, activation=act)
+    dw, = torch.autograd.grad(y, w, dy)
+    columns = torch.tensor([0, 1, 17, N // 2, N - 9, N - 1, *range(N - 40, N - 12)], device='cuda')
+    dz = dy[:, columns].double()
+    if act == 'silu':                                              # with the z that the kernel keeps, rounded to the type, and dz rounded
+        z = (x.double() @ w.detach()[:, columns].double()).to(dtype).double()
+        s = torch.sigmoid(z)
+        dz = dz * s * (1 + z * (1 - s))
+    rows = torch.cat([torch.arange(min(K, 48), device='cuda'), torch.tensor([K - 1], device='cuda')])
+    want = x[:, rows].double().t() @ dz
+    # SiLU: dz of M rows is rounded before it is summed, z too (its slope changes by at most 0.5 a unit, z is below 1): even, M of them
+    _check(dw[rows][:, columns], want, dtype, added=8 * HALF[dtype] / M ** 0.5 if act == 'silu' else 0.0)
+    assert spmm_cpp.dense_status() == 0
+    again, = torch.autograd.grad(spmm_cpp.linear(x, w, activation=act), w, dy)
+    assert torch.equal(again, dw)
+
+
+@pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize('M,K,N,act', [(70_001, 24, 40, None), (66_000, 300, 520, None), (66_000, 72, 24_000, 'relu'), (70_003, 40, 24_008, None)])
+def test_whole_numbers_of_many_rows_are_exact(M, K, N, act, dtype):
+    """Sums below 2^24 of whole numbers: bit for bit, whatever chains and ranges they come in; bias gradients with them."""
+    import spmm_cpp
+    gen = torch.Generator(device='cuda').manual_seed(M + K)
+    x = torch.randint(-2, 3, (M, K), device='cuda', generator=gen).to(dtype)
+    w = torch.randint(-1, 2, (K, N), device='cuda', generator=gen).to(dtype).requires_grad_()
+    b = torch.full((N,), 0.5, device='cuda', dtype=dtype, requires_grad=True)
+    dy = torch.randint(-1, 2, (M, N), device='cuda', generator=gen, dtype=torch.int8).to(dtype)
+    dw, db = torch.autograd.grad(spmm_cpp.linear(x, w, b, activation=act), [w, b], dy)
+    columns = torch.tensor([0, 3, N // 2, N - 8, N - 1], device='cuda')
+    z = x.double() @ w.detach()[:, columns].double() + 0.5
+    dz = dy[:, columns].double() * ((z > 0) if act else 1)
+    assert torch.equal(dw[:, columns], (x.double().t() @ dz).to(dtype)) and torch.equal(db[columns], dz.sum(0).to(dtype))
+    assert spmm_cpp.dense_status() == 0
