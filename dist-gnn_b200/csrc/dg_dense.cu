@@ -145,6 +145,7 @@ template <int EPI> __device__ __forceinline__ void store_rows(const DenseArgs& a
         [[maybe_unused]] float4 shift;
         if (EPI >= kLinear && pieces && mine16) shift = bias_piece(a, col4);
         uint32_t r[32];
+        __syncwarp();                                             // tcgen05.ld is warp-collective, and lanes have asked for as many rows as there are
         tmem_ld16(acc + (uint32_t)c0, r);
         if (c0 + 16 < a.n_pad) tmem_ld16(acc + (uint32_t)c0 + 16, r + 16);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
@@ -582,6 +583,7 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                 }
                 {
                     uint32_t r[32];
+                    __syncwarp();
                     tmem_ld16(acc + (uint32_t)c0, r);
                     tmem_ld16(acc + (uint32_t)c0 + 16, r + 16);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
@@ -1198,6 +1200,7 @@ __device__ __forceinline__ void dense_tn(const CUtensorMap& tmP, const CUtensorM
                     const int two = c0 + 16 < a.q_store;          // warp-uniform
                     uint32_t r[32];
                     const uint32_t acc = tmem + (uint32_t)(b * 256) + ((uint32_t)(q * 32) << 16) + (uint32_t)c0;
+                    __syncwarp();                                 // lanes beyond the stored rows have skipped the last columns
                     tmem_ld16(acc, r);
                     if (two) tmem_ld16(acc + 16, r + 16);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");

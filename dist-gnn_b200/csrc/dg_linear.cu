@@ -270,6 +270,7 @@ k_linear_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
             }
             for (int c0 = first; c0 < a.n_tile; c0 += step, s ^= 1) {
                 uint32_t r[kPiece];
+                __syncwarp();                                     // one lane has stored the last piece
                 tmem_ld16(acc + (uint32_t)c0, r);
                 tmem_ld16(acc + (uint32_t)c0 + 16, r + 16);
                 const int col0 = n0 + c0;
@@ -414,6 +415,7 @@ template <class T> __device__ __forceinline__ void flush_dw(const LinearDwArgs& 
         float4* to_part = a.partial + ((int64_t)part.range * part.panels + part.panel) * (a.q_store / 4) * a.p_store + row;
         for (int c0 = 0; c0 < part.q_pad; c0 += 16) {
             uint32_t r[16];
+            __syncwarp();                                         // tcgen05.ld is warp-collective, and lanes have stored as many columns as they have
             tmem_ld16(tmem + (uint32_t)(h * 256 + c0) + ((uint32_t)(q * 32) << 16), r);
             asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
             if (a.partial) {
@@ -430,19 +432,20 @@ template <class T> __device__ __forceinline__ void flush_dw(const LinearDwArgs& 
                     }
                 continue;
             }
-            if (p >= a.p_cols) continue;
             T* to = static_cast<T*>(a.dw) + p * a.row_stride + (part.q0 + c0) * a.col_stride;
-            if (whole && part.q0 + c0 + 16 <= a.q_cols) {
-                uint32_t v[8];
+            if (p < a.p_cols) {
+                if (whole && part.q0 + c0 + 16 <= a.q_cols) {
+                    uint32_t v[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = Pair<T>::narrow(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
-                reinterpret_cast<uint4*>(to)[0] = make_uint4(v[0], v[1], v[2], v[3]);
-                reinterpret_cast<uint4*>(to)[1] = make_uint4(v[4], v[5], v[6], v[7]);
-                continue;
+                    for (int j = 0; j < 8; ++j) v[j] = Pair<T>::narrow(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+                    reinterpret_cast<uint4*>(to)[0] = make_uint4(v[0], v[1], v[2], v[3]);
+                    reinterpret_cast<uint4*>(to)[1] = make_uint4(v[4], v[5], v[6], v[7]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        if (part.q0 + c0 + j < a.q_cols) to[j * a.col_stride] = Pair<T>::round(__uint_as_float(r[j]));
+                }
             }
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-                if (part.q0 + c0 + j < a.q_cols) to[j * a.col_stride] = Pair<T>::round(__uint_as_float(r[j]));
         }
     }
 }
@@ -705,6 +708,7 @@ k_linear_back(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ C
                     const float2 f = halves(sum[j][e]);
                     sums[t * kBackSumPitch + 2 * e] = f.x, sums[t * kBackSumPitch + 2 * e + 1] = f.y;
                 }
+                __syncwarp();
                 asm volatile("bar.sync 1, %0;" ::"n"(32 * kBackMakers) : "memory");
                 const int c = part.q0 + 64 * j + t;
                 if (t < 64 && c < a.q_cols) {
@@ -714,6 +718,7 @@ k_linear_back(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ C
                     if (a.db_partial) a.db_partial[(int64_t)part.range * a.q_cols + c] = total;
                     else static_cast<T*>(a.db)[c] = Pair<T>::round(total);
                 }
+                __syncwarp();
                 asm volatile("bar.sync 1, %0;" ::"n"(32 * kBackMakers) : "memory");
             }
         }

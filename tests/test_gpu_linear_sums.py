@@ -65,3 +65,22 @@ def test_whole_numbers_of_many_rows_are_exact(M, K, N, act, dtype):
     dz = dy[:, columns].double() * ((z > 0) if act else 1)
     assert torch.equal(dw[:, columns], (x.double().t() @ dz).to(dtype)) and torch.equal(db[columns], dz.sum(0).to(dtype))
     assert spmm_cpp.dense_status() == 0
+
+
+@pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize('M,K,N', [(300, 33, 40), (511, 301, 530), (100, 1, 300), (600, 99, 19_306), (1_000, 70, 19_201)])
+@pytest.mark.parametrize('act', [None, 'relu'])
+def test_gradients_of_one_range_and_odd_widths(M, K, N, act, dtype):
+    """Few rows, or so many panels that each has all rows: accumulators go to the result directly, where lanes of a warp have rows and others have none."""
+    import spmm_cpp
+    gen = torch.Generator(device='cuda').manual_seed(M + K)
+    x = torch.randint(-2, 3, (M, K), device='cuda', generator=gen).to(dtype)
+    w = torch.randint(-1, 2, (K, N), device='cuda', generator=gen).to(dtype)
+    dy = torch.randint(-1, 2, (M, N), device='cuda', generator=gen).to(dtype)
+    for weight in (w.clone(), w.t().contiguous().t()):
+        weight.requires_grad_()
+        b = torch.full((N,), 0.5, device='cuda', dtype=dtype, requires_grad=True)
+        dw, db = torch.autograd.grad(spmm_cpp.linear(x, weight, b, activation=act), [weight, b], dy)
+        dz = dy.double() * ((x.double() @ w.double() + 0.5 > 0) if act else 1)
+        assert torch.equal(dw, (x.double().t() @ dz).to(dtype)) and torch.equal(db, dz.sum(0).to(dtype))
+    assert spmm_cpp.dense_status() == 0
