@@ -504,25 +504,30 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_linear_dw(const __grid_consta
         const bool issuer = elect_one();
         auto wait = [&](uint32_t bar, int parity) { return __any_sync(0xffffffffu, issuer && mbar_wait(bar, parity)) != 0; };
         const uint32_t idesc = umma_idesc_f16(Pair<T>::kFormat, 128, part.q_pad, true, true);
-        int s = 0, phase = 0, in_chain = 0, chain = 0;
-        for (int i = 0; i < part.slabs && ok; ++i) {
-            if (in_chain == kChain) ok = wait(acc_empty, chain++ & 1), in_chain = 0;      // the chain before has left the accumulators
-            ok = ok && wait(full0 + 8 * s, phase);
-            if (!ok) break;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            if (issuer) {
-                const uint32_t st = base + s * stage_bytes, more = in_chain > 0;
-                const uint64_t p = umma_desc_mn16(st, kDwBox), q = umma_desc_mn16(st + a.p_boxes * kDwBox, kDwBox);
-                for (int h = 0; h < part.halves; ++h)
+        int s = 0, phase = 0;
+        for (int chain = 0, left = part.slabs; left > 0 && ok; ++chain, left -= kChain) {
+            // The chain before has left the accumulators.  All lanes ask: with one asking, as below, every stage's turn took 300 clocks more (65,536 rows 1024 x 1024 90 us -> 113).
+            if (chain > 0) ok = __all_sync(0xffffffffu, mbar_wait(acc_empty, (chain - 1) & 1)) != 0;
+            const int slabs = ok ? min(left, kChain) : 0;
+            for (int i = 0; i < slabs && ok; ++i) {
+                ok = wait(full0 + 8 * s, phase);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (issuer) {
+                    const uint32_t st = base + s * stage_bytes;
+                    const uint64_t p = umma_desc_mn16(st, kDwBox), q = umma_desc_mn16(st + a.p_boxes * kDwBox, kDwBox);
+                    for (int h = 0; h < part.halves; ++h)
 #pragma unroll
-                    for (int k = 0; k < kDwRows / 16; ++k)        // 16 rows: 2048 bytes
-                        umma_f16(tmem + (uint32_t)(h * 256), p + (uint32_t)((h * 2 * kDwBox + k * 2048) >> 4), q + (uint32_t)(k * 2048 >> 4), idesc, k > 0 ? 1u : more);
-                umma_commit(empty0 + 8 * s);
-                if (in_chain == kChain - 1 || i == part.slabs - 1) umma_commit(acc_full);
+                        for (int k = 0; k < kDwRows / 16; ++k)    // 16 rows: 2048 bytes
+                            umma_f16(tmem + (uint32_t)(h * 256), p + (uint32_t)((h * 2 * kDwBox + k * 2048) >> 4), q + (uint32_t)(k * 2048 >> 4), idesc,
+                                     i > 0 || k > 0 ? 1u : 0u);
+                    umma_commit(empty0 + 8 * s);
+                }
+                __syncwarp();
+                if (++s == a.stages) s = 0, phase ^= 1;
             }
-            ++in_chain;
+            if (ok && issuer) umma_commit(acc_full);
             __syncwarp();
-            if (++s == a.stages) s = 0, phase ^= 1;
         }
         if (issuer) await_mmas(done);
         __syncwarp();
@@ -616,25 +621,29 @@ k_linear_back(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ C
         const bool issuer = elect_one();
         auto wait = [&](uint32_t bar, int parity) { return __any_sync(0xffffffffu, issuer && mbar_wait(bar, parity)) != 0; };
         const uint32_t idesc = umma_idesc_f16(Pair<T>::kFormat, 128, part.q_pad, true, true);
-        int s = 0, phase = 0, in_chain = 0, chain = 0;
-        for (int i = 0; i < part.slabs && ok; ++i) {
-            if (in_chain == kChain) ok = wait(acc_empty, chain++ & 1), in_chain = 0;
-            ok = ok && wait(ready0 + 8 * s, phase);
-            if (!ok) break;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            if (issuer) {
-                const uint32_t st = base + s * stage_bytes, more = in_chain > 0;
-                const uint64_t p = umma_desc_mn16(st, kBackBox), q = umma_desc_mn16(st + q_at, kBackBox);
-                for (int h = 0; h < part.halves; ++h)
+        int s = 0, phase = 0;
+        for (int chain = 0, left = part.slabs; left > 0 && ok; ++chain, left -= kChain) {
+            if (chain > 0) ok = __all_sync(0xffffffffu, mbar_wait(acc_empty, (chain - 1) & 1)) != 0;
+            const int slabs = ok ? min(left, kChain) : 0;
+            for (int i = 0; i < slabs && ok; ++i) {
+                ok = wait(ready0 + 8 * s, phase);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (issuer) {
+                    const uint32_t st = base + s * stage_bytes;
+                    const uint64_t p = umma_desc_mn16(st, kBackBox), q = umma_desc_mn16(st + q_at, kBackBox);
+                    for (int h = 0; h < part.halves; ++h)
 #pragma unroll
-                    for (int k = 0; k < kBackRows / 16; ++k)      // 16 rows: 2048 bytes
-                        umma_f16(tmem + (uint32_t)(h * 256), p + (uint32_t)((h * 2 * kBackBox + k * 2048) >> 4), q + (uint32_t)(k * 2048 >> 4), idesc, k > 0 ? 1u : more);
-                umma_commit(empty0 + 8 * s);
-                if (in_chain == kChain - 1 || i == part.slabs - 1) umma_commit(acc_full);
+                        for (int k = 0; k < kBackRows / 16; ++k)  // 16 rows: 2048 bytes
+                            umma_f16(tmem + (uint32_t)(h * 256), p + (uint32_t)((h * 2 * kBackBox + k * 2048) >> 4), q + (uint32_t)(k * 2048 >> 4), idesc,
+                                     i > 0 || k > 0 ? 1u : 0u);
+                    umma_commit(empty0 + 8 * s);
+                }
+                __syncwarp();
+                if (++s == a.stages) s = 0, phase ^= 1;
             }
-            ++in_chain;
+            if (ok && issuer) umma_commit(acc_full);
             __syncwarp();
-            if (++s == a.stages) s = 0, phase ^= 1;
         }
         if (issuer) await_mmas(done);
         __syncwarp();
