@@ -365,7 +365,12 @@ __device__ __forceinline__ void umma_tf32_pair(uint32_t tmem_d, uint64_t a_desc,
         ::"r"(tmem_d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
 }
 
-template <int EPI>
+// DEEP: more than kChain half slabs, 1,024 columns.  The tensor cores truncate when they add into an accumulator, so a chain of additions ends there (K in even shares);
+// the epilogue warps take the head passes' accumulator and add it, rounded to nearest, to what they hold of the tile, beside the next chain's MMAs.  (The tail passes', a 2,048th
+// of them, stay in theirs.)  The error is that of 1,024 columns, 2.7e-6 for N(0, 1) operands and 6.7e-6 for positive ones, whatever K is; in one chain it was 1e-5 and 2.8e-5
+// at 4,096 and 3.9e-5 and 1.1e-4 at 16,384.  Shorter chains are not free: reading an accumulator out holds the MMAs up (232,965 rows 602 -> 256 in two chains 354 us -> 450).
+constexpr int kChain = 64;
+template <int EPI, bool DEEP>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadsPair, 1)
 k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmBh,
                 const __grid_constant__ CUtensorMap tmBt, const DenseArgs args, const int n_tiles, const int stages)
@@ -388,6 +393,7 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     const int nhalves = (a.K + PK - 1) / PK;
+    [[maybe_unused]] const int chains = DEEP ? (nhalves + kChain - 1) / kChain : 1, in_chain = DEEP ? ((nhalves + chains - 1) / chains + 1) / 2 * 2 : nhalves;
     constexpr bool kApart = EPI >= kLinear;      // the tail passes' sums, a 2,048th of the head passes', are not rounded with them: accumulators of their own, columns 128 / 384
     constexpr int kTmemCols = 512;                                // two accumulators of up to 256 columns
 
@@ -442,15 +448,19 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             const uint32_t next_stage = (uint32_t)stage_bytes >> 4, tail = a_bytes >> 4, b_head = 2 * tail, b_tail = b_head + ((uint32_t)b_bytes >> 4);
             int s = 0, phase = 0, lt = 0;
             [[maybe_unused]] bool early = false;
-            for (int tile = pair; tile < n_tiles && ok; tile += pairs, ++lt) {
+            [[maybe_unused]] int chain = 0, side = 0;
+            for (int tile = pair; tile < n_tiles && ok; ++lt) {
                 const int b = lt & 1, v = lt >> 1;
+                const int count = DEEP ? min(in_chain, nhalves - chain * in_chain) : nhalves;
+                [[maybe_unused]] const uint32_t tails = tmem + (uint32_t)((DEEP ? side : b) * 256 + 128), tails_add = DEEP && chain > 0;
+                if (!DEEP || ++chain == chains) tile += pairs, chain = 0, side ^= 1;
                 if (lt >= 2) ok = wait(acc_empty0 + 8 * b, (v - 1) & 1);     // both epilogues have drained this accumulator
                 const uint32_t acc = tmem + (uint32_t)(b * 256);
                 // What goes around the MMAs costs the issuing warp 500 clocks a turn (200 of them the barrier's answer), six MMAs 90 to issue and 540 to run at 128 columns:
                 // hence two stages a turn, and the next two asked for before these are issued (382,902 rows 488 -> 8 265 us -> 199, 150,001 rows 256 -> 256 127 -> 110).
                 if constexpr (kApart) {
-                    for (int i = 0; i < nhalves && ok; i += 2) {
-                        const bool two = i + 1 < nhalves;
+                    for (int i = 0; i < count && ok; i += 2) {
+                        const bool two = i + 1 < count;
                         const int s1 = s + 1 == stages ? 0 : s + 1, phase1 = phase ^ (s + 1 == stages);
                         if (!early) ok = __any_sync(0xffffffffu, issuer && mbar_wait(ready0 + 8 * s, phase) && (!two || mbar_wait(ready0 + 8 * s1, phase1))) != 0;
                         if (!ok) break;
@@ -465,8 +475,8 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                                 const uint64_t d = desc0 + (uint32_t)stage * next_stage;
 #pragma unroll
                                 for (int k = 0; k < PK / 8; ++k) {
-                                    umma_tf32_pair(acc + 128, d + tail + 2 * k, d + b_head + 2 * k, idesc, k > 0 ? 1u : add);
-                                    umma_tf32_pair(acc + 128, d + 2 * k, d + b_tail + 2 * k, idesc, 1u);
+                                    umma_tf32_pair(tails, d + tail + 2 * k, d + b_head + 2 * k, idesc, k > 0 ? 1u : add | tails_add);
+                                    umma_tf32_pair(tails, d + 2 * k, d + b_tail + 2 * k, idesc, 1u);
                                     umma_tf32_pair(acc, d + 2 * k, d + b_head + 2 * k, idesc, k > 0 ? 1u : add);
                                 }
                                 umma_commit_pair(empty0 + 8 * stage);
@@ -556,10 +566,39 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         const bool vec = a.ldc % 4 == 0 && (reinterpret_cast<uintptr_t>(a.C) & 15) == 0 &&
                          (EPI == kPlain || !a.mask || (a.ldm % 4 == 0 && (reinterpret_cast<uintptr_t>(a.mask) & 15) == 0)) &&
                          (EPI < kLinear || !a.z || (a.ldz % 4 == 0 && (reinterpret_cast<uintptr_t>(a.z) & 15) == 0));
-        const bool side = EPI == kMasked || (EPI >= kLinear && a.mask);
+        const bool masked = EPI == kMasked || (EPI >= kLinear && a.mask);
         const int r4 = lane >> 3, piece = lane & 7;
         int lt = 0;
+        [[maybe_unused]] int side = 0;
         for (int tile = pair; tile < n_tiles; tile += pairs, ++lt) {
+            [[maybe_unused]] float held[2][32];                   // of this warp's two pieces, the chains before the last
+            if constexpr (DEEP) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) held[0][j] = held[1][j] = 0.f;
+                for (int chain = 1; chain < chains; ++chain, ++lt) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(acc_full0 + 8 * (lt & 1), lt >> 1 & 1));
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+                    for (int p = 0; p < 2; ++p) {
+                        if (first + p * step >= a.n_pad) break;
+                        const uint32_t at = tmem + (uint32_t)((lt & 1) * 256 + first + p * step) + ((uint32_t)(q * 32) << 16);
+#pragma unroll
+                        for (int h = 0; h < 32; h += 16) {
+                            uint32_t r[16];
+                            tmem_ld16(at + h, r);
+                            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) held[p][h + j] += __uint_as_float(r[j]);
+                        }
+                    }
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(leader_acc_empty0 + 8 * (lt & 1));
+                    __syncwarp();
+                }
+                if (!ok) break;
+            }
             const int b = lt & 1, v = lt >> 1;
             const int64_t row0 = (int64_t)tile * (2 * BM) + rank * BM + q * 32;
             const int rows = (int)max((int64_t)0, min((int64_t)32, a.M - row0));
@@ -568,7 +607,7 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                 const bool some = EPI >= kLinear && a.N % 4 == 0 && c0 < a.N, mine16 = !some || c0 + piece * 4 < a.N;
                 const bool whole = vec && (c0 + 32 <= a.N || some);      // 128-byte pieces of every row, whole or their first columns, four rows an instruction
                 [[maybe_unused]] float4 mk[8];
-                if (side && whole) {                              // under way while the accumulator is waited for and read
+                if (masked && whole) {                            // under way while the accumulator is waited for and read
                     const float* m = a.mask + (row0 + r4) * a.ldm + c0 + piece * 4;
 #pragma unroll
                     for (int i = 0; i < 8; ++i, m += 4 * a.ldm)
@@ -587,7 +626,11 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                     tmem_ld16(acc + (uint32_t)c0, r);
                     tmem_ld16(acc + (uint32_t)c0 + 16, r + 16);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                    if constexpr (kApart) add_tails(r, acc + 128 + (uint32_t)c0, true);
+                    if constexpr (DEEP) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + (c0 == first ? held[0][j] : held[1][j]));
+                    }
+                    if constexpr (kApart) add_tails(r, (DEEP ? tmem + (uint32_t)(side * 256 + 128) + ((uint32_t)(q * 32) << 16) : acc + 128) + (uint32_t)c0, true);
                     if (c0 + step >= a.n_pad) {                   // the accumulator has been read: its next tile may start
                         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                         __syncwarp();
@@ -628,7 +671,7 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                     const float* flat = reinterpret_cast<const float*>(stage);
                     for (int i0 = 0; i0 < rows; i0 += 8) {        // eight rows' mask values in flight
                         [[maybe_unused]] float mrow[8];
-                        if (side) {
+                        if (masked) {
 #pragma unroll
                             for (int i = 0; i < 8; ++i)
                                 if (i0 + i < rows) mrow[i] = __ldg(a.mask + (row0 + i0 + i) * a.ldm + c0 + lane);
@@ -654,6 +697,7 @@ k_dense_nt_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                 __syncwarp();
             }
             if (!ok) break;
+            if (DEEP) side ^= 1;
         }
     }
     if (!ok) atomicExch(a.status, 1);
@@ -766,7 +810,8 @@ int launch_nt(const float* A, int64_t lda, const float* Bt_head, const float* Bt
     if (!a.status) return DG_ERR_STATE;
     const int sms = sm_count();
     if (sms <= 0) return DG_ERR_STATE;
-    const bool pair = by_pairs((a.M + BM - 1) / BM * a.panels, a.n_pad, a.K, a.mask != nullptr, sms, linear);
+    const bool deep = linear && a.K > kChain * PK;
+    const bool pair = deep || by_pairs((a.M + BM - 1) / BM * a.panels, a.n_pad, a.K, a.mask != nullptr, sms, linear);
     CUtensorMap tmA, tmBh, tmBt;
     int rc;
     if (!pair) {
@@ -801,8 +846,9 @@ int launch_nt(const float* A, int64_t lda, const float* Bt_head, const float* Bt
         return (int)cudaGetLastError();
     };
     return by_epilogue(epilogue, [&](auto e) {
-        static std::atomic<bool> granted[64];
-        return run(k_dense_nt_pair<decltype(e)::value>, granted);
+        static std::atomic<bool> granted[2][64];
+        constexpr int EPI = decltype(e)::value;
+        return deep ? run(k_dense_nt_pair<EPI, (EPI >= kLinear)>, granted[0]) : run(k_dense_nt_pair<EPI, false>, granted[1]);
     });
 }
 

@@ -2,14 +2,14 @@
 truncates adds up, against float64.  Needs a GPU.
 
 An accumulation into the tensor cores' accumulator is off by up to three steps (2^-23) of the running sum, on average over a sum that grows evenly three halves of a step of
-the whole.  Chains of them end, and their sums are added in fp32: after 512 (fp16), 2,048 (bf16) and 32 (fp32, of 8 columns) accumulations, CHAIN below.  The result
+the whole.  Chains of them end, and their sums are added in fp32: after 512 (fp16), 2,048 (bf16) and 128 (fp32, of 8 columns) accumulations, CHAIN below.  The result
 rounds by half a step of its type, evenly in both directions: over n elements the mean of that is zero within 6 half steps / sqrt(3 n)."""
 import pytest
 import torch
 
 pytestmark = pytest.mark.gpu
 HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
-CHAIN = {torch.float32: 32 * 1.5 * 2.0 ** -23, torch.bfloat16: 2048 * 1.5 * 2.0 ** -23, torch.float16: 512 * 1.5 * 2.0 ** -23}
+CHAIN = {torch.float32: 128 * 1.5 * 2.0 ** -23, torch.bfloat16: 2048 * 1.5 * 2.0 ** -23, torch.float16: 512 * 1.5 * 2.0 ** -23}
 
 
 def _positive(gen, *shape, dtype):
@@ -83,4 +83,52 @@ def test_gradients_of_one_range_and_odd_widths(M, K, N, act, dtype):
         dw, db = torch.autograd.grad(spmm_cpp.linear(x, weight, b, activation=act), [weight, b], dy)
         dz = dy.double() * ((x.double() @ w.double() + 0.5 > 0) if act else 1)
         assert torch.equal(dw, (x.double().t() @ dz).to(dtype)) and torch.equal(db, dz.sum(0).to(dtype))
+    assert spmm_cpp.dense_status() == 0
+
+
+@pytest.mark.parametrize('M,K,N', [(2000, 257, 128), (2000, 602, 128), (300, 1024, 41), (5000, 4096, 200), (40, 4097, 96), (700, 16_384, 130), (20_000, 300, 64)])
+@pytest.mark.parametrize('signs', ['one', 'both'])
+def test_products_of_many_columns_fp32(M, K, N, signs):
+    """Three TF32 passes: chains of at most 1,024 columns whatever K is, forward and in x's gradient.  Of the sum of magnitudes S each element is off by the chain's share,
+    2^-20.8 for the terms that the passes leave out and for the weight's tails, and the additions of K / 1,024 chains in fp32.  On average an accumulation is off by a step of
+    the running sum at most: over a chain of n, n / 2 steps of a sum that grows evenly, and two thirds of n of one that grows with the square root, as those of both signs do."""
+    import spmm_cpp
+    gen = torch.Generator(device='cuda').manual_seed(K)
+    make = torch.rand if signs == 'one' else torch.randn
+    x, w = (make(s, device='cuda', generator=gen) for s in ((M, K), (K, N)))
+    chains = 2.0 ** -24 * ((K + 1023) // 1024) + 2.0 ** -20.8
+    want, size = x.double() @ w.double(), x.double().abs() @ w.double().abs()
+    back = (torch.rand if signs == 'one' else torch.randn)(M, K, device='cuda', generator=gen)
+    v = w.t().contiguous().requires_grad_(False)                   # [N x K]: x's gradient of a layer N -> K sums over K columns
+    a = torch.zeros(M, N, device='cuda', requires_grad=True)
+    dx, = torch.autograd.grad(spmm_cpp.linear(a, v), a, back)
+    for got, exact, total in ((spmm_cpp.linear(x, w), want, size), (dx, back.double() @ v.double().t(), back.double().abs() @ v.double().abs().t())):
+        assert float(((got.double() - exact).abs() / total).max()) <= CHAIN[torch.float32] * 2 + chains
+        assert float((got.double() - exact).norm() / exact.norm()) <= 128 * 2.0 ** -23 * (1 / 2 if signs == 'one' else 2 / 3) + chains
+    assert spmm_cpp.dense_status() == 0
+
+
+@pytest.mark.parametrize('M,K,N', [(600, 1100, 257), (2001, 1030, 47), (150, 1600, 1600), (17, 1025, 1), (260, 4097, 128), (3000, 1040, 130), (40_000, 2100, 300)])
+@pytest.mark.parametrize('act', [None, 'relu', 'gelu', 'silu'])
+def test_whole_numbers_of_many_columns_are_exact_fp32(M, K, N, act):
+    """Several chains with every epilogue: bias, activation, residual, what is kept for the gradient, panels and rows that end inside a tile.  Whole numbers: bit for bit
+    but for GELU and SiLU, which see the exact z (an even number, so that there are none between -2 and 2 but 0)."""
+    import spmm_cpp
+    gen = torch.Generator(device='cuda').manual_seed(M + K + N)
+    x, w, r, dy = (torch.randint(-1, 2, s, device='cuda', generator=gen).float() for s in ((M, K), (K, N), (M, N), (M, N)))
+    x *= 2
+    b = torch.ones(N, device='cuda') * 2
+    leaves = [t.requires_grad_() for t in (x, w, b, r)]
+    y = spmm_cpp.linear(x, w, b, residual=r, activation=act)
+    z = x.detach().double() @ w.detach().double() + 2
+    if act in ('gelu', 'silu'):
+        value = z * (torch.sigmoid(z) if act == 'silu' else 0.5 * torch.erfc(-z * 0.5 ** 0.5))
+        assert float((y.detach().double() - value - r.detach().double()).abs().max()) <= 2.0 ** -21 * float(z.abs().max())
+        assert all(bool(torch.isfinite(g).all()) for g in torch.autograd.grad(y, leaves, dy))
+    else:
+        value, slope = (z.clamp(min=0), z > 0) if act else (z, torch.ones_like(z))
+        assert torch.equal(y.detach(), (value + r.detach().double()).float())
+        dz = dy.double() * slope
+        for got, exact in zip(torch.autograd.grad(y, leaves, dy), (dz @ w.detach().double().t(), x.detach().double().t() @ dz, dz.sum(0), dy.double())):
+            assert torch.equal(got, exact.float())
     assert spmm_cpp.dense_status() == 0
