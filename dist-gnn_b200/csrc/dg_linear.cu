@@ -65,6 +65,11 @@ template <> struct Pair<float> {
     static __device__ __forceinline__ float round(float v) { return v; }
 };
 
+// The tensor cores truncate when they add into an accumulator: where all terms are of one sign a chain of n accumulations, 16 terms each, is some n 2^-23 too small.  So
+// long sums are taken in chains, whose results are added rounded to nearest: fp16, which rounds by 2^-11, after 512 accumulations (6e-5), bf16, by 2^-8, after 2,048.
+constexpr int chain_terms(bool bf16) { return bf16 ? 32768 : 8192; }
+template <class T> constexpr int kChainTerms = chain_terms(std::is_same<T, __nv_bfloat16>::value);
+
 // ---- the product on the tensor cores ------------------------------------------------------------------------------------
 constexpr int BM = 128, BK = 64;                  // rows of a CTA, K-columns of a stage: 128 bytes
 constexpr int kEpilogueWarps = 16, kThreadsPair = 32 * (2 + kEpilogueWarps);
@@ -129,7 +134,8 @@ __device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t a_desc, uint6
 // epilogue warp and buffer for its residual's pieces.
 // What bounds it: HBM up to some 500 columns (400,000 x 256 -> 256 bf16 with GELU, bias, residual and z 139 us, 5.9 TB/s; without them 67 us, 6.15 TB/s), the tensor
 // cores beyond (65,536 x 1024 -> 1024 100 us, 1,379 TFLOP/s; with SiLU, residual and z 137).
-template <class T, int ACT>
+// DEEP: K beyond a chain; tiles of up to 128 columns, so that a warp has one piece, which it holds in registers while the tile's other chains run.
+template <class T, int ACT, bool DEEP>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadsPair, 1)
 k_linear_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmY,
               const __grid_constant__ CUtensorMap tmR, const __grid_constant__ CUtensorMap tmZ, const LinearPairArgs a)
@@ -148,6 +154,7 @@ k_linear_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     const int slabs = (a.K + BK - 1) / BK;
+    [[maybe_unused]] const int chains = DEEP ? (a.K + kChainTerms<T> - 1) / kChainTerms<T> : 1, in_chain = DEEP ? (slabs + chains - 1) / chains : slabs;
     constexpr int kTmemCols = 512;
 
     if (threadIdx.x == 0) {
@@ -205,11 +212,14 @@ k_linear_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
             const uint32_t next_stage = (uint32_t)stage_bytes >> 4, b_step = a.b_boxes ? 16 * 128 >> 4 : 2;      // 16 K-columns
             int s = 0, phase = 0, lt = 0;
             bool early = false;
-            for (int tile = pair; tile < a.tiles && ok; tile += pairs, ++lt) {
+            [[maybe_unused]] int chain = 0;
+            for (int tile = pair; tile < a.tiles && ok; ++lt) {
                 const int b = lt & 1, v = lt >> 1;
+                const int count = DEEP ? min(in_chain, slabs - chain * in_chain) : slabs;
+                if (!DEEP || ++chain == chains) tile += pairs, chain = 0;
                 if (lt >= 2) ok = wait(acc_empty0 + 8 * b, (v - 1) & 1);     // both epilogues have drained this accumulator
                 const uint32_t acc = tmem + (uint32_t)(b * 256);
-                for (int i = 0; i < slabs && ok; ++i) {
+                for (int i = 0; i < count && ok; ++i) {
                     if (!early) ok = wait(full0 + 8 * s, phase);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -256,6 +266,30 @@ k_linear_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
         int lt = 0, s = 0;
         if (a.residual && lane == 0 && pair < a.tiles && first < a.n_tile) fetch(pair, first, 0);
         for (int tile = pair; tile < a.tiles && ok; tile += pairs, ++lt) {
+            [[maybe_unused]] float held[kPiece];
+            if constexpr (DEEP) {
+#pragma unroll
+                for (int j = 0; j < kPiece; ++j) held[j] = 0.f;
+                for (int chain = 1; chain < chains; ++chain, ++lt) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(acc_full0 + 8 * (lt & 1), lt >> 1 & 1));
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (first < a.n_tile) {
+                        const uint32_t at = tmem + (uint32_t)((lt & 1) * 256 + first) + ((uint32_t)(q * 32) << 16);
+                        uint32_t r[kPiece];
+                        __syncwarp();
+                        tmem_ld16(at, r);
+                        tmem_ld16(at + 16, r + 16);
+                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                        for (int j = 0; j < kPiece; ++j) held[j] += __uint_as_float(r[j]);
+                    }
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(leader_acc_empty0 + 8 * (lt & 1));
+                }
+                if (!ok) break;
+            }
             const int b = lt & 1, v = lt >> 1;
             const int n0 = tile % a.n_panels * a.n_tile;
             const int64_t row0 = row_of(tile);
@@ -284,6 +318,10 @@ k_linear_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
                 }
                 __syncwarp();
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                if constexpr (DEEP) {
+#pragma unroll
+                    for (int j = 0; j < kPiece; ++j) r[j] = __float_as_uint(held[j] + __uint_as_float(r[j]));
+                }
                 if (c0 + step >= a.n_tile) {                      // the accumulator has been read: its next tile may start
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                     __syncwarp();
@@ -364,13 +402,10 @@ k_linear_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
 // side; a second kernel adds the ranges in order.
 // One range (fewer than 512 rows, or more than 74 panels) of one chain is written as it is.
 // What bounds it: the tensor cores for wide layers (65,536 rows 1024 x 1024 93 us, 1,480 TFLOP/s), HBM for the others (232,965 rows 602 x 41 65 us, 4.6 TB/s).
-// The tensor cores truncate when they add into an accumulator: where all terms are of one sign a chain of n accumulations, 16 rows each, is some n 2^-23 too small.  So a
-// chain ends after chain_rows, and the CTA adds the accumulators to its partial result: fp16, which rounds by 2^-11, after 512 accumulations (6e-5), bf16, by 2^-8, after
-// 2,048.  With ranges of one chain each, 300,000 x 264, 2304 fp16 were 2.3e-4 too small and 131,072 x 2304, 2304, whose 81 panels leave one range, 7.8e-4.
+// A chain of accumulations ends after kChainTerms rows, and the CTA adds the accumulators to its partial result: with ranges of one chain each, 300,000 x 264, 2304 fp16 were
+// 2.3e-4 too small and 131,072 x 2304, 2304, whose 81 panels leave one range, 7.8e-4.
 constexpr int kDwRows = 64, kDwBox = kDwRows * 128, kDwThreads = 32 * 6, kDwMaxStages = 8;
 constexpr int kDwBarBytes = 8 * (2 * kDwMaxStages + 3) + 8;
-constexpr int chain_rows(bool bf16) { return bf16 ? 32768 : 8192; }
-template <class T> constexpr int kChainRows = chain_rows(std::is_same<T, __nv_bfloat16>::value);
 
 struct LinearDwArgs {
     float4* partial;                              // [range][panel][q_store / 4][p_store]; null: the one range's sums are the result
@@ -463,7 +498,7 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_linear_dw(const __grid_consta
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbase + a.stages * stage_bytes + 8 * (2 * kDwMaxStages + 3));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const DwPart part(a, kDwRows);
-    constexpr int kTmemCols = 512, kChain = kChainRows<T> / kDwRows;      // slabs of a chain
+    constexpr int kTmemCols = 512, kChain = kChainTerms<T> / kDwRows;      // slabs of a chain
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < a.stages; ++s) {
@@ -575,7 +610,7 @@ k_linear_back(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ C
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbase + a.stages * stage_bytes + kBackSumBytes + 8 * (4 * kBackMaxStages + 3));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const DwPart part(a, kBackRows);
-    constexpr int kTmemCols = 512, kChain = kChainRows<T> / kBackRows;
+    constexpr int kTmemCols = 512, kChain = kChainTerms<T> / kBackRows;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < a.stages; ++s) {
@@ -1371,11 +1406,14 @@ int make_map16(CUtensorMap* map, const void* ptr, int32_t type, int64_t rows, in
 
 template <class T, int ACT> int launch_pair(const CUtensorMap* maps, const LinearPairArgs& a, unsigned ctas, size_t smem, cudaStream_t stream)
 {
-    static std::atomic<bool> granted[64];
-    const int rc = allow_smem((const void*)k_linear_pair<T, ACT>, granted);
-    if (rc) return rc;
-    k_linear_pair<T, ACT><<<ctas, kThreadsPair, smem, stream>>>(maps[0], maps[1], maps[2], maps[3], maps[4], a);
-    return (int)cudaGetLastError();
+    auto run = [&](auto* kernel, std::atomic<bool>* granted) {
+        const int rc = allow_smem((const void*)kernel, granted);
+        if (rc) return rc;
+        kernel<<<ctas, kThreadsPair, smem, stream>>>(maps[0], maps[1], maps[2], maps[3], maps[4], a);
+        return (int)cudaGetLastError();
+    };
+    static std::atomic<bool> granted[2][64];
+    return a.K > kChainTerms<T> ? run(k_linear_pair<T, ACT, true>, granted[0]) : run(k_linear_pair<T, ACT, false>, granted[1]);
 }
 template <class T> int launch_pair(int act, const CUtensorMap* maps, const LinearPairArgs& a, unsigned ctas, size_t smem, cudaStream_t stream)
 {
@@ -1407,6 +1445,7 @@ int linear16(const dg_linear_args* g, cudaStream_t stream)
     a.bias = g->bias, a.bits = g->bits, a.ldbits = g->ldbits, a.M = g->M, a.N = g->N, a.K = g->K;
     const int64_t m_tiles = (g->M + 2 * BM - 1) / (2 * BM);
     a.n_tile = tile_columns(m_tiles, g->N, sms / 2);
+    if (g->K > chain_terms(g->type == DG_BFLOAT16)) a.n_tile = std::min(a.n_tile, kEpilogueWarps / 4 * kPiece);
     a.n_panels = (g->N + a.n_tile - 1) / a.n_tile;
     if (m_tiles * a.n_panels >= (int64_t)1 << 30) return DG_ERR_UNSUPPORTED;
     a.tiles = (int)(m_tiles * a.n_panels);
@@ -1475,7 +1514,7 @@ DwShape dw_shape(int64_t M, int32_t N, int32_t K, int32_t type)
     const int64_t ranges = std::max<int64_t>(1, std::min<int64_t>(148 / panels, slabs / 4));
     s.rows_per_range = (slabs + ranges - 1) / ranges * kDwRows;
     s.ranges = (int)((M + s.rows_per_range - 1) / s.rows_per_range);
-    s.floats = s.ranges > 1 || M > chain_rows(type == DG_BFLOAT16) ? s.ranges * panels * s.p_store * s.q_store : 0;
+    s.floats = s.ranges > 1 || M > chain_terms(type == DG_BFLOAT16) ? s.ranges * panels * s.p_store * s.q_store : 0;
     return s;
 }
 
