@@ -140,13 +140,14 @@ __device__ __forceinline__ void decode(uint2 c, float scale, float_pair* v)
 }
 
 // The square root, by Newton's step with the remainder from a fused product (Markstein, IBM Journal of Research and Development, 1990): the correctly
-// rounded one but for a few arguments in a million, where it is the neighbour.  Below fp32's smallest normal number it is too small by up to a third.
+// rounded one but for a few arguments in a million, where it is the neighbour, and below fp32's smallest normal number that of the approximation, within 2^-22.
+// Zero is taken for the smallest number above it, whose reciprocal root is finite.
 __device__ __forceinline__ float_pair square_root(float_pair v)
 {
     const float2 f = halves(v);
     float a, b;
-    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(fmaxf(f.x, 0x1p-126f)));
-    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(fmaxf(f.y, 0x1p-126f)));
+    asm("rsqrt.approx.f32 %0, %1;" : "=f"(a) : "f"(fmaxf(f.x, 0x1p-149f)));
+    asm("rsqrt.approx.f32 %0, %1;" : "=f"(b) : "f"(fmaxf(f.y, 0x1p-149f)));
     const float_pair y = pair_of(a, b), s = mul2(v, y);
     return fma2(fma2(mul2(s, both(-1.f)), s, v), mul2(y, both(0.5f)), s);
 }
