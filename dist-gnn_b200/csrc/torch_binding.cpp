@@ -451,51 +451,61 @@ Weight stored(const Tensor& w)
     return {in_out ? w : w.contiguous(), false};
 }
 
+// What the gradients read goes through saved variables, so that changes in place are noticed and saved-tensor hooks (offloading, checkpoints) have all of it: x where the weight wants
+// its gradient, the weight, and what the product made.  Where the product read a copy of x or of the weight (odd rows, odd strides) the copy is kept in its place.
 struct LinearNode : public torch::autograd::Node {
-    SavedVariable x_saved, w_saved;       // x and w, to notice that they were changed in place
-    Tensor x, w, splits, z, bits;         // the operands as the product read them; w as it lies in memory
-    int64_t N = 0, K = 0;
+    SavedVariable x_saved, w_saved, splits_saved, z_saved, bits_saved;
+    at::TensorOptions options;            // of x
+    int64_t M = 0, N = 0, K = 0;
     int32_t act = 0;
-    bool out_in = false;
+    bool w_copied = false, w_out_in = false;      // the kept copy, as it lies in memory
 
     std::string name() const override { return "LinearBackward"; }
     void release_variables() override
     {
-        x_saved.reset_data(), w_saved.reset_data();
-        x.reset(), w.reset(), splits.reset(), z.reset(), bits.reset();
+        for (SavedVariable* v : {&x_saved, &w_saved, &splits_saved, &z_saved, &bits_saved}) v->reset_data();
     }
     variable_list apply(variable_list&& grads) override
     {
         variable_list out(4);
         if (!grads[0].defined()) return out;
-        TORCH_CHECK(x.defined(), "Trying to backward through the graph a second time");
         TORCH_CHECK(!at::GradMode::is_enabled(), "the gradient of linear cannot be differentiated again");
-        x_saved.unpack(), w_saved.unpack();
         const bool dx = task_should_compute_output(0), dw = task_should_compute_output(1), db = task_should_compute_output(2), dr = task_should_compute_output(3);
-        c10::cuda::CUDAGuard guard(x.device());
-        void* stream = stream_of(x);
-        const int64_t M = x.size(0), item = item_of(x);
-        const int32_t type = type_of(x);
-        const Tensor dy = grads[0].scalar_type() == x.scalar_type() ? grads[0] : grads[0].to(x.scalar_type());
+        c10::cuda::CUDAGuard guard(options.device());
+        const Tensor x = x_saved.unpack(), splits = splits_saved.unpack(), bits = bits_saved.unpack();
+        Tensor z = z_saved.unpack();
+        if (z.defined()) z = by_rows(z);
+        Weight weight{w_saved.unpack(), w_out_in};
+        if (weight.t.defined() && !w_copied) weight = stored(weight.t);
+        Tensor& w = weight.t;
+        const bool out_in = weight.out_in;
+        const at::ScalarType dtype = options.dtype().toScalarType();
+        const Tensor dy = grads[0].scalar_type() == dtype ? grads[0] : grads[0].to(dtype);
+        void* stream = stream_of(dy);
+        const int64_t item = item_of(dy);
+        const int32_t type = type_of(dy);
         if (dr) out[3] = dy;
         if (M == 0) {
-            if (dx) out[0] = at::empty({M, K}, x.options());
-            if (dw) out[1] = at::zeros({K, N}, x.options());
-            if (db) out[2] = at::zeros({N}, x.options());
+            if (dx) out[0] = at::empty({M, K}, options);
+            if (dw) out[1] = at::zeros({K, N}, options);
+            if (db) out[2] = at::zeros({N}, options);
             return out;
         }
         int64_t launches = 0;
         Tensor g = by_rows(dy);
-        if (db) out[2] = at::empty({N}, x.options());
+        if (db) out[2] = at::empty({N}, options);
         const uint32_t* signs = bits.defined() ? reinterpret_cast<const uint32_t*>(bits.data_ptr<int32_t>()) : nullptr;
         const int64_t ldbits = bits.defined() ? bits.size(1) : 0;
         if (N <= 32 && K <= 32) {                                 // narrow: all of them in one pass
-            const Tensor d = !dw ? Tensor() : out_in ? at::empty({N, K}, x.options()) : at::empty({K, N}, x.options());
-            const Tensor scratch = dw || db ? at::empty({dg_linear_grad_scratch(M, (int32_t)N, (int32_t)K)}, x.options().dtype(at::kFloat)) : Tensor();
+            const Tensor d = !dw ? Tensor() : out_in ? at::empty({N, K}, options) : at::empty({K, N}, options);
+            const Tensor scratch = dw || db ? at::empty({dg_linear_grad_scratch(M, (int32_t)N, (int32_t)K)}, options.dtype(at::kFloat)) : Tensor();
             dg_linear_grad_args a{};
-            a.x = x.data_ptr(), a.ldx = ld_of(x), a.w = w.data_ptr(), a.ldw = ld_of(w), a.dy = g.data_ptr(), a.lddy = ld_of(g), a.bits = signs, a.ldbits = ldbits;
+            const Tensor rows = dw ? by_rows(x) : Tensor();
+            if (dw) a.x = rows.data_ptr(), a.ldx = ld_of(rows);
+            if (dx) a.w = w.data_ptr(), a.ldw = ld_of(w);
+            a.dy = g.data_ptr(), a.lddy = ld_of(g), a.bits = signs, a.ldbits = ldbits;
             if (z.defined()) a.z = z.data_ptr(), a.ldz = ld_of(z);
-            if (dx) out[0] = at::empty({M, K}, x.options()), a.dx = out[0].data_ptr(), a.lddx = K;
+            if (dx) out[0] = at::empty({M, K}, options), a.dx = out[0].data_ptr(), a.lddx = K;
             if (dw) a.dw = d.data_ptr(), a.row_stride = out_in ? 1 : N, a.col_stride = out_in ? K : 1, out[1] = out_in ? d.t() : d;
             if (db) a.db = out[2].data_ptr();
             if (scratch.defined()) a.scratch = scratch.data_ptr<float>(), a.scratch_floats = scratch.numel();
@@ -505,8 +515,8 @@ struct LinearNode : public torch::autograd::Node {
             return out;
         }
         auto weight_gradient = [&](const Tensor& from, int32_t with, const Tensor* dz) {
-            const Tensor rows = to_rows(x, &launches), d = out_in ? at::empty({N, K}, x.options()) : at::empty({K, N}, x.options());
-            const Tensor partial = at::empty({dg_linear_dw_scratch(M, (int32_t)N, (int32_t)K, type)}, x.options().dtype(at::kFloat));
+            const Tensor rows = to_rows(x, &launches), d = out_in ? at::empty({N, K}, options) : at::empty({K, N}, options);
+            const Tensor partial = at::empty({dg_linear_dw_scratch(M, (int32_t)N, (int32_t)K, type)}, options.dtype(at::kFloat));
             dg_linear_dw_args a{};
             a.x = rows.data_ptr(), a.ldx = ld_of(rows), a.dy = from.data_ptr(), a.lddy = ld_of(from), a.dw = d.data_ptr();
             a.row_stride = out_in ? 1 : N, a.col_stride = out_in ? K : 1, a.M = M, a.N = (int32_t)N, a.K = (int32_t)K, a.type = type, a.act = with;
@@ -523,12 +533,12 @@ struct LinearNode : public torch::autograd::Node {
         // 16 bits, x of up to 256 columns: dz and its sums on the way to the weight gradient
         const bool together = item == 2 && dw && K <= 256 && (act != DG_ACT_NONE || db) && on_rows(g) && (!z.defined() || on_rows(z));
         if (together) {
-            const Tensor dz = dx && act != DG_ACT_NONE ? whole_rows(M, N, x) : Tensor();
+            const Tensor dz = dx && act != DG_ACT_NONE ? whole_rows(M, N, dy) : Tensor();
             weight_gradient(g, act, &dz);
             if (dz.defined()) g = dz;
         } else if (act != DG_ACT_NONE || db || ((dx || dw) && !on_rows(g))) {
-            const Tensor dz = (dx || dw) && (act != DG_ACT_NONE || !on_rows(g)) ? whole_rows(M, N, x) : Tensor();
-            const Tensor scratch = db ? at::empty({dg_linear_dz_scratch(M, (int32_t)N)}, x.options().dtype(at::kFloat)) : Tensor();
+            const Tensor dz = (dx || dw) && (act != DG_ACT_NONE || !on_rows(g)) ? whole_rows(M, N, dy) : Tensor();
+            const Tensor scratch = db ? at::empty({dg_linear_dz_scratch(M, (int32_t)N)}, options.dtype(at::kFloat)) : Tensor();
             if (dz.defined() || db) {
                 check(dg_linear_dz(g.data_ptr(), ld_of(g), z.defined() ? z.data_ptr() : nullptr, z.defined() ? ld_of(z) : 0, signs, ldbits, act,
                                    dz.defined() ? dz.data_ptr() : nullptr, dz.defined() ? dz.stride(0) : 0, db ? out[2].data_ptr() : nullptr, M, (int32_t)N, type,
@@ -538,7 +548,8 @@ struct LinearNode : public torch::autograd::Node {
             if (dz.defined()) g = dz;
         }
         if (dx) {
-            out[0] = result_rows(M, K, x);
+            if (item == 2 && M > dg_linear_few((int32_t)K, (int32_t)N, type)) w = to_rows(w, &launches);
+            out[0] = result_rows(M, K, dy);
             dg_linear_args a{};
             a.x = g.data_ptr(), a.ldx = ld_of(g), a.w = w.data_ptr(), a.ldw = ld_of(w), a.out_in = !out_in;
             a.y = out[0].data_ptr(), a.ldy = out[0].stride(0), a.M = M, a.N = (int32_t)K, a.K = (int32_t)N, a.type = type;
@@ -633,10 +644,16 @@ Tensor linear(const Tensor& x, const Tensor& w, const std::optional<Tensor>& bia
     if (train) {
         auto node = std::shared_ptr<LinearNode>(new LinearNode(), torch::autograd::deleteNode);
         node->set_next_edges(torch::autograd::collect_next_edges(x, w, b, r));
-        node->x_saved = SavedVariable(x, false), node->w_saved = SavedVariable(w, false);
-        node->x = x2.detach(), node->w = weight.t.detach();
-        node->splits = splits, node->z = z, node->bits = bits;
-        node->N = N, node->K = K, node->act = (int32_t)act, node->out_in = weight.out_in;
+        if (wants(w)) node->x_saved = SavedVariable(x2.is_same(x) ? x : x2.detach(), false);
+        if (wants(x) || wants(w)) {
+            node->w_copied = weight.t.data_ptr() != w.data_ptr(), node->w_out_in = weight.out_in;
+            node->w_saved = SavedVariable(node->w_copied ? weight.t.detach() : w, false);
+        }
+        if (splits.defined()) node->splits_saved = SavedVariable(splits, false);
+        if (z.defined()) node->z_saved = SavedVariable(z, false);
+        if (bits.defined()) node->bits_saved = SavedVariable(bits, false);
+        node->options = y.options().requires_grad(false);
+        node->M = M, node->N = N, node->K = K, node->act = (int32_t)act;
         torch::autograd::set_history(y, node);
     }
     return y;
