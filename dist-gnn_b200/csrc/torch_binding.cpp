@@ -591,6 +591,8 @@ Tensor linear(const Tensor& x, const Tensor& w, const std::optional<Tensor>& bia
         if (residual->dim() != 2 || residual->size(0) != M || residual->size(1) != N) refuse("residual must have the shape of the result");
     }
     const Tensor b = bias.value_or(Tensor()), r = residual.value_or(Tensor());
+    for (const Tensor* t : {&x, &w, &b, &r})
+        if (t->defined() && t->_fw_grad(0).defined()) refuse("tangents of forward-mode differentiation are not carried on");
     auto wants = [](const Tensor& t) { return t.defined() && t.requires_grad(); };
     const bool train = at::GradMode::is_enabled() && (wants(x) || wants(w) || wants(b) || wants(r));
     c10::cuda::CUDAGuard guard(x.device());

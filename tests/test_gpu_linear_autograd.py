@@ -99,3 +99,18 @@ def test_graphs_that_are_kept_and_that_are_not():
     assert all(torch.equal(p, q) for p, q in zip(first, second))
     with pytest.raises(RuntimeError, match='second time'):
         torch.autograd.grad(y, leaves, dy)
+
+
+def test_forward_mode_is_refused():
+    """A tangent would be lost without a word."""
+    import spmm_cpp
+    import torch.autograd.forward_ad as fwd
+    leaves, dy = _leaves(40, 40, 48, torch.float32)
+    for i in range(4):
+        with fwd.dual_level():
+            args = [t.detach() for t in leaves]
+            args[i] = fwd.make_dual(args[i], torch.ones_like(args[i]))
+            with pytest.raises(RuntimeError, match='linear: tangents'):
+                spmm_cpp.linear(args[0], args[1], args[2], residual=args[3])
+    with fwd.dual_level():
+        assert spmm_cpp.linear(*[t.detach() for t in leaves[:3]]).shape == (40, 48)
