@@ -913,7 +913,15 @@ class AdamW(torch.optim.Optimizer):
         self._table = None
 
     def load_state_dict(self, state_dict):
-        super().load_state_dict(state_dict)
+        loaded = []                                                # what is loaded, after hooks that change it
+        last = self.register_load_state_dict_pre_hook(lambda _, given: loaded.append(given))
+        first = self.register_load_state_dict_post_hook(lambda _: self._take_state(loaded[0]), prepend=True)
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            last.remove(), first.remove()
+
+    def _take_state(self, state_dict):
         # the base class casts a parameter's state to the parameter's type; these means have types of their own
         saved = [i for group in state_dict['param_groups'] for i in group['params']]
         own = [p for group in self.param_groups for p in group['params']]
