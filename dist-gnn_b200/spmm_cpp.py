@@ -875,6 +875,8 @@ class AdamW(torch.optim.Optimizer):
                 They are rounded at random (a mean that moves by 0.05 % a step would stand still on a grid of 6 %), with numbers that are a
                 function of `seed`, the step and the element's place, so that a run can be repeated; ranks that hold copies of a weight
                 keep equal copies if they have the same seed.
+                A state dict of torch.optim.AdamW over fp32 parameters loads into 32 bits; one of steps that are not these (amsgrad, maximize, torch.optim.Adam's with
+                weight decay) is refused.
     max_norm    gradients are scaled by min(1, max_norm / (norm + 1e-6)), norm being the 2-norm of all of them, inside the step (the .grad
                 tensors stay as they are); grad_norm is that norm, a 0-dim CUDA tensor.  None: no clipping.
 
@@ -914,7 +916,18 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         loaded = []                                                # what is loaded, after hooks that change it
-        last = self.register_load_state_dict_pre_hook(lambda _, given: loaded.append(given))
+
+        def check(_, given):
+            for group in given['param_groups']:
+                for name in ('amsgrad', 'maximize'):
+                    if group.get(name):
+                        raise ValueError(f'a state of an optimiser with {name} cannot be taken over: AdamW has no such steps')
+                if group.get('weight_decay') and not group.get('decoupled_weight_decay', True):
+                    raise ValueError('a state of an optimiser whose weight decay goes through the means cannot be taken over')
+                self._check_group({**self.defaults, **group, 'lr': float(group['lr'])})      # a rate may be kept in a tensor there
+            loaded.append(given)
+
+        last = self.register_load_state_dict_pre_hook(check)
         first = self.register_load_state_dict_post_hook(lambda _: self._take_state(loaded[0]), prepend=True)
         try:
             super().load_state_dict(state_dict)
@@ -929,6 +942,8 @@ class AdamW(torch.optim.Optimizer):
             if i in state_dict['state']:
                 self.state[p] = {name: torch.as_tensor(value, device=p.device, dtype=torch.int64 if name == 'step' else None).clone()
                                  for name, value in state_dict['state'][i].items()}
+        for group in self.param_groups:
+            group['lr'] = float(group['lr'])
         self._table = None
 
     def _new_state(self, p):

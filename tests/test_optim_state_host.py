@@ -48,3 +48,30 @@ def test_hooks_around_loading(bits):
     assert opt.state[params[0]]['exp_avg'].data_ptr() != other['state'][0]['exp_avg'].data_ptr()
     opt.load_state_dict(given)                                     # the hooks of the first call are gone, the user's are not
     assert len(opt._optimizer_load_state_dict_pre_hooks) == 1 and len(opt._optimizer_load_state_dict_post_hooks) == 1
+
+
+def test_states_of_other_steps_are_refused():
+    """Nothing has changed after a refusal; what differs in nothing but its name is taken."""
+    opt, params = _optimiser(torch.float32, lr=0.5)
+
+    def saved(kind, **options):
+        twins = [torch.nn.Parameter(p.detach().clone()) for p in params]
+        other = kind(twins, **options)
+        for p in twins:
+            p.grad = torch.ones_like(p)
+        other.step()
+        return other.state_dict()
+
+    for bad in (saved(torch.optim.AdamW, amsgrad=True), saved(torch.optim.AdamW, maximize=True), saved(torch.optim.Adam, weight_decay=0.1)):
+        with pytest.raises(ValueError, match='cannot be taken over'):
+            opt.load_state_dict(bad)
+        assert opt.param_groups[0]['lr'] == 0.5 and not opt.state
+    bad = saved(torch.optim.AdamW)
+    bad['param_groups'][0]['betas'] = (1.5, 0.9)
+    with pytest.raises(ValueError, match='betas'):
+        opt.load_state_dict(bad)
+    assert opt.param_groups[0]['betas'] == (0.9, 0.999) and not opt.state
+    for good in (saved(torch.optim.AdamW, lr=0.25), saved(torch.optim.Adam, lr=0.25), saved(torch.optim.AdamW, lr=torch.tensor(0.25), foreach=False)):
+        opt.load_state_dict(good)
+        assert opt.param_groups[0]['lr'] == 0.25 and type(opt.param_groups[0]['lr']) is float and int(opt.state[params[0]]['step']) == 1
+        assert opt.state[params[0]]['step'].dtype == torch.int64
