@@ -904,7 +904,11 @@ class AdamW(torch.optim.Optimizer):
 
     def add_param_group(self, param_group):
         super().add_param_group(param_group)
-        self._check_group(self.param_groups[-1])
+        try:
+            self._check_group(self.param_groups[-1])
+        except ValueError:
+            self.param_groups.pop()
+            raise
         self._table = None
 
     def __getstate__(self):

@@ -75,3 +75,14 @@ def test_states_of_other_steps_are_refused():
         opt.load_state_dict(good)
         assert opt.param_groups[0]['lr'] == 0.25 and type(opt.param_groups[0]['lr']) is float and int(opt.state[params[0]]['step']) == 1
         assert opt.state[params[0]]['step'].dtype == torch.int64
+
+
+def test_a_refused_group_is_not_kept():
+    opt, params = _optimiser()
+    more = torch.nn.Parameter(torch.ones(3))
+    for bad in (dict(betas=(2.0, 0.9)), dict(lr=-1.0), dict(eps=float('nan')), dict(lr=torch.tensor(0.1))):
+        with pytest.raises(ValueError):
+            opt.add_param_group(dict(params=[more], **bad))
+        assert len(opt.param_groups) == 1
+    opt.add_param_group(dict(params=[more], lr=0.1))
+    assert len(opt.param_groups) == 2 and opt.param_groups[1]['lr'] == 0.1
