@@ -6,6 +6,7 @@
 // of include/dist_gnn_b200.h; torch owns memory, streams and the graph, as everywhere in this package.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
@@ -675,6 +676,7 @@ struct AdamwTable {
     std::vector<py::object> seen;         // every parameter of the state, its dict and that dict's values, in their order
     Tensor workspace, norm;
     int32_t bits;
+    bool captured = false;                // a graph holds addresses of these tensors: they have to live on
 
     static void walk(PyObject* state, const std::function<bool(PyObject*)>& use)
     {
@@ -765,6 +767,7 @@ struct AdamwTable {
         }
         if (all.empty()) return;
         void* stream = stream_of(entries[0].p);
+        captured |= c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None;
         const bool clipped = max_norm > 0;
         if (clipped) check(dg_grad_norm(all.data(), (int32_t)all.size(), max_norm, norm.data_ptr<float>(), workspace.data_ptr(), workspace.numel(), stream));
         size_t first = 0;
@@ -794,6 +797,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
         .def(py::init<const py::dict&, const std::vector<std::tuple<Tensor, Tensor, Tensor, std::optional<Tensor>, std::optional<Tensor>, Tensor, int64_t, int32_t>>&, int32_t>())
         .def("same_state", &AdamwTable::same_state)
         .def("step", &AdamwTable::step)
+        .def_readonly("captured", &AdamwTable::captured)
         .def_readonly("norm", &AdamwTable::norm);
     m.def("linear", &linear);
     m.def("spmm", &spmm);

@@ -883,7 +883,8 @@ class AdamW(torch.optim.Optimizer):
     Parameters are contiguous CUDA tensors of one device; those without a gradient are left as they are.  An infinity, a NaN or a
     number whose square leaves fp32's range (1.8e19, after clipping) in a gradient makes its element's parameter and means non-finite, with 8 bits the means of its block of 256, and with max_norm all of them.
     Steps are counted on the device (state 'step', int64), so a step can be captured into a CUDA graph and replayed; the hyperparameters
-    are those of the capture.  Steps of one optimiser run one after the other: a graph of it and an eager step, or two graphs, not at once."""
+    are those of the capture, and so is the state: a graph goes on with the state that it was captured with when another has been loaded, which lives
+    as long as the optimiser.  Steps of one optimiser run one after the other: a graph of it and an eager step, or two graphs, not at once."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, max_norm=None, seed=0):
         if state_bits not in (8, 32):
@@ -892,6 +893,7 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f'max_norm must be None or a positive number, got {max_norm}')
         self._check_group(dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
         self.state_bits, self.max_norm, self.seed, self._table = state_bits, max_norm, int(seed) & 0xFFFFFFFF, None
+        self._captured = []                                        # earlier tables that a graph steps with
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
 
     @staticmethod
@@ -909,6 +911,11 @@ class AdamW(torch.optim.Optimizer):
         except ValueError:
             self.param_groups.pop()
             raise
+        self._drop_table()
+
+    def _drop_table(self):
+        if self._table is not None and self._table.captured:
+            self._captured.append(self._table)
         self._table = None
 
     def __getstate__(self):
@@ -916,7 +923,10 @@ class AdamW(torch.optim.Optimizer):
 
     def __setstate__(self, state):
         super().__setstate__(state)
-        self._table = None
+        if '_table' in self.__dict__:                              # loading a state, not making a copy
+            self._drop_table()
+        else:
+            self._table, self._captured = None, []
 
     def load_state_dict(self, state_dict):
         loaded = []                                                # what is loaded, after hooks that change it
@@ -948,7 +958,7 @@ class AdamW(torch.optim.Optimizer):
                                  for name, value in state_dict['state'][i].items()}
         for group in self.param_groups:
             group['lr'] = float(group['lr'])
-        self._table = None
+        self._drop_table()
 
     def _new_state(self, p):
         options = dict(device=p.device)
@@ -991,7 +1001,9 @@ class AdamW(torch.optim.Optimizer):
         table = self._table
         if table is None or not table.same_state(self.state):
             with torch.no_grad():
-                table = self._table = self._make_table()
+                table = self._make_table()
+            self._drop_table()
+            self._table = table
         groups = []
         for group in self.param_groups:
             b1, b2 = group['betas']
