@@ -488,6 +488,22 @@ class SumOverRanks(torch.autograd.Function):
         return grad_output
 
 
+def _time_backward(y, timer):
+    """The backward pass of the operation that made y as a region 'mm' of the timer, as its forward pass is: between the marks of hooks in front of its node and behind."""
+    if y.grad_fn is not None:
+        running = []
+
+        def enter(grads):
+            running.append(timer.timing_cuda('mm').__enter__())
+
+        def leave(inputs, grads):
+            running.pop().__exit__(None, None, None)
+
+        y.grad_fn.register_prehook(enter)
+        y.grad_fn.register_hook(leave)
+    return y
+
+
 class GCN(nn.Module):
     """num_layers DistGCNLayers with ReLU between them, no bias (gcn.py:56-72).  Weights are drawn as the reference
     draws them - torch.rand on the host after manual_seed(0), layer by layer - unless `weights` injects them.
@@ -544,9 +560,11 @@ class GCN(nn.Module):
         for l, w in enumerate(self.weights()):
             b = SumOverRanks.apply(getattr(self, f'bias{l + 1}')) if self.bias else None
             z = Aggregate.apply(h, self.g.adj_parts, f'L{l + 1}', l == 0)
-            with DistEnv.env.timer.timing_cuda('mm'):
+            timer = DistEnv.env.timer
+            with timer.timing_cuda('mm'):
                 h = spmm_cpp.linear(z, SumOverRanks.apply(w), b, residual=h if self.residual and 0 < l < last else None,
                                     activation=self.activation if l < last else None)
+            _time_backward(h, timer)
         return h
 
     def input_product(self, features):

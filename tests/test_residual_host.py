@@ -35,3 +35,32 @@ def test_gradients_of_shared_weights_are_summed_once(monkeypatch):
         x = torch.ones(3, requires_grad=True)
         gcn.SumOverRanks.apply(x).sum().backward()                   # an expanded gradient
         assert torch.equal(x.grad, torch.full((3,), float(world)))
+
+
+def test_backward_of_an_operation_is_timed():
+    """One region from before its node to behind it, for every backward pass; none where nothing is differentiated."""
+    from models import gcn
+    events = []
+
+    class Region:
+        def __enter__(self):
+            events.append('enter')
+            return self
+
+        def __exit__(self, *exc):
+            events.append('leave')
+
+    class Timer:
+        def timing_cuda(self, tag):
+            assert tag == 'mm'
+            return Region()
+
+    w = torch.ones(3, 2, requires_grad=True)
+    x = torch.ones(4, 3, requires_grad=True)
+    x.register_hook(lambda g: events.append('x'))
+    y = gcn._time_backward(x @ w, Timer())
+    (y * 2).sum().backward(retain_graph=True)
+    assert events == ['enter', 'leave', 'x']
+    (y * 2).sum().backward()
+    assert events == ['enter', 'leave', 'x'] * 2
+    gcn._time_backward(x.detach() @ w.detach(), Timer())
