@@ -1065,20 +1065,41 @@ __global__ void __launch_bounds__(32 * kFewWarps) k_few_rows16(const FewArgs a)
 #pragma unroll
     for (int j = 0; j < kLoads; ++j)
         from[j] = OUT_IN ? w + (int64_t)min(n0 + 8 * j + g, a.N - 1) * a.ldw : w + (int64_t)j * a.ldw + min(n0 + 4 * g, (a.N - 1) / 4 * 4);
+    // A chain's sums, to or on the warp's own.  Chains end as those of the tensor cores' kernels do: 16 x 1,048,576 -> 48 fp16 was 4e-4 too small in one.
+    constexpr int kChain = kChainTerms<T> / 16;
+    bool more = false;
+    auto put = [&]() {
+#pragma unroll
+        for (int j = 0; j < kMmas; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int in_mma = 2 * t + (e & 1), col = OUT_IN ? 8 * j + in_mma : 4 * in_mma + j;
+                float* const to = &sums[warp][g + (e & 2) * 4][col];
+                *to = more ? *to + acc[j][e] : acc[j][e];
+                acc[j][e] = 0.f;
+            }
+        more = true;
+    };
     int step = warp;
     if (a.whole_x && a.whole_w) {
         const int whole_steps = a.K / 16;
+        while (true) {
+            const int stop = min(whole_steps, step + kChain * kFewWarps);
 #pragma unroll 4
-        for (; step < whole_steps; step += kFewWarps) {
-            const int k = step * 16 + 4 * t;
-            const uint2 u0 = __ldg(reinterpret_cast<const uint2*>(x0 + k)), u1 = __ldg(reinterpret_cast<const uint2*>(x1 + k));
-            uint2 b[kLoads];
+            for (; step < stop; step += kFewWarps) {
+                const int k = step * 16 + 4 * t;
+                const uint2 u0 = __ldg(reinterpret_cast<const uint2*>(x0 + k)), u1 = __ldg(reinterpret_cast<const uint2*>(x1 + k));
+                uint2 b[kLoads];
 #pragma unroll
-            for (int j = 0; j < kLoads; ++j) b[j] = __ldg(reinterpret_cast<const uint2*>(from[j] + (OUT_IN ? (int64_t)k : k * a.ldw)));
-            multiply(u0, u1, b);
+                for (int j = 0; j < kLoads; ++j) b[j] = __ldg(reinterpret_cast<const uint2*>(from[j] + (OUT_IN ? (int64_t)k : k * a.ldw)));
+                multiply(u0, u1, b);
+            }
+            if (step >= whole_steps) break;
+            put();
         }
     }
-    for (; step * 16 < a.K; step += kFewWarps) {                  // other alignments, and the last step of an odd K
+    for (int n = 0; step * 16 < a.K; step += kFewWarps, ++n) {    // other alignments, and the last step of an odd K
+        if (n > 0 && n % kChain == 0) put();
         const int k = step * 16 + 4 * t, nk = a.K - k, nn = a.N - min(n0 + 4 * g, (a.N - 1) / 4 * 4);
         uint2 b[kLoads];
 #pragma unroll
@@ -1086,13 +1107,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) k_few_rows16(const FewArgs a)
             b[j] = OUT_IN ? load4(from[j] + k, nk, a.whole_w) : j < nk ? load4(from[j] + k * a.ldw, nn, a.whole_w) : make_uint2(0u, 0u);
         multiply(load4(x0 + k, nk, a.whole_x), load4(x1 + k, nk, a.whole_x), b);
     }
-#pragma unroll
-    for (int j = 0; j < kMmas; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int in_mma = 2 * t + (e & 1), col = OUT_IN ? 8 * j + in_mma : 4 * in_mma + j;
-            sums[warp][g + (e & 2) * 4][col] = acc[j][e];
-        }
+    put();
     __syncthreads();
     const int m = threadIdx.x / kCols, col = threadIdx.x % kCols;      // a warp has 32 columns of a row, or 16 of two
     if (m >= kFewRows) return;

@@ -170,3 +170,15 @@ def test_whole_numbers_of_many_columns_are_exact(M, K, N, act, dtype):
     db, = torch.autograd.grad(y, b, dy)
     assert torch.equal(db, (dy.double() * ((z > 0) if act else 1)).sum(0).to(dtype))
     assert spmm_cpp.dense_status() == 0
+
+
+@pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize('M,K,N', [(16, 1 << 20, 48), (32, 1_500_001, 40), (1, 1 << 21, 64), (5, 600_006, 33)])
+@pytest.mark.parametrize('transposed', [False, True])
+def test_products_of_few_rows_and_many_columns(M, K, N, transposed, dtype):
+    """Every warp's chains of a share of K, with whole and with odd alignments."""
+    import spmm_cpp
+    gen = torch.Generator(device='cuda').manual_seed(K + M)
+    x, w = _positive(gen, M, K, dtype=dtype), _positive(gen, K, N, dtype=dtype) * (64 / K)
+    w = w.t().contiguous().t() if transposed else w
+    _check(spmm_cpp.linear(x, w), x.double() @ w.double(), dtype)
