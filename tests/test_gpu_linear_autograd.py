@@ -114,3 +114,50 @@ def test_forward_mode_is_refused():
                 spmm_cpp.linear(args[0], args[1], args[2], residual=args[3])
     with fwd.dual_level():
         assert spmm_cpp.linear(*[t.detach() for t in leaves[:3]]).shape == (40, 48)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('M,K,N', [(5, 40, 24), (700, 40, 24), (700, 40, 41), (300, 7, 11)])
+def test_broadcast_inputs(M, K, N, dtype):
+    """A row for all of x, a number for all of a row of the residual: autograd sums the gradients.  Whole numbers below the type's exact ones in every row, and sums of them
+    that fp32 holds: the rounded sum itself."""
+    import spmm_cpp
+    g = torch.Generator(device='cuda').manual_seed(M + N)
+    row = torch.ones(1, K, device='cuda', dtype=dtype, requires_grad=True)
+    side = torch.ones(M, 1, device='cuda', dtype=dtype, requires_grad=True)
+    w = torch.randint(-2, 3, (K, N), device='cuda', generator=g).to(dtype)
+    y = spmm_cpp.linear(row.expand(M, K), w, residual=side.expand(M, N))
+    y.backward(torch.ones((), device='cuda', dtype=dtype).expand(M, N))
+    assert torch.equal(row.grad, (w.double().sum(1) * M).to(dtype)[None])
+    assert torch.equal(side.grad, torch.full((M, 1), float(N), device='cuda', dtype=torch.float64).to(dtype))
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.float16])
+@pytest.mark.parametrize('M,K,N', [(12, 40, 48), (5000, 24, 16), (700, 256, 264), (700, 300, 40), (900, 40, 41), (600, 1100, 33)])
+@pytest.mark.parametrize('act', [None, 'relu', 'gelu', 'silu'])
+def test_every_subset_of_gradients(M, K, N, act, dtype):
+    """Which gradients are asked for decides which kernels run; the numbers are those of all of them, but for the bias's, which kernels sum in different orders: one step
+    of the result and the order of M sums."""
+    import spmm_cpp
+    gen = torch.Generator(device='cuda').manual_seed(M + N)
+    base = [torch.randn(*s, device='cuda', generator=gen).to(dtype) for s in ((M, K), (K, N), (N,), (M, N))]
+    dy = torch.randn(M, N, device='cuda', generator=gen).to(dtype)
+
+    def grads(asked):
+        leaves = [t.clone().requires_grad_(bool(asked >> i & 1)) for i, t in enumerate(base)]
+        y = spmm_cpp.linear(*leaves[:3], residual=leaves[3], activation=act)
+        got = iter(torch.autograd.grad(y, [t for t in leaves if t.requires_grad], dy))
+        return [next(got) if t.requires_grad else None for t in leaves]
+
+    want = grads(15)
+    for asked in range(1, 15):
+        for i, (p, q) in enumerate(zip(grads(asked), want)):
+            assert (p is not None) == bool(asked >> i & 1)
+            if p is None:
+                continue
+            if i == 2:
+                step = {torch.float32: 2.0 ** -23, torch.float16: 2.0 ** -10}[dtype]
+                assert float((p.double() - q.double()).abs().max()) <= (step + M * 2.0 ** -24) * float(q.abs().max())
+            else:
+                assert torch.equal(p, q), (asked, i)
+    assert spmm_cpp.dense_status() == 0
