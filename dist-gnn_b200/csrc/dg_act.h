@@ -73,7 +73,7 @@ template <int ACT> __device__ __forceinline__ float act_slope(float z)
 // the pair above.  With a = |z| and e = exp(-z^2 / 2):  gelu(z) = max(z, 0) - a e R(a),  gelu'(z) = w + 1 for z > 0, else -w, with w = e (a / sqrt(2 pi) - R(a)).
 // R(a) = t P(t) as above, t = 1 / (1 + 0.3 a) and P of degree 5: within 1.8e-5 of R everywhere on [0, 14], a 27th of half a step of fp16, and 3e-7 of the value.  (A polynomial in
 // a, fitted for the value alone, was 11 % off at gelu(-4.5) and several times the value below -5.)  SiLU and GELU take one reciprocal for a pair: 1 / u = v / (u v).
-// 2,449,029 x 256 -> 256 bf16, forward alone (scalar -> pairs, and 8 -> 16 epilogue warps): GELU 741 us -> 595, SiLU 555 -> 478.
+// 2,449,029 x 256 -> 256 bf16, forward alone (scalar -> pairs, and 8 -> 16 epilogue warps): GELU 741 us -> 584, SiLU 555 -> 507.
 __device__ __forceinline__ float_pair reciprocals(float_pair u)      // of numbers whose product is within fp32's range
 {
     const float2 d = halves(u);

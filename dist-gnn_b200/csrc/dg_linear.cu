@@ -132,7 +132,7 @@ __device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t a_desc, uint6
 // in turn).  A stage is 64 K-columns of the CTA's 128 rows of x and of its half of the panel's columns of w.  Two accumulators (columns 0 / 256).
 // Barriers: full (even CTA, the loads of both), empty and acc_full (both CTAs, by commit), acc_empty (even CTA: the epilogue warps of both), and one an
 // epilogue warp and buffer for its residual's pieces.
-// What bounds it: HBM up to some 500 columns (400,000 x 256 -> 256 bf16 with GELU, bias, residual and z 139 us, 5.9 TB/s; without them 67 us, 6.15 TB/s), the tensor
+// What bounds it: HBM up to some 500 columns (400,000 x 256 -> 256 bf16 with GELU, bias, residual and z 143 us, 5.7 TB/s; without them 67 us, 6.1 TB/s), the tensor
 // cores beyond (65,536 x 1024 -> 1024 100 us, 1,379 TFLOP/s; with SiLU, residual and z 137).
 // DEEP: K beyond a chain; tiles of up to 128 columns, so that a warp has one piece, which it holds in registers while the tile's other chains run.
 template <class T, int ACT, bool DEEP>
@@ -401,7 +401,7 @@ k_linear_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
 // the MMA's 128 rows, so a panel wider than 128 takes two accumulators.  The range's partial goes to scratch, four columns of dz and all of x's side by
 // side; a second kernel adds the ranges in order.
 // One range (fewer than 512 rows, or more than 74 panels) of one chain is written as it is.
-// What bounds it: the tensor cores for wide layers (65,536 rows 1024 x 1024 93 us, 1,480 TFLOP/s), HBM for the others (232,965 rows 602 x 41 65 us, 4.6 TB/s).
+// What bounds it: the tensor cores for wide layers (65,536 rows 1024 x 1024 91 us, 1,502 TFLOP/s), HBM for the others (232,965 rows 602 x 41 63 us, 4.8 TB/s).
 // A chain of accumulations ends after kChainTerms rows, and the CTA adds the accumulators to its partial result: with ranges of one chain each, 300,000 x 264, 2304 fp16 were
 // 2.3e-4 too small and 131,072 x 2304, 2304, whose 81 panels leave one range, 7.8e-4.
 constexpr int kDwRows = 64, kDwBox = kDwRows * 128, kDwThreads = 32 * 6, kDwMaxStages = 8;
@@ -587,7 +587,7 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_linear_dw(const __grid_consta
 
 // The same product with dz made on the way, for x of up to 256 columns: dy arrives where dz is put together, z beside it; the operand that the tensor cores
 // then read is also what TMA stores, and its column sums are taken by the threads that make it.  So the gradients of w and b and dz itself, which x's
-// gradient needs, take one pass over x, dy and z; dz by a pass of its own reads and writes as much again (2,449,029 x 256, 256 bf16: 617 + 384 us, 725 this way).
+// gradient needs, take one pass over x, dy and z; dz by a pass of its own reads and writes as much again (2,449,029 x 256, 256 bf16: 656 + 388 us, 732 this way).
 // Warps: 0 TMA, 1 MMA issue + tensor-memory allocation, 2-9 dz (a row's 16-byte piece a thread and box of 32 rows x 64 columns), of which 2-5 flush, 10 stores dz.
 constexpr int kBackRows = 32, kBackBox = kBackRows * 128, kBackMakers = 8, kBackThreads = 32 * (3 + kBackMakers), kBackMaxStages = 8;
 constexpr int kBackBarBytes = 8 * (4 * kBackMaxStages + 3) + 8, kBackSumPitch = 9, kBackSumBytes = 32 * kBackMakers * kBackSumPitch * 4;
@@ -1175,7 +1175,7 @@ template <bool OUT_IN, int ROWS> __global__ void __launch_bounds__(32 * kFewWarp
 
 // ---- narrow layers ------------------------------------------------------------------------------------------------------------------
 // Up to 32 inputs and 32 outputs: a tile of the tensor cores' kernels costs some 2 us whatever its width, and rows that are no whole 16-byte pieces have to be
-// copied for them (1,611,877 x 7 -> 11 fp32 SiLU took 321 us, a sixteenth of it for the bytes, and takes 66), so these multiply on the CUDA cores, a row a thread, any strides, sums in fp32: K N products a row, for 32 x 32 about as long as the
+// copied for them (1,611,877 x 7 -> 11 fp32 SiLU took 321 us, a sixteenth of it for the bytes, and takes 63; its gradients 154), so these multiply on the CUDA cores, a row a thread, any strides, sums in fp32: K N products a row, for 32 x 32 about as long as the
 // bytes take.  Rows travel through shared memory, so that both ways are whole lines whatever the width; the place of an element by a product and a
 // shift instead of a division.
 constexpr int kThinRows = 128, kThinMost = 32, kThinPitch = 36;      // pitch: rows on 16 bytes, eight of them on all banks

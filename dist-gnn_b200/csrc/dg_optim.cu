@@ -9,8 +9,9 @@
 // of the distance to the neighbour below, with numbers that are a function of (seed, step, place): a step can be repeated bit for bit.  An r above zero is
 // never rounded to zero, or the next step would divide an m that is not by eps.  A block that holds an infinity or a NaN is non-finite from then on.
 //
-// What bounds it: HBM for tables with 32-bit states (28 bytes an element; 157 M fp32 698 us, 6.3 TB/s, and their norm 109 us, 5.8 TB/s), the issue slots with bf16 and
-// 8 bits (10 bytes and 52 instructions an element; 627 M 1,294 us, 4.9 TB/s, slots 67 % busy), the launch for small models (8.9 k elements 4.5 us).
+// What bounds it: HBM for tables with 32-bit states (28 bytes an element; 157 M fp32 702 us, 6.3 TB/s, and their norm 110 us, 5.7 TB/s; bf16 22 bytes, 578 us,
+// 6.0 TB/s), with bf16 and 8 bits (10 bytes and 55 instructions an element; 627 M 1,323 us, 4.8 TB/s) neither HBM nor the issue slots, 70 % busy: the latency that 24 warps
+// an SM leave uncovered; the launch for small models (8.9 k elements 4.8 us).
 #include <algorithm>
 #include <cmath>
 #include <type_traits>

@@ -827,13 +827,14 @@ def linear(x, weight, bias=None, residual=None, activation=None):
     layers here hold it, or the transpose of an [N x K] matrix, bias [N], residual [M x N], all fp32, bf16 or fp16.  activation: None, 'relu', 'gelu'
     (z Phi(z), not its tanh form) or 'silu'.
 
-    Everything between the operands and the result is in fp32 (fp32 products: three TF32 passes, as dense_nt), rounded once.  For the gradients
+    Everything between the operands and the result is in fp32 (fp32 products: three TF32 passes, as dense_nt; 0.6e-6 of the norm off at 100 columns, 2.7e-6
+    from 1,024 on, however many), rounded once.  For the gradients
     ReLU keeps a bit an element; GELU and SiLU keep x @ weight + bias in the type of x, and the gradient behind the activation is rounded to
     that type before it is multiplied.  Operands may have any strides: x, residual and gradients whose rows do not start on 16-byte boundaries are copied
     once, to padded rows, and the rows of the result and of x's gradient are padded to whole 16-byte pieces (a column slice of a wider buffer)
     where M exceeds the few rows (fp32 16, else 32) that smaller kernels take, but for layers of up to 32 inputs and outputs.  What is not finite in a row
     of x, of the residual or of a gradient stays in that row (and in the weight's and bias's gradients); an infinity among fp32 operands of the
-    three-pass product comes out as a NaN."""
+    three-pass product comes out as a NaN.  GELU and SiLU of minus infinity are zero.  Tangents of forward-mode differentiation and gradients of gradients are refused."""
     try:
         act = ACTIVATIONS[activation]
     except KeyError:

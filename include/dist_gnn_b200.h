@@ -388,8 +388,9 @@ int dg_rows_cross_entropy_grad(const float* x, int64_t ld, int64_t n, int32_t C,
                                const float* lse, const float* upstream, float* grad, int64_t ldg, void* stream);
 
 /* ---- linear layer: y = act(x w + b) + r, and its gradients (the reference's layers are torch.mm and F.relu, models/gcn.py:41, :70) ----
- * Types: fp32 (three TF32 passes, fp32 accuracy), bf16, fp16; every operand of a call is of its type, sums, bias, activation and residual are in fp32,
- * rounded once.  "On rows" below: the address is a multiple of 16 bytes and so is the row stride.
+ * Types: fp32 (three TF32 passes: off by 0.6e-6 of the norm at 100 columns, 0.9e-6 at 256, 2.7e-6 from 1,024 on, a plain fp32 product by 0.2e-6 to 0.6e-6), bf16, fp16; every operand of
+ * a call is of its type, sums, bias, activation and residual are in fp32, rounded once.  Sums of any length are taken in chains: what an accumulator truncates stays below an eighth
+ * of the rounding of a 16-bit result.  "On rows" below: the address is a multiple of 16 bytes and so is the row stride.
  *   x [M x K] ldx, w: [K x N] ldw (out_in == 0) or [N x K] ldw (out_in != 0), bias [N] or NULL, residual [M x N] ldr or NULL, y [M x N] ldy
  *   z, ldz    NULL, or where z = x w + b goes, rounded to the type, which the gradient of GELU and SiLU reads
  *   bits      NULL, or with ReLU a bit an element, set where z > 0: ldbits words a row, an even number >= N / 32, 8-byte aligned
