@@ -182,3 +182,39 @@ def test_products_of_few_rows_and_many_columns(M, K, N, transposed, dtype):
     x, w = _positive(gen, M, K, dtype=dtype), _positive(gen, K, N, dtype=dtype) * (64 / K)
     w = w.t().contiguous().t() if transposed else w
     _check(spmm_cpp.linear(x, w), x.double() @ w.double(), dtype)
+
+
+@pytest.mark.parametrize('dtype,M,K,N', [(torch.float32, 600, 2100, 1200), (torch.float16, 600, 20_000, 9_000), (torch.bfloat16, 70_000, 72, 300)])
+def test_chains_captured_and_on_two_streams(dtype, M, K, N):
+    """Layers whose products, x's gradients or weight gradients take several chains, two at once and replayed with other inputs: the eager numbers, bit for bit."""
+    import spmm_cpp
+    gen = torch.Generator(device='cuda').manual_seed(N)
+    x, w, dy = _positive(gen, M, K, dtype=dtype), _positive(gen, K, N, dtype=dtype) * (4 / K), _positive(gen, M, N, dtype=dtype) * (4 / N)
+
+    def both(a, b):
+        y = spmm_cpp.linear(a, b, activation='silu')
+        return (y.detach(), *torch.autograd.grad(y, [a, b], dy))
+
+    a, b = x.clone().requires_grad_(), w.clone().requires_grad_()
+    want = both(a, b)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            there = both(a, b)
+        here = both(a, b)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(p, q) for p, q in zip(want, there)) and all(torch.equal(p, q) for p, q in zip(want, here))
+    torch.cuda.synchronize()
+    del want, there, here
+    c, d = x.clone().requires_grad_(), w.clone().requires_grad_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = both(c, d)
+    with torch.no_grad():
+        c.copy_(_positive(gen, M, K, dtype=dtype))
+    graph.replay()
+    torch.cuda.synchronize()
+    e, f = c.detach().clone().requires_grad_(), d.detach().clone().requires_grad_()
+    assert all(torch.equal(p, q) for p, q in zip(got, both(e, f)))
+    assert spmm_cpp.dense_status() == 0
